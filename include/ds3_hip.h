@@ -44,6 +44,9 @@ typedef int32_t ds3_hip_type_t;
 #define DS3_HIP_TYPE_Q8_0 8
 #define DS3_HIP_TYPE_Q4_K 12
 #define DS3_HIP_TYPE_Q6_K 14
+/* Microscaled types of the *_mx calls, outside the range of GGUF's ids. */
+#define DS3_HIP_TYPE_MXFP4  256
+#define DS3_HIP_TYPE_MXINT8 257
 
 /* Opaque device buffer (reference src/ds3_metal.h:14). */
 typedef struct ds3_hip_buffer ds3_hip_buffer_t;
@@ -302,6 +305,81 @@ int ds3_hip_moe_bucket(const ds3_hip_buffer_t *indices, const ds3_hip_buffer_t *
  * (the parity probe for the block decoders). */
 int ds3_hip_dequantize(const ds3_hip_buffer_t *src, uint64_t src_offset, ds3_hip_type_t type, uint64_t n,
                        ds3_hip_buffer_t *dst);
+
+/* ---------------------------------------------------------------------- */
+/* Microscaled operators (no ds3_metal.h counterpart)                     */
+/* ---------------------------------------------------------------------- */
+
+/* 4-bit weights that the matrix cores take as they are, and rows in 8 bits
+ * for them.  A microscaled matrix [n_rows][n_cols], n_cols a multiple of 32,
+ * is two buffers (the element and scale formats of the OCP MX specification):
+ *   scales [n_rows][n_cols / 32]: a byte c per 32 consecutive values, for
+ *     2^(c - 127); 255 makes the whole block NaN;
+ *   codes, starting on a multiple of 16 bytes, rows without gaps:
+ *     DS3_HIP_TYPE_MXFP4  [n_rows][n_cols / 2]: E2M1 nibbles, bit 3 the sign,
+ *       bits 0..2 the magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6; value 2j in the
+ *       low half of byte j;
+ *     DS3_HIP_TYPE_MXINT8 [n_rows][n_cols]: signed bytes q, for q / 64.
+ * All calls: -1 for a null or too small buffer, sizes that a type does not
+ * take, an output that overlaps an input or another output, or a read-only
+ * output; 0 and nothing done for zero rows.  They need no workspace before
+ * them, so any of them can be captured (but see matmul_mx). */
+
+/* Rounds rows of src (F32, F16, Q8_0, Q4_K or Q6_K rows, src_row_stride bytes
+ * apart; n_cols a multiple of 256 for Q4_K / Q6_K; src and its stride
+ * multiples of 4 / 2 / 2 / 16 / 2 bytes) to a microscaled type, to nearest
+ * with ties to even.  A block's scale is 2^floor(log2 amax) for MXINT8, whose q
+ * saturates at +-127, and for MXFP4 the smallest power of two with amax at
+ * most 7 times it.  A block with an infinity or a NaN gets scale 255, one of
+ * zeros scale 0. */
+int ds3_hip_mx_quantize(const ds3_hip_buffer_t *src, ds3_hip_type_t src_type, uint64_t src_row_stride,
+                        ds3_hip_buffer_t *codes, ds3_hip_buffer_t *scales, ds3_hip_type_t mx_type,
+                        uint32_t n_rows, uint32_t n_cols);
+
+/* The values of a microscaled matrix, to F32 (exact) or F16 (rounded once)
+ * rows without gaps. */
+int ds3_hip_mx_dequantize(const ds3_hip_buffer_t *codes, const ds3_hip_buffer_t *scales, ds3_hip_type_t mx_type,
+                          uint32_t n_rows, uint32_t n_cols, ds3_hip_buffer_t *dst, ds3_hip_type_t dst_type);
+
+/* The prologue of an FFN block in one pass over n_rows rows of n: s = x +
+ * delta (delta NULL: s = x), y = s / sqrt(mean(s^2) + eps) * weight, and y
+ * rounded to MXINT8 rows as ds3_hip_mx_quantize rounds it.  sum (optional)
+ * receives s and may be x or delta; x_norm (optional) receives y, for the
+ * router.  n is a multiple of 32; every row's result is the same on every
+ * call. */
+int ds3_hip_add_rms_norm_mx(const ds3_hip_buffer_t *x, const ds3_hip_buffer_t *delta, const ds3_hip_buffer_t *weight,
+                            float eps, ds3_hip_buffer_t *sum, ds3_hip_buffer_t *x_norm, ds3_hip_buffer_t *codes,
+                            ds3_hip_buffer_t *scales, uint32_t n, uint32_t n_rows);
+
+/* C[M][N] = X[M][K] . W[N][K]^T in fp32 of MXINT8 rows and MXFP4 weights.
+ * Every product is exact and summed in fp32; the order of a sum depends on
+ * the sizes alone.  Rows of x whose scale is below 2^-122 are first rounded to
+ * multiples of 2^-128. */
+int ds3_hip_matmul_mx(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
+                      const ds3_hip_buffer_t *w_codes, const ds3_hip_buffer_t *w_scales, ds3_hip_buffer_t *C,
+                      uint32_t M, uint32_t N, uint32_t K);
+
+/* The same for rows grouped by expert, as ds3_hip_moe_bucket orders them:
+ *   C[r][n] = x[ids ? ids[r] : r] . w[g * N + n],  offsets[g] <= r < offsets[g + 1]
+ * offsets int32 [n_group + 1], never decreasing, n_group at most 1024; ids
+ * int32 [n_rows]; x has n_x rows, w n_group * N.  Groups may be empty and of
+ * any size.  Rows of C outside every group, and rows whose id is no row of x,
+ * are left as they were.  Offsets are taken into 0 .. n_rows; where they
+ * decrease the values of C are unspecified, nothing outside it is touched. */
+int ds3_hip_matmul_mx_grouped(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
+                              const ds3_hip_buffer_t *w_codes, const ds3_hip_buffer_t *w_scales,
+                              const ds3_hip_buffer_t *offsets, const ds3_hip_buffer_t *ids, ds3_hip_buffer_t *C,
+                              uint32_t n_x, uint32_t n_rows, uint32_t n_group, uint32_t N, uint32_t K);
+
+/* The experts' first half: h[r] = silu(x . gate) * (x . up) with rows and
+ * groups as in ds3_hip_matmul_mx_grouped (N = n_ff, K = n_embd), rounded to
+ * MXINT8 rows, the x of the down product.  n_ff is a multiple of 32. */
+int ds3_hip_moe_gate_up_mx(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
+                           const ds3_hip_buffer_t *gate_codes, const ds3_hip_buffer_t *gate_scales,
+                           const ds3_hip_buffer_t *up_codes, const ds3_hip_buffer_t *up_scales,
+                           const ds3_hip_buffer_t *offsets, const ds3_hip_buffer_t *ids,
+                           ds3_hip_buffer_t *h_codes, ds3_hip_buffer_t *h_scales, uint32_t n_x, uint32_t n_rows,
+                           uint32_t n_group, uint32_t n_ff, uint32_t n_embd);
 
 /* Router selection.  0 (default): the certified router (fp64 wavefront sums
  * with a proven error bound, exact sequential sums only where the bound

@@ -73,6 +73,12 @@ SIGNATURES: dict[str, tuple] = {
     "ds3_hip_moe_route": (C.c_int, [P, P, P, P, P, U32, U32, U32, U32, U64, I32, B]),
     "ds3_hip_moe_bucket": (C.c_int, [P, P, U32, U32, U32, P, P, P, P, P]),
     "ds3_hip_dequantize": (C.c_int, [P, U64, I32, U64, P]),
+    "ds3_hip_mx_quantize": (C.c_int, [P, I32, U64, P, P, I32, U32, U32]),
+    "ds3_hip_mx_dequantize": (C.c_int, [P, P, I32, U32, U32, P, I32]),
+    "ds3_hip_add_rms_norm_mx": (C.c_int, [P, P, P, F, P, P, P, P, U32, U32]),
+    "ds3_hip_matmul_mx": (C.c_int, [P, P, P, P, P, U32, U32, U32]),
+    "ds3_hip_matmul_mx_grouped": (C.c_int, [P, P, P, P, P, P, P, U32, U32, U32, U32, U32]),
+    "ds3_hip_moe_gate_up_mx": (C.c_int, [P, P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32]),
     "ds3_hip_set_router_mode": (C.c_int, [C.c_int]),
     "ds3_hip_router_stats": (C.c_int, [C.POINTER(U64), C.POINTER(U64), C.c_int]),
     "ds3_hip_debug_grouped_lists": (C.c_int, [P, P, P, P, P, P, P, P, P]),

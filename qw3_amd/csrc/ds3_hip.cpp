@@ -13,6 +13,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 #include <unistd.h>
 #include <vector>
@@ -1968,4 +1969,320 @@ extern "C" int ds3_hip_device_info(char *arch, size_t arch_len, int *n_cu, uint6
     if (n_cu) *n_cu = p.multiProcessorCount;
     if (hbm_bytes) *hbm_bytes = p.totalGlobalMem;
     return 0;
+}
+
+// ===========================================================================
+// Microscaled operators (no reference counterpart)
+// ===========================================================================
+
+namespace {
+
+// Rows and columns that the kernels index with 32 bits.
+bool mx_sizes_ok(const char *what, std::initializer_list<uint64_t> sizes)
+{
+    for (const uint64_t n : sizes)
+        if (n > 0x7fffffffu) {
+            fprintf(stderr, "ds3_hip: %s: a size of %llu is out of range\n", what, (unsigned long long)n);
+            return false;
+        }
+    return true;
+}
+
+bool mx_cols_ok(const char *what, const char *name, uint32_t n)
+{
+    if (n != 0 && n % 32 == 0) return true;
+    fprintf(stderr, "ds3_hip: %s: %s=%u must be a multiple of 32\n", what, name, n);
+    return false;
+}
+
+bool aligned_to(const ds3_hip_buffer_t *b, size_t n, const char *what, const char *name)
+{
+    if (!b || (uintptr_t)cptr(b) % n == 0) return true;
+    fprintf(stderr, "ds3_hip: %s: %s must start on a multiple of %zu bytes\n", what, name, n);
+    return false;
+}
+
+size_t mx_code_bytes(int type, uint64_t rows, uint32_t cols)
+{
+    return (size_t)rows * (type == T_MXFP4 ? cols / 2 : cols);
+}
+
+// The planes of a rows x cols matrix: large enough, the codes aligned.
+bool mx_planes_ok(const char *what, const char *name, const ds3_hip_buffer_t *codes, const ds3_hip_buffer_t *scales,
+                  int type, uint64_t rows, uint32_t cols)
+{
+    char c[32], s[32];
+    snprintf(c, sizeof c, "%s codes", name);
+    snprintf(s, sizeof s, "%s scales", name);
+    return fits(codes, mx_code_bytes(type, rows, cols), c) && fits(scales, rows * (cols / 32), s) &&
+           aligned_to(codes, 16, what, c);
+}
+
+struct Span {
+    const ds3_hip_buffer_t *buf;
+    size_t bytes;
+    const char *name;
+};
+
+// No byte that the call writes belongs to anything else that it reads or
+// writes, but that `may_be_input`, an output, may be one of the inputs.
+bool apart(const char *what, std::initializer_list<Span> out, std::initializer_list<Span> in,
+           const ds3_hip_buffer_t *may_be_input = nullptr)
+{
+    const auto meet = [](const Span &a, const Span &b) {
+        return a.buf && b.buf && a.bytes && b.bytes && cptr(a.buf) < cptr(b.buf) + b.bytes &&
+               cptr(b.buf) < cptr(a.buf) + a.bytes;
+    };
+    for (const Span *o = out.begin(); o != out.end(); o++) {
+        for (const Span *p = out.begin(); p != o; p++)
+            if (meet(*o, *p)) {
+                fprintf(stderr, "ds3_hip: %s: %s overlaps %s\n", what, o->name, p->name);
+                return false;
+            }
+        for (const Span &i : in)
+            if (meet(*o, i) && !(o->buf == may_be_input && cptr(o->buf) == cptr(i.buf) && o->bytes == i.bytes)) {
+                fprintf(stderr, "ds3_hip: %s: %s overlaps %s\n", what, o->name, i.name);
+                return false;
+            }
+    }
+    return true;
+}
+
+bool writable(const char *what, std::initializer_list<Span> out)
+{
+    for (const Span &o : out)
+        if (o.buf && o.buf->readonly) {
+            fprintf(stderr, "ds3_hip: %s: %s is a read-only buffer (buffer_from_mmap)\n", what, o.name);
+            return false;
+        }
+    return true;
+}
+
+constexpr uint32_t kMxMaxGroups = 1024;
+
+}  // namespace
+
+extern "C" int ds3_hip_mx_quantize(const ds3_hip_buffer_t *src, ds3_hip_type_t src_type, uint64_t src_row_stride,
+                                   ds3_hip_buffer_t *codes, ds3_hip_buffer_t *scales, ds3_hip_type_t mx_type,
+                                   uint32_t n_rows, uint32_t n_cols)
+{
+    const char *what = "mx_quantize";
+    if (!src || !codes || !scales) return -1;
+    if (mx_type != T_MXFP4 && mx_type != T_MXINT8) {
+        fprintf(stderr, "ds3_hip: %s: type %d is no microscaled type\n", what, mx_type);
+        return -1;
+    }
+    if (!mx_sizes_ok(what, { n_rows, n_cols }) || !mx_cols_ok(what, "n_cols", n_cols)) return -1;
+    const bool k_type = src_type == T_Q4_K || src_type == T_Q6_K;
+    const size_t rb = row_bytes(src_type, n_cols);
+    if (rb == 0 || (k_type && n_cols % 256 != 0)) {
+        fprintf(stderr, "ds3_hip: %s: rows of %u values of type %d unsupported\n", what, n_cols, src_type);
+        return -1;
+    }
+    if (n_rows == 0) return 0;
+    if (src_row_stride < rb) {
+        fprintf(stderr, "ds3_hip: %s: src_row_stride=%llu is shorter than one row (%zu bytes)\n", what,
+                (unsigned long long)src_row_stride, rb);
+        return -1;
+    }
+    const size_t need = src_type == T_F32 ? 4 : src_type == T_Q4_K ? 16 : 2;
+    if (!aligned_to(src, need, what, "src")) return -1;
+    if (n_rows > 1 && src_row_stride % need != 0) {
+        fprintf(stderr, "ds3_hip: %s: src_row_stride must be a multiple of %zu bytes\n", what, need);
+        return -1;
+    }
+    if (src_row_stride > (uint64_t)1 << 40) return -1;
+    const size_t sb = span_bytes(n_rows, src_row_stride, rb), cb = mx_code_bytes(mx_type, n_rows, n_cols),
+                 eb = (size_t)n_rows * (n_cols / 32);
+    if (!fits(src, sb, "src") || !mx_planes_ok(what, "the", codes, scales, mx_type, n_rows, n_cols) ||
+        !writable(what, { { codes, cb, "codes" }, { scales, eb, "scales" } }) ||
+        !apart(what, { { codes, cb, "codes" }, { scales, eb, "scales" } }, { { src, sb, "src" } }) || !ensure_init())
+        return -1;
+    KScope ks("mx_quantize");
+    return finish(launch_mx_quantize(src_type, cptr(src), src_row_stride, n_rows, n_cols, mx_type,
+                                     (uint8_t *)dptr(codes), (uint8_t *)dptr(scales), g.stream),
+                  what);
+}
+
+extern "C" int ds3_hip_mx_dequantize(const ds3_hip_buffer_t *codes, const ds3_hip_buffer_t *scales,
+                                     ds3_hip_type_t mx_type, uint32_t n_rows, uint32_t n_cols, ds3_hip_buffer_t *dst,
+                                     ds3_hip_type_t dst_type)
+{
+    const char *what = "mx_dequantize";
+    if (!codes || !scales || !dst) return -1;
+    if ((mx_type != T_MXFP4 && mx_type != T_MXINT8) || (dst_type != T_F32 && dst_type != T_F16)) {
+        fprintf(stderr, "ds3_hip: %s: from type %d to type %d unsupported\n", what, mx_type, dst_type);
+        return -1;
+    }
+    if (!mx_sizes_ok(what, { n_rows, n_cols }) || !mx_cols_ok(what, "n_cols", n_cols)) return -1;
+    if (n_rows == 0) return 0;
+    const size_t n = (size_t)n_rows * n_cols, db = row_bytes(dst_type, 1) * n,
+                 cb = mx_code_bytes(mx_type, n_rows, n_cols), eb = n / 32;
+    if (!mx_planes_ok(what, "the", codes, scales, mx_type, n_rows, n_cols) || !fits(dst, db, "dst") ||
+        !aligned_to(dst, row_bytes(dst_type, 1), what, "dst") || !writable(what, { { dst, db, "dst" } }) ||
+        !apart(what, { { dst, db, "dst" } }, { { codes, cb, "codes" }, { scales, eb, "scales" } }) || !ensure_init())
+        return -1;
+    KScope ks("mx_dequantize");
+    return finish(launch_mx_dequantize(mx_type, cptr(codes), cptr(scales), (int64_t)n, dst_type, dptr(dst), g.stream),
+                  what);
+}
+
+extern "C" int ds3_hip_add_rms_norm_mx(const ds3_hip_buffer_t *x, const ds3_hip_buffer_t *delta,
+                                       const ds3_hip_buffer_t *weight, float eps, ds3_hip_buffer_t *sum,
+                                       ds3_hip_buffer_t *x_norm, ds3_hip_buffer_t *codes, ds3_hip_buffer_t *scales,
+                                       uint32_t n, uint32_t n_rows)
+{
+    const char *what = "add_rms_norm_mx";
+    if (!x || !weight || !codes || !scales || !(eps >= 0.0f)) return -1;
+    if (!mx_sizes_ok(what, { n, n_rows }) || !mx_cols_ok(what, "n", n)) return -1;
+    if (n_rows == 0) return 0;
+    const size_t bytes = (size_t)n * n_rows * 4, wb = (size_t)n * 4, cb = (size_t)n * n_rows, eb = cb / 32;
+    if (!fits(x, bytes, "x") || !fits(delta, bytes, "delta") || !fits(weight, wb, "weight") ||
+        !fits(sum, bytes, "sum") || !fits(x_norm, bytes, "x_norm") ||
+        !mx_planes_ok(what, "the", codes, scales, T_MXINT8, n_rows, n))
+        return -1;
+    for (const ds3_hip_buffer_t *b : { x, delta, weight, (const ds3_hip_buffer_t *)sum, (const ds3_hip_buffer_t *)x_norm })
+        if (!aligned_to(b, 4, what, "an f32 buffer")) return -1;
+    const Span o[4] = { { sum, bytes, "sum" }, { x_norm, bytes, "x_norm" }, { codes, cb, "codes" }, { scales, eb, "scales" } };
+    // sum may be x or delta itself: a row's values are read before they are written
+    if (!writable(what, { o[0], o[1], o[2], o[3] }) ||
+        !apart(what, { o[0], o[1], o[2], o[3] }, { { x, bytes, "x" }, { delta, bytes, "delta" }, { weight, wb, "weight" } },
+               sum) ||
+        !ensure_init())
+        return -1;
+    KScope ks("add_rms_norm_mx");
+    return finish(launch_add_rms_norm_mx(fptr(x), delta ? fptr(delta) : nullptr, fptr(weight), eps,
+                                         sum ? fptr(sum) : nullptr, x_norm ? fptr(x_norm) : nullptr,
+                                         (uint8_t *)dptr(codes), (uint8_t *)dptr(scales), (int)n, n_rows, g.stream),
+                  what);
+}
+
+extern "C" int ds3_hip_matmul_mx(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
+                                 const ds3_hip_buffer_t *w_codes, const ds3_hip_buffer_t *w_scales,
+                                 ds3_hip_buffer_t *C, uint32_t M, uint32_t N, uint32_t K)
+{
+    const char *what = "matmul_mx";
+    if (!x_codes || !x_scales || !w_codes || !w_scales || !C) return -1;
+    if (!mx_sizes_ok(what, { M, N, K }) || !mx_cols_ok(what, "K", K)) return -1;
+    if (M == 0 || N == 0) return 0;
+    const size_t c_b = (size_t)M * N * 4, nb = K / 32;
+    const Span o{ C, c_b, "C" };
+    if (!mx_planes_ok(what, "x", x_codes, x_scales, T_MXINT8, M, K) ||
+        !mx_planes_ok(what, "w", w_codes, w_scales, T_MXFP4, N, K) || !fits(C, c_b, "C") ||
+        !aligned_to(C, 4, what, "C") || !writable(what, { o }) ||
+        !apart(what, { o }, { { x_codes, (size_t)M * K, "x codes" }, { x_scales, M * nb, "x scales" },
+                              { w_codes, (size_t)N * K / 2, "w codes" }, { w_scales, N * nb, "w scales" } }) ||
+        !ensure_init())
+        return -1;
+    MxProduct p{};
+    p.xc = cptr(x_codes);
+    p.xs = cptr(x_scales);
+    p.wc = cptr(w_codes);
+    p.ws = cptr(w_scales);
+    p.c = fptr(C);
+    p.n_x = p.n_rows = (int)M;
+    p.n_group = 1;
+    p.N = (int)N;
+    p.K = (int)K;
+    KScope ks("mx_product");
+    return finish(launch_mx_product(p, g.stream), what);
+}
+
+namespace {
+
+// The checks that the grouped products share; true with *p filled but for the
+// outputs.
+bool mx_grouped_args(const char *what, const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
+                     const ds3_hip_buffer_t *w_codes, const ds3_hip_buffer_t *w_scales, const ds3_hip_buffer_t *u_codes,
+                     const ds3_hip_buffer_t *u_scales, const ds3_hip_buffer_t *offsets, const ds3_hip_buffer_t *ids,
+                     uint32_t n_x, uint32_t n_rows, uint32_t n_group, uint32_t N, uint32_t K, MxProduct *p)
+{
+    if (!x_codes || !x_scales || !w_codes || !w_scales || !offsets) return false;
+    const uint64_t wr = (uint64_t)n_group * N;
+    if (!mx_sizes_ok(what, { n_x, n_rows, N, K }) || !mx_cols_ok(what, "K", K)) return false;
+    if (n_group == 0 || n_group > kMxMaxGroups) {
+        fprintf(stderr, "ds3_hip: %s: n_group=%u (1 to %u)\n", what, n_group, kMxMaxGroups);
+        return false;
+    }
+    if (!ids && n_x < n_rows) {
+        fprintf(stderr, "ds3_hip: %s: x has %u rows, without ids it needs n_rows=%u\n", what, n_x, n_rows);
+        return false;
+    }
+    if (!mx_planes_ok(what, "x", x_codes, x_scales, T_MXINT8, n_x, K) ||
+        !mx_planes_ok(what, "w", w_codes, w_scales, T_MXFP4, wr, K) ||
+        (u_codes && !mx_planes_ok(what, "up", u_codes, u_scales, T_MXFP4, wr, K)) ||
+        !fits(offsets, ((size_t)n_group + 1) * 4, "offsets") || !fits(ids, (size_t)n_rows * 4, "ids") ||
+        !aligned_to(offsets, 4, what, "offsets") || !aligned_to(ids, 4, what, "ids"))
+        return false;
+    *p = MxProduct{};
+    p->xc = cptr(x_codes);
+    p->xs = cptr(x_scales);
+    p->wc = cptr(w_codes);
+    p->ws = cptr(w_scales);
+    p->uc = cptr(u_codes);
+    p->us = cptr(u_scales);
+    p->offsets = (const int32_t *)cptr(offsets);
+    p->ids = (const int32_t *)cptr(ids);
+    p->n_x = (int)n_x;
+    p->n_rows = (int)n_rows;
+    p->n_group = (int)n_group;
+    p->N = (int)N;
+    p->K = (int)K;
+    return true;
+}
+
+}  // namespace
+
+extern "C" int ds3_hip_matmul_mx_grouped(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
+                                         const ds3_hip_buffer_t *w_codes, const ds3_hip_buffer_t *w_scales,
+                                         const ds3_hip_buffer_t *offsets, const ds3_hip_buffer_t *ids,
+                                         ds3_hip_buffer_t *C, uint32_t n_x, uint32_t n_rows, uint32_t n_group,
+                                         uint32_t N, uint32_t K)
+{
+    const char *what = "matmul_mx_grouped";
+    MxProduct p;
+    if (!C || !mx_grouped_args(what, x_codes, x_scales, w_codes, w_scales, nullptr, nullptr, offsets, ids, n_x, n_rows,
+                               n_group, N, K, &p))
+        return -1;
+    if (n_x == 0 || n_rows == 0 || N == 0) return 0;
+    const size_t wr = (size_t)n_group * N, nb = K / 32;
+    const Span o{ C, (size_t)n_rows * N * 4, "C" };
+    if (!fits(C, o.bytes, "C") || !aligned_to(C, 4, what, "C") || !writable(what, { o }) ||
+        !apart(what, { o }, { { x_codes, (size_t)n_x * K, "x codes" }, { x_scales, n_x * nb, "x scales" },
+                              { w_codes, wr * K / 2, "w codes" }, { w_scales, wr * nb, "w scales" },
+                              { offsets, ((size_t)n_group + 1) * 4, "offsets" }, { ids, (size_t)n_rows * 4, "ids" } }) ||
+        !ensure_init())
+        return -1;
+    p.c = fptr(C);
+    KScope ks("mx_product");
+    return finish(launch_mx_product(p, g.stream), what);
+}
+
+extern "C" int ds3_hip_moe_gate_up_mx(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
+                                      const ds3_hip_buffer_t *gate_codes, const ds3_hip_buffer_t *gate_scales,
+                                      const ds3_hip_buffer_t *up_codes, const ds3_hip_buffer_t *up_scales,
+                                      const ds3_hip_buffer_t *offsets, const ds3_hip_buffer_t *ids,
+                                      ds3_hip_buffer_t *h_codes, ds3_hip_buffer_t *h_scales, uint32_t n_x,
+                                      uint32_t n_rows, uint32_t n_group, uint32_t n_ff, uint32_t n_embd)
+{
+    const char *what = "moe_gate_up_mx";
+    MxProduct p;
+    if (!up_codes || !up_scales || !h_codes || !h_scales || !mx_cols_ok(what, "n_ff", n_ff) ||
+        !mx_grouped_args(what, x_codes, x_scales, gate_codes, gate_scales, up_codes, up_scales, offsets, ids, n_x,
+                         n_rows, n_group, n_ff, n_embd, &p))
+        return -1;
+    if (n_x == 0 || n_rows == 0) return 0;
+    const size_t wr = (size_t)n_group * n_ff, nb = n_embd / 32, hb = (size_t)n_rows * n_ff;
+    const Span o{ h_codes, hb, "h codes" }, os{ h_scales, hb / 32, "h scales" };
+    if (!mx_planes_ok(what, "h", h_codes, h_scales, T_MXINT8, n_rows, n_ff) || !writable(what, { o, os }) ||
+        !apart(what, { o, os }, { { x_codes, (size_t)n_x * n_embd, "x codes" }, { x_scales, n_x * nb, "x scales" },
+                                  { gate_codes, wr * n_embd / 2, "gate codes" }, { gate_scales, wr * nb, "gate scales" },
+                                  { up_codes, wr * n_embd / 2, "up codes" }, { up_scales, wr * nb, "up scales" },
+                                  { offsets, ((size_t)n_group + 1) * 4, "offsets" }, { ids, (size_t)n_rows * 4, "ids" } }) ||
+        !ensure_init())
+        return -1;
+    p.hc = (uint8_t *)dptr(h_codes);
+    p.hs = (uint8_t *)dptr(h_scales);
+    KScope ks("mx_gate_up");
+    return finish(launch_mx_product(p, g.stream), what);
 }

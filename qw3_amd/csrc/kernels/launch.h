@@ -10,6 +10,8 @@ namespace ds3k {
 
 // GGUF type ids (reference src/ds3.h:201-216).
 enum : int { T_F32 = 0, T_F16 = 1, T_Q8_0 = 8, T_Q4_K = 12, T_Q6_K = 14 };
+// Microscaled types (mx.h), outside the range of GGUF's ids.
+enum : int { T_MXFP4 = 256, T_MXINT8 = 257 };
 
 // Where the three expert matrices of expert e start: either e * rows * stride
 // or, if `table` is non-null, table[3e + {0,1,2}] (gate, up, down) bytes.
@@ -252,5 +254,36 @@ hipError_t launch_scatter_add(const float *src, const float *scores, const int32
                               int n_cols, int count, int64_t n_rows, hipStream_t s);
 hipError_t launch_silu_mul(const float *g, const float *u, float *out, int64_t n, hipStream_t s);
 hipError_t launch_axpy(const float *x, float w, float *y, int64_t n, hipStream_t s);
+
+// Microscaled rows (mx.h).  codes 16-byte aligned, n_cols a multiple of 32
+// (of 256 from Q4_K / Q6_K); src as its type's blocks need (F32 4, F16 / Q6_K /
+// Q8_0 2, Q4_K 16 bytes), rows `stride` bytes apart.
+hipError_t launch_mx_quantize(int type, const uint8_t *src, uint64_t stride, int64_t n_rows, int64_t n_cols, int mx,
+                              uint8_t *codes, uint8_t *scales, hipStream_t s);
+// n values (a multiple of 32) to dst of T_F32 or T_F16.
+hipError_t launch_mx_dequantize(int mx, const uint8_t *codes, const uint8_t *scales, int64_t n, int dst_type, void *dst,
+                                hipStream_t s);
+// s = x + delta (delta optional); y = rms_norm(s) * g; MXINT8 rows of y, and s
+// and y where sum and y are given.  sum may be x or delta.
+hipError_t launch_add_rms_norm_mx(const float *x, const float *delta, const float *g, float eps, float *sum, float *y,
+                                  uint8_t *codes, uint8_t *scales, int n, int64_t n_rows, hipStream_t s);
+
+// Products of MXINT8 rows with MXFP4 weights.  Row r of the n_rows belongs to
+// the group that offsets [n_group + 1] puts it in (offsets null: one group) and
+// takes row ids[r] of x (ids null: row r) of n_x; group g's weights are rows
+// g N .. g N + N - 1 of the weight matrix.  Rows of no group and rows whose id
+// is no row of x are left as they are.
+//   hc null: c[r][n] = x . w
+//   else:    h[r][n] = silu(x . w) * (x . u), rounded to MXINT8 (N % 32 = 0)
+struct MxProduct {
+    const uint8_t *xc, *xs;             // x codes, scales
+    const uint8_t *wc, *ws, *uc, *us;   // weights (gate), up
+    const int32_t *offsets, *ids;
+    float *c;
+    uint8_t *hc, *hs;
+    int n_x, n_rows, n_group, N, K;
+    int c_vec;                          // c rows take 16-byte stores
+};
+hipError_t launch_mx_product(const MxProduct &p, hipStream_t s);
 
 }  // namespace ds3k

@@ -1,0 +1,371 @@
+// mx_rows.hip -- rows to and from the microscaled formats (mx.h): rounding of
+// F32 / F16 / GGUF-quantised rows, its inverse, and the FFN block's prologue
+// (residual addition, RMS norm, rounding) in one pass.
+#include "mx.h"
+
+#include <algorithm>
+
+namespace ds3k {
+
+constexpr int MXR_TPB = 256;
+
+// ---------------------------------------------------------------------------
+// Rounding.  One pass, bound by its reads: eight lanes take a block, four
+// values each (16-byte loads of F32), so that a wave reads 1 KiB and writes
+// whole lines.
+// ---------------------------------------------------------------------------
+
+// Four consecutive values; VEC: the address is a multiple of their size.
+template <bool F16, bool VEC>
+__device__ __forceinline__ void load4(const uint8_t *p, float (&v)[4])
+{
+    if constexpr (F16) {
+        if constexpr (VEC) {
+            const half4_t h = *(const half4_t *)p;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = (float)h[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = (float)((const _Float16 *)p)[i];
+        }
+    } else if constexpr (VEC) {
+        const float4 f = *(const float4 *)p;
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = ((const float *)p)[i];
+    }
+}
+
+// The eight lanes of a block: values v of lane s = lane % 8, block `b` of the
+// matrix (row major).
+template <int MX>
+__device__ __forceinline__ void store_block8(const float (&v)[4], int64_t b, int s, uint8_t *codes, uint8_t *scales)
+{
+    uint32_t m = abs_bits(v[0]);
+#pragma unroll
+    for (int i = 1; i < 4; i++) m = max(m, abs_bits(v[i]));
+    const uint32_t c = mx_scale<MX>(max8(m));
+    const uint32_t w = mx_round4<MX>(v, c);
+    if constexpr (MX == T_MXINT8) *(uint32_t *)(codes + b * 32 + 4 * s) = w;
+    else *(uint16_t *)(codes + b * 16 + 2 * s) = (uint16_t)w;
+    if (s == 0) scales[b] = (uint8_t)c;
+}
+
+// nb blocks a row, rows `stride` bytes apart (dense rows are given as one).
+template <int MX, bool F16, bool VEC>
+__global__ void __launch_bounds__(MXR_TPB) k_mx_round(const uint8_t *src, uint64_t stride, int64_t n_blocks, int64_t nb,
+                                                      uint8_t *codes, uint8_t *scales)
+{
+    const int s = threadIdx.x & 7;
+    const int64_t step = (int64_t)gridDim.x * (MXR_TPB / 8);
+    for (int64_t b = (int64_t)blockIdx.x * (MXR_TPB / 8) + (threadIdx.x >> 3); b < n_blocks; b += step) {
+        const int64_t row = nb == n_blocks ? 0 : b / nb;
+        const int64_t col = (b - row * nb) * 32 + 4 * s;
+        float v[4];
+        load4<F16, VEC>(src + row * stride + col * (F16 ? 2 : 4), v);
+        store_block8<MX>(v, b, s, codes, scales);
+    }
+}
+
+// GGUF blocks: a thread decodes one 32-weight unit (common.h) into LDS, where
+// the units of a 256-weight block lie interleaved, then rounds one block.  The
+// LDS rows of 32 are 33 floats apart: a wave's 32-float rows would otherwise
+// start in the same bank.
+template <int MX, int TYPE>
+__global__ void __launch_bounds__(MXR_TPB) k_mx_round_gguf(const uint8_t *src, uint64_t stride, int64_t n_blocks,
+                                                           int64_t nb, uint8_t *codes, uint8_t *scales)
+{
+    __shared__ float lds[MXR_TPB * 33];
+    const int64_t step = (int64_t)gridDim.x * MXR_TPB;
+    for (int64_t b0 = (int64_t)blockIdx.x * MXR_TPB; b0 < n_blocks; b0 += step) {
+        const int64_t b = b0 + threadIdx.x;
+        const bool in = b < n_blocks;
+        float w[32];
+        if (in) {
+            const int64_t row = b / nb;
+            int k0[4];
+            unit_decode<TYPE>(src + row * stride, (int)(b - row * nb), w, k0);
+            if constexpr (TYPE != T_Q8_0) {
+                // rows are whole 256-weight blocks, so unit b's block starts 8 * (b / 8) units in
+                float *base = lds + (threadIdx.x & ~7) * 33;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const int o = k0[s] & 255;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) base[o + (o >> 5) + i] = w[8 * s + i];
+                }
+            }
+        }
+        if constexpr (TYPE != T_Q8_0) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 32; i++) w[i] = lds[threadIdx.x * 33 + i];
+            __syncthreads();
+        }
+        if (!in) continue;
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 32; i++) m = max(m, abs_bits(w[i]));
+        const uint32_t c = mx_scale<MX>(m);
+        uint32_t q[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float v[4] = { w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3] };
+            q[i] = mx_round4<MX>(v, c);
+        }
+        if constexpr (MX == T_MXINT8) {
+            *(uint4 *)(codes + b * 32) = make_uint4(q[0], q[1], q[2], q[3]);
+            *(uint4 *)(codes + b * 32 + 16) = make_uint4(q[4], q[5], q[6], q[7]);
+        } else {
+            *(uint4 *)(codes + b * 16) = make_uint4(q[0] | (q[1] << 16), q[2] | (q[3] << 16), q[4] | (q[5] << 16),
+                                                    q[6] | (q[7] << 16));
+        }
+        scales[b] = (uint8_t)c;
+    }
+}
+
+// The workgroups of a grid-stride kernel over n units of `per` a workgroup.
+static unsigned strided_grid(int64_t n, int per)
+{
+    const int64_t wg = (n + per - 1) / per;
+    return (unsigned)std::min<int64_t>(wg, (int64_t)1 << 20);
+}
+
+template <int MX>
+static hipError_t launch_round(int type, const uint8_t *src, uint64_t stride, int64_t n_rows, int64_t n_cols,
+                               uint8_t *codes, uint8_t *scales, hipStream_t s)
+{
+    const int64_t n_blocks = n_rows * (n_cols / 32);
+    int64_t nb = n_cols / 32;
+    if (type == T_F32 || type == T_F16) {
+        const int size = type == T_F32 ? 4 : 2;
+        if (stride == (uint64_t)n_cols * size) nb = n_blocks;                   // one long row
+        const bool vec = ((uintptr_t)src | (nb == n_blocks ? 0 : stride)) % (4 * size) == 0;
+        const dim3 grid(strided_grid(n_blocks, MXR_TPB / 8)), tpb(MXR_TPB);
+        if (type == T_F32) {
+            if (vec) hipLaunchKernelGGL((k_mx_round<MX, false, true>), grid, tpb, 0, s, src, stride, n_blocks, nb, codes, scales);
+            else hipLaunchKernelGGL((k_mx_round<MX, false, false>), grid, tpb, 0, s, src, stride, n_blocks, nb, codes, scales);
+        } else {
+            if (vec) hipLaunchKernelGGL((k_mx_round<MX, true, true>), grid, tpb, 0, s, src, stride, n_blocks, nb, codes, scales);
+            else hipLaunchKernelGGL((k_mx_round<MX, true, false>), grid, tpb, 0, s, src, stride, n_blocks, nb, codes, scales);
+        }
+        return hipGetLastError();
+    }
+    const dim3 grid(strided_grid(n_blocks, MXR_TPB)), tpb(MXR_TPB);
+    switch (type) {
+    case T_Q8_0: hipLaunchKernelGGL((k_mx_round_gguf<MX, T_Q8_0>), grid, tpb, 0, s, src, stride, n_blocks, nb, codes, scales); break;
+    case T_Q4_K: hipLaunchKernelGGL((k_mx_round_gguf<MX, T_Q4_K>), grid, tpb, 0, s, src, stride, n_blocks, nb, codes, scales); break;
+    case T_Q6_K: hipLaunchKernelGGL((k_mx_round_gguf<MX, T_Q6_K>), grid, tpb, 0, s, src, stride, n_blocks, nb, codes, scales); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_mx_quantize(int type, const uint8_t *src, uint64_t stride, int64_t n_rows, int64_t n_cols, int mx,
+                              uint8_t *codes, uint8_t *scales, hipStream_t s)
+{
+    return mx == T_MXFP4 ? launch_round<T_MXFP4>(type, src, stride, n_rows, n_cols, codes, scales, s)
+                         : launch_round<T_MXINT8>(type, src, stride, n_rows, n_cols, codes, scales, s);
+}
+
+// ---------------------------------------------------------------------------
+// The values of a matrix.  Four a thread; every product is exact in fp32 but
+// for a 6 * 2^127 or 2^128 that overflows to infinity.
+// ---------------------------------------------------------------------------
+template <int MX, bool F16, bool VEC>
+__global__ void __launch_bounds__(MXR_TPB) k_mx_values(const uint8_t *codes, const uint8_t *scales, int64_t n4, void *dst)
+{
+    const int64_t step = (int64_t)gridDim.x * MXR_TPB;
+    for (int64_t i = (int64_t)blockIdx.x * MXR_TPB + threadIdx.x; i < n4; i += step) {
+        const int c = scales[i >> 3];
+        float v[4];
+        if constexpr (MX == T_MXINT8) {
+            const uint32_t w = ((const uint32_t *)codes)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __builtin_amdgcn_ldexpf((float)(int8_t)byte_of(w, j), c - 133);
+        } else {
+            const uint32_t w = ((const uint16_t *)codes)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                // twice the magnitudes, as bytes 0, 1, 2, 3 and 4, 6, 8, 12
+                const uint32_t n = (w >> (4 * j)) & 15u, k = n & 7u;
+                const float m = (float)byte_of(k < 4u ? 0x03020100u : 0x0c080604u, (int)(k & 3u));
+                v[j] = __builtin_amdgcn_ldexpf(n & 8u ? -m : m, c - 128);
+            }
+        }
+        if (c == 255)
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __uint_as_float(0x7fc00000u);
+        if constexpr (F16) {
+            const half4_t h = { (_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3] };
+            if constexpr (VEC) ((half4_t *)dst)[i] = h;
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++) ((_Float16 *)dst)[4 * i + j] = h[j];
+        } else if constexpr (VEC) {
+            ((float4 *)dst)[i] = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) ((float *)dst)[4 * i + j] = v[j];
+        }
+    }
+}
+
+template <int MX, bool F16>
+static void values(const uint8_t *codes, const uint8_t *scales, int64_t n4, void *dst, hipStream_t s)
+{
+    const dim3 grid(strided_grid(n4, MXR_TPB)), tpb(MXR_TPB);
+    if ((uintptr_t)dst % (F16 ? 8 : 16) == 0)
+        hipLaunchKernelGGL((k_mx_values<MX, F16, true>), grid, tpb, 0, s, codes, scales, n4, dst);
+    else
+        hipLaunchKernelGGL((k_mx_values<MX, F16, false>), grid, tpb, 0, s, codes, scales, n4, dst);
+}
+
+hipError_t launch_mx_dequantize(int mx, const uint8_t *codes, const uint8_t *scales, int64_t n, int dst_type, void *dst,
+                                hipStream_t s)
+{
+    if (mx == T_MXFP4) dst_type == T_F16 ? values<T_MXFP4, true>(codes, scales, n / 4, dst, s)
+                                         : values<T_MXFP4, false>(codes, scales, n / 4, dst, s);
+    else dst_type == T_F16 ? values<T_MXINT8, true>(codes, scales, n / 4, dst, s)
+                           : values<T_MXINT8, false>(codes, scales, n / 4, dst, s);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// y = s * (1 / sqrt(mean(s^2) + eps)) * g of s = x + delta, rounded to MXINT8,
+// with the reference's RMSNorm formula (src/ds3_reference.c:329-342).  s (when
+// delta is given) and y are also written where asked for.
+//
+// A row is read once and stays in registers between the sum of squares and the
+// rounding: TPR threads a row, four columns a thread and chunk, so a block of
+// 32 is eight neighbouring lanes.  Rows of more than CH chunks (CH = 0) are
+// read a second time, from the cache.
+// ---------------------------------------------------------------------------
+struct NormArgs {
+    const float *x, *delta, *g;
+    float *sum, *y;
+    uint8_t *codes, *scales;
+    float eps;
+    int n;
+    int64_t n_rows;
+};
+
+template <bool VEC>
+__device__ __forceinline__ void store4f(float *p, const float (&v)[4])
+{
+    if constexpr (VEC) {
+        *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = v[i];
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load_sum4(const NormArgs &a, int64_t at, float (&v)[4])
+{
+    load4<false, VEC>((const uint8_t *)(a.x + at), v);
+    if (a.delta) {
+        float d[4];
+        load4<false, VEC>((const uint8_t *)(a.delta + at), d);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = v[i] + d[i];
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void finish4(const NormArgs &a, int64_t row, int col, float rms, const float (&v)[4])
+{
+#pragma clang fp contract(off)
+    const int64_t at = row * a.n + col;
+    float g[4], y[4];
+    load4<false, VEC>((const uint8_t *)(a.g + col), g);
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = v[i] * rms * g[i];
+    if (a.sum) store4f<VEC>(a.sum + at, v);
+    if (a.y) store4f<VEC>(a.y + at, y);
+    store_block8<T_MXINT8>(y, at / 32, (col / 4) & 7, a.codes, a.scales);
+}
+
+// Eight lanes hold a block, and columns come in 32s, so a block's lanes are in
+// or out together.
+template <int TPR, int CH, bool VEC>
+__global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
+{
+    constexpr int ROWS = MXR_TPB / TPR, WPR = TPR / WAVE;
+    __shared__ float part[MXR_TPB / WAVE];
+    const int t = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+    if (WPR == 1 && row >= a.n_rows) return;               // whole waves; WPR > 1 has one row a workgroup
+    float v[CH > 0 ? CH : 1][4];
+    float ss = 0.f;
+    const int64_t base = row * a.n;
+    if constexpr (CH > 0) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int col = (c * TPR + t) * 4;
+            if (col < a.n) {
+                load_sum4<VEC>(a, base + col, v[c]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[c][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) ss += v[c][i] * v[c][i];
+    } else {
+        for (int col = 4 * t; col < a.n; col += 4 * TPR) {
+            load_sum4<VEC>(a, base + col, v[0]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) ss += v[0][i] * v[0][i];
+        }
+    }
+    ss = wave_sum(ss);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & (WAVE - 1)) == 0) part[threadIdx.x / WAVE] = ss;
+        __syncthreads();
+        ss = part[0];
+#pragma unroll
+        for (int w = 1; w < WPR; w++) ss += part[w];
+    }
+    const float rms = 1.0f / sqrtf(ss / (float)a.n + a.eps);
+    if constexpr (CH > 0) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int col = (c * TPR + t) * 4;
+            if (col < a.n) finish4<VEC>(a, row, col, rms, v[c]);
+        }
+    } else {
+        for (int col = 4 * t; col < a.n; col += 4 * TPR) {
+            load_sum4<VEC>(a, base + col, v[0]);
+            finish4<VEC>(a, row, col, rms, v[0]);
+        }
+    }
+}
+
+template <int TPR, int CH>
+static hipError_t norm_launch(const NormArgs &a, bool vec, hipStream_t s)
+{
+    const dim3 grid((unsigned)((a.n_rows + MXR_TPB / TPR - 1) / (MXR_TPB / TPR))), tpb(MXR_TPB);
+    if (vec) hipLaunchKernelGGL((k_add_rms_norm_mx<TPR, CH, true>), grid, tpb, 0, s, a);
+    else hipLaunchKernelGGL((k_add_rms_norm_mx<TPR, CH, false>), grid, tpb, 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_add_rms_norm_mx(const float *x, const float *delta, const float *g, float eps, float *sum, float *y,
+                                  uint8_t *codes, uint8_t *scales, int n, int64_t n_rows, hipStream_t s)
+{
+    const NormArgs a{ x, delta, g, sum, y, codes, scales, eps, n, n_rows };
+    const bool vec = (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)g | (uintptr_t)sum | (uintptr_t)y) & 15) == 0;
+    if (n <= 256) return norm_launch<WAVE, 1>(a, vec, s);
+    if (n <= 1024) return norm_launch<WAVE, 4>(a, vec, s);
+    if (n <= 2048) return norm_launch<MXR_TPB, 2>(a, vec, s);
+    if (n <= 4096) return norm_launch<MXR_TPB, 4>(a, vec, s);
+    if (n <= 8192) return norm_launch<MXR_TPB, 8>(a, vec, s);
+    return norm_launch<MXR_TPB, 0>(a, vec, s);
+}
+
+}  // namespace ds3k

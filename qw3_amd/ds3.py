@@ -16,6 +16,8 @@ from ._native import hip
 
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 0, 1, 8, 12, 14
 TYPE_NAMES = {TYPE_F32: "F32", TYPE_F16: "F16", TYPE_Q8_0: "Q8_0", TYPE_Q4_K: "Q4_K", TYPE_Q6_K: "Q6_K"}
+# microscaled types (include/ds3_hip.h), outside the range of GGUF's ids
+TYPE_MXFP4, TYPE_MXINT8 = 256, 257
 # (values per block, bytes per block) -- reference src/ds3_reference.c:59-184
 BLOCK = {TYPE_F32: (1, 4), TYPE_F16: (1, 2), TYPE_Q8_0: (32, 34), TYPE_Q4_K: (256, 144), TYPE_Q6_K: (256, 210)}
 
@@ -215,6 +217,98 @@ def moe_ffn(x: Buffer, router: Buffer, router_type: int, ex: ExpertTensors, out:
         out, logits, _h(expert_offsets), scratch, scratch, scratch,
         ex.n_embd, n_expert, n_used, ex.n_ff, n_ff_shared, row_bytes(router_type, ex.n_embd), router_type, norm),
         "moe_ffn")
+
+
+@dataclass
+class MxMatrix:
+    """A microscaled matrix (include/ds3_hip.h): codes and one scale byte per
+    32 consecutive values, of TYPE_MXFP4 (weights) or TYPE_MXINT8 (rows)."""
+    codes: Buffer
+    scales: Buffer
+    type: int
+    rows: int
+    cols: int
+
+    @staticmethod
+    def nbytes(type_: int, rows: int, cols: int) -> tuple[int, int]:
+        """Bytes of the code and the scale plane."""
+        if type_ not in (TYPE_MXFP4, TYPE_MXINT8):
+            raise ValueError(f"type {type_} is no microscaled type")
+        if cols % 32 or cols <= 0:
+            raise ValueError(f"{cols} columns do not fill blocks of 32")
+        return rows * (cols // 2 if type_ == TYPE_MXFP4 else cols), rows * (cols // 32)
+
+    @classmethod
+    def alloc(cls, type_: int, rows: int, cols: int) -> "MxMatrix":
+        c, s = cls.nbytes(type_, rows, cols)
+        return cls(Buffer.alloc(max(c, 1)), Buffer.alloc(max(s, 1)), type_, rows, cols)
+
+
+def _mx(m: MxMatrix, type_: int, what: str) -> None:
+    if m.type != type_:
+        raise ValueError(f"{what} must be of type {type_}, not {m.type}")
+
+
+def mx_quantize(src: Buffer, src_type: int, dst: MxMatrix, src_row_stride: int | None = None) -> None:
+    """Rounds rows of F32, F16, Q8_0, Q4_K or Q6_K values to dst's type (ds3_hip_mx_quantize)."""
+    stride = row_bytes(src_type, dst.cols) if src_row_stride is None else src_row_stride
+    _check(hip().ds3_hip_mx_quantize(src, src_type, stride, dst.codes, dst.scales, dst.type, dst.rows, dst.cols),
+           "mx_quantize")
+
+
+def mx_dequantize(src: MxMatrix, dst: Buffer, dst_type: int = TYPE_F32) -> None:
+    """The values of a microscaled matrix, to F32 or F16."""
+    _check(hip().ds3_hip_mx_dequantize(src.codes, src.scales, src.type, src.rows, src.cols, dst, dst_type),
+           "mx_dequantize")
+
+
+def add_rms_norm_mx(x: Buffer, weight: Buffer, eps: float, out: MxMatrix, delta: Buffer | None = None,
+                    sum_out: Buffer | None = None, x_norm: Buffer | None = None) -> None:
+    """rms_norm(x + delta) * weight in MXINT8 rows; the sum and the f32 rows where asked for (ds3_hip_add_rms_norm_mx)."""
+    _mx(out, TYPE_MXINT8, "out")
+    _check(hip().ds3_hip_add_rms_norm_mx(x, _h(delta), weight, eps, _h(sum_out), _h(x_norm), out.codes, out.scales,
+                                         out.cols, out.rows), "add_rms_norm_mx")
+
+
+def _mx_product(x: MxMatrix, w: MxMatrix) -> None:
+    _mx(x, TYPE_MXINT8, "x")
+    _mx(w, TYPE_MXFP4, "w")
+    if x.cols != w.cols:
+        raise ValueError(f"x has rows of {x.cols}, w of {w.cols}")
+
+
+def matmul_mx(x: MxMatrix, w: MxMatrix, c: Buffer) -> None:
+    """c [x.rows][w.rows] = x . w^T in f32 (ds3_hip_matmul_mx)."""
+    _mx_product(x, w)
+    _check(hip().ds3_hip_matmul_mx(x.codes, x.scales, w.codes, w.scales, c, x.rows, w.rows, x.cols), "matmul_mx")
+
+
+def _per_group(w: MxMatrix, n_group: int) -> int:
+    if n_group <= 0 or w.rows % n_group:
+        raise ValueError(f"{w.rows} weight rows do not divide into {n_group} groups")
+    return w.rows // n_group
+
+
+def matmul_mx_grouped(x: MxMatrix, w: MxMatrix, offsets: Buffer, c: Buffer, n_rows: int, n_group: int,
+                      ids: Buffer | None = None) -> None:
+    """c [n_rows][w.rows / n_group]: each row of x times its group's weights (ds3_hip_matmul_mx_grouped)."""
+    _mx_product(x, w)
+    _check(hip().ds3_hip_matmul_mx_grouped(x.codes, x.scales, w.codes, w.scales, offsets, _h(ids), c, x.rows, n_rows,
+                                           n_group, _per_group(w, n_group), x.cols), "matmul_mx_grouped")
+
+
+def moe_gate_up_mx(x: MxMatrix, gate: MxMatrix, up: MxMatrix, offsets: Buffer, h: MxMatrix, n_group: int,
+                   ids: Buffer | None = None) -> None:
+    """h = silu(x . gate) * (x . up) of each row's group, in MXINT8 rows (ds3_hip_moe_gate_up_mx)."""
+    _mx_product(x, gate)
+    _mx_product(x, up)
+    _mx(h, TYPE_MXINT8, "h")
+    n_ff = _per_group(gate, n_group)
+    if up.rows != gate.rows or h.cols != n_ff:
+        raise ValueError(f"gate has {gate.rows} rows, up {up.rows}, h {h.cols} columns")
+    _check(hip().ds3_hip_moe_gate_up_mx(x.codes, x.scales, gate.codes, gate.scales, up.codes, up.scales, offsets,
+                                        _h(ids), h.codes, h.scales, x.rows, h.rows, n_group, n_ff, x.cols),
+           "moe_gate_up_mx")
 
 
 class Graph:

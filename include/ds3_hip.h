@@ -311,8 +311,9 @@ int ds3_hip_dequantize(const ds3_hip_buffer_t *src, uint64_t src_offset, ds3_hip
 /* ---------------------------------------------------------------------- */
 
 /* 4-bit weights that the matrix cores take as they are, and rows in 8 bits
- * for them.  A microscaled matrix [n_rows][n_cols], n_cols a multiple of 32,
- * is two buffers (the element and scale formats of the OCP MX specification):
+ * for them.  A microscaled matrix [n_rows][n_cols], n_cols a multiple of 32
+ * up to 2^27, is two buffers (the element and scale formats of the OCP MX
+ * specification):
  *   scales [n_rows][n_cols / 32]: a byte c per 32 consecutive values, for
  *     2^(c - 127); 255 makes the whole block NaN;
  *   codes, starting on a multiple of 16 bytes, rows without gaps:
@@ -322,8 +323,8 @@ int ds3_hip_dequantize(const ds3_hip_buffer_t *src, uint64_t src_offset, ds3_hip
  *     DS3_HIP_TYPE_MXINT8 [n_rows][n_cols]: signed bytes q, for q / 64.
  * All calls: -1 for a null or too small buffer, sizes that a type does not
  * take, an output that overlaps an input or another output, or a read-only
- * output; 0 and nothing done for zero rows.  They need no workspace before
- * them, so any of them can be captured (but see matmul_mx). */
+ * output; 0 and nothing done for zero rows.  They need no workspace, so any of
+ * them can be captured without a call before. */
 
 /* Rounds rows of src (F32, F16, Q8_0, Q4_K or Q6_K rows, src_row_stride bytes
  * apart; n_cols a multiple of 256 for Q4_K / Q6_K; src and its stride

@@ -1988,10 +1988,11 @@ bool mx_sizes_ok(const char *what, std::initializer_list<uint64_t> sizes)
     return true;
 }
 
+// Rows of whole blocks, up to 2^27 values (16 rows are addressed with 32 bits).
 bool mx_cols_ok(const char *what, const char *name, uint32_t n)
 {
-    if (n != 0 && n % 32 == 0) return true;
-    fprintf(stderr, "ds3_hip: %s: %s=%u must be a multiple of 32\n", what, name, n);
+    if (n != 0 && n % 32 == 0 && n <= 1u << 27) return true;
+    fprintf(stderr, "ds3_hip: %s: %s=%u must be a multiple of 32, at most 2^27\n", what, name, n);
     return false;
 }
 
@@ -2059,6 +2060,12 @@ bool writable(const char *what, std::initializer_list<Span> out)
 }
 
 constexpr uint32_t kMxMaxGroups = 1024;
+
+int run_mx_product(MxProduct *p, const char *kernel, const char *what)
+{
+    KScope ks(kernel);
+    return finish(launch_mx_product(*p, g.stream), what);
+}
 
 }  // namespace
 
@@ -2184,8 +2191,7 @@ extern "C" int ds3_hip_matmul_mx(const ds3_hip_buffer_t *x_codes, const ds3_hip_
     p.n_group = 1;
     p.N = (int)N;
     p.K = (int)K;
-    KScope ks("mx_product");
-    return finish(launch_mx_product(p, g.stream), what);
+    return run_mx_product(&p, "mx_product", what);
 }
 
 namespace {
@@ -2254,8 +2260,7 @@ extern "C" int ds3_hip_matmul_mx_grouped(const ds3_hip_buffer_t *x_codes, const 
         !ensure_init())
         return -1;
     p.c = fptr(C);
-    KScope ks("mx_product");
-    return finish(launch_mx_product(p, g.stream), what);
+    return run_mx_product(&p, "mx_product", what);
 }
 
 extern "C" int ds3_hip_moe_gate_up_mx(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
@@ -2283,6 +2288,5 @@ extern "C" int ds3_hip_moe_gate_up_mx(const ds3_hip_buffer_t *x_codes, const ds3
         return -1;
     p.hc = (uint8_t *)dptr(h_codes);
     p.hs = (uint8_t *)dptr(h_scales);
-    KScope ks("mx_gate_up");
-    return finish(launch_mx_product(p, g.stream), what);
+    return run_mx_product(&p, "mx_gate_up", what);
 }

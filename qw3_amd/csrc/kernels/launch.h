@@ -282,7 +282,7 @@ struct MxProduct {
     float *c;
     uint8_t *hc, *hs;
     int n_x, n_rows, n_group, N, K;
-    int c_vec;                          // c rows take 16-byte stores
+    int c_vec;                          // c rows take 16-byte stores (set by the launcher)
 };
 hipError_t launch_mx_product(const MxProduct &p, hipStream_t s);
 

@@ -15,7 +15,7 @@
 // operands keep every bit down to the fp32 sum (no difference from a 64-bit
 // sum over 10^5 random tiles of equal scales, 2^-22 of the sum of magnitudes
 // with scales 2^30 apart).  So a row byte q is split as
-//   q = 8 hi + lo,  hi = the nearest integer to q / 8 (ties to even), |lo| <= 4
+//   q = 8 hi + lo,  hi = floor((q + 4) / 8),  -4 <= lo <= 3
 // hi / 8 is an E2M3 value (6 bits: steps of 1/8 up to 2) and lo / 2 an E2M1
 // value, both exactly, and q / 64 = hi / 8 + 2^-5 (lo / 2): two matrix
 // instructions at the 4-bit rate (8.4 PFLOP/s measured, 4.2 for the pair; one
@@ -32,7 +32,11 @@ namespace ds3k {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x6 __attribute__((ext_vector_type(6)));
 typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32_any __attribute__((aligned(1)));     // at any address
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half32_t __attribute__((ext_vector_type(32)));
 
@@ -111,54 +115,150 @@ struct XFrag {
     uint32_t sc;       // byte 0: scale of hi, byte 1: of lo
 };
 
-// Splits 32 signed bytes (w, in order) with scale byte c.  A block whose scale
-// is below 2^-122 (c < 5), for which lo would need one below 2^-127, is first
-// rounded to multiples of 2^-128: what is lost lies under the smallest normal
-// fp32 number.
-__device__ __forceinline__ XFrag x_frag(const uint32_t (&w)[8], uint32_t c)
+// 32 bytes of a row of x with their scale byte, as loaded.
+struct RawBlock {
+    uint32_t w[8], sc;
+};
+
+__device__ __forceinline__ RawBlock raw_block(const uint8_t *xc, const uint8_t *xs, int b)
 {
-    half32_t q;
+    RawBlock q;
+    const uint4 x0 = *(const uint4 *)(xc + (int64_t)b * 32), x1 = *(const uint4 *)(xc + (int64_t)b * 32 + 16);
+    q.w[0] = x0.x; q.w[1] = x0.y; q.w[2] = x0.z; q.w[3] = x0.w;
+    q.w[4] = x1.x; q.w[5] = x1.y; q.w[6] = x1.z; q.w[7] = x1.w;
+    q.sc = xs[b];
+    return q;
+}
+
+// The digits of 32 signed bytes; `in` false: of zeros.  With b = q + 128 the
+// digits are hi = floor((b + 4) / 8) - 16 and lo = (b + 4) % 8 - 4.  b is put in
+// the mantissa of 1024 = 0x6400: 8 (hi + 16) is it with 4 added and the low bits
+// cleared, so that one conversion finds hi with nothing to round, and lo's code
+// is looked up by the low three bits, four at a time.  (By the way of hi rounded
+// and subtracted again it took one more conversion of 90 cycles and 16 of 10.)
+//
+// lo's scale byte is 5 less than hi's, so a block with a byte below 5 (values
+// under 2^-121) is first taken to the nearest multiples of 2^-128, what its bytes
+// stand for with scale byte 5: 1024 + b' = (1024 + b) s + 1152 (1 - s), rounded
+// once, as f16 holds 1152 (1 - s) for every s = 2^0 .. 2^-5 and 0.  Without a
+// branch: one in the loop of k_mx_few keeps the loads behind it from being issued
+// early (37 tokens in 8 of 128 experts each: 78 us with it, 48 without).
+__device__ __forceinline__ XFrag x_frag(const RawBlock &raw, bool in)
+{
+    const uint32_t s1 = in ? 0x3c00u - (uint32_t)(5 - min((int)raw.sc, 5)) * 0x400u : 0u;
+    const half2_t s = __builtin_bit_cast(half2_t, s1 * 0x10001u);
+    const half2_t m = { (_Float16)1152.f, (_Float16)1152.f }, k = m - m * s;
+    u32x16 q;
+    uint32_t n[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        // byte + 128 in the mantissa of 1024 = 0x6400, less 1152
-        const uint32_t b = w[i] ^ 0x80808080u;
-        const half2_t k = { (_Float16)1152.f, (_Float16)1152.f };
-        const half2_t a = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - k;
-        const half2_t d = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - k;
-        q[4 * i] = a[0];
-        q[4 * i + 1] = a[1];
-        q[4 * i + 2] = d[0];
-        q[4 * i + 3] = d[1];
+        const uint32_t b = raw.w[i] ^ 0x80808080u;
+        const uint32_t u0 = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+        const uint32_t v0 = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+        const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, u0), s, k));
+        const uint32_t v = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, v0), s, k));
+        const uint32_t u8 = (u + 0x00040004u) & 0xfff8fff8u, v8 = (v + 0x00040004u) & 0xfff8fff8u;
+        const half2_t a = __builtin_bit_cast(half2_t, u8) - m, d = __builtin_bit_cast(half2_t, v8) - m;
+        q[2 * i] = __builtin_bit_cast(uint32_t, a);
+        q[2 * i + 1] = __builtin_bit_cast(uint32_t, d);
+        // 0, 1, 2, 3, -4, -3, -2, -1 for the low bits 0 .. 7
+        const uint32_t c = __builtin_amdgcn_perm(0x090a0b0cu, 0x03020100u,
+                                                 __builtin_amdgcn_perm(v, u, 0x06040200u) & 0x07070707u);
+        n[i] = c | (c >> 4);
     }
-    if (__builtin_expect(c < 5u, 0)) {
-        q = q * (_Float16)__builtin_amdgcn_ldexpf(1.0f, (int)c - 5);
-        c = 5u;
-    }
+    const uint32_t sc = in ? max(raw.sc, 5u) : 127u;
     XFrag f;
-    f.hi = __builtin_bit_cast(u32x6, __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(q, 64.f));
-    q = q - __builtin_amdgcn_cvt_scalef32_pk32_f16_fp6(f.hi, 64.f);
+    f.hi = __builtin_bit_cast(u32x6, __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(__builtin_bit_cast(half32_t, q), 64.f));
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        uint32_t o = 0;
-        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, half2_t{ q[8 * i], q[8 * i + 1] }, 2.f, 0);
-        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, half2_t{ q[8 * i + 2], q[8 * i + 3] }, 2.f, 1);
-        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, half2_t{ q[8 * i + 4], q[8 * i + 5] }, 2.f, 2);
-        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o, half2_t{ q[8 * i + 6], q[8 * i + 7] }, 2.f, 3);
-        f.lo[i] = (int)o;
-    }
-    f.sc = c | ((c - 5u) << 8);
+    for (int i = 0; i < 4; i++) f.lo[i] = (int)__builtin_amdgcn_perm(n[2 * i + 1], n[2 * i], 0x06040200u);
+    f.sc = sc | ((sc - 5u) << 8);
     return f;
 }
 
-// acc += weights (32 E2M1 codes a lane, scale byte 0 of wsc) . x
-__device__ __forceinline__ f32x4 mx_mfma(i32x4 w, uint32_t wsc, const XFrag &x, f32x4 acc)
+// acc += weights (32 E2M1 codes a lane, scale byte S of wsc) . x, in two parts.
+// The second waits for the first's sum, so several of the first go before.
+template <int S>
+__device__ __forceinline__ f32x4 mx_mfma_hi(i32x4 w, uint32_t wsc, const XFrag &x, f32x4 acc)
 {
     const i32x8 a = __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
-    const i32x8 h = { (int)x.hi[0], (int)x.hi[1], (int)x.hi[2], (int)x.hi[3], (int)x.hi[4], (int)x.hi[5], 0, 0 };
-    const i32x8 l = __builtin_shufflevector(x.lo, x.lo, 0, 1, 2, 3, -1, -1, -1, -1);
+    const i32x6 t = __builtin_bit_cast(i32x6, x.hi);
+    const i32x8 h = __builtin_shufflevector(t, t, 0, 1, 2, 3, 4, 5, -1, -1);
     // formats: 4 = E2M1, 2 = E2M3
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, h, acc, 4, 2, 0, (int)wsc, 0, (int)x.sc);
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, l, acc, 4, 4, 0, (int)wsc, 1, (int)x.sc);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, h, acc, 4, 2, S, (int)wsc, 0, (int)x.sc);
+}
+
+template <int S>
+__device__ __forceinline__ f32x4 mx_mfma_lo(i32x4 w, uint32_t wsc, const XFrag &x, f32x4 acc)
+{
+    const i32x8 a = __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
+    const i32x8 l = __builtin_shufflevector(x.lo, x.lo, 0, 1, 2, 3, -1, -1, -1, -1);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, l, acc, 4, 4, S, (int)wsc, 1, (int)x.sc);
+}
+
+// ---------------------------------------------------------------------------
+// From memory to the operands' places
+//
+// A load is fast when four neighbouring lanes read 64 bytes in a row, and
+// fastest on whole lines: 16 rows x 64 bytes with neighbouring lanes on
+// neighbouring rows reach 15 B/clk a CU from L2, 4 rows x 256 bytes 52.  An
+// operand wants neighbouring lanes on neighbouring rows.  So 16 rows of a chunk
+// of 16 blocks (512 columns) are loaded as four times 4 rows x 16 blocks: in
+// load j, lane 16 g + 4 R + p takes block 4 g + p of row 4 R + j, and a 4 x 4
+// transposition among the four lanes of a quad (two exchanges between
+// neighbouring lanes, one instruction a register each) leaves lane 16 g + r
+// with the blocks 4 g + 0..3 of row r.  Step k of a chunk thus multiplies the
+// blocks 4 g + k, and the scale bytes of a lane's four steps are one dword.
+// ---------------------------------------------------------------------------
+constexpr int CHUNK_BLOCKS = 16;
+
+template <int XOR>
+__device__ __forceinline__ int quad_xor(int v)
+{
+    return __builtin_amdgcn_mov_dpp(v, XOR == 1 ? 0xb1 : 0x4e, 0xf, 0xf, true);
+}
+
+// v[j] of lane p of each quad <-> v[p] of lane j: an exchange and a choice a
+// register and stage.  (v_cndmask_b32 can do both with a DPP operand, but takes
+// its mask from VCC alone: 16 registers took 800 cycles with a new VCC for each
+// of the four masks, 270 like this.)
+__device__ __forceinline__ void quad_transpose(int (&v)[4])
+{
+    const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
+    // every exchange before the choices: under a branch it would miss the other lanes
+    const int x0 = quad_xor<1>(v[0]), x1 = quad_xor<1>(v[1]), x2 = quad_xor<1>(v[2]), x3 = quad_xor<1>(v[3]);
+    const int a0 = b0 ? x1 : v[0], a1 = b0 ? v[1] : x0, a2 = b0 ? x3 : v[2], a3 = b0 ? v[3] : x2;
+    const int y0 = quad_xor<2>(a0), y1 = quad_xor<2>(a1), y2 = quad_xor<2>(a2), y3 = quad_xor<2>(a3);
+    v[0] = b1 ? y2 : a0;
+    v[2] = b1 ? a2 : y0;
+    v[1] = b1 ? y3 : a1;
+    v[3] = b1 ? a3 : y1;
+}
+
+__device__ __forceinline__ void quad_transpose(i32x4 (&v)[4])
+{
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+        int t[4] = { v[0][d], v[1][d], v[2][d], v[3][d] };
+        quad_transpose(t);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j][d] = t[j];
+    }
+}
+
+// The scale dwords of 16 rows are loaded with lane 4 r + g on dword g of row r;
+// one pass through the LDS crossbar takes them to lane 16 g + r.
+__device__ __forceinline__ uint32_t scales_to_place(uint32_t v)
+{
+    const int lane = threadIdx.x & (WAVE - 1);
+    return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (4 * (lane & 15) + (lane >> 4)), (int)v);
+}
+
+// 127 in the bytes of blocks b .. b + 3 that are nb or more.
+__device__ __forceinline__ uint32_t scales_within(uint32_t v, int b, int nb)
+{
+    const int n = min(max(nb - b, 0), 4);
+    const uint32_t m = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+    return (v & m) | (0x7f7f7f7fu & ~m);
 }
 
 }  // namespace ds3k

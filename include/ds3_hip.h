@@ -323,8 +323,9 @@ int ds3_hip_dequantize(const ds3_hip_buffer_t *src, uint64_t src_offset, ds3_hip
  *     DS3_HIP_TYPE_MXINT8 [n_rows][n_cols]: signed bytes q, for q / 64.
  * All calls: -1 for a null or too small buffer, sizes that a type does not
  * take, an output that overlaps an input or another output, or a read-only
- * output; 0 and nothing done for zero rows.  They need no workspace, so any of
- * them can be captured without a call before. */
+ * output; 0 and nothing done for zero rows.  All but
+ * ds3_hip_moe_block_mx need no workspace and can be captured without a call
+ * before. */
 
 /* Rounds rows of src (F32, F16, Q8_0, Q4_K or Q6_K rows, src_row_stride bytes
  * apart; n_cols a multiple of 256 for Q4_K / Q6_K; src and its stride
@@ -381,6 +382,32 @@ int ds3_hip_moe_gate_up_mx(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer
                            const ds3_hip_buffer_t *offsets, const ds3_hip_buffer_t *ids,
                            ds3_hip_buffer_t *h_codes, ds3_hip_buffer_t *h_scales, uint32_t n_x, uint32_t n_rows,
                            uint32_t n_group, uint32_t n_ff, uint32_t n_embd);
+
+/* The experts' outputs back in token order: out[t] (+)= the sum over j, in
+ * order, of scores[t][j] * y[slot_pos[t][j]], y f32 [n_rows][n_cols] (as
+ * ds3_hip_matmul_mx_grouped writes it for ds3_hip_moe_bucket's lists), slot_pos
+ * int32 and scores f32 [n_tokens][n_used], out f32 [n_tokens][n_cols].  Slots
+ * that are no row of y (moe_bucket marks dropped ones -1) add nothing. */
+int ds3_hip_moe_combine(const ds3_hip_buffer_t *y, const ds3_hip_buffer_t *slot_pos, const ds3_hip_buffer_t *scores,
+                        ds3_hip_buffer_t *out, uint32_t n_tokens, uint32_t n_used, uint32_t n_rows, uint32_t n_cols,
+                        bool accumulate);
+
+/* ds3_hip_moe_block with microscaled experts, in place: hidden[t] += delta[t]
+ * (delta may be NULL), then hidden[t] += MoE(rms_norm(hidden[t]) * ffn_norm).
+ * The experts are MXFP4 matrices: gate and up [n_expert * n_ff_exp][n_embd], down
+ * [n_expert * n_embd][n_ff_exp]; the router reads the normalised rows in f32,
+ * the experts the same rows in MXINT8, and h is rounded to MXINT8.  gate_logits /
+ * indices / scores (optional) as in ds3_hip_moe_ffn_batch, with its limits on
+ * n_expert and n_used.  It uses the library's workspace: before a capture the
+ * call is made once. */
+int ds3_hip_moe_block_mx(ds3_hip_buffer_t *hidden, const ds3_hip_buffer_t *delta, const ds3_hip_buffer_t *ffn_norm,
+                         float eps, const ds3_hip_buffer_t *w_gate_inp,
+                         const ds3_hip_buffer_t *gate_codes, const ds3_hip_buffer_t *gate_scales,
+                         const ds3_hip_buffer_t *up_codes, const ds3_hip_buffer_t *up_scales,
+                         const ds3_hip_buffer_t *down_codes, const ds3_hip_buffer_t *down_scales,
+                         ds3_hip_buffer_t *gate_logits, ds3_hip_buffer_t *indices, ds3_hip_buffer_t *scores,
+                         uint32_t n_tokens, uint32_t n_embd, uint32_t n_expert, uint32_t n_used, uint32_t n_ff_exp,
+                         uint64_t router_row_stride, ds3_hip_type_t router_type, bool norm_topk_prob);
 
 /* Router selection.  0 (default): the certified router (fp64 wavefront sums
  * with a proven error bound, exact sequential sums only where the bound

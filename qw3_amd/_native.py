@@ -79,6 +79,8 @@ SIGNATURES: dict[str, tuple] = {
     "ds3_hip_matmul_mx": (C.c_int, [P, P, P, P, P, U32, U32, U32]),
     "ds3_hip_matmul_mx_grouped": (C.c_int, [P, P, P, P, P, P, P, U32, U32, U32, U32, U32]),
     "ds3_hip_moe_gate_up_mx": (C.c_int, [P, P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32]),
+    "ds3_hip_moe_combine": (C.c_int, [P, P, P, P, U32, U32, U32, U32, B]),
+    "ds3_hip_moe_block_mx": (C.c_int, [P, P, P, F, P, P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32, U64, I32, B]),
     "ds3_hip_set_router_mode": (C.c_int, [C.c_int]),
     "ds3_hip_router_stats": (C.c_int, [C.POINTER(U64), C.POINTER(U64), C.c_int]),
     "ds3_hip_debug_grouped_lists": (C.c_int, [P, P, P, P, P, P, P, P, P]),

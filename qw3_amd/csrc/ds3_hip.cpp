@@ -2290,3 +2290,158 @@ extern "C" int ds3_hip_moe_gate_up_mx(const ds3_hip_buffer_t *x_codes, const ds3
     p.hs = (uint8_t *)dptr(h_scales);
     return run_mx_product(&p, "mx_gate_up", what);
 }
+
+extern "C" int ds3_hip_moe_combine(const ds3_hip_buffer_t *y, const ds3_hip_buffer_t *slot_pos,
+                                   const ds3_hip_buffer_t *scores, ds3_hip_buffer_t *out, uint32_t n_tokens,
+                                   uint32_t n_used, uint32_t n_rows, uint32_t n_cols, bool accumulate)
+{
+    const char *what = "moe_combine";
+    if (!y || !slot_pos || !scores || !out || n_used == 0 || n_cols == 0) return -1;
+    if (!mx_sizes_ok(what, { n_tokens, n_used, n_rows, n_cols })) return -1;
+    if (n_tokens == 0) return 0;
+    const size_t s_b = (size_t)n_tokens * n_used * 4, y_b = (size_t)n_rows * n_cols * 4, o_b = (size_t)n_tokens * n_cols * 4;
+    if (!fits(y, y_b, "y") || !fits(slot_pos, s_b, "slot_pos") || !fits(scores, s_b, "scores") || !fits(out, o_b, "out"))
+        return -1;
+    for (const ds3_hip_buffer_t *b : { y, slot_pos, scores, (const ds3_hip_buffer_t *)out })
+        if (!aligned_to(b, 4, what, "a buffer")) return -1;
+    const Span o{ out, o_b, "out" };
+    if (!writable(what, { o }) ||
+        !apart(what, { o }, { { y, y_b, "y" }, { slot_pos, s_b, "slot_pos" }, { scores, s_b, "scores" } }) || !ensure_init())
+        return -1;
+    KScope ks("moe_combine");
+    return finish(launch_combine_f32(fptr(y), n_rows, (const int32_t *)cptr(slot_pos), fptr(scores), n_tokens, (int)n_used,
+                                     (int)n_cols, fptr(out), accumulate, g.stream),
+                  what);
+}
+
+extern "C" int ds3_hip_moe_block_mx(
+    ds3_hip_buffer_t *hidden, const ds3_hip_buffer_t *delta, const ds3_hip_buffer_t *ffn_norm, float eps,
+    const ds3_hip_buffer_t *w_gate_inp, const ds3_hip_buffer_t *gate_codes, const ds3_hip_buffer_t *gate_scales,
+    const ds3_hip_buffer_t *up_codes, const ds3_hip_buffer_t *up_scales, const ds3_hip_buffer_t *down_codes,
+    const ds3_hip_buffer_t *down_scales, ds3_hip_buffer_t *gate_logits, ds3_hip_buffer_t *indices,
+    ds3_hip_buffer_t *scores, uint32_t n_tokens, uint32_t n_embd, uint32_t n_expert, uint32_t n_used,
+    uint32_t n_ff_exp, uint64_t router_row_stride, ds3_hip_type_t router_type, bool norm_topk_prob)
+{
+    const char *what = "moe_block_mx";
+    if (!hidden || !ffn_norm || !w_gate_inp || !gate_codes || !gate_scales || !up_codes || !up_scales || !down_codes ||
+        !down_scales || !(eps >= 0.0f) || n_expert == 0 || n_used == 0 || n_used > n_expert)
+        return -1;
+    if (!mx_sizes_ok(what, { n_tokens, n_embd, n_ff_exp, (uint64_t)n_tokens * n_used }) ||
+        !mx_cols_ok(what, "n_embd", n_embd) || !mx_cols_ok(what, "n_ff_exp", n_ff_exp) || !moe_limits_ok(n_expert, n_used))
+        return -1;
+    const size_t rb = row_bytes(router_type, n_embd);
+    if (!router_seq_type_ok(router_type, (int)n_embd) || rb == 0 || router_row_stride < rb ||
+        router_row_stride > (uint64_t)1 << 40) {
+        fprintf(stderr, "ds3_hip: %s: router rows of %u values of type %d, %llu bytes apart, unsupported\n", what, n_embd,
+                router_type, (unsigned long long)router_row_stride);
+        return -1;
+    }
+    if (n_tokens == 0) return 0;
+    const size_t T = n_tokens, x_b = T * n_embd * 4, l_b = T * n_expert * 4, i_b = T * n_used * 4,
+                 r_b = span_bytes(n_expert, router_row_stride, rb), gr = (size_t)n_expert * n_ff_exp,
+                 dr = (size_t)n_expert * n_embd, wc_b = gr * n_embd / 2, ws_b = wc_b / 16;
+    if (!fits(hidden, x_b, "hidden") || !fits(delta, x_b, "delta") || !fits(ffn_norm, (size_t)n_embd * 4, "ffn_norm") ||
+        !fits(w_gate_inp, r_b, "router") || !fits(gate_logits, l_b, "gate_logits") || !fits(indices, i_b, "indices") ||
+        !fits(scores, i_b, "scores") || !mx_planes_ok(what, "gate", gate_codes, gate_scales, T_MXFP4, gr, n_embd) ||
+        !mx_planes_ok(what, "up", up_codes, up_scales, T_MXFP4, gr, n_embd) ||
+        !mx_planes_ok(what, "down", down_codes, down_scales, T_MXFP4, dr, n_ff_exp))
+        return -1;
+    for (const ds3_hip_buffer_t *b : { (const ds3_hip_buffer_t *)hidden, delta, ffn_norm, (const ds3_hip_buffer_t *)gate_logits,
+                                       (const ds3_hip_buffer_t *)indices, (const ds3_hip_buffer_t *)scores })
+        if (!aligned_to(b, 4, what, "a 32-bit buffer")) return -1;
+    if (router_type == T_F32 && (!aligned_to(w_gate_inp, 4, what, "the router") || router_row_stride % 4 != 0)) return -1;
+    const Span o[4] = { { hidden, x_b, "hidden" }, { gate_logits, l_b, "gate_logits" }, { indices, i_b, "indices" },
+                        { scores, i_b, "scores" } };
+    if (!writable(what, { o[0], o[1], o[2], o[3] }) ||
+        !apart(what, { o[0], o[1], o[2], o[3] },
+               { { delta, x_b, "delta" }, { ffn_norm, (size_t)n_embd * 4, "ffn_norm" }, { w_gate_inp, r_b, "router" },
+                 { gate_codes, wc_b, "gate codes" }, { gate_scales, ws_b, "gate scales" }, { up_codes, wc_b, "up codes" },
+                 { up_scales, ws_b, "up scales" }, { down_codes, wc_b, "down codes" }, { down_scales, ws_b, "down scales" } }) ||
+        !ensure_init())
+        return -1;
+
+    // The norm and the router over all tokens, the experts by chunks of what bucketing holds.
+    const size_t Tc = std::min(T, (size_t)prefill_chunk(n_expert)), S = Tc * n_used;
+    const int max_tiles = (int)((S + 63) / 64) + (int)n_expert;
+    Bump bp;
+    const RouteScratch rs = route_scratch((int)T, n_embd, n_expert);
+    const size_t o_xn = bp.take(x_b), o_xc = bp.take(T * n_embd), o_xs = bp.take(T * n_embd / 32), o_l = bp.take(l_b),
+                 o_i = bp.take(i_b), o_s = bp.take(i_b), o_r = bp.take(rs.bytes), o_cnt = bp.take((size_t)n_expert * 4),
+                 o_off = bp.take(((size_t)n_expert + 1) * 4), o_ids = bp.take(S * 4), o_wts = bp.take(S * 4),
+                 o_pos = bp.take(S * 4), o_t = bp.take((size_t)max_tiles * 4), o_n = bp.take(4),
+                 o_hc = bp.take(S * n_ff_exp), o_hs = bp.take(S * n_ff_exp / 32), o_y = bp.take(S * n_embd * 4);
+    uint8_t *ws = ws_get(bp.off + kAllocPad);            // the products read whole dwords of scales
+    if (!ws) return -1;
+    float *xn = (float *)(ws + o_xn), *y = (float *)(ws + o_y), *out = fptr(hidden);
+    const RouteBufs rbuf = route_bufs(ws + o_r, rs, gate_logits ? fptr(gate_logits) : (float *)(ws + o_l),
+                                      indices ? (int32_t *)dptr(indices) : (int32_t *)(ws + o_i),
+                                      scores ? fptr(scores) : (float *)(ws + o_s), nullptr);
+    hipError_t e;
+    {
+        KScope ks("add_rms_norm_mx");
+        e = launch_add_rms_norm_mx(out, delta ? fptr(delta) : nullptr, fptr(ffn_norm), eps, delta ? out : nullptr, xn,
+                                   ws + o_xc, ws + o_xs, (int)n_embd, n_tokens, g.stream);
+    }
+    if (e != hipSuccess) return report(e, what);
+    ExactTail xt{};
+    if (route_tokens(xn, w_gate_inp, router_row_stride, router_type, (int)T, n_embd, n_expert, n_used, norm_topk_prob, rbuf,
+                     nullptr, true, nullptr, nullptr, &xt) != 0)
+        return -1;
+    if (xt.w != nullptr) {
+        KScope ks("exact_weights");
+        e = launch_exact_weights(xn, n_embd, xt, (int)n_embd, g.stream);
+        if (e != hipSuccess) return report(e, what);
+    }
+    const BucketOut bo{ (int32_t *)(ws + o_cnt), (int32_t *)(ws + o_off), (int32_t *)(ws + o_ids), (float *)(ws + o_wts),
+                        (int32_t *)(ws + o_pos), (int32_t *)(ws + o_t), (int32_t *)(ws + o_n), max_tiles, 64 };
+    for (size_t t0 = 0; t0 < T; t0 += Tc) {
+        const size_t tc = std::min(Tc, T - t0);
+        {
+            KScope ks("bucket");
+            e = launch_bucket(rbuf.idx + t0 * n_used, rbuf.scores + t0 * n_used, (int)tc, (int)n_used, (int)n_expert, bo,
+                              g.stream);
+        }
+        MxProduct p{};
+        p.offsets = bo.offsets;
+        p.n_rows = (int)(tc * n_used);
+        p.n_group = (int)n_expert;
+        if (e == hipSuccess) {
+            p.xc = ws + o_xc + t0 * n_embd;
+            p.xs = ws + o_xs + t0 * (n_embd / 32);
+            p.wc = cptr(gate_codes);
+            p.ws = cptr(gate_scales);
+            p.uc = cptr(up_codes);
+            p.us = cptr(up_scales);
+            p.ids = bo.ids;
+            p.hc = ws + o_hc;
+            p.hs = ws + o_hs;
+            p.n_x = (int)tc;
+            p.N = (int)n_ff_exp;
+            p.K = (int)n_embd;
+            KScope ks("mx_gate_up");
+            e = launch_mx_product(p, g.stream);
+        }
+        if (e == hipSuccess) {
+            p.xc = ws + o_hc;
+            p.xs = ws + o_hs;
+            p.wc = cptr(down_codes);
+            p.ws = cptr(down_scales);
+            p.uc = p.us = nullptr;
+            p.ids = nullptr;
+            p.hc = p.hs = nullptr;
+            p.c = y;
+            p.n_x = p.n_rows;
+            p.N = (int)n_embd;
+            p.K = (int)n_ff_exp;
+            KScope ks("mx_product");
+            e = launch_mx_product(p, g.stream);
+        }
+        if (e == hipSuccess) {
+            KScope ks("moe_combine");
+            e = launch_combine_f32(y, p.n_rows, bo.slot_pos, rbuf.scores + t0 * n_used, (int64_t)tc, (int)n_used, (int)n_embd,
+                                   out + t0 * n_embd, true, g.stream);
+        }
+        if (e != hipSuccess) return report(e, what);
+    }
+    return finish(hipSuccess, what);
+}

@@ -8,6 +8,9 @@
 #include "common.h"
 #include "launch.h"
 
+#include <algorithm>
+#include <cstdint>
+
 namespace ds3k {
 
 constexpr int EW_TPB = 256;
@@ -108,21 +111,21 @@ __global__ void k_to_f32(const _Float16 *x, float *y, int64_t n)
 }
 
 // out[t][j] = (acc ? out[t][j] : 0) + w_0 y[p_0][j] + ... in k order, then + residual.
-// VEC consecutive columns per thread: 8 (16-byte y loads) or one.
-template <int VEC>
-__global__ void k_combine(const _Float16 *__restrict__ y, const int32_t *__restrict__ slot_pos,
+// VEC consecutive columns per thread: 16-byte y loads or one value.
+template <typename T, int VEC>
+__global__ void k_combine(const T *__restrict__ y, const int32_t *__restrict__ slot_pos,
                           const float *__restrict__ wts, int k, int N, float *__restrict__ out, int64_t ldo,
-                          const float *__restrict__ residual, int accumulate)
+                          const float *__restrict__ residual, int accumulate, uint32_t n_rows)
 {
 #pragma clang fp contract(off)
     typedef float vec_t __attribute__((ext_vector_type(VEC)));
-    typedef _Float16 hvec_t __attribute__((ext_vector_type(VEC)));
-    const int t = blockIdx.y;
+    typedef T hvec_t __attribute__((ext_vector_type(VEC)));
+    const int64_t t = blockIdx.y;
     const int j = (blockIdx.x * EW_TPB + threadIdx.x) * VEC;
     if (j >= N) return;
-    constexpr int KMAX = VEC == 8 ? 8 : 16;   // slots whose loads are issued together
-    static_assert(VEC == 8 || VEC == 1, "8 columns per thread or one");
-    float *o = out + (int64_t)t * ldo + j;
+    constexpr int KMAX = VEC > 1 ? 8 : 16;    // slots whose loads are issued together
+    static_assert(VEC * sizeof(T) == 16 || VEC == 1, "16 bytes per thread or one value");
+    float *o = out + t * ldo + j;
     vec_t acc = accumulate ? *(const vec_t *)o : (vec_t)0.0f;
     for (int k0 = 0; k0 < k; k0 += KMAX) {
         vec_t v[KMAX];
@@ -131,6 +134,7 @@ __global__ void k_combine(const _Float16 *__restrict__ y, const int32_t *__restr
 #pragma unroll
         for (int kk = 0; kk < KMAX; kk++) {
             p[kk] = k0 + kk < k ? slot_pos[t * k + k0 + kk] : -1;
+            if ((uint32_t)p[kk] >= n_rows) p[kk] = -1;
             w[kk] = p[kk] >= 0 ? wts[t * k + k0 + kk] : 0.0f;
             v[kk] = p[kk] >= 0 ? __builtin_convertvector(*(const hvec_t *)(y + (int64_t)p[kk] * N + j), vec_t)
                                : (vec_t)0.0f;
@@ -139,7 +143,7 @@ __global__ void k_combine(const _Float16 *__restrict__ y, const int32_t *__restr
         for (int kk = 0; kk < KMAX; kk++)
             if (p[kk] >= 0) acc = acc + w[kk] * v[kk];          // dropped slots add nothing
     }
-    if (residual) acc = acc + *(const vec_t *)(residual + (int64_t)t * ldo + j);
+    if (residual) acc = acc + *(const vec_t *)(residual + t * ldo + j);
     *(vec_t *)o = acc;
 }
 
@@ -255,23 +259,37 @@ hipError_t launch_to_f32(const _Float16 *x, float *y, int64_t n, hipStream_t s)
     return hipGetLastError();
 }
 
+template <typename T>
+static hipError_t launch_combine_rows(const T *y, int64_t n_rows, const int32_t *slot_pos, const float *wts, int64_t n_tok,
+                                      int k, int N, float *out, int64_t ldo, const float *residual, bool accumulate,
+                                      hipStream_t s)
+{
+    // 16-byte y loads whenever the rows allow it (the grouped path's n_embd is
+    // a multiple of 128); one value a thread otherwise
+    constexpr int VEC = 16 / sizeof(T);
+    const bool vec = N % VEC == 0 && ldo % 4 == 0 &&
+                     ((((uintptr_t)y) | ((uintptr_t)out) | ((uintptr_t)residual)) & 15) == 0;
+    const int cols = vec ? VEC * EW_TPB : EW_TPB;
+    const uint32_t rows = (uint32_t)std::min<int64_t>(n_rows, INT32_MAX);
+    for (int64_t t0 = 0; t0 < n_tok; t0 += 65535) {
+        const dim3 grid((unsigned)(((int64_t)N + cols - 1) / cols), (unsigned)std::min<int64_t>(n_tok - t0, 65535));
+        const auto kernel = vec ? k_combine<T, VEC> : k_combine<T, 1>;
+        hipLaunchKernelGGL(kernel, grid, dim3(EW_TPB), 0, s, y, slot_pos + t0 * k, wts + t0 * k, k, N, out + t0 * ldo, ldo,
+                           residual ? residual + t0 * ldo : nullptr, accumulate ? 1 : 0, rows);
+    }
+    return hipGetLastError();
+}
+
 hipError_t launch_combine(const _Float16 *y, const int32_t *slot_pos, const float *wts, int T, int k, int N, float *out,
                           int64_t ldo, const float *residual, bool accumulate, hipStream_t s)
 {
-    // 8 columns per thread (16-byte y loads) whenever the rows allow it (the
-    // grouped path's n_embd is a multiple of 128); one otherwise
-    const bool vec8 = N % 8 == 0 && ldo % 4 == 0 &&
-                      ((((uintptr_t)y) | ((uintptr_t)out) | ((uintptr_t)residual)) & 15) == 0;
-    if (vec8) {
-        const dim3 grid((unsigned)((N / 8 + EW_TPB - 1) / EW_TPB), (unsigned)T);
-        hipLaunchKernelGGL(k_combine<8>, grid, dim3(EW_TPB), 0, s, y, slot_pos, wts, k, N, out, ldo, residual,
-                           accumulate ? 1 : 0);
-    } else {
-        const dim3 grid((unsigned)((N + EW_TPB - 1) / EW_TPB), (unsigned)T);
-        hipLaunchKernelGGL(k_combine<1>, grid, dim3(EW_TPB), 0, s, y, slot_pos, wts, k, N, out, ldo, residual,
-                           accumulate ? 1 : 0);
-    }
-    return hipGetLastError();
+    return launch_combine_rows(y, INT32_MAX, slot_pos, wts, T, k, N, out, ldo, residual, accumulate, s);
+}
+
+hipError_t launch_combine_f32(const float *y, int64_t n_rows, const int32_t *slot_pos, const float *wts, int64_t n_tok, int k,
+                              int N, float *out, bool accumulate, hipStream_t s)
+{
+    return launch_combine_rows(y, n_rows, slot_pos, wts, n_tok, k, N, out, N, nullptr, accumulate, s);
 }
 
 }  // namespace ds3k

@@ -236,6 +236,11 @@ hipError_t launch_combine(const _Float16 *y, const int32_t *slot_pos, const floa
                           int N, float *out, int64_t ldo, const float *residual, bool accumulate,
                           hipStream_t s);
 
+// The same of fp32 rows: n_rows of y, N apart as those of out; a slot that is none
+// of them adds nothing.
+hipError_t launch_combine_f32(const float *y, int64_t n_rows, const int32_t *slot_pos, const float *wts, int64_t n_tok, int k,
+                              int N, float *out, bool accumulate, hipStream_t s);
+
 // RMSNorm of n_rows rows of n floats (row strides ldx, ldo):
 // out = x * (1 / sqrt(mean(x^2) + eps)) * w (reference src/ds3_reference.c:329-342).
 hipError_t launch_rms_norm(const float *x, const float *w, float *out, int n, int n_rows, float eps, int64_t ldx,

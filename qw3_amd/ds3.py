@@ -311,6 +311,29 @@ def moe_gate_up_mx(x: MxMatrix, gate: MxMatrix, up: MxMatrix, offsets: Buffer, h
            "moe_gate_up_mx")
 
 
+def moe_combine(y: Buffer, slot_pos: Buffer, scores: Buffer, out: Buffer, n_tokens: int, n_used: int, n_rows: int,
+                n_cols: int, accumulate: bool = False) -> None:
+    """out[t] (+)= sum over j of scores[t][j] * y[slot_pos[t][j]] (ds3_hip_moe_combine)."""
+    _check(hip().ds3_hip_moe_combine(y, slot_pos, scores, out, n_tokens, n_used, n_rows, n_cols, accumulate),
+           "moe_combine")
+
+
+def moe_block_mx(hidden: Buffer, ffn_norm: Buffer, eps: float, router: Buffer, router_type: int, gate: MxMatrix,
+                 up: MxMatrix, down: MxMatrix, n_tokens: int, n_expert: int, n_used: int, delta: Buffer | None = None,
+                 logits: Buffer | None = None, indices: Buffer | None = None, scores: Buffer | None = None,
+                 norm: bool = True) -> None:
+    """hidden += delta, then hidden += MoE(rms_norm(hidden) * ffn_norm) with MXFP4 experts (ds3_hip_moe_block_mx)."""
+    for m, what in ((gate, "gate"), (up, "up"), (down, "down")):
+        _mx(m, TYPE_MXFP4, what)
+    n_ff, n_embd = _per_group(gate, n_expert), gate.cols
+    if (up.rows, up.cols, down.rows, down.cols) != (gate.rows, n_embd, n_expert * n_embd, n_ff):
+        raise ValueError(f"gate {gate.rows} x {gate.cols}, up {up.rows} x {up.cols}, down {down.rows} x {down.cols}")
+    _check(hip().ds3_hip_moe_block_mx(
+        hidden, _h(delta), ffn_norm, eps, router, gate.codes, gate.scales, up.codes, up.scales, down.codes, down.scales,
+        _h(logits), _h(indices), _h(scores), n_tokens, n_embd, n_expert, n_used, n_ff, row_bytes(router_type, n_embd),
+        router_type, norm), "moe_block_mx")
+
+
 class Graph:
     """Calls made inside `with ds3.Graph() as gr:` are captured, not run;
     gr.launch() replays them (ds3_hip_graph_begin / _end / _launch)."""

@@ -229,9 +229,7 @@ __device__ __forceinline__ int quad_xor(int v)
 }
 
 // v[j] of lane p of each quad <-> v[p] of lane j: an exchange and a choice a
-// register and stage.  (v_cndmask_b32 can do both with a DPP operand, but takes
-// its mask from VCC alone: 16 registers took 800 cycles with a new VCC for each
-// of the four masks, 270 like this.)
+// register and stage.
 __device__ __forceinline__ void quad_transpose(int (&v)[4])
 {
     const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
@@ -254,6 +252,57 @@ __device__ __forceinline__ void quad_transpose(i32x4 (&v)[4])
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j][d] = t[j];
     }
+}
+
+// The same beside matrix products: v_cndmask_b32 takes its exchange as a DPP
+// operand, half the instructions, but its mask from VCC, which a new mask is slow to
+// reach.  Alone 16 registers take 700 cycles like this and 270 as above; where the
+// SIMD's other wave and the matrix cores have work meanwhile, the instructions
+// count (16384 rows in 128 groups of 768 x 2 outputs 131.6 us, 136.4 as above).  The
+// compiler does not see that vector instructions write the results: a product reads
+// them two instructions later at the earliest, as every use in a loop's next turn does.
+__device__ __forceinline__ void quad_transpose_beside(i32x4 (&v)[4])
+{
+    const int b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
+#define QUAD_XOR1 " quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf bound_ctrl:0\n"
+#define QUAD_XOR2 " quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf bound_ctrl:0\n"
+#pragma unroll
+    for (int d = 0; d < 4; d += 2) {
+        int s0, s1, s2, s3, t0, t1, t2, t3;              // after the first exchange
+        int o0, o1, o2, o3, q0, q1, q2, q3;
+        // a DPP operand is read two instructions after it was written at the earliest
+        asm("s_nop 0\n"
+            "v_cmp_eq_u32_e32 vcc, 0, %[b0]\n"
+            "v_cndmask_b32_dpp %[s0], %[a1], %[a0], vcc" QUAD_XOR1
+            "v_cndmask_b32_dpp %[s2], %[a3], %[a2], vcc" QUAD_XOR1
+            "v_cndmask_b32_dpp %[t0], %[c1], %[c0], vcc" QUAD_XOR1
+            "v_cndmask_b32_dpp %[t2], %[c3], %[c2], vcc" QUAD_XOR1
+            "v_cmp_ne_u32_e32 vcc, 0, %[b0]\n"
+            "v_cndmask_b32_dpp %[s1], %[a0], %[a1], vcc" QUAD_XOR1
+            "v_cndmask_b32_dpp %[s3], %[a2], %[a3], vcc" QUAD_XOR1
+            "v_cndmask_b32_dpp %[t1], %[c0], %[c1], vcc" QUAD_XOR1
+            "v_cndmask_b32_dpp %[t3], %[c2], %[c3], vcc" QUAD_XOR1
+            "v_cmp_eq_u32_e32 vcc, 0, %[b1]\n"
+            "v_cndmask_b32_dpp %[o0], %[s2], %[s0], vcc" QUAD_XOR2
+            "v_cndmask_b32_dpp %[o1], %[s3], %[s1], vcc" QUAD_XOR2
+            "v_cndmask_b32_dpp %[q0], %[t2], %[t0], vcc" QUAD_XOR2
+            "v_cndmask_b32_dpp %[q1], %[t3], %[t1], vcc" QUAD_XOR2
+            "v_cmp_ne_u32_e32 vcc, 0, %[b1]\n"
+            "v_cndmask_b32_dpp %[o2], %[s0], %[s2], vcc" QUAD_XOR2
+            "v_cndmask_b32_dpp %[o3], %[s1], %[s3], vcc" QUAD_XOR2
+            "v_cndmask_b32_dpp %[q2], %[t0], %[t2], vcc" QUAD_XOR2
+            "v_cndmask_b32_dpp %[q3], %[t1], %[t3], vcc" QUAD_XOR2
+            : [s0] "=&v"(s0), [s1] "=&v"(s1), [s2] "=&v"(s2), [s3] "=&v"(s3), [t0] "=&v"(t0), [t1] "=&v"(t1),
+              [t2] "=&v"(t2), [t3] "=&v"(t3), [o0] "=&v"(o0), [o1] "=&v"(o1), [o2] "=&v"(o2), [o3] "=&v"(o3),
+              [q0] "=&v"(q0), [q1] "=&v"(q1), [q2] "=&v"(q2), [q3] "=&v"(q3)
+            : [a0] "v"(v[0][d]), [a1] "v"(v[1][d]), [a2] "v"(v[2][d]), [a3] "v"(v[3][d]), [c0] "v"(v[0][d + 1]),
+              [c1] "v"(v[1][d + 1]), [c2] "v"(v[2][d + 1]), [c3] "v"(v[3][d + 1]), [b0] "v"(b0), [b1] "v"(b1)
+            : "vcc");
+        v[0][d] = o0, v[1][d] = o1, v[2][d] = o2, v[3][d] = o3;
+        v[0][d + 1] = q0, v[1][d + 1] = q1, v[2][d + 1] = q2, v[3][d + 1] = q3;
+    }
+#undef QUAD_XOR1
+#undef QUAD_XOR2
 }
 
 // The scale dwords of 16 rows are loaded with lane 4 r + g on dword g of row r;

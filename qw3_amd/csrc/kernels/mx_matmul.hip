@@ -67,8 +67,10 @@ template <int BM> struct GroupTiles {
         for (int i = 0; i < 4; i++) {
             const uint32_t n = (uint32_t)__builtin_amdgcn_readlane(tiles[i], src);
             if (left < n || i == 3) {
-                const int row = __builtin_amdgcn_readlane(at[i], src) + (int)left * BM;
-                return { g0 + 4 * src + i, row, min(BM, __builtin_amdgcn_readlane(at[i + 1], src) - row) };
+                // (offsets that decrease can make more tiles than 32 bits count)
+                const int from = __builtin_amdgcn_readlane(at[i], src), row = (int)((uint32_t)from + left * BM);
+                const int rows = min(BM, __builtin_amdgcn_readlane(at[i + 1], src) - row);
+                return { g0 + 4 * src + i, row, row < from ? 0 : max(rows, 0) };
             }
             left -= n;
         }
@@ -368,10 +370,11 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32
 #pragma unroll
             for (int t = 0; t < NT; t++) swn[t] = *(const u32_any *)(ws[t] + s_row + (uint32_t)(chunk * CHUNK_BLOCKS));
         };
-        const auto place_w = [&](int t, int chunk) {
+        const auto place_w = [&](int t, int chunk, auto beside) {
 #pragma unroll
             for (int j = 0; j < 4; j++) w[t][j] = wn[t][j];
-            quad_transpose(w[t]);
+            if constexpr (decltype(beside)::value != 0) quad_transpose_beside(w[t]);
+            else quad_transpose(w[t]);
             sw[t] = scales_within(scales_to_place(swn[t]), chunk * CHUNK_BLOCKS + 4 * g, nb);
         };
         // x: a wave splits units of 16 rows x 4 blocks, one for each step of a chunk.  Blocks
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32
         }
         __syncthreads();
 #pragma unroll
-        for (int t = 0; t < NT; t++) place_w(t, 0);
+        for (int t = 0; t < NT; t++) place_w(t, 0, Int<0>{});
 
         for (q = first + wave; q <= last; q += WAVES) {
             f32x4 acc[NT][MT];
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32
 #pragma unroll
                         for (int t = 0; t < NT; t++) {
                             acc[t][m] = mx_mfma_lo<k>(w[t][k], sw[t], f, acc[t][m]);
-                            if (k == 3 && m == MT - 1) place_w(t, next_c);
+                            if (k == 3 && m == MT - 1) place_w(t, next_c, Int<1>{});
                         }
                         if (m == MT - 1 && k == 1) {             // the registers of two steps are free
 #pragma unroll

@@ -517,8 +517,9 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32
 
 constexpr int CUS = 256, LDS_BYTES = 160 * 1024;
 
-// Row tiles of bm: the most that n_rows rows in n_group groups can make, and as
-// many as groups of all sizes make on average.
+// Row tiles of bm: the most that n_rows rows in n_group groups can make, and about
+// as many as groups of unlike sizes make (half of the last one empty in each, or one
+// a group where rows are few).
 static int64_t most_tiles(const MxProduct &p, int bm)
 {
     return std::min<int64_t>(p.n_rows, ((int64_t)p.n_rows + bm - 1) / bm + p.n_group - 1);
@@ -526,7 +527,8 @@ static int64_t most_tiles(const MxProduct &p, int bm)
 
 static int64_t usual_tiles(const MxProduct &p, int bm)
 {
-    return std::min<int64_t>(p.n_rows, ((int64_t)p.n_rows + bm - 1) / bm + p.n_group / 2);
+    const int64_t rows = p.n_rows;
+    return std::max(std::min<int64_t>(rows, (rows + bm - 1) / bm + p.n_group / 2), std::min<int64_t>(rows, p.n_group));
 }
 
 // Row tiles times tiles of `cols` output columns; false beyond 32 bits, which

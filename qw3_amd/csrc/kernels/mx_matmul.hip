@@ -554,17 +554,24 @@ static int tile_lds(const MxProduct &p, int mt)
 // (about as long as six of its tiles with eight waves a workgroup, four with four)
 // and its tiles, one a SIMD at a time.  4096 x 1536, K = 2048: 24 tiles in two parts
 // 25.5 us, in three 35; 16384 rows in 128 groups, 24 tiles in one part 142, in two 142,
-// in three 153.
+// in three 153; 296 rows in 128 groups, in three parts 47.5, in four 44.5.
+//
+// (Equal shares of all tiles for every workgroup, that end within row tiles, were no
+// faster: 128 against 131 us for those 16384 rows, 144 against 135 for groups of equal
+// sizes, 62 against 57 for 8000 rows, K = 768.  Nor were two halves of the columns for
+// the waves that have no tile: 512 x 4096 15.9 us with and without.)
 static int64_t tile_span(const MxProduct &p, int bm, int out, int at_once, int split)
 {
     const int64_t tiles = ((int64_t)p.N + out - 1) / out, rows = usual_tiles(p, bm);
-    int64_t best = tiles, best_cost = INT64_MAX;
+    int64_t best = tiles, best_cost = INT64_MAX, best_rounds = 0;
     for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, at_once); parts++) {
-        const int64_t span = (tiles + parts - 1) / parts;
-        const int64_t cost = (rows * parts + at_once - 1) / at_once * (split + (span + 3) / 4 * 4);
-        if (cost < best_cost) {
+        const int64_t span = (tiles + parts - 1) / parts, rounds = (rows * parts + at_once - 1) / at_once;
+        const int64_t cost = rounds * (split + (span + 3) / 4 * 4);
+        // of equals the shorter one that still has a tile for each SIMD: more workgroups share the end
+        if (cost < best_cost || (cost == best_cost && rounds == best_rounds && span >= 4)) {
             best = span;
             best_cost = cost;
+            best_rounds = rounds;
         }
     }
     return best;

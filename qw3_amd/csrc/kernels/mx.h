@@ -98,17 +98,6 @@ __device__ __forceinline__ uint32_t mx_round4(const float (&v)[4], uint32_t c)
     }
 }
 
-// silu(g) u = g u t' / (1 + t), t = e^-|g|, t' = 1 or t: no exponential leaves its
-// range.  exp2's argument is rounded by |g| 2^-24 of the result, the constant, exp2,
-// the sum, the reciprocal and the three products by 2^-24 or one ulp each.  (With
-// expf and a rounded division it took 30 instructions, a quarter of what the lanes
-// of k_mx_tile execute.)
-__device__ __forceinline__ float silu_mul(float g, float u)
-{
-    const float t = __builtin_amdgcn_exp2f(fabsf(g) * -1.44269504f);
-    return g * u * ((g < 0.f ? t : 1.f) * __builtin_amdgcn_rcpf(1.f + t));
-}
-
 // ---------------------------------------------------------------------------
 // Matrix-core operands
 //

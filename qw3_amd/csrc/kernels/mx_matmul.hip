@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(WAVES * WAVE) k_mx_few(MxProduct p, uint32_t n
                 }
                 float h[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) h[e] = silu_mul(gt[e], up[e]);
+                for (int e = 0; e < 4; e++) h[e] = swiglu(gt[e], up[e]);
                 uint32_t mx = abs_bits(h[0]);
 #pragma unroll
                 for (int e = 1; e < 4; e++) mx = max(mx, abs_bits(h[e]));
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32
                         for (int j = 0; j < 2; j++)
 #pragma unroll
                             for (int i4 = 0; i4 < 4; i4++) {
-                                h[j][i4] = silu_mul(acc[2 * e + j][m][i4], acc[NT / 2 + 2 * e + j][m][i4]);
+                                h[j][i4] = swiglu(acc[2 * e + j][m][i4], acc[NT / 2 + 2 * e + j][m][i4]);
                                 mx = max(mx, abs_bits(h[j][i4]));
                             }
                         mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, WAVE));

@@ -68,59 +68,96 @@ __global__ void __launch_bounds__(MXR_TPB) k_mx_round(const uint8_t *src, uint64
     }
 }
 
-// GGUF blocks: a thread decodes one 32-weight unit (common.h) into LDS, where
-// the units of a 256-weight block lie interleaved, then rounds one block.  The
-// LDS rows of 32 are 33 floats apart: a wave's 32-float rows would otherwise
-// start in the same bank.
+// GGUF blocks: a thread decodes one 32-weight unit (common.h) and rounds it with
+// the scales of the blocks of 32 that its parts lie in.  A Q4_K unit is 16 weights
+// each of two blocks that it shares with the next lane, a Q6_K unit 8 each of four
+// that a quad shares; their codes are exchanged so that every lane stores the
+// whole of one block.  98304 x 2048 weights to MXFP4: Q4_K 56 us (3.9 TB/s read and
+// written; 72 with the weights themselves exchanged through LDS), Q6_K 83, Q8_0 85
+// (its 34-byte blocks are read as dwords in halves); the vector units' decoding and
+// rounding bound it, a copy of as much would take 42, 53 and 62.
+template <int N>
+__device__ __forceinline__ uint32_t amax_of(const float *v)
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) m = max(m, abs_bits(v[i]));
+    return m;
+}
+
+// The codes of N values, in dwords.
+template <int MX, int N>
+__device__ __forceinline__ void round_dwords(const float *v, uint32_t c, int *out)
+{
+#pragma unroll
+    for (int i = 0; i < N / 4; i++) {
+        const float x[4] = { v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3] };
+        const uint32_t q = mx_round4<MX>(x, c);
+        if constexpr (MX == T_MXINT8) out[i] = (int)q;
+        else if (i % 2 == 0) out[i / 2] = (int)q;
+        else out[i / 2] |= (int)(q << 16);
+    }
+}
+
 template <int MX, int TYPE>
 __global__ void __launch_bounds__(MXR_TPB) k_mx_round_gguf(const uint8_t *src, uint64_t stride, int64_t n_blocks,
                                                            int64_t nb, uint8_t *codes, uint8_t *scales)
 {
-    __shared__ float lds[MXR_TPB * 33];
+    constexpr int D = MX == T_MXINT8 ? 8 : 4;            // dwords of a block's codes
     const int64_t step = (int64_t)gridDim.x * MXR_TPB;
-    for (int64_t b0 = (int64_t)blockIdx.x * MXR_TPB; b0 < n_blocks; b0 += step) {
-        const int64_t b = b0 + threadIdx.x;
-        const bool in = b < n_blocks;
+    // rows are whole GGUF blocks of eight units (Q8_0: one), which stay together
+    for (int64_t b = (int64_t)blockIdx.x * MXR_TPB + threadIdx.x; b < n_blocks; b += step) {
+        const int64_t row = b / nb;
         float w[32];
-        if (in) {
-            const int64_t row = b / nb;
-            int k0[4];
-            unit_decode<TYPE>(src + row * stride, (int)(b - row * nb), w, k0);
-            if constexpr (TYPE != T_Q8_0) {
-                // rows are whole 256-weight blocks, so unit b's block starts 8 * (b / 8) units in
-                float *base = lds + (threadIdx.x & ~7) * 33;
+        int k0[4], q[D];
+        unit_decode<TYPE>(src + row * stride, (int)(b - row * nb), w, k0);
+        uint32_t c;
+        if constexpr (TYPE == T_Q4_K) {
+            int lo[D / 2], hi[D / 2];
+            uint32_t ml = amax_of<16>(w), mh = amax_of<16>(w + 16);
+            ml = max(ml, (uint32_t)quad_xor<1>((int)ml));
+            mh = max(mh, (uint32_t)quad_xor<1>((int)mh));
+            const uint32_t cl = mx_scale<MX>(ml), ch = mx_scale<MX>(mh);
+            round_dwords<MX, 16>(w, cl, lo);
+            round_dwords<MX, 16>(w + 16, ch, hi);
+            const bool odd = threadIdx.x & 1;            // of the two blocks the even lane stores the first
 #pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    const int o = k0[s] & 255;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) base[o + (o >> 5) + i] = w[8 * s + i];
-                }
+            for (int i = 0; i < D / 2; i++) {
+                const int got = quad_xor<1>(odd ? lo[i] : hi[i]);
+                q[i] = odd ? got : lo[i];
+                q[D / 2 + i] = odd ? hi[i] : got;
             }
-        }
-        if constexpr (TYPE != T_Q8_0) {
-            __syncthreads();
+            c = odd ? ch : cl;
+        } else if constexpr (TYPE == T_Q6_K) {
+            const int p = threadIdx.x & 3;               // of the four blocks lane p stores the p-th
+            c = 0;
+            int part[D / 4][4];
 #pragma unroll
-            for (int i = 0; i < 32; i++) w[i] = lds[threadIdx.x * 33 + i];
-            __syncthreads();
-        }
-        if (!in) continue;
-        uint32_t m = 0;
+            for (int t = 0; t < 4; t++) {
+                uint32_t m = amax_of<8>(w + 8 * t);
+                m = max(m, (uint32_t)quad_xor<1>((int)m));
+                m = max(m, (uint32_t)quad_xor<2>((int)m));
+                const uint32_t ct = mx_scale<MX>(m);
+                int d[D / 4];
+                round_dwords<MX, 8>(w + 8 * t, ct, d);
 #pragma unroll
-        for (int i = 0; i < 32; i++) m = max(m, abs_bits(w[i]));
-        const uint32_t c = mx_scale<MX>(m);
-        uint32_t q[8];
+                for (int i = 0; i < D / 4; i++) part[i][t] = d[i];
+                c = p == t ? ct : c;
+            }
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float v[4] = { w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3] };
-            q[i] = mx_round4<MX>(v, c);
-        }
-        if constexpr (MX == T_MXINT8) {
-            *(uint4 *)(codes + b * 32) = make_uint4(q[0], q[1], q[2], q[3]);
-            *(uint4 *)(codes + b * 32 + 16) = make_uint4(q[4], q[5], q[6], q[7]);
+            for (int i = 0; i < D / 4; i++) {
+                quad_transpose(part[i]);
+#pragma unroll
+                for (int t = 0; t < 4; t++) q[D / 4 * t + i] = part[i][t];
+            }
         } else {
-            *(uint4 *)(codes + b * 16) = make_uint4(q[0] | (q[1] << 16), q[2] | (q[3] << 16), q[4] | (q[5] << 16),
-                                                    q[6] | (q[7] << 16));
+            c = mx_scale<MX>(amax_of<32>(w));
+            round_dwords<MX, 32>(w, c, q);
         }
+        uint4 *out = (uint4 *)(codes + b * (4 * D));
+#pragma unroll
+        for (int i = 0; i < D / 4; i++)
+            out[i] = make_uint4((uint32_t)q[4 * i], (uint32_t)q[4 * i + 1], (uint32_t)q[4 * i + 2], (uint32_t)q[4 * i + 3]);
         scales[b] = (uint8_t)c;
     }
 }

@@ -2008,7 +2008,9 @@ size_t mx_code_bytes(int type, uint64_t rows, uint32_t cols)
     return (size_t)rows * (type == T_MXFP4 ? cols / 2 : cols);
 }
 
-// The planes of a rows x cols matrix: large enough, the codes aligned.
+// The planes of a rows x cols matrix: large enough, the codes aligned.  (Where
+// the bytes of the codes pass 64 bits, those of the scales are still more than a
+// buffer holds.)
 bool mx_planes_ok(const char *what, const char *name, const ds3_hip_buffer_t *codes, const ds3_hip_buffer_t *scales,
                   int type, uint64_t rows, uint32_t cols)
 {
@@ -2098,7 +2100,10 @@ extern "C" int ds3_hip_mx_quantize(const ds3_hip_buffer_t *src, ds3_hip_type_t s
         fprintf(stderr, "ds3_hip: %s: src_row_stride must be a multiple of %zu bytes\n", what, need);
         return -1;
     }
-    if (src_row_stride > (uint64_t)1 << 40) return -1;
+    if (src_row_stride > ((uint64_t)1 << 62) / n_rows) {
+        fprintf(stderr, "ds3_hip: %s: src_row_stride=%llu is out of range\n", what, (unsigned long long)src_row_stride);
+        return -1;
+    }
     const size_t sb = span_bytes(n_rows, src_row_stride, rb), cb = mx_code_bytes(mx_type, n_rows, n_cols),
                  eb = (size_t)n_rows * (n_cols / 32);
     if (!fits(src, sb, "src") || !mx_planes_ok(what, "the", codes, scales, mx_type, n_rows, n_cols) ||

@@ -147,6 +147,23 @@ def test_block_is_its_steps(hip_ready, T, embd, E, k, ff, router_type):
         assert (np.abs(a - b) <= tol * y + (2 * k + 2) * 2.0 ** -24 * (y + np.abs(m.x + m.delta))).all()
 
 
+@pytest.mark.parametrize("mode", [1, 2])
+def test_block_in_the_other_router_modes(hip_ready, mode):
+    """The sequential router for one token, the certified one for many."""
+    T, k = (1, 3) if mode == 1 else (40, 3)
+    m = Block(T, 256, 8, k, 64)
+    old = ds3.hip().ds3_hip_set_router_mode(mode)
+    try:
+        hidden = m.hidden()
+        m.block(hidden)
+        got, idx, scores = hidden.read(np.float32, m.x.shape), m.idx.read(np.int32, (T, k)), m.scores.read(np.float32, (T, k))
+    finally:
+        ds3.hip().ds3_hip_set_router_mode(old)
+    want, err = m.reference(idx, scores)
+    assert (np.abs(got - want) <= err).all()
+    assert np.allclose(scores.sum(1), 1, atol=1e-5) and all(len(set(r)) == k for r in idx)
+
+
 def test_block_of_more_than_a_chunk(hip_ready):
     """More tokens than are bucketed at once: as in two calls."""
     T, embd, E, k, ff = 2500, 128, 16, 3, 64

@@ -91,6 +91,10 @@ def test_sizes_and_types(lib, capfd):
     refused(lib, capfd, "mx_quantize", changed(QUANT, a2=4 * 64 + 2), "multiple of 4 bytes")
     refused(lib, capfd, "mx_quantize", changed(QUANT, a0=odder), "multiple of 4 bytes")
     refused(lib, capfd, "mx_quantize", changed(QUANT, a6=1 << 31), "out of range")
+    huge = [buf(1 << 40, (i + 1) << 44) for i in range(2)]
+    # the span of the rows passes 64 bits
+    refused(lib, capfd, "mx_quantize", changed(QUANT, a2=1 << 40, a3=huge[0], a4=huge[1], a6=(1 << 24) + 1), "out of range")
+    refused(lib, capfd, "matmul_mx_grouped", changed(GROUPED, a9=1024, a10=1 << 30, a11=1 << 27), "holds")
     refused(lib, capfd, "mx_dequantize", changed(VALUES, a2=F32), "unsupported")
     refused(lib, capfd, "mx_dequantize", changed(VALUES, a6=ds3.TYPE_Q8_0), "unsupported")
     refused(lib, capfd, "mx_dequantize", changed(VALUES, a4=33), "multiple of 32")

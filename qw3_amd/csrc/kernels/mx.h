@@ -175,6 +175,18 @@ __device__ __forceinline__ XFrag x_frag(const RawBlock &raw, bool in)
     return f;
 }
 
+// Lane `from`'s.
+__device__ __forceinline__ XFrag frag_from(const XFrag &x, int from)
+{
+    XFrag f;
+#pragma unroll
+    for (int i = 0; i < 6; i++) f.hi[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)x.hi[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) f.lo[i] = __builtin_amdgcn_ds_bpermute(4 * from, x.lo[i]);
+    f.sc = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)x.sc);
+    return f;
+}
+
 // acc += weights (32 E2M1 codes a lane, scale byte S of wsc) . x, in two parts.
 // The second waits for the first's sum, so several of the first go before.
 template <int S>

@@ -124,10 +124,14 @@ __device__ __forceinline__ Job job_of(uint32_t job, uint32_t n_tiles)
 // ---------------------------------------------------------------------------
 // Few rows: a workgroup takes 16 rows of x and NT blocks of 16 weight rows (GU:
 // half of them gate rows, half the same up rows); its waves take the chunks of
-// 512 columns in turn, straight from memory, and their sums meet in LDS.
+// 512 columns in turn, straight from memory, and their sums meet in LDS.  Two to
+// three waves a SIMD hide each other's loads.  Bound by memory where the weights
+// are many (1 x 2048 . 151936 34.1 us, 4.9 TB/s), else by the chain of offsets,
+// ids, rows and weights (27 x 2048 . 768 4.5 us, gate/up of one token in 8 of 128
+// experts 8.6).
 // ---------------------------------------------------------------------------
 template <int WAVES, int NT, bool GU>
-__global__ void __launch_bounds__(WAVES * WAVE) k_mx_few(MxProduct p, uint32_t n_jobs, uint32_t n_tiles)
+__global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProduct p, uint32_t n_jobs, uint32_t n_tiles)
 {
     static_assert(!GU || NT == 4, "the gate/up tile is two blocks of each matrix");
     constexpr int BM = 16, NW = GU ? 32 : 16 * NT;       // output columns a workgroup
@@ -153,6 +157,8 @@ __global__ void __launch_bounds__(WAVES * WAVE) k_mx_few(MxProduct p, uint32_t n
 #pragma unroll
         for (int j = 0; j < 4; j++) xc[j] = p.xc + max(x_row((r & 12) + j), (int64_t)0) * p.K;
         const uint8_t *xs = p.xs + max(x_row(lane >> 2), (int64_t)0) * nb + 4 * (lane & 3);
+        const int64_t row4 = max(x_row(r >> 2), (int64_t)0);
+        const uint8_t *xc4 = p.xc + row4 * p.K, *xs4 = p.xs + row4 * nb;
         // The weight rows of block t: n_of(t) .. + 15, moved down where they would pass the
         // end (those below n0 + 16 t are then not stored).
         const auto n_of = [&](int t) {
@@ -173,52 +179,76 @@ __global__ void __launch_bounds__(WAVES * WAVE) k_mx_few(MxProduct p, uint32_t n
         f32x4 acc[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[t] = f32x4{ 0.f, 0.f, 0.f, 0.f };
-        for (int c = wave; c < n_chunk; c += WAVES) {
-            // Blocks behind the last are read as the last (their x becomes zero); scales up to
-            // 15 bytes on, which every allocation has.
-            const int b0 = c * CHUNK_BLOCKS, b = min(b0 + lb, nb - 1);
-            i32x4 x0[4], x1[4], w[NT][4];
-            uint32_t sx, sw[NT];
+        // Up to four rows: a lane splits one block, lane 16 g + 4 R + p block 4 g + p of row R,
+        // and step k takes them from there through the LDS crossbar.  More rows: a lane splits
+        // the four blocks that it multiplies (for one row of 151936 outputs 38.4 us, not 34.1:
+        // the vector units were busy two thirds of it).
+        const auto chunks = [&](auto four_rows) {
+            constexpr bool FOUR = decltype(four_rows)::value != 0;
+            for (int c = wave; c < n_chunk; c += WAVES) {
+                // Blocks behind the last are read as the last (their x becomes zero); scales up to
+                // 15 bytes on, which every allocation has.
+                const int b0 = c * CHUNK_BLOCKS, b = min(b0 + lb, nb - 1);
+                i32x4 x0[4], x1[4], w[NT][4];
+                uint32_t sx, sw[NT];
+                RawBlock own;
+                if constexpr (FOUR) {
+                    own = raw_block(xc4, xs4, b);
+                } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                x0[j] = *(const i32x4 *)(xc[j] + (int64_t)b * 32);
-                x1[j] = *(const i32x4 *)(xc[j] + (int64_t)b * 32 + 16);
-            }
-            sx = *(const u32_any *)(xs + b0);
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) w[t][j] = *(const i32x4 *)(wc[t] + c_row[j] + (uint32_t)b * 16);
-                sw[t] = *(const u32_any *)(ws[t] + s_row + b0);
-            }
-            quad_transpose(x0);
-            quad_transpose(x1);
-            sx = scales_to_place(sx);
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                quad_transpose(w[t]);
-                sw[t] = scales_within(scales_to_place(sw[t]), b0 + 4 * g, nb);
-            }
-            const auto step = [&](auto kc) {
-                constexpr int k = decltype(kc)::value;
-                RawBlock q;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    q.w[i] = (uint32_t)x0[k][i];
-                    q.w[4 + i] = (uint32_t)x1[k][i];
+                    for (int j = 0; j < 4; j++) {
+                        x0[j] = *(const i32x4 *)(xc[j] + (int64_t)b * 32);
+                        x1[j] = *(const i32x4 *)(xc[j] + (int64_t)b * 32 + 16);
+                    }
+                    sx = *(const u32_any *)(xs + b0);
                 }
-                q.sc = byte_of(sx, k);
-                const XFrag f = x_frag(q, b0 + 4 * g + k < nb);
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[t] = mx_mfma_hi<k>(w[t][k], sw[t], f, acc[t]);
+                for (int t = 0; t < NT; t++) {
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[t] = mx_mfma_lo<k>(w[t][k], sw[t], f, acc[t]);
-            };
-            step(Int<0>{});
-            step(Int<1>{});
-            step(Int<2>{});
-            step(Int<3>{});
-        }
+                    for (int j = 0; j < 4; j++) w[t][j] = *(const i32x4 *)(wc[t] + c_row[j] + (uint32_t)b * 16);
+                    sw[t] = *(const u32_any *)(ws[t] + s_row + b0);
+                }
+                XFrag mine;
+                if constexpr (FOUR) {
+                    mine = x_frag(own, b0 + lb < nb);
+                } else {
+                    quad_transpose(x0);
+                    quad_transpose(x1);
+                    sx = scales_to_place(sx);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    quad_transpose(w[t]);
+                    sw[t] = scales_within(scales_to_place(sw[t]), b0 + 4 * g, nb);
+                }
+                const auto step = [&](auto kc) {
+                    constexpr int k = decltype(kc)::value;
+                    XFrag f;
+                    if constexpr (FOUR) {
+                        f = frag_from(mine, 16 * g + ((4 * r + k) & 15));
+                    } else {
+                        RawBlock q;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            q.w[i] = (uint32_t)x0[k][i];
+                            q.w[4 + i] = (uint32_t)x1[k][i];
+                        }
+                        q.sc = byte_of(sx, k);
+                        f = x_frag(q, b0 + 4 * g + k < nb);
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; t++) acc[t] = mx_mfma_hi<k>(w[t][k], sw[t], f, acc[t]);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) acc[t] = mx_mfma_lo<k>(w[t][k], sw[t], f, acc[t]);
+                };
+                step(Int<0>{});
+                step(Int<1>{});
+                step(Int<2>{});
+                step(Int<3>{});
+            }
+        };
+        if (tile.rows <= 4) chunks(Int<1>{});
+        else chunks(Int<0>{});
 #pragma unroll
         for (int t = 0; t < NT; t++) red[wave][t][lane] = acc[t];
         __syncthreads();
@@ -274,7 +304,13 @@ __global__ void __launch_bounds__(WAVES * WAVE) k_mx_few(MxProduct p, uint32_t n
 // The rows of x are split into digits once and stay in LDS, in the matrix
 // cores' lane order, for all columns.  After that a wave runs by itself, with no
 // barrier: its weights go from memory to its registers a chunk of 512 columns
-// ahead, over the end of a tile into its next one.
+// ahead, over the end of a tile into its next one.  Two waves a SIMD.
+//
+// 16384 rows in 128 groups of 768 x 2 outputs, K = 2048: 131 us, 0.79 PFLOP/s; the
+// vector units are busy 61 % of the waves' time (half of that the exchange of the
+// weights between lanes, a fifth the epilogue, a sixth the split of x), the matrix
+// cores 27 %.  296 rows in those groups: 43 us, memory at 4.4 TB/s.  512 x 4096:
+// 15 us, of which 4.4 the split of x and 5 the launch and the last stores.
 // ---------------------------------------------------------------------------
 constexpr int FRAG_LO = 0, FRAG_HI = 1024, FRAG_HI2 = 2048, FRAG_SC = 2560, FRAG_BYTES = 2688;
 // 32 bytes between the steps' fragments: the four lanes that write a row's
@@ -613,10 +649,11 @@ static hipError_t launch_few(const MxProduct &p, hipStream_t s)
 // Both sides of each line, in us, K = 2048 unless said:
 //  - k_mx_few below 512 blocks, where the CUs are not full and splitting x in
 //    every workgroup costs less than a prologue: 64 x 4096, 256 blocks, 7.1
-//    against 9.7; at 512 blocks (128 x 4096) 11.3 against 10.0.  Beyond, too, with at
-//    most one row a group and three chunks or more: 128 rows in 128 groups of
-//    768 x 2 outputs 36 against 39 (K = 768, 2048 outputs: 22 against 19), one row of
-//    65536 outputs, K = 4096, 30 against 34;
+//    against 9.7; at 512 blocks (128 x 4096) 11.3 against 10.0.  Beyond, too, with few
+//    rows to split, at most one a group: 128 rows in 128 groups of 768 x 2 outputs 32.0
+//    against 39, K = 768 and 2048 outputs 17.9 against 18.6 (with two a group 23.8
+//    against 21.3); or four rows of one matrix: one of 65536 outputs, K = 768, 7.8 against
+//    10.7, K = 4096, 27.6 against 34;
 //  - in it, one block of weight rows a workgroup below 128 blocks (64 blocks 5.1, two
 //    5.3; 128 blocks 6.5 against 5.6), two below 512 and four waves (64 x 4096: 7.1,
 //    with four by two waves 8.4), or with the two chunks of K = 768 below 256 (128 x
@@ -632,7 +669,7 @@ template <bool GU>
 static hipError_t launch_product(const MxProduct &p, hipStream_t s)
 {
     const int64_t blocks = usual_tiles(p, 16) * (((int64_t)p.N * (GU ? 2 : 1) + 63) / 64);
-    if (blocks < 512 || (p.n_rows <= p.n_group && p.K > 1024) || tile_lds(p, 1) > LDS_BYTES) {
+    if (blocks < 512 || p.n_rows <= (p.offsets ? p.n_group : 4) || tile_lds(p, 1) > LDS_BYTES) {
         if constexpr (GU) return blocks < 512 ? launch_few<4, 4, true>(p, s) : launch_few<2, 4, true>(p, s);
         else if (blocks < 128) return launch_few<4, 1, false>(p, s);
         else if (blocks < (p.K > 1024 ? 512 : 256)) return launch_few<4, 2, false>(p, s);

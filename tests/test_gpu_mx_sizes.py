@@ -12,7 +12,8 @@ pytestmark = pytest.mark.gpu
 
 DENSE = [(20, 4000, 128), (33, 2700, 256), (70, 4100, 1024), (70, 4100, 1056), (200, 2600, 96), (200, 2600, 3584),
          (200, 2600, 3616), (500, 1040, 7680), (500, 1040, 7712), (1000, 2100, 544), (500, 4200, 64), (1000, 2100, 3584),
-         (1000, 2100, 3616), (1, 33000, 1056), (1, 33000, 1024)]
+         (1000, 2100, 3616), (1, 33000, 1056), (1, 33000, 1024),
+         (4, 33000, 288), (5, 33000, 288), (4, 300, 1600), (5, 300, 1600), (2, 70, 96)]
 
 
 @pytest.mark.parametrize("m,n,k", DENSE)

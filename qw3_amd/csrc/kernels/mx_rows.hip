@@ -270,9 +270,15 @@ hipError_t launch_mx_dequantize(int mx, const uint8_t *codes, const uint8_t *sca
 }
 
 // ---------------------------------------------------------------------------
-// y = s * (1 / sqrt(mean(s^2) + eps)) * g of s = x + delta, rounded to MXINT8,
-// with the reference's RMSNorm formula (src/ds3_reference.c:329-342).  s (when
-// delta is given) and y are also written where asked for.
+// y = s / sqrt(mean(s^2) + eps) * g of s = x + delta (the reference's RMSNorm,
+// src/ds3_reference.c:329-342), rounded to MXINT8.  s (when delta is given) and y
+// are also written where asked for.
+//
+// s is one fp32 addition; everything from its squares on is in 64 bits, and y
+// rounded once: a factor rounded to 32 bits would move a whole row the same way, and
+// squares in 32 bits would overflow from 1.8e19 on.  Memory bounds the kernel (6001 x
+// 4096 with delta and sum 67 us, 4.8 TB/s; 68.5 in 32 bits), and the vector units have
+// the time.
 //
 // A row is read once and stays in registers between the sum of squares and the
 // rounding: TPR threads a row, four columns a thread and chunk, so a block of
@@ -312,17 +318,45 @@ __device__ __forceinline__ void load_sum4(const NormArgs &a, int64_t at, float (
 }
 
 template <bool VEC>
-__device__ __forceinline__ void finish4(const NormArgs &a, int64_t row, int col, float rms, const float (&v)[4])
+__device__ __forceinline__ void finish4(const NormArgs &a, int64_t row, int col, double rms, const float (&v)[4])
 {
-#pragma clang fp contract(off)
     const int64_t at = row * a.n + col;
     float g[4], y[4];
     load4<false, VEC>((const uint8_t *)(a.g + col), g);
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = v[i] * rms * g[i];
+    for (int i = 0; i < 4; i++) y[i] = (float)((double)v[i] * rms * (double)g[i]);
     if (a.sum) store4f<VEC>(a.sum + at, v);
     if (a.y) store4f<VEC>(a.y + at, y);
     store_block8<T_MXINT8>(y, at / 32, (col / 4) & 7, a.codes, a.scales);
+}
+
+// v + v of the lane that DPP takes, in both halves.
+template <int CTRL>
+__device__ __forceinline__ double add_dpp(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return v + __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
+__device__ __forceinline__ double lane_of(double v, int lane)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
+// The sum over the wavefront: neighbours, quads, halves and rows of 16, then the
+// four rows.
+__device__ __forceinline__ double wave_sum64(double v)
+{
+    v = add_dpp<0xb1>(v);
+    v = add_dpp<0x4e>(v);
+    v = add_dpp<0x141>(v);
+    v = add_dpp<0x140>(v);
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 
 // Eight lanes hold a block, and columns come in 32s, so a block's lanes are in
@@ -331,12 +365,12 @@ template <int TPR, int CH, bool VEC>
 __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
 {
     constexpr int ROWS = MXR_TPB / TPR, WPR = TPR / WAVE;
-    __shared__ float part[MXR_TPB / WAVE];
+    __shared__ double part[MXR_TPB / WAVE];
     const int t = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
     if (WPR == 1 && row >= a.n_rows) return;               // whole waves; WPR > 1 has one row a workgroup
     float v[CH > 0 ? CH : 1][4];
-    float ss = 0.f;
+    double ss = 0.0;
     const int64_t base = row * a.n;
     if constexpr (CH > 0) {
 #pragma unroll
@@ -352,15 +386,15 @@ __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
 #pragma unroll
         for (int c = 0; c < CH; c++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) ss += v[c][i] * v[c][i];
+            for (int i = 0; i < 4; i++) ss = fma((double)v[c][i], (double)v[c][i], ss);
     } else {
         for (int col = 4 * t; col < a.n; col += 4 * TPR) {
             load_sum4<VEC>(a, base + col, v[0]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) ss += v[0][i] * v[0][i];
+            for (int i = 0; i < 4; i++) ss = fma((double)v[0][i], (double)v[0][i], ss);
         }
     }
-    ss = wave_sum(ss);
+    ss = wave_sum64(ss);
     if constexpr (WPR > 1) {
         if ((threadIdx.x & (WAVE - 1)) == 0) part[threadIdx.x / WAVE] = ss;
         __syncthreads();
@@ -368,7 +402,7 @@ __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
 #pragma unroll
         for (int w = 1; w < WPR; w++) ss += part[w];
     }
-    const float rms = 1.0f / sqrtf(ss / (float)a.n + a.eps);
+    const double rms = 1.0 / sqrt(ss / a.n + a.eps);
     if constexpr (CH > 0) {
 #pragma unroll
         for (int c = 0; c < CH; c++) {

@@ -161,6 +161,24 @@ def test_add_rms_norm(hip_ready, n, rows):
         assert (err <= step * np.where(top, 1.0, 0.5) + bound * np.abs(y64)).all()
 
 
+@pytest.mark.parametrize("n", [64, 1024, 2048, 8192, 8224])
+def test_add_rms_norm_range(hip_ready, n):
+    """Rows whose squares leave the range of 32 bits, and y within one rounding."""
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal((6, n)) * np.r_[1e30, 3e18, 1.0, 1e-18, 1e-25, 1e-30][:, None]).astype(np.float32)
+    g = (1 + 0.2 * rng.standard_normal(n)).astype(np.float32)
+    for eps in (0.0, 1e-6):
+        m, y = ds3.MxMatrix.alloc(I8, 6, n), ds3.Buffer.alloc(x.nbytes)
+        ds3.add_rms_norm_mx(ds3.Buffer.from_array(x), ds3.Buffer.from_array(g), eps, m, x_norm=y)
+        x64 = x.astype(np.float64)
+        want = x64 / np.sqrt((x64 ** 2).mean(1, keepdims=True) + np.float32(eps)) * g
+        got = y.read(np.float32, x.shape)
+        # half a step of the result, and what n additions in 64 bits may lose
+        assert (np.abs(got - want) <= (2.0 ** -24 + n * 2.0 ** -52) * np.abs(want) + 2.0 ** -150).all()
+        codes = X.encode(I8, got)
+        assert all(np.array_equal(a, b) for a, b in zip(read_mx(m), codes))
+
+
 def test_add_rms_norm_rows_of_nothing(hip_ready):
     """Rows of zeros, of infinities and of NaN: only their own outputs show them."""
     n = 512

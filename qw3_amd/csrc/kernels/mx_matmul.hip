@@ -341,7 +341,6 @@ template <int WAVES, int NT, int MT, int LEAD, bool GU>
 __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32_t n_jobs, uint32_t n_tiles, int span,
                                                              int spread)
 {
-    static_assert(WAVES % MT == 0, "a wave splits units of one 16-row block");
     static_assert(!GU || NT % 4 == 0, "a wave's gate and up rows make whole blocks of 32 outputs");
     constexpr int BM = 16 * MT, OUT = GU ? 8 * NT : 16 * NT, STEP = step_bytes(MT);
     extern __shared__ __align__(16) uint8_t lds[];       // n_chunk x 4 steps
@@ -417,31 +416,40 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32
         // behind the last become zeros, whatever their weights (the last block's, whose NaN
         // scale the row has anyway).  Its first loads go before those of the weights: loads
         // return in order.
-        int64_t xr = tile.row + min(16 * (wave % MT) + rl, tile.rows - 1);
-        if (p.ids) xr = p.ids[xr];
-        if (xr < 0 || xr >= p.n_x) xr = 0;
-        const uint8_t *xc = p.xc + xr * p.K, *xs = p.xs + xr * nb;
-        constexpr int AT_ONCE = 4, EACH = WAVES / MT;
+        // (A wave keeps to one block of 16 rows where the waves divide by them.)
+        constexpr bool ONE = WAVES % MT == 0;
+        constexpr int MS = ONE ? 1 : MT, EACH = ONE ? WAVES / MT : WAVES, AT_ONCE = ONE ? 4 : MT;
+        const uint8_t *xc[MS], *xs[MS];
+#pragma unroll
+        for (int i = 0; i < MS; i++) {
+            int64_t xr = tile.row + min(16 * (ONE ? wave % MT : i) + rl, tile.rows - 1);
+            if (p.ids) xr = p.ids[xr];
+            if (xr < 0 || xr >= p.n_x) xr = 0;
+            xc[i] = p.xc + xr * p.K;
+            xs[i] = p.xs + xr * nb;
+        }
         RawBlock raw[AT_ONCE];
         const auto load_x = [&](int u) {
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; i++) raw[i] = raw_block(xc, xs, min(4 * (u + i * EACH) + gl, nb - 1));
+            for (int i = 0; i < AT_ONCE; i++)
+                raw[i] = raw_block(xc[i % MS], xs[i % MS], min(4 * (u + i / MS * EACH) + gl, nb - 1));
         };
-        load_x(wave / MT);
+        const int u0 = ONE ? wave / MT : wave;
+        load_x(u0);
         int q = min(first + wave, last);
         at_tile(q);
         load_sw(0);
 #pragma unroll
         for (int j = 0; j < 4; j++) load_w(0, j);
-        for (int u = wave / MT; u < 4 * n_chunk; u += AT_ONCE * EACH) {
+        for (int u = u0; u < 4 * n_chunk; u += AT_ONCE / MS * EACH) {
 #pragma unroll
             for (int i = 0; i < AT_ONCE; i++) {
-                const int v = u + i * EACH;
+                const int v = u + i / MS * EACH;
                 if (v < 4 * n_chunk)
-                    frag_store(lds + (4 * (v / 4) + gl) * STEP + (wave % MT) * FRAG_BYTES, 16 * (v % 4) + rl,
+                    frag_store(lds + (4 * (v / 4) + gl) * STEP + (ONE ? wave % MT : i % MS) * FRAG_BYTES, 16 * (v % 4) + rl,
                                x_frag(raw[i], 4 * v + gl < nb));
             }
-            load_x(u + AT_ONCE * EACH);
+            load_x(u + AT_ONCE / MS * EACH);
         }
         __syncthreads();
 #pragma unroll
@@ -585,28 +593,39 @@ static int tile_lds(const MxProduct &p, int mt)
     return (int)std::min<int64_t>(n, 1 << 30);
 }
 
-// Column tiles a workgroup takes.  With `parts` workgroups for a row tile, they
-// run in rounds of as many as the CUs hold, each for its rows of x to be split
-// (about as long as six of its tiles with eight waves a workgroup, four with four)
-// and its tiles, one a SIMD at a time.  4096 x 1536, K = 2048: 24 tiles in two parts
-// 25.5 us, in three 35; 16384 rows in 128 groups, 24 tiles in one part 142, in two 142,
-// in three 153; 296 rows in 128 groups, in three parts 47.5, in four 44.5.
+// How many column tiles a workgroup takes, and for how long it all runs.  With
+// `parts` workgroups for a row tile, they run in rounds of as many as the CUs hold,
+// each for its rows of x to be split (about as long as six of its tiles with eight
+// waves a workgroup, four with four) and its tiles, one a SIMD at a time.  4096 x
+// 1536, K = 2048: 24 tiles in two parts 25.5 us, in three 35; 16384 rows in 128 groups,
+// 24 tiles in one part 142, in two 142, in three 153; 296 rows in 128 groups, in three
+// parts 47.5, in four 44.5.
 //
 // (Equal shares of all tiles for every workgroup, that end within row tiles, were no
 // faster: 128 against 131 us for those 16384 rows, 144 against 135 for groups of equal
 // sizes, 62 against 57 for 8000 rows, K = 768.  Nor were two halves of the columns for
 // the waves that have no tile: 512 x 4096 15.9 us with and without.)
-static int64_t tile_span(const MxProduct &p, int bm, int out, int at_once, int split)
+struct Plan {
+    int64_t span, cost;         // the cost in 1/20 of a tile of 32 rows
+};
+
+template <int WAVES, int NT, int MT, bool GU>
+static Plan tile_plan(const MxProduct &p)
 {
-    const int64_t tiles = ((int64_t)p.N + out - 1) / out, rows = usual_tiles(p, bm);
-    int64_t best = tiles, best_cost = INT64_MAX, best_rounds = 0;
+    constexpr int OUT = GU ? 8 * NT : 16 * NT;
+    // workgroups a CU holds: eight waves' registers
+    const int at_once = WAVES == 8 || 2 * tile_lds(p, MT) > LDS_BYTES ? CUS : 2 * CUS;
+    const int64_t tiles = ((int64_t)p.N + OUT - 1) / OUT, rows = usual_tiles(p, 16 * MT);
+    // (48 rows: the split takes half as long again, a tile a tenth)
+    const int64_t split = (at_once == CUS ? 6 : 4) * (MT == 3 ? 30 : 20), tile = MT == 3 ? 22 : 20;
+    Plan best{ tiles, INT64_MAX };
+    int64_t best_rounds = 0;
     for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, at_once); parts++) {
         const int64_t span = (tiles + parts - 1) / parts, rounds = (rows * parts + at_once - 1) / at_once;
-        const int64_t cost = rounds * (split + (span + 3) / 4 * 4);
+        const int64_t cost = rounds * (split + (span + 3) / 4 * 4 * tile);
         // of equals the shorter one that still has a tile for each SIMD: more workgroups share the end
-        if (cost < best_cost || (cost == best_cost && rounds == best_rounds && span >= 4)) {
-            best = span;
-            best_cost = cost;
+        if (cost < best.cost || (cost == best.cost && rounds == best_rounds && span >= 4)) {
+            best = { span, cost };
             best_rounds = rounds;
         }
     }
@@ -624,8 +643,7 @@ static hipError_t launch_tile(const MxProduct &p, hipStream_t s)
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
         if (e != hipSuccess) return e;
     }
-    const int each = WAVES == 8 || 2 * lds > LDS_BYTES ? 1 : 2;  // workgroups a CU: eight waves' registers
-    const int64_t span = tile_span(p, BM, OUT, CUS * each, each == 1 ? 6 : 4);
+    const int64_t span = tile_plan<WAVES, NT, MT, GU>(p).span;
     uint32_t n_jobs, n_tiles;
     if (!count_jobs(p, BM, OUT * span, n_jobs, n_tiles)) return hipErrorInvalidValue;
     const uint32_t items = n_jobs / n_tiles;
@@ -660,7 +678,10 @@ static hipError_t launch_few(const MxProduct &p, hipStream_t s)
 //    2048: 6.9 against 6.0);
 //  - 32 rows instead of 16 from 16 rows a group (16: 54 against 65, gate/up; 8: 62
 //    against 51) or, for one matrix, 2048 blocks (512 x 4096: 15.3 against 17.7; 256 x
-//    4096: 13.3 against 11.6), as long as they fit the LDS;
+//    4096: 13.3 against 11.6), as long as they fit the LDS; 48 where their plan is the
+//    shorter one (16384 rows in 128 groups, gate/up: 119 against 139; 4096 rows 81 against
+//    68; K = 768: 16000 rows 87 against 96, 4096 rows 40.8 against 44.2, 2048 rows 33
+//    against 30; 2048 x 16384: 101 against 113, 2048 x 4096: 34 against 31);
 //  - four waves instead of eight where two such workgroups fit a CU: for 16 rows 128 x
 //    4096: 10.0 against 10.5 (at K = 4096, where they do not, 2048 x 2048: 45.9 against
 //    41.2); for 32 rows of groups of unequal sizes, 16000 rows in 128 groups x 2048, K =
@@ -677,7 +698,13 @@ static hipError_t launch_product(const MxProduct &p, hipStream_t s)
     }
     const bool wide = p.offsets ? (int64_t)p.n_rows >= 16 * (int64_t)p.n_group : blocks >= 2048;
     if (wide && tile_lds(p, 2) <= LDS_BYTES) {
-        if (p.offsets && 2 * tile_lds(p, 2) <= LDS_BYTES) return launch_tile<4, 4, 2, 2, GU>(p, s);
+        if (p.offsets && 2 * tile_lds(p, 2) <= LDS_BYTES) {
+            if (2 * tile_lds(p, 3) <= LDS_BYTES && tile_plan<4, 4, 3, GU>(p).cost < tile_plan<4, 4, 2, GU>(p).cost)
+                return launch_tile<4, 4, 3, 0, GU>(p, s);
+            return launch_tile<4, 4, 2, 2, GU>(p, s);
+        }
+        if (tile_lds(p, 3) <= LDS_BYTES && tile_plan<8, 4, 3, GU>(p).cost < tile_plan<8, 4, 2, GU>(p).cost)
+            return launch_tile<8, 4, 3, 0, GU>(p, s);
         return launch_tile<8, 4, 2, 2, GU>(p, s);
     }
     if (2 * tile_lds(p, 1) <= LDS_BYTES) return launch_tile<4, 4, 1, 4, GU>(p, s);

@@ -13,7 +13,8 @@ pytestmark = pytest.mark.gpu
 DENSE = [(20, 4000, 128), (33, 2700, 256), (70, 4100, 1024), (70, 4100, 1056), (200, 2600, 96), (200, 2600, 3584),
          (200, 2600, 3616), (500, 1040, 7680), (500, 1040, 7712), (1000, 2100, 544), (500, 4200, 64), (1000, 2100, 3584),
          (1000, 2100, 3616), (1, 33000, 1056), (1, 33000, 1024),
-         (4, 33000, 288), (5, 33000, 288), (4, 300, 1600), (5, 300, 1600), (2, 70, 96)]
+         (4, 33000, 288), (5, 33000, 288), (4, 300, 1600), (5, 300, 1600), (2, 70, 96),
+         (512, 4096, 288), (3001, 1197, 96), (1500, 2200, 2560), (1500, 2200, 2592)]
 
 
 @pytest.mark.parametrize("m,n,k", DENSE)
@@ -33,7 +34,8 @@ def sizes_of(rng, groups, rows):
 
 # groups, rows, n, k
 GROUPED = [(260, 200, 224, 1056), (260, 200, 224, 1024), (300, 1000, 160, 512), (300, 1000, 160, 3616), (40, 640, 608, 1536),
-           (40, 640, 608, 1568), (40, 639, 608, 320), (1024, 1024, 64, 96), (24, 900, 480, 3616), (24, 900, 480, 7712)]
+           (40, 640, 608, 1568), (40, 639, 608, 320), (1024, 1024, 64, 96), (24, 900, 480, 3616), (24, 900, 480, 7712),
+           (9, 3000, 320, 96), (9, 6000, 608, 96), (9, 3000, 608, 2080), (9, 2000, 608, 1056)]
 
 
 @pytest.mark.parametrize("groups,rows,n,k", GROUPED)

@@ -259,8 +259,8 @@ __device__ __forceinline__ void quad_transpose(i32x4 (&v)[4])
 // operand, half the instructions, but its mask from VCC, which a new mask is slow to
 // reach.  Alone 16 registers take 700 cycles like this and 270 as above; where the
 // SIMD's other wave and the matrix cores have work meanwhile, the instructions
-// count (16384 rows in 128 groups of 768 x 2 outputs 131.6 us, 136.4 as above).  The
-// compiler does not see that vector instructions write the results: a product reads
+// count (16384 rows in 128 groups of 768 x 2 outputs, 32 rows a workgroup: 131.6 us,
+// 136.4 as above).  The compiler does not see that vector instructions write the results: a product reads
 // them two instructions later at the earliest, as every use in a loop's next turn does.
 __device__ __forceinline__ void quad_transpose_beside(i32x4 (&v)[4])
 {

@@ -306,11 +306,11 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
 // barrier: its weights go from memory to its registers a chunk of 512 columns
 // ahead, over the end of a tile into its next one.  Two waves a SIMD.
 //
-// 16384 rows in 128 groups of 768 x 2 outputs, K = 2048: 131 us, 0.79 PFLOP/s; the
-// vector units are busy 61 % of the waves' time (half of that the exchange of the
-// weights between lanes, a fifth the epilogue, a sixth the split of x), the matrix
-// cores 27 %.  296 rows in those groups: 43 us, memory at 4.4 TB/s.  512 x 4096:
-// 15 us, of which 4.4 the split of x and 5 the launch and the last stores.
+// 16384 rows in 128 groups of 768 x 2 outputs, K = 2048: 115 us, 0.9 PFLOP/s; the
+// vector units are busy 62 % of the waves' time (a third of that the exchange of the
+// weights between lanes, a quarter the epilogue, as much the split of x), the
+// matrix cores 33 %.  296 rows in those groups: 43 us, memory at 4.4 TB/s.  512 x
+// 4096: 15 us, of which 4.4 the split of x and 5 the launch and the last stores.
 // ---------------------------------------------------------------------------
 constexpr int FRAG_LO = 0, FRAG_HI = 1024, FRAG_HI2 = 2048, FRAG_SC = 2560, FRAG_BYTES = 2688;
 // 32 bytes between the steps' fragments: the four lanes that write a row's

@@ -2388,15 +2388,10 @@ extern "C" int ds3_hip_moe_block_mx(
                                    ws + o_xc, ws + o_xs, (int)n_embd, n_tokens, g.stream);
     }
     if (e != hipSuccess) return report(e, what);
-    ExactTail xt{};
+    // (the certified router's own weights, from sums in 64 bits, are the closer ones)
     if (route_tokens(xn, w_gate_inp, router_row_stride, router_type, (int)T, n_embd, n_expert, n_used, norm_topk_prob, rbuf,
-                     nullptr, true, nullptr, nullptr, &xt) != 0)
+                     nullptr, true) != 0)
         return -1;
-    if (xt.w != nullptr) {
-        KScope ks("exact_weights");
-        e = launch_exact_weights(xn, n_embd, xt, (int)n_embd, g.stream);
-        if (e != hipSuccess) return report(e, what);
-    }
     const BucketOut bo{ (int32_t *)(ws + o_cnt), (int32_t *)(ws + o_off), (int32_t *)(ws + o_ids), (float *)(ws + o_wts),
                         (int32_t *)(ws + o_pos), (int32_t *)(ws + o_t), (int32_t *)(ws + o_n), max_tiles, 64 };
     for (size_t t0 = 0; t0 < T; t0 += Tc) {

@@ -619,14 +619,17 @@ static Plan tile_plan(const MxProduct &p)
     // (48 rows: the split takes half as long again, a tile a tenth)
     const int64_t split = (at_once == CUS ? 6 : 4) * (MT == 3 ? 30 : 20), tile = MT == 3 ? 22 : 20;
     Plan best{ tiles, INT64_MAX };
-    int64_t best_rounds = 0;
-    for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, at_once); parts++) {
-        const int64_t span = (tiles + parts - 1) / parts, rounds = (rows * parts + at_once - 1) / at_once;
-        const int64_t cost = rounds * (split + (span + 3) / 4 * 4 * tile);
-        // of equals the shorter one that still has a tile for each SIMD: more workgroups share the end
-        if (cost < best.cost || (cost == best.cost && rounds == best_rounds && span >= 4)) {
-            best = { span, cost };
-            best_rounds = rounds;
+    // by the number q of tiles a SIMD, the shortest span of each number of parts
+    for (int64_t q = (tiles + 3) / 4; q > 0; q--) {
+        const int64_t parts = (tiles + 4 * q - 1) / (4 * q);
+        q = (tiles + 4 * parts - 1) / (4 * parts);
+        const int64_t rounds = (rows * parts + at_once - 1) / at_once, cost = rounds * (split + 4 * q * tile);
+        if (cost < best.cost) {
+            // as many more workgroups as the last round has room for, with a tile for each
+            // SIMD: they share the end
+            const int64_t most = q > 1 ? (tiles - 1) / (4 * (q - 1)) : std::max(parts, tiles / 4);
+            const int64_t more = std::max(parts, std::min(most, rounds * at_once / rows));
+            best = { (tiles + more - 1) / more, cost };
         }
     }
     return best;

@@ -597,12 +597,12 @@ static int tile_lds(const MxProduct &p, int mt)
 // `parts` workgroups for a row tile, they run in rounds of as many as the CUs hold,
 // each for its rows of x to be split (about as long as six of its tiles with eight
 // waves a workgroup, four with four) and its tiles, one a SIMD at a time.  4096 x
-// 1536, K = 2048: 24 tiles in two parts 25.5 us, in three 35; 16384 rows in 128 groups,
-// 24 tiles in one part 142, in two 142, in three 153; 296 rows in 128 groups, in three
-// parts 47.5, in four 44.5.
+// 1536, K = 2048: 24 tiles in two parts 25.5 us, in three 35; 16384 rows in 128 groups, 32
+// a workgroup, 24 tiles in one part 142, in two 142, in three 153; 296 rows in 128 groups,
+// in three parts 47.5, in four 44.5.
 //
 // (Equal shares of all tiles for every workgroup, that end within row tiles, were no
-// faster: 128 against 131 us for those 16384 rows, 144 against 135 for groups of equal
+// faster: 128 against 131 us for those 16384 rows, 32 a workgroup, 144 against 135 for groups of equal
 // sizes, 62 against 57 for 8000 rows, K = 768.  Nor were two halves of the columns for
 // the waves that have no tile: 512 x 4096 15.9 us with and without.)
 struct Plan {

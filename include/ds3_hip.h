@@ -347,7 +347,8 @@ int ds3_hip_mx_dequantize(const ds3_hip_buffer_t *codes, const ds3_hip_buffer_t 
  * delta (delta NULL: s = x), y = s / sqrt(mean(s^2) + eps) * weight, and y
  * rounded to MXINT8 rows as ds3_hip_mx_quantize rounds it.  sum (optional)
  * receives s and may be x or delta; x_norm (optional) receives y, for the
- * router.  s is one fp32 addition, y is computed in 64 bits and rounded once.
+ * router.  sum is rounded once; y is computed in 64 bits from the unrounded
+ * s and rounded once.
  * n is a multiple of 32; every row's result is the same on every call. */
 int ds3_hip_add_rms_norm_mx(const ds3_hip_buffer_t *x, const ds3_hip_buffer_t *delta, const ds3_hip_buffer_t *weight,
                             float eps, ds3_hip_buffer_t *sum, ds3_hip_buffer_t *x_norm, ds3_hip_buffer_t *codes,

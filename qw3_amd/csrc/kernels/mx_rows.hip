@@ -274,11 +274,11 @@ hipError_t launch_mx_dequantize(int mx, const uint8_t *codes, const uint8_t *sca
 // src/ds3_reference.c:329-342), rounded to MXINT8.  s (when delta is given) and y
 // are also written where asked for.
 //
-// s is one fp32 addition; everything from its squares on is in 64 bits, and y
-// rounded once: a factor rounded to 32 bits would move a whole row the same way, and
-// squares in 32 bits would overflow from 1.8e19 on.  Memory bounds the kernel (6001 x
-// 4096 with delta and sum 67 us, 4.8 TB/s; 68.5 in 32 bits), and the vector units have
-// the time.
+// The s that is written is rounded once; y comes from the unrounded sum, in 64
+// bits, and is rounded once: a factor rounded to 32 bits would move a whole row the
+// same way, and squares in 32 bits would overflow from 1.8e19 on.  Memory bounds the
+// kernel (6001 x 4096 with delta and sum 67 us, 4.8 TB/s; 68.5 in 32 bits), and the
+// vector units have the time.
 //
 // A row is read once and stays in registers between the sum of squares and the
 // rounding: TPR threads a row, four columns a thread and chunk, so a block of
@@ -305,27 +305,37 @@ __device__ __forceinline__ void store4f(float *p, const float (&v)[4])
     }
 }
 
+// Four columns' x and delta.
+struct Terms {
+    float x[4], d[4];
+
+    __device__ __forceinline__ double sum(int i) const { return (double)x[i] + (double)d[i]; }
+};
+
 template <bool VEC>
-__device__ __forceinline__ void load_sum4(const NormArgs &a, int64_t at, float (&v)[4])
+__device__ __forceinline__ void load_terms(const NormArgs &a, int64_t at, Terms &v)
 {
-    load4<false, VEC>((const uint8_t *)(a.x + at), v);
+    load4<false, VEC>((const uint8_t *)(a.x + at), v.x);
     if (a.delta) {
-        float d[4];
-        load4<false, VEC>((const uint8_t *)(a.delta + at), d);
+        load4<false, VEC>((const uint8_t *)(a.delta + at), v.d);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = v[i] + d[i];
+        for (int i = 0; i < 4; i++) v.d[i] = 0.f;
     }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void finish4(const NormArgs &a, int64_t row, int col, double rms, const float (&v)[4])
+__device__ __forceinline__ void finish4(const NormArgs &a, int64_t row, int col, double rms, const Terms &v)
 {
     const int64_t at = row * a.n + col;
     float g[4], y[4];
     load4<false, VEC>((const uint8_t *)(a.g + col), g);
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = (float)((double)v[i] * rms * (double)g[i]);
-    if (a.sum) store4f<VEC>(a.sum + at, v);
+    for (int i = 0; i < 4; i++) y[i] = (float)(v.sum(i) * rms * (double)g[i]);
+    if (a.sum) {
+        const float s[4] = { v.x[0] + v.d[0], v.x[1] + v.d[1], v.x[2] + v.d[2], v.x[3] + v.d[3] };
+        store4f<VEC>(a.sum + at, s);
+    }
     if (a.y) store4f<VEC>(a.y + at, y);
     store_block8<T_MXINT8>(y, at / 32, (col / 4) & 7, a.codes, a.scales);
 }
@@ -369,7 +379,7 @@ __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
     const int t = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
     if (WPR == 1 && row >= a.n_rows) return;               // whole waves; WPR > 1 has one row a workgroup
-    float v[CH > 0 ? CH : 1][4];
+    Terms v[CH > 0 ? CH : 1];
     double ss = 0.0;
     const int64_t base = row * a.n;
     if constexpr (CH > 0) {
@@ -377,21 +387,20 @@ __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
         for (int c = 0; c < CH; c++) {
             const int col = (c * TPR + t) * 4;
             if (col < a.n) {
-                load_sum4<VEC>(a, base + col, v[c]);
+                load_terms<VEC>(a, base + col, v[c]);
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[c][i] = 0.f;
+                v[c] = Terms{};
             }
         }
 #pragma unroll
         for (int c = 0; c < CH; c++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) ss = fma((double)v[c][i], (double)v[c][i], ss);
+            for (int i = 0; i < 4; i++) ss = fma(v[c].sum(i), v[c].sum(i), ss);
     } else {
         for (int col = 4 * t; col < a.n; col += 4 * TPR) {
-            load_sum4<VEC>(a, base + col, v[0]);
+            load_terms<VEC>(a, base + col, v[0]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) ss = fma((double)v[0][i], (double)v[0][i], ss);
+            for (int i = 0; i < 4; i++) ss = fma(v[0].sum(i), v[0].sum(i), ss);
         }
     }
     ss = wave_sum64(ss);
@@ -411,7 +420,7 @@ __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
         }
     } else {
         for (int col = 4 * t; col < a.n; col += 4 * TPR) {
-            load_sum4<VEC>(a, base + col, v[0]);
+            load_terms<VEC>(a, base + col, v[0]);
             finish4<VEC>(a, row, col, rms, v[0]);
         }
     }

@@ -166,11 +166,13 @@ def test_add_rms_norm_range(hip_ready, n):
     """Rows whose squares leave the range of 32 bits, and y within one rounding."""
     rng = np.random.default_rng(n)
     x = (rng.standard_normal((6, n)) * np.r_[1e30, 3e18, 1.0, 1e-18, 1e-25, 1e-30][:, None]).astype(np.float32)
+    d = (x * rng.standard_normal(x.shape)).astype(np.float32)
     g = (1 + 0.2 * rng.standard_normal(n)).astype(np.float32)
-    for eps in (0.0, 1e-6):
+    for eps, delta in ((0.0, None), (1e-6, None), (0.0, d), (1e-6, d)):
         m, y = ds3.MxMatrix.alloc(I8, 6, n), ds3.Buffer.alloc(x.nbytes)
-        ds3.add_rms_norm_mx(ds3.Buffer.from_array(x), ds3.Buffer.from_array(g), eps, m, x_norm=y)
-        x64 = x.astype(np.float64)
+        ds3.add_rms_norm_mx(ds3.Buffer.from_array(x), ds3.Buffer.from_array(g), eps, m, x_norm=y,
+                            delta=None if delta is None else ds3.Buffer.from_array(delta))
+        x64 = x.astype(np.float64) + (0 if delta is None else delta)      # not rounded in between
         want = x64 / np.sqrt((x64 ** 2).mean(1, keepdims=True) + np.float32(eps)) * g
         got = y.read(np.float32, x.shape)
         # half a step of the result, and what n additions in 64 bits may lose

@@ -72,17 +72,20 @@ __global__ void __launch_bounds__(MXR_TPB) k_mx_round(const uint8_t *src, uint64
 // the scales of the blocks of 32 that its parts lie in.  A Q4_K unit is 16 weights
 // each of two blocks that it shares with the next lane, a Q6_K unit 8 each of four
 // that a quad shares; their codes are exchanged so that every lane stores the
-// whole of one block.  98304 x 2048 weights to MXFP4: Q4_K 56 us (3.9 TB/s read and
-// written; 72 with the weights themselves exchanged through LDS), Q6_K 83, Q8_0 85
+// whole of one block.  98304 x 2048 weights to MXFP4: Q4_K 54 us (4.1 TB/s read and
+// written; 72 with the weights themselves exchanged through LDS), Q6_K 82, Q8_0 78
 // (its 34-byte blocks are read as dwords in halves); the vector units' decoding and
 // rounding bound it, a copy of as much would take 42, 53 and 62.
+// The largest magnitude's bits.  The values have one scale in common: one that is
+// not finite makes all of them infinite or NaN, the first too, while the maximum
+// itself passes over NaN.
 template <int N>
 __device__ __forceinline__ uint32_t amax_of(const float *v)
 {
-    uint32_t m = 0;
+    float m = fabsf(v[0]);
 #pragma unroll
-    for (int i = 0; i < N; i++) m = max(m, abs_bits(v[i]));
-    return m;
+    for (int i = 1; i < N; i++) m = __builtin_fmaxf(m, fabsf(v[i]));
+    return max(__float_as_uint(m), abs_bits(v[0]));
 }
 
 // The codes of N values, in dwords.

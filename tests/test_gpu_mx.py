@@ -102,6 +102,35 @@ def test_quantize_gguf_rows(hip_ready, to, t, rows, blocks):
         assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0]), st
 
 
+@pytest.mark.parametrize("to", [FP4, I8])
+@pytest.mark.parametrize("t", [ds3.TYPE_Q8_0, ds3.TYPE_Q4_K, ds3.TYPE_Q6_K])
+def test_quantize_gguf_scales_that_are_not_finite(hip_ready, to, t):
+    """Infinite and NaN block scales, also times sub-block scales of zero: the MX blocks they reach get 255."""
+    rng = np.random.default_rng(t)
+    rows, cols = 9, 1024
+    per, nb = ds3.BLOCK[t]
+    blk = rng.integers(0, 256, (rows, cols // per, nb), dtype=np.uint8)
+    at = {ds3.TYPE_Q8_0: (0,), ds3.TYPE_Q4_K: (0, 2), ds3.TYPE_Q6_K: (208,)}[t]
+    for i in at:
+        blk[:, :, i:i + 2] = rng.uniform(1e-4, 2e-3, blk.shape[:2] + (1,)).astype(np.float16).view(np.uint8)
+    if t != ds3.TYPE_Q8_0:                              # some sub-block scales of zero
+        sub = slice(4, 16) if t == ds3.TYPE_Q4_K else slice(192, 208)
+        blk[:, :, sub] *= rng.integers(0, 2, blk[:, :, sub].shape, dtype=np.uint8)
+    for r, v in ((1, np.inf), (3, np.nan), (5, -np.inf), (7, np.inf)):
+        i = at[-1] if r > 4 else at[0]
+        blk[r, r % 3, i:i + 2] = np.array([v], np.float16).view(np.uint8)
+    raw = blk.reshape(rows, -1)
+    with np.errstate(invalid="ignore"):
+        v = O.dequantize(t, raw.reshape(-1), rows * cols).reshape(rows, cols)
+        want = X.encode(to, v)
+    m = ds3.MxMatrix.alloc(to, rows, cols)
+    ds3.mx_quantize(ds3.Buffer.from_array(raw), t, m)
+    codes, scales = read_mx(m)
+    bad = ~np.isfinite(v).reshape(rows, -1, 32).all(2)
+    assert bad.any() and np.array_equal(scales == 255, bad)
+    assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0])
+
+
 @pytest.mark.parametrize("t", [FP4, I8])
 @pytest.mark.parametrize("dst,size", [(ds3.TYPE_F32, 4), (ds3.TYPE_F16, 2)])
 def test_dequantize(hip_ready, t, dst, size):

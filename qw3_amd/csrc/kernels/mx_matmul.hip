@@ -127,8 +127,8 @@ __device__ __forceinline__ Job job_of(uint32_t job, uint32_t n_tiles)
 // 512 columns in turn, straight from memory, and their sums meet in LDS.  Two to
 // three waves a SIMD hide each other's loads.  Bound by memory where the weights
 // are many (1 x 2048 . 151936 34.1 us, 4.9 TB/s), else by the chain of offsets,
-// ids, rows and weights (27 x 2048 . 768 4.5 us, gate/up of one token in 8 of 128
-// experts 8.6).
+// ids, rows and weights (in a graph 27 x 2048 . 768 4.6 us, 1 x 2048 . 2048 3.4,
+// gate/up of one token in 8 of 128 experts, with the values of h, 8.3).
 // ---------------------------------------------------------------------------
 template <int WAVES, int NT, bool GU>
 __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProduct p, uint32_t n_jobs, uint32_t n_tiles)
@@ -153,12 +153,6 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
             return id >= 0 && id < p.n_x ? id : (int64_t)-1;
         };
         const bool ok = r < tile.rows && x_row(r) >= 0;  // this lane's outputs exist
-        const uint8_t *xc[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) xc[j] = p.xc + max(x_row((r & 12) + j), (int64_t)0) * p.K;
-        const uint8_t *xs = p.xs + max(x_row(lane >> 2), (int64_t)0) * nb + 4 * (lane & 3);
-        const int64_t row4 = max(x_row(r >> 2), (int64_t)0);
-        const uint8_t *xc4 = p.xc + row4 * p.K, *xs4 = p.xs + row4 * nb;
         // The weight rows of block t: n_of(t) .. + 15, moved down where they would pass the
         // end (those below n0 + 16 t are then not stored).
         const auto n_of = [&](int t) {
@@ -185,6 +179,16 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
         // the vector units were busy two thirds of it).
         const auto chunks = [&](auto four_rows) {
             constexpr bool FOUR = decltype(four_rows)::value != 0;
+            const uint8_t *xc[4], *xs;                   // FOUR: one row, else as the loads take them
+            if constexpr (FOUR) {
+                const int64_t row = max(x_row(r >> 2), (int64_t)0);
+                xc[0] = p.xc + row * p.K;
+                xs = p.xs + row * nb;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) xc[j] = p.xc + max(x_row((r & 12) + j), (int64_t)0) * p.K;
+                xs = p.xs + max(x_row(lane >> 2), (int64_t)0) * nb + 4 * (lane & 3);
+            }
             for (int c = wave; c < n_chunk; c += WAVES) {
                 // Blocks behind the last are read as the last (their x becomes zero); scales up to
                 // 15 bytes on, which every allocation has.
@@ -193,7 +197,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
                 uint32_t sx, sw[NT];
                 RawBlock own;
                 if constexpr (FOUR) {
-                    own = raw_block(xc4, xs4, b);
+                    own = raw_block(xc[0], xs, b);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {

@@ -68,14 +68,6 @@ __global__ void __launch_bounds__(MXR_TPB) k_mx_round(const uint8_t *src, uint64
     }
 }
 
-// GGUF blocks: a thread decodes one 32-weight unit (common.h) and rounds it with
-// the scales of the blocks of 32 that its parts lie in.  A Q4_K unit is 16 weights
-// each of two blocks that it shares with the next lane, a Q6_K unit 8 each of four
-// that a quad shares; their codes are exchanged so that every lane stores the
-// whole of one block.  98304 x 2048 weights to MXFP4: Q4_K 54 us (4.1 TB/s read and
-// written; 72 with the weights themselves exchanged through LDS), Q6_K 82, Q8_0 78
-// (its 34-byte blocks are read as dwords in halves); the vector units' decoding and
-// rounding bound it, a copy of as much would take 42, 53 and 62.
 // The largest magnitude's bits.  The values have one scale in common: one that is
 // not finite makes all of them infinite or NaN, the first too, while the maximum
 // itself passes over NaN.
@@ -102,6 +94,14 @@ __device__ __forceinline__ void round_dwords(const float *v, uint32_t c, int *ou
     }
 }
 
+// GGUF blocks: a thread decodes one 32-weight unit (common.h) and rounds it with
+// the scales of the blocks of 32 that its parts lie in.  A Q4_K unit is 16 weights
+// each of two blocks that it shares with the next lane, a Q6_K unit 8 each of four
+// that a quad shares; their codes are exchanged so that every lane stores the
+// whole of one block.  98304 x 2048 weights to MXFP4: Q4_K 54 us (4.1 TB/s read and
+// written; 72 with the weights themselves exchanged through LDS), Q6_K 82, Q8_0 78
+// (its 34-byte blocks are read as dwords in halves); the vector units' decoding and
+// rounding bound it, a copy of as much would take 42, 53 and 62.
 template <int MX, int TYPE>
 __global__ void __launch_bounds__(MXR_TPB) k_mx_round_gguf(const uint8_t *src, uint64_t stride, int64_t n_blocks,
                                                            int64_t nb, uint8_t *codes, uint8_t *scales)
@@ -373,7 +373,8 @@ __device__ __forceinline__ double wave_sum64(double v)
 }
 
 // Eight lanes hold a block, and columns come in 32s, so a block's lanes are in
-// or out together.
+// or out together.  y is rounded to 32 bits before its block is: a value that 64 bits
+// put a hair below a power of two would else halve its block's scale and saturate.
 template <int TPR, int CH, bool VEC>
 __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
 {

@@ -173,15 +173,16 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
         f32x4 acc[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[t] = f32x4{ 0.f, 0.f, 0.f, 0.f };
-        // Up to four rows: a lane splits one block, lane 16 g + 4 R + p block 4 g + p of row R,
-        // and step k takes them from there through the LDS crossbar.  More rows: a lane splits
-        // the four blocks that it multiplies (for one row of 151936 outputs 38.4 us, not 34.1:
-        // the vector units were busy two thirds of it).
-        const auto chunks = [&](auto four_rows) {
-            constexpr bool FOUR = decltype(four_rows)::value != 0;
-            const uint8_t *xc[4], *xs;                   // FOUR: one row, else as the loads take them
-            if constexpr (FOUR) {
-                const int64_t row = max(x_row(r >> 2), (int64_t)0);
+        // Up to 4 PER rows: a lane splits PER blocks, lanes 16 g + 4 / PER R .. the four blocks
+        // 4 g + 0..3 of row R, and step k takes them from there through the LDS crossbar.  More
+        // rows (PER = 4): a lane splits the four blocks that it multiplies (for one row of
+        // 151936 outputs 38.4 us, not 34.1: the vector units were busy two thirds of it; for
+        // eight rows, K = 4096, 4096 outputs 6.7, not 5.5).
+        const auto chunks = [&](auto per) {
+            constexpr int PER = decltype(per)::value, LANES = 4 / PER;
+            const uint8_t *xc[4], *xs;                   // of one row, PER = 4: as the loads take them
+            if constexpr (PER < 4) {
+                const int64_t row = max(x_row(r / LANES), (int64_t)0);
                 xc[0] = p.xc + row * p.K;
                 xs = p.xs + row * nb;
             } else {
@@ -195,9 +196,11 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
                 const int b0 = c * CHUNK_BLOCKS, b = min(b0 + lb, nb - 1);
                 i32x4 x0[4], x1[4], w[NT][4];
                 uint32_t sx, sw[NT];
-                RawBlock own;
-                if constexpr (FOUR) {
-                    own = raw_block(xc[0], xs, b);
+                const int own = b0 + 4 * g + PER * (r % LANES);
+                RawBlock raw[PER];
+                if constexpr (PER < 4) {
+#pragma unroll
+                    for (int i = 0; i < PER; i++) raw[i] = raw_block(xc[0], xs, min(own + i, nb - 1));
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
@@ -212,9 +215,10 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
                     for (int j = 0; j < 4; j++) w[t][j] = *(const i32x4 *)(wc[t] + c_row[j] + (uint32_t)b * 16);
                     sw[t] = *(const u32_any *)(ws[t] + s_row + b0);
                 }
-                XFrag mine;
-                if constexpr (FOUR) {
-                    mine = x_frag(own, b0 + lb < nb);
+                XFrag mine[PER];
+                if constexpr (PER < 4) {
+#pragma unroll
+                    for (int i = 0; i < PER; i++) mine[i] = x_frag(raw[i], own + i < nb);
                 } else {
                     quad_transpose(x0);
                     quad_transpose(x1);
@@ -228,8 +232,8 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
                 const auto step = [&](auto kc) {
                     constexpr int k = decltype(kc)::value;
                     XFrag f;
-                    if constexpr (FOUR) {
-                        f = frag_from(mine, 16 * g + ((4 * r + k) & 15));
+                    if constexpr (PER < 4) {
+                        f = frag_from(mine[k % PER], 16 * g + ((LANES * r + k / PER) & 15));
                     } else {
                         RawBlock q;
 #pragma unroll
@@ -252,7 +256,8 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
             }
         };
         if (tile.rows <= 4) chunks(Int<1>{});
-        else chunks(Int<0>{});
+        else if (tile.rows <= 8) chunks(Int<2>{});
+        else chunks(Int<4>{});
 #pragma unroll
         for (int t = 0; t < NT; t++) red[wave][t][lane] = acc[t];
         __syncthreads();
@@ -677,8 +682,8 @@ static hipError_t launch_few(const MxProduct &p, hipStream_t s)
 //    against 9.7; at 512 blocks (128 x 4096) 11.3 against 10.0.  Beyond, too, with few
 //    rows to split, at most one a group: 128 rows in 128 groups of 768 x 2 outputs 32.0
 //    against 39, K = 768 and 2048 outputs 17.9 against 18.6 (with two a group 23.8
-//    against 21.3); or four rows of one matrix: one of 65536 outputs, K = 768, 7.8 against
-//    10.7, K = 4096, 27.6 against 34;
+//    against 21.3); or eight rows of one matrix: one of 65536 outputs, K = 768, 7.8
+//    against 10.7, K = 4096, 27.6 against 34, eight 30.3 against 34.4;
 //  - in it, one block of weight rows a workgroup below 128 blocks (64 blocks 5.1, two
 //    5.3; 128 blocks 6.5 against 5.6), two below 512 and four waves (64 x 4096: 7.1,
 //    with four by two waves 8.4), or with the two chunks of K = 768 below 256 (128 x
@@ -697,7 +702,7 @@ template <bool GU>
 static hipError_t launch_product(const MxProduct &p, hipStream_t s)
 {
     const int64_t blocks = usual_tiles(p, 16) * (((int64_t)p.N * (GU ? 2 : 1) + 63) / 64);
-    if (blocks < 512 || p.n_rows <= (p.offsets ? p.n_group : 4) || tile_lds(p, 1) > LDS_BYTES) {
+    if (blocks < 512 || p.n_rows <= (p.offsets ? p.n_group : 8) || tile_lds(p, 1) > LDS_BYTES) {
         if constexpr (GU) return blocks < 512 ? launch_few<4, 4, true>(p, s) : launch_few<2, 4, true>(p, s);
         else if (blocks < 128) return launch_few<4, 1, false>(p, s);
         else if (blocks < (p.K > 1024 ? 512 : 256)) return launch_few<4, 2, false>(p, s);

@@ -14,6 +14,7 @@ DENSE = [(20, 4000, 128), (33, 2700, 256), (70, 4100, 1024), (70, 4100, 1056), (
          (200, 2600, 3616), (500, 1040, 7680), (500, 1040, 7712), (1000, 2100, 544), (500, 4200, 64), (1000, 2100, 3584),
          (1000, 2100, 3616), (1, 33000, 1056), (1, 33000, 1024),
          (4, 33000, 288), (5, 33000, 288), (4, 300, 1600), (5, 300, 1600), (2, 70, 96),
+         (8, 33000, 288), (9, 33000, 288), (8, 300, 1600), (9, 300, 1600), (6, 2000, 2080),
          (512, 4096, 288), (3001, 1197, 96), (1500, 2200, 2560), (1500, 2200, 2592)]
 
 

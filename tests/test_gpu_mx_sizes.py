@@ -91,3 +91,46 @@ def test_scales(hip_ready, m, n, k):
     # scale bytes below 5 round x to multiples of 2^-128: half of one for each term
     slack = np.abs(w.values).sum(1)[None] * 2.0 ** -129
     assert (np.abs(got[rows] - want) <= X.sum_bound(mag, k) + slack).all()
+
+
+def test_outputs_beyond_32_bits(hip_ready):
+    """C of more than 2^32 bytes: its first, middle and last rows."""
+    rng = np.random.default_rng(4)
+    m, n, k = 33000, 33000, 32
+    x, w = X.random_matrix(rng, I8, m, k), X.random_matrix(rng, FP4, n, k)
+    c = ds3.Buffer.alloc(4 * m * n)
+    print(f"  matmul_mx {m}x{n}x{k}", flush=True)
+    ds3.matmul_mx(x.dev, w.dev, c)
+    for row in (0, 1, 2 ** 30 // n, 2 ** 30 // n + 1, 2 ** 31 // n, m - 2, m - 1):
+        row = min(row, m - 1)
+        got = c.view(4 * row * n, 4 * n).read(np.float32, (1, n))
+        check(got, *X.product(x.values[row:row + 1], w.values), k)
+
+
+@pytest.mark.parametrize("rows,groups", [(1, 1), (40, 1), (6, 2)])
+def test_weights_beyond_32_bits(hip_ready, rows, groups):
+    """More than 2^32 bytes of weights, zeros but for the first and the last rows."""
+    rng = np.random.default_rng(rows)
+    n, k, some = 70016 // groups, 131072, 20
+    x, part = X.random_matrix(rng, I8, rows, k), X.random_matrix(rng, FP4, 2 * some, k)
+    w = ds3.MxMatrix.alloc(FP4, n * groups, k)          # zeroed
+    last = n * groups - some
+    for at, r in ((0, slice(0, some)), (last, slice(some, None))):
+        w.codes.view(at * k // 2, some * k // 2).write(part.codes[r])
+        w.scales.view(at * k // 32, some * k // 32).write(part.scales[r])
+    c = ds3.Buffer.alloc(4 * rows * n)
+    print(f"  {rows} rows, {n * groups} x {k} weights in {groups} groups", flush=True)
+    want, mag = X.product(x.values, part.values)
+    if groups == 1:
+        ds3.matmul_mx(x.dev, w, c)
+        got = c.read(np.float32, (rows, n))
+        check(got[:, :some], want[:, :some], mag[:, :some], k)
+        check(got[:, -some:], want[:, some:], mag[:, some:], k)
+        assert not got[:, some:-some].any()
+    else:
+        half = rows // 2
+        ds3.matmul_mx_grouped(x.dev, w, ds3.Buffer.from_array(np.array([0, half, rows], np.int32)), c, rows, 2)
+        got = c.read(np.float32, (rows, n))
+        check(got[:half, :some], want[:half, :some], mag[:half, :some], k)
+        check(got[half:, -some:], want[half:, some:], mag[half:, some:], k)
+        assert not got[:half, some:].any() and not got[half:, :-some].any()

@@ -256,39 +256,46 @@ __device__ __forceinline__ void quad_transpose(i32x4 (&v)[4])
 }
 
 // The same beside matrix products: v_cndmask_b32 takes its exchange as a DPP
-// operand, half the instructions, but its mask from VCC, which a new mask is slow to
-// reach.  Alone 16 registers take 700 cycles like this and 270 as above; where the
-// SIMD's other wave and the matrix cores have work meanwhile, the instructions
-// count (16384 rows in 128 groups of 768 x 2 outputs, 32 rows a workgroup: 131.6 us,
-// 136.4 as above).  The compiler does not see that vector instructions write the results: a product reads
-// them two instructions later at the earliest, as every use in a loop's next turn does.
+// operand, half the instructions, but its mask from VCC.  Where the SIMD's other wave
+// and the matrix cores have work meanwhile, the instructions count (16384 rows in 128
+// groups of 768 x 2 outputs: 120.2 us, 125.6 as above; 2048 x 4096, K = 2048: 32.7,
+// 34.6); where a SIMD has one wave, the waits for VCC do (512 x 4096: 16.1, 15.0).
+//
+// The masks are constants that scalar instructions write: a vector instruction may
+// read a VCC that a scalar one wrote in the very next place, one that a comparison
+// wrote two places later (such waits in place of them: 16.5, 121.8).  The compiler does
+// not look inside, so the block keeps the distances itself: two places from a vector
+// write to a DPP read of it and three from a product that reads a register as its sum to
+// the register's next write (before the block by s_nop and two s_mov, inside by four
+// selections), two from its last write to a product that reads it (products of other
+// weights or the next turn's first loads).
 __device__ __forceinline__ void quad_transpose_beside(i32x4 (&v)[4])
 {
-    const int b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
 #define QUAD_XOR1 " quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf bound_ctrl:0\n"
 #define QUAD_XOR2 " quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf bound_ctrl:0\n"
 #pragma unroll
     for (int d = 0; d < 4; d += 2) {
         int s0, s1, s2, s3, t0, t1, t2, t3;              // after the first exchange
         int o0, o1, o2, o3, q0, q1, q2, q3;
-        // a DPP operand is read two instructions after it was written at the earliest
         asm("s_nop 0\n"
-            "v_cmp_eq_u32_e32 vcc, 0, %[b0]\n"
+            "s_mov_b32 vcc_lo, 0x55555555\n"            // the even lanes
+            "s_mov_b32 vcc_hi, 0x55555555\n"
             "v_cndmask_b32_dpp %[s0], %[a1], %[a0], vcc" QUAD_XOR1
             "v_cndmask_b32_dpp %[s2], %[a3], %[a2], vcc" QUAD_XOR1
             "v_cndmask_b32_dpp %[t0], %[c1], %[c0], vcc" QUAD_XOR1
             "v_cndmask_b32_dpp %[t2], %[c3], %[c2], vcc" QUAD_XOR1
-            "v_cmp_ne_u32_e32 vcc, 0, %[b0]\n"
+            "s_not_b64 vcc, vcc\n"
             "v_cndmask_b32_dpp %[s1], %[a0], %[a1], vcc" QUAD_XOR1
             "v_cndmask_b32_dpp %[s3], %[a2], %[a3], vcc" QUAD_XOR1
             "v_cndmask_b32_dpp %[t1], %[c0], %[c1], vcc" QUAD_XOR1
             "v_cndmask_b32_dpp %[t3], %[c2], %[c3], vcc" QUAD_XOR1
-            "v_cmp_eq_u32_e32 vcc, 0, %[b1]\n"
+            "s_mov_b32 vcc_lo, 0x33333333\n"            // the first two of each quad
+            "s_mov_b32 vcc_hi, 0x33333333\n"
             "v_cndmask_b32_dpp %[o0], %[s2], %[s0], vcc" QUAD_XOR2
             "v_cndmask_b32_dpp %[o1], %[s3], %[s1], vcc" QUAD_XOR2
             "v_cndmask_b32_dpp %[q0], %[t2], %[t0], vcc" QUAD_XOR2
             "v_cndmask_b32_dpp %[q1], %[t3], %[t1], vcc" QUAD_XOR2
-            "v_cmp_ne_u32_e32 vcc, 0, %[b1]\n"
+            "s_not_b64 vcc, vcc\n"
             "v_cndmask_b32_dpp %[o2], %[s0], %[s2], vcc" QUAD_XOR2
             "v_cndmask_b32_dpp %[o3], %[s1], %[s3], vcc" QUAD_XOR2
             "v_cndmask_b32_dpp %[q2], %[t0], %[t2], vcc" QUAD_XOR2
@@ -297,8 +304,8 @@ __device__ __forceinline__ void quad_transpose_beside(i32x4 (&v)[4])
               [t2] "=&v"(t2), [t3] "=&v"(t3), [o0] "=&v"(o0), [o1] "=&v"(o1), [o2] "=&v"(o2), [o3] "=&v"(o3),
               [q0] "=&v"(q0), [q1] "=&v"(q1), [q2] "=&v"(q2), [q3] "=&v"(q3)
             : [a0] "v"(v[0][d]), [a1] "v"(v[1][d]), [a2] "v"(v[2][d]), [a3] "v"(v[3][d]), [c0] "v"(v[0][d + 1]),
-              [c1] "v"(v[1][d + 1]), [c2] "v"(v[2][d + 1]), [c3] "v"(v[3][d + 1]), [b0] "v"(b0), [b1] "v"(b1)
-            : "vcc");
+              [c1] "v"(v[1][d + 1]), [c2] "v"(v[2][d + 1]), [c3] "v"(v[3][d + 1])
+            : "vcc", "scc");
         v[0][d] = o0, v[1][d] = o1, v[2][d] = o2, v[3][d] = o3;
         v[0][d + 1] = q0, v[1][d + 1] = q1, v[2][d + 1] = q2, v[3][d + 1] = q3;
     }

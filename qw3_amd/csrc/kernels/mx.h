@@ -259,7 +259,8 @@ __device__ __forceinline__ void quad_transpose(i32x4 (&v)[4])
 // operand, half the instructions, but its mask from VCC.  Where the SIMD's other wave
 // and the matrix cores have work meanwhile, the instructions count (16384 rows in 128
 // groups of 768 x 2 outputs: 120.2 us, 125.6 as above; 2048 x 4096, K = 2048: 32.7,
-// 34.6); where a SIMD has one wave, the waits for VCC do (512 x 4096: 16.1, 15.0).
+// 34.6); where a SIMD has one wave, the waits for VCC do (512 x 4096: 16.1, 15.0), and
+// the transposition above serves.
 //
 // The masks are constants that scalar instructions write: a vector instruction may
 // read a VCC that a scalar one wrote in the very next place, one that a comparison

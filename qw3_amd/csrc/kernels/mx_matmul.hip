@@ -346,7 +346,7 @@ __device__ __forceinline__ XFrag frag_load(const uint8_t *frag, int at)
     return f;
 }
 
-template <int WAVES, int NT, int MT, int LEAD, bool GU>
+template <int WAVES, int NT, int MT, int LEAD, bool GU, bool BESIDE>
 __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32_t n_jobs, uint32_t n_tiles, int span,
                                                              int spread)
 {
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32
 #pragma unroll
                         for (int t = 0; t < NT; t++) {
                             acc[t][m] = mx_mfma_lo<k>(w[t][k], sw[t], f, acc[t][m]);
-                            if (k == 3 && m == MT - 1) place_w(t, next_c, Int<1>{});
+                            if (k == 3 && m == MT - 1) place_w(t, next_c, Int<BESIDE>{});
                         }
                         if (m == MT - 1 && k == 1) {             // the registers of two steps are free
 #pragma unroll
@@ -650,9 +650,14 @@ static hipError_t launch_tile(const MxProduct &p, hipStream_t s)
     constexpr int BM = 16 * MT, OUT = GU ? 8 * NT : 16 * NT;
     const int lds = tile_lds(p, MT);
     if (lds > LDS_BYTES) return hipErrorInvalidValue;
+    // Whether every SIMD has two waves with a tile each (K = 2048: 512 x 4096, 1024 tiles,
+    // 16.9 us with the transposition for that, 16.0 without; 768 x 4096, 1536 tiles, 19.25,
+    // 18.9; 1024 x 4096, 2048 tiles, 20.15, 20.5).
+    const bool beside = usual_tiles(p, BM) * (((int64_t)p.N + OUT - 1) / OUT) >= 8 * CUS;
+    const auto kernel = beside ? k_mx_tile<WAVES, NT, MT, LEAD, GU, true> : k_mx_tile<WAVES, NT, MT, LEAD, GU, false>;
     if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void *)k_mx_tile<WAVES, NT, MT, LEAD, GU>,
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
+        const hipError_t e =
+            hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
         if (e != hipSuccess) return e;
     }
     const int64_t span = tile_plan<WAVES, NT, MT, GU>(p).span;
@@ -661,8 +666,7 @@ static hipError_t launch_tile(const MxProduct &p, hipStream_t s)
     const uint32_t items = n_jobs / n_tiles;
     const int spread = items >= 32 ? 1 : 0;
     if (spread) n_jobs = (items + 7) / 8 * 8 * n_tiles;          // row tiles past the last are empty
-    hipLaunchKernelGGL((k_mx_tile<WAVES, NT, MT, LEAD, GU>), job_grid(n_jobs), dim3(WAVES * WAVE), (size_t)lds, s, p, n_jobs,
-                       n_tiles, (int)span, spread);
+    hipLaunchKernelGGL(kernel, job_grid(n_jobs), dim3(WAVES * WAVE), (size_t)lds, s, p, n_jobs, n_tiles, (int)span, spread);
     return hipGetLastError();
 }
 

@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) k_mx_tile(MxProduct p, uint32
     const int r = lane & 15, g = lane >> 4;              // a lane's place in the products
     const int rl = lane >> 2, gl = lane & 3;             // and in loads of four blocks of 16 rows
     const int nb = p.K / 32, n_chunk = (nb + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS;
-    const int col_tiles = (p.N + OUT - 1) / OUT;
+    const int col_tiles = (int)(((uint32_t)p.N + OUT - 1) / OUT);
     const uint32_t n_items = spread ? row_tiles<BM>(p.offsets, p.n_group, p.n_rows) : 0;
 
     for (uint32_t at = blockIdx.x; at < n_jobs; at += gridDim.x) {

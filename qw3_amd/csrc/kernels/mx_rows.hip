@@ -381,8 +381,8 @@ __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
     constexpr int ROWS = MXR_TPB / TPR, WPR = TPR / WAVE;
     __shared__ double part[MXR_TPB / WAVE];
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-    if (WPR == 1 && row >= a.n_rows) return;               // whole waves; WPR > 1 has one row a workgroup
+    const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / TPR;
+    if (row >= a.n_rows) return;                            // whole waves; WPR > 1 has one row a workgroup
     Terms v[CH > 0 ? CH : 1];
     double ss = 0.0;
     const int64_t base = row * a.n;
@@ -433,7 +433,9 @@ __global__ void __launch_bounds__(MXR_TPB) k_add_rms_norm_mx(NormArgs a)
 template <int TPR, int CH>
 static hipError_t norm_launch(const NormArgs &a, bool vec, hipStream_t s)
 {
-    const dim3 grid((unsigned)((a.n_rows + MXR_TPB / TPR - 1) / (MXR_TPB / TPR))), tpb(MXR_TPB);
+    // a launch takes fewer than 2^32 threads in x
+    const int64_t wg = (a.n_rows + MXR_TPB / TPR - 1) / (MXR_TPB / TPR), gx = std::min<int64_t>(wg, 1 << 20);
+    const dim3 grid((unsigned)gx, (unsigned)((wg + gx - 1) / gx)), tpb(MXR_TPB);
     if (vec) hipLaunchKernelGGL((k_add_rms_norm_mx<TPR, CH, true>), grid, tpb, 0, s, a);
     else hipLaunchKernelGGL((k_add_rms_norm_mx<TPR, CH, false>), grid, tpb, 0, s, a);
     return hipGetLastError();

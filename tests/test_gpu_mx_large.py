@@ -37,3 +37,27 @@ def test_most_columns(hip_ready, m, n):
             got = c.view(4 * (row * n + at), 4 * SOME).read(np.float32, SOME)
             cols = slice(i * SOME, (i + 1) * SOME)
             check(got, want[row, cols], mag[row, cols], k)
+
+
+@pytest.mark.parametrize("rows,n", [(2 ** 26 + 5, 32), (2 ** 24 + 3, 1056)])
+def test_norm_of_most_rows(hip_ready, rows, n):
+    """More rows than one dimension of a launch has threads for (89 GB): zero rows but for the first, some middle and
+    the last ones, whose results are those of a call of their own."""
+    rng = np.random.default_rng(n)
+    some, eps = 7, 1e-6
+    places = [0, 2 ** 20 - 3, 2 ** 22 - 3, 2 ** 23, rows - some]
+    part = rng.standard_normal((some * len(places), n)).astype(np.float32)
+    g = ds3.Buffer.from_array((1 + 0.2 * rng.standard_normal(n)).astype(np.float32))
+    x, m = ds3.Buffer.alloc(4 * rows * n), ds3.MxMatrix.alloc(I8, rows, n)
+    for i, at in enumerate(places):
+        x.view(4 * at * n, 4 * some * n).write(part[i * some:(i + 1) * some])
+    print(f"  norm {rows}x{n}", flush=True)
+    ds3.add_rms_norm_mx(x, g, eps, m)
+    own = ds3.MxMatrix.alloc(I8, len(part), n)
+    ds3.add_rms_norm_mx(ds3.Buffer.from_array(part), g, eps, own)
+    codes, scales = own.codes.read(np.uint8, part.shape), own.scales.read(np.uint8, (len(part), n // 32))
+    assert scales.any(1).all()
+    for i, at in enumerate(places):
+        r = slice(i * some, (i + 1) * some)
+        assert np.array_equal(m.codes.view(at * n, some * n).read(np.uint8, (some, n)), codes[r]), at
+        assert np.array_equal(m.scales.view(at * (n // 32), some * (n // 32)).read(np.uint8, (some, n // 32)), scales[r]), at

@@ -52,7 +52,7 @@ template <int BM> struct GroupTiles {
         for (int i = 0; i < 5; i++) at[i] = min(max(offsets[min(g0 + 4 * lane + i, n_group)], 0), n_rows);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            tiles[i] = max(at[i + 1] - at[i] + BM - 1, 0) / BM;
+            tiles[i] = (int)(((uint32_t)max(at[i + 1] - at[i], 0) + BM - 1) / BM);
             sum += tiles[i];
         }
         incl = wave_scan(sum);

@@ -61,3 +61,24 @@ def test_norm_of_most_rows(hip_ready, rows, n):
         r = slice(i * some, (i + 1) * some)
         assert np.array_equal(m.codes.view(at * n, some * n).read(np.uint8, (some, n)), codes[r]), at
         assert np.array_equal(m.scales.view(at * (n // 32), some * (n // 32)).read(np.uint8, (some, n // 32)), scales[r]), at
+
+
+def test_largest_group(hip_ready):
+    """A group of nearly 2^31 rows (17 GB with their ids), and one behind it."""
+    rng = np.random.default_rng(6)
+    rows, n, k, n_x = 2 ** 31 - 1, 1, 32, 9
+    offsets = np.array([0, rows - 5, rows], np.int32)
+    x, w = X.random_matrix(rng, I8, n_x, k), X.random_matrix(rng, FP4, 2 * n, k)
+    ids, c = ds3.Buffer.alloc(4 * rows), ds3.Buffer.alloc(4 * rows)      # zeroed: x's first row
+    places = [0, 2 ** 29 - 3, 2 ** 30 + 77, rows - 2 ** 20, rows - 1000]
+    own = rng.integers(0, n_x, (len(places), 1000)).astype(np.int32)
+    for at, v in zip(places, own):
+        ids.write(v, 4 * at)
+    print(f"  matmul_mx_grouped {rows}x{n}x{k}", flush=True)
+    ds3.matmul_mx_grouped(x.dev, w.dev, ds3.Buffer.from_array(offsets), c, rows, 2, ids=ids)
+    want, mag = X.product(x.values, w.values)
+    for at, v in zip(places, own):
+        group = (np.arange(at, at + 1000) >= offsets[1]).astype(int)
+        check(c.read(np.float32, 1000, 4 * at), want[v, group], mag[v, group], k)
+    for at in (5000, 2 ** 30 - 99, rows - 2 ** 21):
+        check(c.read(np.float32, 99, 4 * at), want[0, 0], mag[0, 0], k)

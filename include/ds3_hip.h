@@ -400,8 +400,8 @@ int ds3_hip_moe_combine(const ds3_hip_buffer_t *y, const ds3_hip_buffer_t *slot_
  * the experts the same rows in MXINT8, and h is rounded to MXINT8.  gate_logits /
  * indices / scores (optional) as in ds3_hip_moe_ffn_batch, with its limits on
  * n_expert and n_used, but that the certified router's scores come from its
- * logits in 64 bits.  It uses the library's workspace: before a capture the
- * call is made once. */
+ * logits in 64 bits.  n_tokens is below 2^26.  It uses the library's workspace:
+ * before a capture the call is made once. */
 int ds3_hip_moe_block_mx(ds3_hip_buffer_t *hidden, const ds3_hip_buffer_t *delta, const ds3_hip_buffer_t *ffn_norm,
                          float eps, const ds3_hip_buffer_t *w_gate_inp,
                          const ds3_hip_buffer_t *gate_codes, const ds3_hip_buffer_t *gate_scales,

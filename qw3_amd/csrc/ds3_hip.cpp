@@ -2334,6 +2334,11 @@ extern "C" int ds3_hip_moe_block_mx(
     if (!mx_sizes_ok(what, { n_tokens, n_embd, n_ff_exp, (uint64_t)n_tokens * n_used }) ||
         !mx_cols_ok(what, "n_embd", n_embd) || !mx_cols_ok(what, "n_ff_exp", n_ff_exp) || !moe_limits_ok(n_expert, n_used))
         return -1;
+    // (refused before anything is written: the router takes 64 threads a token in one dimension of a launch)
+    if (n_tokens >= 1u << 26) {
+        fprintf(stderr, "ds3_hip: %s: n_tokens=%u is out of range (below 2^26)\n", what, n_tokens);
+        return -1;
+    }
     const size_t rb = row_bytes(router_type, n_embd);
     if (!router_seq_type_ok(router_type, (int)n_embd) || rb == 0 || router_row_stride < rb ||
         router_row_stride > (uint64_t)1 << 40) {

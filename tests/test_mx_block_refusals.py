@@ -72,3 +72,9 @@ def test_python_refusals():
     for mats, n_expert in (((g, bad, d), 8), ((g, g, g), 8), ((g, g, d), 7), ((g, d, d), 8)):
         with pytest.raises(ValueError):
             ds3.moe_block_mx(None, None, 1e-6, None, F32, *mats, 3, n_expert, 2)
+
+
+def test_more_tokens_than_a_launch_routes(lib, capfd):
+    """The router's launch ends below 2^26 tokens; the call says so before hidden is written."""
+    refused(lib, capfd, "moe_block_mx", changed(BLOCK, a14=1 << 26), "n_tokens=67108864 is out of range")
+    refused(lib, capfd, "moe_block_mx", changed(BLOCK, a14=(1 << 26) - 1), "holds")

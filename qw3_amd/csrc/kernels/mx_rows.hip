@@ -323,7 +323,7 @@ __device__ __forceinline__ void load_terms(const NormArgs &a, int64_t at, Terms 
         load4<false, VEC>((const uint8_t *)(a.delta + at), v.d);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v.d[i] = 0.f;
+        for (int i = 0; i < 4; i++) v.d[i] = -0.f;           // x + -0 is x, for -0 too
     }
 }
 

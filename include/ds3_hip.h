@@ -463,6 +463,16 @@ int ds3_hip_debug_grouped_descs(int32_t *desc_gu, int32_t *desc_dn);
 int ds3_hip_debug_product_plan(ds3_hip_type_t type, uint32_t M, uint32_t N, uint32_t K, uint64_t weight_row_stride,
                                uint64_t weight_offset, int64_t *plan);
 
+/* No ds3_metal.h counterpart (a test hook): the kernel that the microscaled
+ * products take for n_rows rows in n_group groups (0: ds3_hip_matmul_mx; gate_up:
+ * ds3_hip_moe_gate_up_mx with N = n_ff, else ds3_hip_matmul_mx_grouped).  plan =
+ * { kernel (0 few rows, 1 many), waves and rows of x a workgroup, output columns
+ * a tile (gate_up: of h), tiles of output columns, how many of them a workgroup
+ * takes, for kernel 1 whether its waves transpose weights beside others' work }.
+ * A wave of kernel 1 takes every `waves`-th tile of its workgroup's.
+ * Launches nothing and needs no device; -1 for sizes that no product takes. */
+int ds3_hip_debug_mx_plan(uint32_t n_rows, uint32_t n_group, uint32_t N, uint32_t K, bool gate_up, int64_t *plan);
+
 /* No ds3_metal.h counterpart: the row count of A from which
  * ds3_hip_matmul_quantized_batch takes its fp16 MFMA path (see there).  0
  * restores the default (64).  Returns the previous value. */

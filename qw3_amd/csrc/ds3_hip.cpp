@@ -2296,6 +2296,25 @@ extern "C" int ds3_hip_moe_gate_up_mx(const ds3_hip_buffer_t *x_codes, const ds3
     return run_mx_product(&p, "mx_gate_up", what);
 }
 
+extern "C" int ds3_hip_debug_mx_plan(uint32_t n_rows, uint32_t n_group, uint32_t N, uint32_t K, bool gate_up, int64_t *plan)
+{
+    const char *what = "debug_mx_plan";
+    if (!plan || n_rows == 0 || N == 0 || n_group > kMxMaxGroups || (gate_up && (n_group == 0 || N % 32 != 0)) ||
+        !mx_sizes_ok(what, { n_rows, N, K }) || !mx_cols_ok(what, "K", K))
+        return -1;
+    static const int32_t some = 0;
+    MxProduct p{};
+    p.offsets = n_group ? &some : nullptr;               // only whether there are any counts
+    p.n_rows = (int)n_rows;
+    p.n_group = n_group ? (int)n_group : 1;
+    p.N = (int)N;
+    p.K = (int)K;
+    const MxPlan f = mx_product_plan(p, gate_up);
+    const int64_t v[7] = { f.kernel, f.waves, f.rows, f.outputs, f.tiles, f.span, f.beside };
+    memcpy(plan, v, sizeof v);
+    return 0;
+}
+
 extern "C" int ds3_hip_moe_combine(const ds3_hip_buffer_t *y, const ds3_hip_buffer_t *slot_pos,
                                    const ds3_hip_buffer_t *scores, ds3_hip_buffer_t *out, uint32_t n_tokens,
                                    uint32_t n_used, uint32_t n_rows, uint32_t n_cols, bool accumulate)

@@ -291,4 +291,13 @@ struct MxProduct {
 };
 hipError_t launch_mx_product(const MxProduct &p, hipStream_t s);
 
+// What launch_mx_product takes for these sizes (pointers but for offsets null or
+// not do not count).  kernel: 0 k_mx_few, 1 k_mx_tile.
+struct MxPlan {
+    int kernel, waves, rows, outputs;   // waves and rows of x a workgroup, output columns a tile
+    int beside;                         // k_mx_tile's transposition
+    int64_t tiles, span;                // tiles of output columns, and of them a workgroup's
+};
+MxPlan mx_product_plan(const MxProduct &p, bool gate_up);
+
 }  // namespace ds3k

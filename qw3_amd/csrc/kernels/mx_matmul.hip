@@ -614,12 +614,12 @@ static int tile_lds(const MxProduct &p, int mt)
 // faster: 128 against 131 us for those 16384 rows, 32 a workgroup, 144 against 135 for groups of equal
 // sizes, 62 against 57 for 8000 rows, K = 768.  Nor were two halves of the columns for
 // the waves that have no tile: 512 x 4096 15.9 us with and without.)
-struct Plan {
+struct Span {
     int64_t span, cost;         // the cost in 1/20 of a tile of 32 rows
 };
 
 template <int WAVES, int NT, int MT, bool GU>
-static Plan tile_plan(const MxProduct &p)
+static Span tile_span(const MxProduct &p)
 {
     constexpr int OUT = GU ? 8 * NT : 16 * NT;
     // workgroups a CU holds: eight waves' registers
@@ -627,7 +627,7 @@ static Plan tile_plan(const MxProduct &p)
     const int64_t tiles = ((int64_t)p.N + OUT - 1) / OUT, rows = usual_tiles(p, 16 * MT);
     // (48 rows: the split takes half as long again, a tile a tenth)
     const int64_t split = (at_once == CUS ? 6 : 4) * (MT == 3 ? 30 : 20), tile = MT == 3 ? 22 : 20;
-    Plan best{ tiles, INT64_MAX };
+    Span best{ tiles, INT64_MAX };
     // by the number q of tiles a SIMD, the shortest span of each number of parts
     for (int64_t q = (tiles + 3) / 4; q > 0; q--) {
         const int64_t parts = (tiles + 4 * q - 1) / (4 * q);
@@ -645,28 +645,23 @@ static Plan tile_plan(const MxProduct &p)
 }
 
 template <int WAVES, int NT, int MT, int LEAD, bool GU>
-static hipError_t launch_tile(const MxProduct &p, hipStream_t s)
+static hipError_t launch_tile(const MxProduct &p, const MxPlan &plan, hipStream_t s)
 {
-    constexpr int BM = 16 * MT, OUT = GU ? 8 * NT : 16 * NT;
     const int lds = tile_lds(p, MT);
     if (lds > LDS_BYTES) return hipErrorInvalidValue;
-    // Whether every SIMD has two waves with a tile each (K = 2048: 512 x 4096, 1024 tiles,
-    // 16.9 us with the transposition for that, 16.0 without; 768 x 4096, 1536 tiles, 19.25,
-    // 18.9; 1024 x 4096, 2048 tiles, 20.15, 20.5).
-    const bool beside = usual_tiles(p, BM) * (((int64_t)p.N + OUT - 1) / OUT) >= 8 * CUS;
-    const auto kernel = beside ? k_mx_tile<WAVES, NT, MT, LEAD, GU, true> : k_mx_tile<WAVES, NT, MT, LEAD, GU, false>;
+    const auto kernel = plan.beside ? k_mx_tile<WAVES, NT, MT, LEAD, GU, true> : k_mx_tile<WAVES, NT, MT, LEAD, GU, false>;
     if (lds > 64 * 1024) {
         const hipError_t e =
             hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
         if (e != hipSuccess) return e;
     }
-    const int64_t span = tile_plan<WAVES, NT, MT, GU>(p).span;
     uint32_t n_jobs, n_tiles;
-    if (!count_jobs(p, BM, OUT * span, n_jobs, n_tiles)) return hipErrorInvalidValue;
+    if (!count_jobs(p, 16 * MT, plan.outputs * plan.span, n_jobs, n_tiles)) return hipErrorInvalidValue;
     const uint32_t items = n_jobs / n_tiles;
     const int spread = items >= 32 ? 1 : 0;
     if (spread) n_jobs = (items + 7) / 8 * 8 * n_tiles;          // row tiles past the last are empty
-    hipLaunchKernelGGL(kernel, job_grid(n_jobs), dim3(WAVES * WAVE), (size_t)lds, s, p, n_jobs, n_tiles, (int)span, spread);
+    hipLaunchKernelGGL(kernel, job_grid(n_jobs), dim3(WAVES * WAVE), (size_t)lds, s, p, n_jobs, n_tiles, (int)plan.span,
+                       spread);
     return hipGetLastError();
 }
 
@@ -677,6 +672,25 @@ static hipError_t launch_few(const MxProduct &p, hipStream_t s)
     if (!count_jobs(p, 16, GU ? 32 : 16 * NT, n_jobs, n_tiles)) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_mx_few<WAVES, NT, GU>), job_grid(n_jobs), dim3(WAVES * WAVE), 0, s, p, n_jobs, n_tiles);
     return hipGetLastError();
+}
+
+template <int WAVES, int NT, bool GU>
+static MxPlan few_of(const MxProduct &p)
+{
+    const int64_t outputs = GU ? 32 : 16 * NT;
+    return { 0, WAVES, 16, (int)outputs, 0, ((int64_t)p.N + outputs - 1) / outputs, 1 };
+}
+
+template <int WAVES, int NT, int MT, bool GU>
+static MxPlan tile_of(const MxProduct &p)
+{
+    constexpr int64_t outputs = GU ? 8 * NT : 16 * NT;
+    const int64_t tiles = ((int64_t)p.N + outputs - 1) / outputs;
+    // Whether every SIMD has two waves with a tile each (K = 2048: 512 x 4096, 1024 tiles,
+    // 16.9 us with the transposition for that, 16.0 without; 768 x 4096, 1536 tiles, 19.25,
+    // 18.9; 1024 x 4096, 2048 tiles, 20.15, 20.5).
+    const int beside = usual_tiles(p, 16 * MT) * tiles >= 8 * CUS;
+    return { 1, WAVES, 16 * MT, (int)outputs, beside, tiles, tile_span<WAVES, NT, MT, GU>(p).span };
 }
 
 // The variant, by the number of 16 x 64 blocks of products and the rows a group.
@@ -703,29 +717,45 @@ static hipError_t launch_few(const MxProduct &p, hipStream_t s)
 //    41.2); for 32 rows of groups of unequal sizes, 16000 rows in 128 groups x 2048, K =
 //    768: 98 against 108 (2048 rows of one matrix: 15.1 against 13.6).
 template <bool GU>
-static hipError_t launch_product(const MxProduct &p, hipStream_t s)
+static MxPlan product_plan(const MxProduct &p)
 {
     const int64_t blocks = usual_tiles(p, 16) * (((int64_t)p.N * (GU ? 2 : 1) + 63) / 64);
     if (blocks < 512 || p.n_rows <= (p.offsets ? p.n_group : 8) || tile_lds(p, 1) > LDS_BYTES) {
-        if constexpr (GU) return blocks < 512 ? launch_few<4, 4, true>(p, s) : launch_few<2, 4, true>(p, s);
-        else if (blocks < 128) return launch_few<4, 1, false>(p, s);
-        else if (blocks < (p.K > 1024 ? 512 : 256)) return launch_few<4, 2, false>(p, s);
-        else return launch_few<2, 4, false>(p, s);
+        if constexpr (GU) return blocks < 512 ? few_of<4, 4, true>(p) : few_of<2, 4, true>(p);
+        else if (blocks < 128) return few_of<4, 1, false>(p);
+        else if (blocks < (p.K > 1024 ? 512 : 256)) return few_of<4, 2, false>(p);
+        else return few_of<2, 4, false>(p);
     }
     const bool wide = p.offsets ? (int64_t)p.n_rows >= 16 * (int64_t)p.n_group : blocks >= 2048;
     if (wide && tile_lds(p, 2) <= LDS_BYTES) {
         if (p.offsets && 2 * tile_lds(p, 2) <= LDS_BYTES) {
-            if (2 * tile_lds(p, 3) <= LDS_BYTES && tile_plan<4, 4, 3, GU>(p).cost < tile_plan<4, 4, 2, GU>(p).cost)
-                return launch_tile<4, 4, 3, 0, GU>(p, s);
-            return launch_tile<4, 4, 2, 2, GU>(p, s);
+            if (2 * tile_lds(p, 3) <= LDS_BYTES && tile_span<4, 4, 3, GU>(p).cost < tile_span<4, 4, 2, GU>(p).cost)
+                return tile_of<4, 4, 3, GU>(p);
+            return tile_of<4, 4, 2, GU>(p);
         }
-        if (tile_lds(p, 3) <= LDS_BYTES && tile_plan<8, 4, 3, GU>(p).cost < tile_plan<8, 4, 2, GU>(p).cost)
-            return launch_tile<8, 4, 3, 0, GU>(p, s);
-        return launch_tile<8, 4, 2, 2, GU>(p, s);
+        if (tile_lds(p, 3) <= LDS_BYTES && tile_span<8, 4, 3, GU>(p).cost < tile_span<8, 4, 2, GU>(p).cost)
+            return tile_of<8, 4, 3, GU>(p);
+        return tile_of<8, 4, 2, GU>(p);
     }
-    if (2 * tile_lds(p, 1) <= LDS_BYTES) return launch_tile<4, 4, 1, 4, GU>(p, s);
-    return launch_tile<8, 4, 1, 4, GU>(p, s);
+    if (2 * tile_lds(p, 1) <= LDS_BYTES) return tile_of<4, 4, 1, GU>(p);
+    return tile_of<8, 4, 1, GU>(p);
 }
+
+template <bool GU>
+static hipError_t launch_product(const MxProduct &p, hipStream_t s)
+{
+    const MxPlan f = product_plan<GU>(p);
+    if (f.kernel == 0) {
+        if constexpr (GU) return f.waves == 4 ? launch_few<4, 4, true>(p, s) : launch_few<2, 4, true>(p, s);
+        else if (f.waves == 2) return launch_few<2, 4, false>(p, s);
+        else return f.outputs == 16 ? launch_few<4, 1, false>(p, s) : launch_few<4, 2, false>(p, s);
+    }
+    if (f.rows == 48) return f.waves == 4 ? launch_tile<4, 4, 3, 0, GU>(p, f, s) : launch_tile<8, 4, 3, 0, GU>(p, f, s);
+    if (f.rows == 32) return f.waves == 4 ? launch_tile<4, 4, 2, 2, GU>(p, f, s) : launch_tile<8, 4, 2, 2, GU>(p, f, s);
+    return f.waves == 4 ? launch_tile<4, 4, 1, 4, GU>(p, f, s) : launch_tile<8, 4, 1, 4, GU>(p, f, s);
+}
+
+MxPlan mx_product_plan(const MxProduct &p, bool gate_up) { return gate_up ? product_plan<true>(p) : product_plan<false>(p); }
 
 hipError_t launch_mx_product(const MxProduct &p0, hipStream_t s)
 {

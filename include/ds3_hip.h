@@ -338,8 +338,9 @@ int ds3_hip_mx_quantize(const ds3_hip_buffer_t *src, ds3_hip_type_t src_type, ui
                         ds3_hip_buffer_t *codes, ds3_hip_buffer_t *scales, ds3_hip_type_t mx_type,
                         uint32_t n_rows, uint32_t n_cols);
 
-/* The values of a microscaled matrix, to F32 (exact) or F16 (rounded once)
- * rows without gaps. */
+/* The values of a microscaled matrix, to F32 or F16 rows without gaps: exact in
+ * F32 but for magnitudes of 2^128 and more (scale 254 only), which become
+ * infinite, and rounded once to F16. */
 int ds3_hip_mx_dequantize(const ds3_hip_buffer_t *codes, const ds3_hip_buffer_t *scales, ds3_hip_type_t mx_type,
                           uint32_t n_rows, uint32_t n_cols, ds3_hip_buffer_t *dst, ds3_hip_type_t dst_type);
 
@@ -356,8 +357,8 @@ int ds3_hip_add_rms_norm_mx(const ds3_hip_buffer_t *x, const ds3_hip_buffer_t *d
 
 /* C[M][N] = X[M][K] . W[N][K]^T in fp32 of MXINT8 rows and MXFP4 weights.
  * Every product is exact and summed in fp32; the order of a sum depends on
- * the sizes alone.  Rows of x whose scale is below 2^-122 are first rounded to
- * multiples of 2^-128. */
+ * the sizes alone.  Blocks of x whose scale is below 2^-122 are the exception:
+ * their values are first rounded to multiples of 2^-128. */
 int ds3_hip_matmul_mx(const ds3_hip_buffer_t *x_codes, const ds3_hip_buffer_t *x_scales,
                       const ds3_hip_buffer_t *w_codes, const ds3_hip_buffer_t *w_scales, ds3_hip_buffer_t *C,
                       uint32_t M, uint32_t N, uint32_t K);
@@ -394,7 +395,8 @@ int ds3_hip_moe_combine(const ds3_hip_buffer_t *y, const ds3_hip_buffer_t *slot_
                         bool accumulate);
 
 /* ds3_hip_moe_block with microscaled experts, in place: hidden[t] += delta[t]
- * (delta may be NULL), then hidden[t] += MoE(rms_norm(hidden[t]) * ffn_norm).
+ * (delta may be NULL), then hidden[t] += MoE(rms_norm(s[t]) * ffn_norm), s the sum
+ * before its rounding, as in ds3_hip_add_rms_norm_mx.
  * The experts are MXFP4 matrices: gate and up [n_expert * n_ff_exp][n_embd], down
  * [n_expert * n_embd][n_ff_exp]; the router reads the normalised rows in f32,
  * the experts the same rows in MXINT8, and h is rounded to MXINT8.  gate_logits /

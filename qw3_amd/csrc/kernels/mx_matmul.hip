@@ -315,11 +315,11 @@ __global__ void __launch_bounds__(WAVES * WAVE, NT == 4 ? 2 : 3) k_mx_few(MxProd
 // barrier: its weights go from memory to its registers a chunk of 512 columns
 // ahead, over the end of a tile into its next one.  Two waves a SIMD.
 //
-// 16384 rows in 128 groups of 768 x 2 outputs, K = 2048: 115 us, 0.9 PFLOP/s; the
-// vector units are busy 62 % of the waves' time (a third of that the exchange of the
+// 16384 rows in 128 groups of 768 x 2 outputs, K = 2048: 116 us, 0.9 PFLOP/s; the
+// vector units are busy 60 % of the waves' time (a third of that the exchange of the
 // weights between lanes, a quarter the epilogue, as much the split of x), the
 // matrix cores 33 %.  296 rows in those groups: 43 us, memory at 4.4 TB/s.  512 x
-// 4096: 15 us, of which 4.4 the split of x and 5 the launch and the last stores.
+// 4096: 15.3 us, of which 4.4 the split of x and 5 the launch and the last stores.
 // ---------------------------------------------------------------------------
 constexpr int FRAG_LO = 0, FRAG_HI = 1024, FRAG_HI2 = 2048, FRAG_SC = 2560, FRAG_BYTES = 2688;
 // 32 bytes between the steps' fragments: the four lanes that write a row's
@@ -701,7 +701,9 @@ static MxPlan tile_of(const MxProduct &p)
 //    rows to split, at most one a group: 128 rows in 128 groups of 768 x 2 outputs 32.0
 //    against 39, K = 768 and 2048 outputs 17.9 against 18.6 (with two a group 23.8
 //    against 21.3); or eight rows of one matrix: one of 65536 outputs, K = 768, 7.8
-//    against 10.7, K = 4096, 27.6 against 34, eight 30.3 against 34.4;
+//    against 10.7, K = 4096, 27.6 against 34, eight 30.3 against 34.4; nor do digits of
+//    16 rows fit the LDS above K = 7680 (4096 outputs of 64 rows 19.5 us at 7680, 20.4 at
+//    8192, of 512 rows 46.8 and 91.4, of 2048 rows 127 and 282);
 //  - in it, one block of weight rows a workgroup below 128 blocks (64 blocks 5.1, two
 //    5.3; 128 blocks 6.5 against 5.6), two below 512 and four waves (64 x 4096: 7.1,
 //    with four by two waves 8.4), or with the two chunks of K = 768 below 256 (128 x

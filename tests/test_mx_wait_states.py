@@ -47,9 +47,7 @@ class Instruction:
         self.states = int(args[0], 0) + 1 if self.op == "s_nop" else 1
         self.branch = args[0] if self.op.startswith(("s_branch", "s_cbranch")) else None
         self.ends = self.op in ("s_branch", "s_endpgm", "s_setpc_b64")
-        n_out = 2 if "_co_" in self.op or self.op.startswith(("v_div_scale", "v_swap")) else 1
-        if self.op.startswith("v_cmp") and self.op.endswith("_e32"):
-            n_out = 1                                    # vcc, named in the listing
+        n_out = 2 if "_co_" in self.op or self.op.startswith(("v_div_scale", "v_swap", "v_mad_u64", "v_mad_i64")) else 1
         if not self.valu or self.op == "v_nop":
             self.writes, self.reads, self.dpp_reads, self.c_reads = set(), set(), set(), set()
             return

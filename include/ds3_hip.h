@@ -413,6 +413,136 @@ int ds3_hip_moe_block_mx(ds3_hip_buffer_t *hidden, const ds3_hip_buffer_t *delta
                          uint32_t n_tokens, uint32_t n_embd, uint32_t n_expert, uint32_t n_used, uint32_t n_ff_exp,
                          uint64_t router_row_stride, ds3_hip_type_t router_type, bool norm_topk_prob);
 
+/* Attention and sampling operators (no ds3_metal.h counterpart): what lies
+ * between a layer's q / k / v products and its output product, and between the
+ * output head and the next token.
+ *
+ * A paged cache of one layer is two F16 buffers, k and v, each
+ * [n_blocks][n_head_kv][block_size][head_dim]; block_size is a power of two.  A
+ * slot is block * block_size + row of the block.  Request i's block_table row
+ * ([max_blocks] int32) names the blocks of its positions in order.  The tokens of
+ * a call lie request after request: rows q_offsets[i] .. q_offsets[i + 1] - 1 of
+ * n_seq + 1 int32 belong to request i; rows from q_offsets[n_seq] on belong to none.
+ * What device buffers hold cannot be refused by the host: slots and block ids
+ * outside the cache are passed over (not written, not read), and each entry point
+ * says what other values do.
+ * Buffers: int32 and F32 ones start on multiples of 4 bytes, heads and caches on
+ * multiples of 16 (of 8 where they hold fewer than 16 bytes a head half). */
+
+/* Angles of rotary positions, computed on the host in 64 bits and written to
+ * `table` (rotary_dim / 2 + 1 doubles): pair i turns by position * f(theta_i),
+ * theta_i = base^(-2 i / rotary_dim).  With r_i = original_ctx * theta_i / (2 pi),
+ * the turns of pair i over the trained context:
+ *   PLAIN       f = theta
+ *   LINEAR      f = theta / factor
+ *   WAVELENGTH  f = theta * (s + (1 - s) / factor), s = (r - low) / (high - low)
+ *               held to 0 .. 1
+ *   YARN        f = theta * (1 - s + s / factor), s = (i - a) / (b - a) held to
+ *               0 .. 1, a and b the pair indices (rounded down and up, held to 0 ..
+ *               rotary_dim - 1) at which r is `high` and `low`; rotated values are
+ *               scaled by 0.1 ln(factor) + 1 where factor > 1.
+ * rotary_dim is even, up to 512.  Not allowed during graph capture. */
+#define DS3_HIP_ROPE_PLAIN      0
+#define DS3_HIP_ROPE_LINEAR     1
+#define DS3_HIP_ROPE_WAVELENGTH 2
+#define DS3_HIP_ROPE_YARN       3
+int ds3_hip_rope_table(ds3_hip_buffer_t *table, uint32_t rotary_dim, double base, int32_t scaling, double factor,
+                       double low, double high, uint32_t original_ctx);
+
+/* out = x rotated by its tokens' positions (int32, any value).  A row of x holds
+ * n_head heads of head_dim values (F32 or F16), rows x_row_stride bytes apart; out
+ * likewise.  With norm (F32 [head_dim]) each head is first x * rsqrt(mean(x^2) +
+ * eps) * norm, in F32.  The first rotary_dim values of a head turn: value i with
+ * value i + rotary_dim / 2, or interleaved, 2 i with 2 i + 1; the rest are copied
+ * (normalised).  Angles are reduced in 64 bits.  out may be x itself (one type,
+ * one stride).  head_dim is a multiple of 8 up to 512, rotary_dim even. */
+int ds3_hip_rope(const ds3_hip_buffer_t *x, ds3_hip_type_t x_type, uint64_t x_row_stride,
+                 const ds3_hip_buffer_t *positions, const ds3_hip_buffer_t *table, const ds3_hip_buffer_t *norm,
+                 float eps, ds3_hip_buffer_t *out, ds3_hip_type_t out_type, uint64_t out_row_stride, uint32_t n_tokens,
+                 uint32_t n_head, uint32_t head_dim, uint32_t rotary_dim, bool interleaved);
+
+/* New tokens of a layer in one launch: q_out = q and the cache's k rows = k, both
+ * normalised (q_norm, k_norm, optional) and rotated as in ds3_hip_rope, and the
+ * cache's v rows = v, k and v at slots[t] (int32; a slot outside the cache: the
+ * row is not written).  q, k, v are rows of `type`, their strides in bytes (of one
+ * packed buffer: views); q_out is dense.  table may be NULL: no rotation,
+ * positions (then unused) may be NULL too.  q and q_out may be NULL: k and v only.
+ * The slots of a call differ; of rows with one slot it is not defined which is
+ * kept.  Values beyond F16's range become infinite in the cache. */
+int ds3_hip_rope_append(const ds3_hip_buffer_t *q, const ds3_hip_buffer_t *k, const ds3_hip_buffer_t *v,
+                        ds3_hip_type_t type, uint64_t q_row_stride, uint64_t k_row_stride, uint64_t v_row_stride,
+                        const ds3_hip_buffer_t *positions, const ds3_hip_buffer_t *slots,
+                        const ds3_hip_buffer_t *table, const ds3_hip_buffer_t *q_norm, const ds3_hip_buffer_t *k_norm,
+                        float eps, ds3_hip_buffer_t *q_out, ds3_hip_type_t q_out_type, ds3_hip_buffer_t *k_cache,
+                        ds3_hip_buffer_t *v_cache, uint32_t n_tokens, uint32_t n_head, uint32_t n_head_kv,
+                        uint32_t head_dim, uint32_t rotary_dim, bool interleaved, uint32_t n_blocks,
+                        uint32_t block_size);
+
+/* The step's plan from lengths on the device: request i has kv_lens[i] tokens in
+ * the cache and new_lens[i] to come (below 0: none).  Its table row gets the blocks
+ * that it lacks, taken from the end of free_blocks[0 .. n_free - 1] in the order of
+ * requests (the r-th block taken is free_blocks[n_free - 1 - r]).  Written:
+ *   kv_lens_out[i] = kv_lens[i] + new_lens[i], n_free_out (kv_lens and n_free
+ *   themselves, or buffers of their own), q_offsets[n_seq + 1], and for each of
+ *   max_tokens rows its position and slot (rows of no request: 0 and -1).
+ *   status[4] = { new tokens, blocks taken, blocks lacking, requests longer than
+ *   max_blocks blocks }.
+ * A plan that lacks blocks, has such a request or more than max_tokens tokens is
+ * not carried out: lengths, table and n_free stay, every offset is 0, every slot
+ * -1.  Each of them is then safe to run the layer's calls on, which do nothing.
+ * free_blocks holds n_blocks entries; n_free is held to 0 .. n_blocks. */
+int ds3_hip_kv_plan(const ds3_hip_buffer_t *new_lens, const ds3_hip_buffer_t *kv_lens, ds3_hip_buffer_t *kv_lens_out,
+                    ds3_hip_buffer_t *block_table, const ds3_hip_buffer_t *free_blocks, const ds3_hip_buffer_t *n_free,
+                    ds3_hip_buffer_t *n_free_out, ds3_hip_buffer_t *q_offsets, ds3_hip_buffer_t *positions,
+                    ds3_hip_buffer_t *slots, ds3_hip_buffer_t *status, uint32_t n_seq, uint32_t max_blocks,
+                    uint32_t n_blocks, uint32_t block_size, uint32_t max_tokens);
+
+/* Requests with done[i] != 0 give their blocks back: the table entries of their
+ * kv_lens[i] tokens go to the end of free_blocks, in the order of requests and
+ * positions, n_free grows by their number and kv_lens[i] becomes 0.  Blocks that do
+ * not fit (more than n_blocks in all: one was given back twice): nothing changes. */
+int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t *kv_lens, const ds3_hip_buffer_t *block_table,
+                       ds3_hip_buffer_t *free_blocks, ds3_hip_buffer_t *n_free, uint32_t n_seq, uint32_t max_blocks,
+                       uint32_t n_blocks, uint32_t block_size);
+
+/* Attention of new tokens over the paged cache, which holds their own k and v
+ * already: token j of request i's m new ones is at position p = kv_lens[i] - m + j
+ * and sees positions 0 .. p, or with window != 0 the last `window` of those.
+ * out = softmax(scale * q . k) . v by head; q head h reads kv head h / (n_head /
+ * n_head_kv).  A token that sees nothing gets zeros: one at a position below 0, or
+ * whose blocks all lie outside the cache.  Rows of out that belong to no request
+ * are left as they were.  q and out are of `type`, rows of n_head heads.
+ *   F32: products to 22 bits of q and of the softmax's weights (two F16 parts each),
+ *        against the cache's exact F16 values
+ *   F16: q as it is, the softmax's weights rounded to F16
+ * Sums and the softmax are F32.  head_dim is a multiple of 8 up to 256.
+ * It uses the library's workspace: before a capture the call is made once. */
+int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint64_t q_row_stride,
+                            const ds3_hip_buffer_t *k_cache, const ds3_hip_buffer_t *v_cache,
+                            const ds3_hip_buffer_t *block_table, const ds3_hip_buffer_t *q_offsets,
+                            const ds3_hip_buffer_t *kv_lens, ds3_hip_buffer_t *out, uint64_t out_row_stride,
+                            uint32_t n_tokens, uint32_t n_seq, uint32_t n_head, uint32_t n_head_kv, uint32_t head_dim,
+                            uint32_t n_blocks, uint32_t block_size, uint32_t max_blocks, float scale, uint32_t window);
+
+/* One token a row from logits (F32 [n_rows][n_vocab], rows row_stride bytes apart)
+ * and given random numbers: uniform[r] in 0 <= u < 1 (others are held to it).  The
+ * row's tokens are ordered by logit, equal ones by index; NaN counts as -inf.
+ * Weights are exp((x - largest) / temperature).  Kept are
+ *   the first top_k tokens (0 or less: all), of those
+ *   the shortest run whose weights reach top_p of theirs (1 or more, NaN: all), of those
+ *   the ones of at least min_p times the first's weight (0 or less, NaN: all),
+ * always the first one.  Drawn is the first kept token in that order at which the summed
+ * weights pass u times all kept ones'.  probs[r] (optional) is its share of them.
+ * temperature 0 or less, or a logit of +inf: the first token, share 1.  A row of nothing but
+ * -inf and NaN: token -1, share 0.  The settings are one F32 (top_k: int32) a row;
+ * NULL: temperature 1, all tokens.
+ * Weights are summed as whole numbers of 2^-44 of the first's, so a token does not
+ * depend on the order of sums.  n_vocab is at most 2^18. */
+int ds3_hip_sample(const ds3_hip_buffer_t *logits, uint64_t row_stride, const ds3_hip_buffer_t *uniform,
+                   const ds3_hip_buffer_t *temperature, const ds3_hip_buffer_t *top_k, const ds3_hip_buffer_t *top_p,
+                   const ds3_hip_buffer_t *min_p, ds3_hip_buffer_t *tokens, ds3_hip_buffer_t *probs, uint32_t n_rows,
+                   uint32_t n_vocab);
+
 /* Router selection.  0 (default): the certified router (fp64 wavefront sums
  * with a proven error bound, exact sequential sums only where the bound
  * cannot certify the top-k order) in ds3_hip_moe_ffn and, up to 16 tokens,

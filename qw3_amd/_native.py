@@ -81,6 +81,15 @@ SIGNATURES: dict[str, tuple] = {
     "ds3_hip_moe_gate_up_mx": (C.c_int, [P, P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32]),
     "ds3_hip_moe_combine": (C.c_int, [P, P, P, P, U32, U32, U32, U32, B]),
     "ds3_hip_moe_block_mx": (C.c_int, [P, P, P, F, P, P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32, U64, I32, B]),
+    "ds3_hip_rope_table": (C.c_int, [P, U32, D, I32, D, D, D, U32]),
+    "ds3_hip_rope": (C.c_int, [P, I32, U64, P, P, P, F, P, I32, U64, U32, U32, U32, U32, B]),
+    "ds3_hip_rope_append": (C.c_int, [P, P, P, I32, U64, U64, U64, P, P, P, P, P, F, P, I32, P, P, U32, U32, U32, U32,
+                                      U32, B, U32, U32]),
+    "ds3_hip_kv_plan": (C.c_int, [P, P, P, P, P, P, P, P, P, P, P, U32, U32, U32, U32, U32]),
+    "ds3_hip_kv_release": (C.c_int, [P, P, P, P, P, U32, U32, U32, U32]),
+    "ds3_hip_attention_paged": (C.c_int, [P, I32, U64, P, P, P, P, P, P, U64, U32, U32, U32, U32, U32, U32, U32, U32, F,
+                                          U32]),
+    "ds3_hip_sample": (C.c_int, [P, U64, P, P, P, P, P, P, P, U32, U32]),
     "ds3_hip_set_router_mode": (C.c_int, [C.c_int]),
     "ds3_hip_router_stats": (C.c_int, [C.POINTER(U64), C.POINTER(U64), C.c_int]),
     "ds3_hip_debug_grouped_lists": (C.c_int, [P, P, P, P, P, P, P, P, P]),

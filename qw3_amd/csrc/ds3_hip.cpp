@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -2468,4 +2469,401 @@ extern "C" int ds3_hip_moe_block_mx(
         if (e != hipSuccess) return report(e, what);
     }
     return finish(hipSuccess, what);
+}
+
+// ===========================================================================
+// Attention and sampling operators (no reference counterpart)
+// ===========================================================================
+
+namespace {
+
+bool size_in(const char *what, const char *name, uint64_t v, uint64_t lo, uint64_t hi)
+{
+    if (v >= lo && v <= hi) return true;
+    fprintf(stderr, "ds3_hip: %s: %s=%llu is not in %llu .. %llu\n", what, name, (unsigned long long)v,
+            (unsigned long long)lo, (unsigned long long)hi);
+    return false;
+}
+
+bool float_type_ok(const char *what, int type)
+{
+    if (type == T_F32 || type == T_F16) return true;
+    fprintf(stderr, "ds3_hip: %s: type %d is neither F32 nor F16\n", what, type);
+    return false;
+}
+
+// A cache of n_blocks blocks of block_size rows: a power of two, its slots int32.
+bool pages_ok(const char *what, uint32_t n_blocks, uint32_t block_size, int *log_block)
+{
+    if (block_size == 0 || (block_size & (block_size - 1)) != 0 || block_size > 1u << 16) {
+        fprintf(stderr, "ds3_hip: %s: block_size=%u is no power of two up to 65536\n", what, block_size);
+        return false;
+    }
+    *log_block = __builtin_ctz(block_size);
+    return size_in(what, "n_blocks", n_blocks, 1, 0x7fffffffu >> *log_block);
+}
+
+// Rows of n_head heads `stride` bytes apart: *span gets their bytes.
+bool heads_ok(const char *what, const char *name, const ds3_hip_buffer_t *b, int type, uint64_t stride, uint64_t rows,
+              uint64_t n_head, uint64_t head_dim, size_t *span)
+{
+    const uint64_t row = n_head * head_dim * (type == T_F32 ? 4 : 2);
+    if (stride < row || stride % 16 != 0 || stride > (uint64_t)1 << 31) {
+        fprintf(stderr, "ds3_hip: %s: rows of %s %llu bytes apart: at least one row (%llu bytes), a multiple of 16\n", what,
+                name, (unsigned long long)stride, (unsigned long long)row);
+        return false;
+    }
+    *span = (size_t)span_bytes(rows, stride, row);
+    return fits(b, *span, name) && aligned_to(b, 16, what, name);
+}
+
+bool ints_ok(const char *what, std::initializer_list<Span> bufs)
+{
+    for (const Span &s : bufs)
+        if (!fits(s.buf, s.bytes, s.name) || !aligned_to(s.buf, 4, what, s.name)) return false;
+    return true;
+}
+
+// Heads that q rows of 2^31 bytes hold, kv heads that divide them.
+bool head_counts_ok(const char *what, uint32_t n_head, uint32_t n_head_kv, uint32_t head_dim, uint32_t most_dim)
+{
+    if (!size_in(what, "head_dim", head_dim, 8, most_dim) || !size_in(what, "n_head", n_head, 1, 1u << 16) ||
+        !size_in(what, "n_head_kv", n_head_kv, 1, n_head))
+        return false;
+    if (head_dim % 8 != 0 || n_head % n_head_kv != 0) {
+        fprintf(stderr, "ds3_hip: %s: head_dim=%u must be a multiple of 8, n_head=%u of n_head_kv=%u\n", what, head_dim,
+                n_head, n_head_kv);
+        return false;
+    }
+    return true;
+}
+
+bool rotary_ok(const char *what, uint32_t rotary_dim, uint32_t most)
+{
+    if (rotary_dim != 0 && rotary_dim % 2 == 0 && rotary_dim <= most) return true;
+    fprintf(stderr, "ds3_hip: %s: rotary_dim=%u must be even, 2 .. %u\n", what, rotary_dim, most);
+    return false;
+}
+
+}  // namespace
+
+extern "C" int ds3_hip_rope_table(ds3_hip_buffer_t *table, uint32_t rotary_dim, double base, int32_t scaling,
+                                  double factor, double low, double high, uint32_t original_ctx)
+{
+    const char *what = "rope_table";
+    if (!table) return -1;
+    if (!rotary_ok(what, rotary_dim, 512)) return -1;
+    const bool ramp = scaling == DS3_HIP_ROPE_WAVELENGTH || scaling == DS3_HIP_ROPE_YARN;
+    if (scaling < DS3_HIP_ROPE_PLAIN || scaling > DS3_HIP_ROPE_YARN || !(base > 1.0) || !std::isfinite(base) ||
+        (scaling != DS3_HIP_ROPE_PLAIN && (!(factor > 0.0) || !std::isfinite(factor))) ||
+        (ramp && (!(low > 0.0) || !(high > low) || !std::isfinite(high) || original_ctx == 0))) {
+        fprintf(stderr, "ds3_hip: %s: scaling %d with base %g, factor %g, low %g, high %g, original_ctx %u unsupported\n",
+                what, scaling, base, factor, low, high, original_ctx);
+        return -1;
+    }
+    const uint32_t pairs = rotary_dim / 2;
+    const size_t bytes = ((size_t)pairs + 1) * 8;
+    if (!fits(table, bytes, "table") || !aligned_to(table, 8, what, "table") ||
+        !writable(what, { { table, bytes, "table" } }) || refuse_in_capture(what) || !ensure_init())
+        return -1;
+    const double two_pi = 6.283185307179586476925286766559;
+    double v[257], a = 0.0, b = 0.0;
+    if (scaling == DS3_HIP_ROPE_YARN) {
+        const auto pair = [&](double turns) {
+            return rotary_dim * std::log(original_ctx / (turns * two_pi)) / (2.0 * std::log(base));
+        };
+        a = std::max(std::floor(pair(high)), 0.0);
+        b = std::min(std::ceil(pair(low)), (double)rotary_dim - 1.0);
+    }
+    for (uint32_t i = 0; i < pairs; i++) {
+        const double theta = std::pow(base, -2.0 * i / rotary_dim);
+        double f = theta;
+        if (scaling == DS3_HIP_ROPE_LINEAR) f = theta / factor;
+        else if (scaling == DS3_HIP_ROPE_WAVELENGTH) {
+            const double s = std::clamp((original_ctx * theta / two_pi - low) / (high - low), 0.0, 1.0);
+            f = theta * (s + (1.0 - s) / factor);
+        } else if (scaling == DS3_HIP_ROPE_YARN) {
+            const double s = std::clamp((i - a) / std::max(b - a, 0.001), 0.0, 1.0);
+            f = theta * (1.0 - s + s / factor);
+        }
+        v[i] = f / two_pi;
+    }
+    v[pairs] = scaling == DS3_HIP_ROPE_YARN && factor > 1.0 ? 0.1 * std::log(factor) + 1.0 : 1.0;
+    return ds3_hip_buffer_write(table, 0, v, bytes);
+}
+
+extern "C" int ds3_hip_rope(const ds3_hip_buffer_t *x, ds3_hip_type_t x_type, uint64_t x_row_stride,
+                            const ds3_hip_buffer_t *positions, const ds3_hip_buffer_t *table,
+                            const ds3_hip_buffer_t *norm, float eps, ds3_hip_buffer_t *out, ds3_hip_type_t out_type,
+                            uint64_t out_row_stride, uint32_t n_tokens, uint32_t n_head, uint32_t head_dim,
+                            uint32_t rotary_dim, bool interleaved)
+{
+    const char *what = "rope";
+    if (!x || !positions || !table || !out) return -1;
+    if (!float_type_ok(what, x_type) || !float_type_ok(what, out_type) || !head_counts_ok(what, n_head, 1, head_dim, 512) ||
+        !rotary_ok(what, rotary_dim, head_dim) || !mx_sizes_ok(what, { n_tokens }))
+        return -1;
+    if (n_tokens == 0) return 0;
+    const size_t p_b = (size_t)n_tokens * 4, t_b = ((size_t)rotary_dim / 2 + 1) * 8, w_b = (size_t)head_dim * 4;
+    size_t x_b, o_b;
+    if (!heads_ok(what, "x", x, x_type, x_row_stride, n_tokens, n_head, head_dim, &x_b) ||
+        !heads_ok(what, "out", out, out_type, out_row_stride, n_tokens, n_head, head_dim, &o_b) ||
+        !ints_ok(what, { { positions, p_b, "positions" }, { table, t_b, "table" }, { norm, w_b, "norm" } }) ||
+        !aligned_to(table, 8, what, "table") || !aligned_to(norm, 16, what, "norm"))
+        return -1;
+    const bool same = cptr(x) == cptr(out) && x_type == out_type && x_row_stride == out_row_stride;
+    if (!writable(what, { { out, o_b, "out" } }) ||
+        !apart(what, { { out, o_b, "out" } },
+               { { positions, p_b, "positions" }, { table, t_b, "table" }, { norm, w_b, "norm" },
+                 { same ? nullptr : x, x_b, "x" } }) ||
+        !ensure_init())
+        return -1;
+    RopeArgs p{};
+    p.x[0] = dptr(x);
+    p.stride[0] = x_row_stride;
+    p.positions = (const int32_t *)dptr(positions);
+    p.table = (const double *)dptr(table);
+    p.norm[0] = norm ? fptr(norm) : nullptr;
+    p.eps = eps;
+    p.out = dptr(out);
+    p.out_stride = out_row_stride;
+    p.n_tokens = n_tokens;
+    p.n_head = (int)n_head;
+    p.head_dim = (int)head_dim;
+    p.rotary = (int)rotary_dim;
+    KScope ks("rope");
+    return finish(launch_rope(p, x_type, out_type, interleaved, g.stream), what);
+}
+
+extern "C" int ds3_hip_rope_append(const ds3_hip_buffer_t *q, const ds3_hip_buffer_t *k, const ds3_hip_buffer_t *v,
+                                   ds3_hip_type_t type, uint64_t q_row_stride, uint64_t k_row_stride,
+                                   uint64_t v_row_stride, const ds3_hip_buffer_t *positions,
+                                   const ds3_hip_buffer_t *slots, const ds3_hip_buffer_t *table,
+                                   const ds3_hip_buffer_t *q_norm, const ds3_hip_buffer_t *k_norm, float eps,
+                                   ds3_hip_buffer_t *q_out, ds3_hip_type_t q_out_type, ds3_hip_buffer_t *k_cache,
+                                   ds3_hip_buffer_t *v_cache, uint32_t n_tokens, uint32_t n_head, uint32_t n_head_kv,
+                                   uint32_t head_dim, uint32_t rotary_dim, bool interleaved, uint32_t n_blocks,
+                                   uint32_t block_size)
+{
+    const char *what = "rope_append";
+    if (!k || !v || !slots || !k_cache || !v_cache || (table && !positions)) return -1;
+    if (!q != !q_out) {
+        fprintf(stderr, "ds3_hip: %s: q and q_out are given together or neither is\n", what);
+        return -1;
+    }
+    int log_block = 0;
+    if (!float_type_ok(what, type) || (q && !float_type_ok(what, q_out_type)) ||
+        !head_counts_ok(what, q ? n_head : n_head_kv, n_head_kv, head_dim, 512) ||
+        (table && !rotary_ok(what, rotary_dim, head_dim)) || !mx_sizes_ok(what, { n_tokens }) ||
+        !pages_ok(what, n_blocks, block_size, &log_block))
+        return -1;
+    if (n_tokens == 0) return 0;
+    const size_t i_b = (size_t)n_tokens * 4, t_b = table ? ((size_t)rotary_dim / 2 + 1) * 8 : 0, w_b = (size_t)head_dim * 4,
+                 c_b = (size_t)n_blocks * block_size * n_head_kv * head_dim * 2,
+                 o_row = (size_t)n_head * head_dim * (q_out_type == T_F32 ? 4 : 2);
+    size_t q_b = 0, k_b, v_b, o_b = 0;
+    if ((q && (!heads_ok(what, "q", q, type, q_row_stride, n_tokens, n_head, head_dim, &q_b) ||
+               !heads_ok(what, "q_out", q_out, q_out_type, o_row, n_tokens, n_head, head_dim, &o_b))) ||
+        !heads_ok(what, "k", k, type, k_row_stride, n_tokens, n_head_kv, head_dim, &k_b) ||
+        !heads_ok(what, "v", v, type, v_row_stride, n_tokens, n_head_kv, head_dim, &v_b) ||
+        !ints_ok(what, { { table ? positions : nullptr, i_b, "positions" }, { slots, i_b, "slots" }, { table, t_b, "table" },
+                         { q ? q_norm : nullptr, w_b, "q_norm" }, { k_norm, w_b, "k_norm" } }) ||
+        !aligned_to(table, 8, what, "table") || !aligned_to(q_norm, 16, what, "q_norm") ||
+        !aligned_to(k_norm, 16, what, "k_norm") || !fits(k_cache, c_b, "k_cache") || !fits(v_cache, c_b, "v_cache") ||
+        !aligned_to(k_cache, 16, what, "k_cache") || !aligned_to(v_cache, 16, what, "v_cache"))
+        return -1;
+    const Span oq = { q_out, o_b, "q_out" }, ok = { k_cache, c_b, "k_cache" }, ov = { v_cache, c_b, "v_cache" };
+    // (q_out may be q itself, row by row)
+    const bool same = q && cptr(q) == cptr(q_out) && type == q_out_type && q_row_stride == o_row;
+    if (!writable(what, { oq, ok, ov }) ||
+        !apart(what, { oq, ok, ov },
+               { { same ? nullptr : q, q_b, "q" }, { k, k_b, "k" }, { v, v_b, "v" }, { slots, i_b, "slots" },
+                 { table ? positions : nullptr, i_b, "positions" }, { table, t_b, "table" },
+                 { q ? q_norm : nullptr, w_b, "q_norm" }, { k_norm, w_b, "k_norm" } }) ||
+        (same && !apart(what, { ok, ov }, { { q, q_b, "q" } })) || !ensure_init())
+        return -1;
+    RopeArgs p{};
+    p.x[0] = dptr(q);
+    p.x[1] = dptr(k);
+    p.x[2] = dptr(v);
+    p.stride[0] = q_row_stride;
+    p.stride[1] = k_row_stride;
+    p.stride[2] = v_row_stride;
+    p.positions = (const int32_t *)dptr(positions);
+    p.table = (const double *)dptr(table);
+    p.norm[0] = q && q_norm ? fptr(q_norm) : nullptr;
+    p.norm[1] = k_norm ? fptr(k_norm) : nullptr;
+    p.eps = eps;
+    p.out = dptr(q_out);
+    p.out_stride = o_row;
+    p.slots = (const int32_t *)dptr(slots);
+    p.k_cache = dptr(k_cache);
+    p.v_cache = dptr(v_cache);
+    p.n_slots = (int64_t)n_blocks * block_size;
+    p.n_tokens = n_tokens;
+    p.log_block = log_block;
+    p.n_head = q ? (int)n_head : 0;
+    p.n_head_kv = (int)n_head_kv;
+    p.head_dim = (int)head_dim;
+    p.rotary = table ? (int)rotary_dim : 0;
+    KScope ks("rope_append");
+    return finish(launch_rope(p, type, q ? q_out_type : type, interleaved, g.stream), what);
+}
+
+extern "C" int ds3_hip_kv_plan(const ds3_hip_buffer_t *new_lens, const ds3_hip_buffer_t *kv_lens,
+                               ds3_hip_buffer_t *kv_lens_out, ds3_hip_buffer_t *block_table,
+                               const ds3_hip_buffer_t *free_blocks, const ds3_hip_buffer_t *n_free,
+                               ds3_hip_buffer_t *n_free_out, ds3_hip_buffer_t *q_offsets, ds3_hip_buffer_t *positions,
+                               ds3_hip_buffer_t *slots, ds3_hip_buffer_t *status, uint32_t n_seq, uint32_t max_blocks,
+                               uint32_t n_blocks, uint32_t block_size, uint32_t max_tokens)
+{
+    const char *what = "kv_plan";
+    if (!new_lens || !kv_lens || !kv_lens_out || !block_table || !free_blocks || !n_free || !n_free_out || !q_offsets ||
+        !positions || !slots || !status)
+        return -1;
+    int log_block = 0;
+    if (!size_in(what, "n_seq", n_seq, 1, 1u << 20) || !pages_ok(what, n_blocks, block_size, &log_block) ||
+        !size_in(what, "max_blocks", max_blocks, 1, 0x7fffffffu >> log_block) ||
+        !size_in(what, "max_tokens", max_tokens, 1, 1u << 30))
+        return -1;
+    const size_t s_b = (size_t)n_seq * 4, r_b = (size_t)max_tokens * 4;
+    const Span in[4] = { { new_lens, s_b, "new_lens" }, { kv_lens, s_b, "kv_lens" },
+                         { free_blocks, (size_t)n_blocks * 4, "free_blocks" }, { n_free, 4, "n_free" } };
+    const Span out[7] = { { kv_lens_out, s_b, "kv_lens_out" }, { n_free_out, 4, "n_free_out" },
+                          { block_table, s_b * max_blocks, "block_table" }, { q_offsets, s_b + 4, "q_offsets" },
+                          { positions, r_b, "positions" }, { slots, r_b, "slots" }, { status, 16, "status" } };
+    // (the lengths and the count may be written where they are read)
+    const Span lens = cptr(kv_lens) == cptr(kv_lens_out) ? Span{ nullptr, 0, "" } : in[1],
+               left = cptr(n_free) == cptr(n_free_out) ? Span{ nullptr, 0, "" } : in[3];
+    if (!ints_ok(what, { in[0], in[1], in[2], in[3], out[0], out[1], out[2], out[3], out[4], out[5], out[6] }) ||
+        !writable(what, { out[0], out[1], out[2], out[3], out[4], out[5], out[6] }) ||
+        !apart(what, { out[0], out[1], out[2], out[3], out[4], out[5], out[6] }, { in[0], lens, in[2], left }) ||
+        !ensure_init())
+        return -1;
+    Bump bp;
+    const size_t o_h = bp.take(4), o_c = bp.take(s_b), o_f = bp.take(s_b);
+    uint8_t *ws = ws_get(bp.off);
+    if (!ws) return -1;
+    const auto ip = [](const ds3_hip_buffer_t *b) { return (int32_t *)dptr(b); };
+    const PlanArgs p{ ip(new_lens), ip(kv_lens), ip(free_blocks), ip(n_free), ip(kv_lens_out), ip(block_table),
+                      ip(n_free_out), ip(q_offsets), ip(positions), ip(slots), ip(status), (int32_t *)(ws + o_h),
+                      (int32_t *)(ws + o_c), (int32_t *)(ws + o_f), (int)n_seq, (int)max_blocks, (int)n_blocks, log_block,
+                      (int)max_tokens };
+    KScope ks("kv_plan");
+    return finish(launch_kv_plan(p, g.stream), what);
+}
+
+extern "C" int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t *kv_lens,
+                                  const ds3_hip_buffer_t *block_table, ds3_hip_buffer_t *free_blocks,
+                                  ds3_hip_buffer_t *n_free, uint32_t n_seq, uint32_t max_blocks, uint32_t n_blocks,
+                                  uint32_t block_size)
+{
+    const char *what = "kv_release";
+    if (!done || !kv_lens || !block_table || !free_blocks || !n_free) return -1;
+    int log_block = 0;
+    if (!size_in(what, "n_seq", n_seq, 1, 1u << 20) || !pages_ok(what, n_blocks, block_size, &log_block) ||
+        !size_in(what, "max_blocks", max_blocks, 1, 0x7fffffffu >> log_block))
+        return -1;
+    const size_t s_b = (size_t)n_seq * 4;
+    const Span d = { done, s_b, "done" }, t = { block_table, s_b * max_blocks, "block_table" },
+               l = { kv_lens, s_b, "kv_lens" }, f = { free_blocks, (size_t)n_blocks * 4, "free_blocks" },
+               n = { n_free, 4, "n_free" };
+    if (!ints_ok(what, { d, t, l, f, n }) || !writable(what, { l, f, n }) || !apart(what, { l, f, n }, { d, t }) ||
+        !ensure_init())
+        return -1;
+    const ReleaseArgs p{ (const int32_t *)dptr(done), (const int32_t *)dptr(block_table), (int32_t *)dptr(kv_lens),
+                         (int32_t *)dptr(free_blocks), (int32_t *)dptr(n_free), (int)n_seq, (int)max_blocks, (int)n_blocks,
+                         log_block };
+    KScope ks("kv_release");
+    return finish(launch_kv_release(p, g.stream), what);
+}
+
+extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint64_t q_row_stride,
+                                       const ds3_hip_buffer_t *k_cache, const ds3_hip_buffer_t *v_cache,
+                                       const ds3_hip_buffer_t *block_table, const ds3_hip_buffer_t *q_offsets,
+                                       const ds3_hip_buffer_t *kv_lens, ds3_hip_buffer_t *out, uint64_t out_row_stride,
+                                       uint32_t n_tokens, uint32_t n_seq, uint32_t n_head, uint32_t n_head_kv,
+                                       uint32_t head_dim, uint32_t n_blocks, uint32_t block_size, uint32_t max_blocks,
+                                       float scale, uint32_t window)
+{
+    const char *what = "attention_paged";
+    if (!q || !k_cache || !v_cache || !block_table || !q_offsets || !kv_lens || !out) return -1;
+    int log_block = 0;
+    if (!float_type_ok(what, type) || !head_counts_ok(what, n_head, n_head_kv, head_dim, 256) ||
+        !pages_ok(what, n_blocks, block_size, &log_block) || !size_in(what, "n_seq", n_seq, 1, 1u << 20) ||
+        !size_in(what, "max_blocks", max_blocks, 1, 0x7fffffffu >> log_block) ||
+        !size_in(what, "n_tokens", n_tokens, 0, 1u << 20) || !size_in(what, "window", window, 0, 0x7fffffffu))
+        return -1;
+    if (!std::isfinite(scale)) {
+        fprintf(stderr, "ds3_hip: %s: scale is not finite\n", what);
+        return -1;
+    }
+    if (n_tokens == 0) return 0;
+    const size_t c_b = (size_t)n_blocks * block_size * n_head_kv * head_dim * 2, s_b = (size_t)n_seq * 4,
+                 t_b = s_b * max_blocks;
+    size_t q_b, o_b;
+    if (!heads_ok(what, "q", q, type, q_row_stride, n_tokens, n_head, head_dim, &q_b) ||
+        !heads_ok(what, "out", out, type, out_row_stride, n_tokens, n_head, head_dim, &o_b) ||
+        !fits(k_cache, c_b, "k_cache") || !fits(v_cache, c_b, "v_cache") || !aligned_to(k_cache, 16, what, "k_cache") ||
+        !aligned_to(v_cache, 16, what, "v_cache") ||
+        !ints_ok(what, { { block_table, t_b, "block_table" }, { q_offsets, s_b + 4, "q_offsets" },
+                         { kv_lens, s_b, "kv_lens" } }) ||
+        !writable(what, { { out, o_b, "out" } }) ||
+        !apart(what, { { out, o_b, "out" } },
+               { { q, q_b, "q" }, { k_cache, c_b, "k_cache" }, { v_cache, c_b, "v_cache" },
+                 { block_table, t_b, "block_table" }, { q_offsets, s_b + 4, "q_offsets" }, { kv_lens, s_b, "kv_lens" } }) ||
+        !ensure_init())
+        return -1;
+    AttnArgs p{};
+    p.q = dptr(q);
+    p.out = dptr(out);
+    p.q_stride = q_row_stride;
+    p.out_stride = out_row_stride;
+    p.k = (const _Float16 *)dptr(k_cache);
+    p.v = (const _Float16 *)dptr(v_cache);
+    p.table = (const int32_t *)dptr(block_table);
+    p.offsets = (const int32_t *)dptr(q_offsets);
+    p.lens = (const int32_t *)dptr(kv_lens);
+    p.n_tokens = (int)n_tokens;
+    p.n_seq = (int)n_seq;
+    p.n_head = (int)n_head;
+    p.n_head_kv = (int)n_head_kv;
+    p.head_dim = (int)head_dim;
+    p.n_blocks = (int)n_blocks;
+    p.log_block = log_block;
+    p.max_blocks = (int)max_blocks;
+    p.scale = scale;
+    p.window = (int)window;
+    KScope ks("attention_paged");
+    return finish(launch_attention(p, type, g.stream), what);
+}
+
+extern "C" int ds3_hip_sample(const ds3_hip_buffer_t *logits, uint64_t row_stride, const ds3_hip_buffer_t *uniform,
+                              const ds3_hip_buffer_t *temperature, const ds3_hip_buffer_t *top_k,
+                              const ds3_hip_buffer_t *top_p, const ds3_hip_buffer_t *min_p, ds3_hip_buffer_t *tokens,
+                              ds3_hip_buffer_t *probs, uint32_t n_rows, uint32_t n_vocab)
+{
+    const char *what = "sample";
+    if (!logits || !uniform || !tokens) return -1;
+    if (!size_in(what, "n_rows", n_rows, 0, 1u << 20) || !size_in(what, "n_vocab", n_vocab, 1, 1u << 18)) return -1;
+    if (n_rows == 0) return 0;
+    const uint64_t row = (uint64_t)n_vocab * 4;
+    if (row_stride < row || row_stride % 4 != 0 || row_stride > (uint64_t)1 << 31) {
+        fprintf(stderr, "ds3_hip: %s: rows %llu bytes apart: at least one row (%llu bytes), a multiple of 4\n", what,
+                (unsigned long long)row_stride, (unsigned long long)row);
+        return -1;
+    }
+    const size_t l_b = (size_t)span_bytes(n_rows, row_stride, row), r_b = (size_t)n_rows * 4;
+    const Span in[6] = { { logits, l_b, "logits" }, { uniform, r_b, "uniform" }, { temperature, r_b, "temperature" },
+                         { top_k, r_b, "top_k" }, { top_p, r_b, "top_p" }, { min_p, r_b, "min_p" } };
+    const Span out[2] = { { tokens, r_b, "tokens" }, { probs, r_b, "probs" } };
+    if (!ints_ok(what, { in[0], in[1], in[2], in[3], in[4], in[5], out[0], out[1] }) ||
+        !writable(what, { out[0], out[1] }) ||
+        !apart(what, { out[0], out[1] }, { in[0], in[1], in[2], in[3], in[4], in[5] }) || !ensure_init())
+        return -1;
+    const auto fp = [](const ds3_hip_buffer_t *b) { return b ? fptr(b) : nullptr; };
+    const SampleArgs p{ fp(logits), row_stride, fp(uniform), fp(temperature), fp(top_p), fp(min_p),
+                        (const int32_t *)dptr(top_k), (int32_t *)dptr(tokens), fp(probs), (int)n_rows, (int)n_vocab };
+    KScope ks("sample");
+    return finish(launch_sample(p, g.stream), what);
 }

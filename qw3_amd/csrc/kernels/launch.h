@@ -300,4 +300,67 @@ struct MxPlan {
 };
 MxPlan mx_product_plan(const MxProduct &p, bool gate_up);
 
+// Rotary positions and the writing of k and v (kv_cache.hip).  Kinds: 0 q, 1 k, 2 v;
+// without a cache n_head_kv is 0, without q n_head is.  `lanes`, `per` and `chunks`
+// are the launcher's.
+struct RopeArgs {
+    const void *x[3];            // rows of heads, stride[] bytes apart
+    uint64_t stride[3];
+    const int32_t *positions;    // rotary > 0
+    const double *table;         // rotary > 0: rotary / 2 turns a position, the factor
+    const float *norm[2];        // q, k: [head_dim] or null
+    float eps;
+    void *out;
+    uint64_t out_stride;
+    const int32_t *slots;
+    void *k_cache, *v_cache;     // F16 [blocks][n_head_kv][block][head_dim]
+    int64_t n_slots, n_tokens;
+    int log_block, n_head, n_head_kv, head_dim, rotary;
+    int lanes, per, chunks;
+};
+hipError_t launch_rope(RopeArgs p, int in_type, int out_type, bool inter, hipStream_t s);
+
+// The plan of a step (ds3_hip_kv_plan) with its scratch: n_free as it was, and of
+// each request the tokens it had and the new blocks before its own.
+struct PlanArgs {
+    const int32_t *new_lens, *kv_lens, *free_blocks, *n_free;
+    int32_t *kv_lens_out, *table, *n_free_out, *offsets, *positions, *slots, *status;
+    int32_t *head, *cached, *first;      // [1], [n_seq], [n_seq]
+    int n_seq, max_blocks, n_blocks, log_block, max_tokens;
+};
+hipError_t launch_kv_plan(const PlanArgs &p, hipStream_t s);
+
+struct ReleaseArgs {
+    const int32_t *done, *table;
+    int32_t *kv_lens, *free_blocks, *n_free;
+    int n_seq, max_blocks, n_blocks, log_block;
+};
+hipError_t launch_kv_release(const ReleaseArgs &p, hipStream_t s);
+
+// Attention of new tokens over a paged cache (attention.hip).
+struct AttnArgs {
+    const void *q;
+    void *out;
+    uint64_t q_stride, out_stride;       // bytes between tokens' rows
+    const _Float16 *k, *v;               // [n_blocks][n_head_kv][block][head_dim]
+    const int32_t *table, *offsets, *lens;
+    int n_tokens, n_seq, n_head, n_head_kv, head_dim;
+    int n_blocks, log_block, max_blocks;
+    float scale;
+    int window;                          // 0: none
+};
+hipError_t launch_attention(const AttnArgs &p, int type, hipStream_t s);
+
+// Sampling (sample.hip).
+struct SampleArgs {
+    const float *logits;
+    uint64_t stride;                     // bytes between rows
+    const float *uniform, *temperature, *top_p, *min_p;      // the last three: null for none
+    const int32_t *top_k;
+    int32_t *tokens;
+    float *probs;
+    int n_rows, n_vocab;
+};
+hipError_t launch_sample(const SampleArgs &p, hipStream_t s);
+
 }  // namespace ds3k

@@ -334,6 +334,98 @@ def moe_block_mx(hidden: Buffer, ffn_norm: Buffer, eps: float, router: Buffer, r
         router_type, norm), "moe_block_mx")
 
 
+ROPE_PLAIN, ROPE_LINEAR, ROPE_WAVELENGTH, ROPE_YARN = 0, 1, 2, 3
+
+
+def rope_table(rotary_dim: int, base: float, scaling: int = ROPE_PLAIN, factor: float = 1.0, low: float = 0.0,
+               high: float = 0.0, original_ctx: int = 0) -> Buffer:
+    """The angles of rotary positions (ds3_hip_rope_table), for rope and rope_append."""
+    table = Buffer.alloc(8 * (rotary_dim // 2 + 1))
+    _check(hip().ds3_hip_rope_table(table, rotary_dim, base, scaling, factor, low, high, original_ctx), "rope_table")
+    return table
+
+
+@dataclass
+class KvCache:
+    """One layer's paged cache: F16 [n_blocks][n_head_kv][block_size][head_dim] each."""
+    k: Buffer
+    v: Buffer
+    n_blocks: int
+    block_size: int
+    n_head_kv: int
+    head_dim: int
+
+    @classmethod
+    def alloc(cls, n_blocks: int, block_size: int, n_head_kv: int, head_dim: int) -> "KvCache":
+        n = 2 * n_blocks * block_size * n_head_kv * head_dim
+        return cls(Buffer.alloc(n), Buffer.alloc(n), n_blocks, block_size, n_head_kv, head_dim)
+
+
+def rope(x: Buffer, positions: Buffer, table: Buffer, out: Buffer, n_tokens: int, n_head: int, head_dim: int,
+         rotary_dim: int | None = None, type_: int = TYPE_F32, out_type: int | None = None, norm: Buffer | None = None,
+         eps: float = 1e-6, interleaved: bool = False, row_stride: int | None = None,
+         out_row_stride: int | None = None) -> None:
+    """out = the heads of x (RMS-normalised where norm is given) rotated by their positions (ds3_hip_rope)."""
+    out_type = type_ if out_type is None else out_type
+    n = n_head * head_dim
+    _check(hip().ds3_hip_rope(x, type_, row_bytes(type_, n) if row_stride is None else row_stride, positions, table,
+                              _h(norm), eps, out, out_type,
+                              row_bytes(out_type, n) if out_row_stride is None else out_row_stride, n_tokens, n_head,
+                              head_dim, head_dim if rotary_dim is None else rotary_dim, interleaved), "rope")
+
+
+def rope_append(q: Buffer | None, k: Buffer, v: Buffer, positions: Buffer | None, slots: Buffer, cache: KvCache,
+                q_out: Buffer | None, n_tokens: int, n_head: int, type_: int = TYPE_F32, out_type: int | None = None,
+                table: Buffer | None = None, rotary_dim: int | None = None, q_norm: Buffer | None = None,
+                k_norm: Buffer | None = None, eps: float = 1e-6, interleaved: bool = False,
+                strides: tuple[int, int, int] | None = None) -> None:
+    """New tokens' q to q_out, k and v into the cache at `slots` (ds3_hip_rope_append); strides: bytes between rows of
+    q, k and v where they are not dense."""
+    d = cache.head_dim
+    dense = row_bytes(type_, n_head * d), row_bytes(type_, cache.n_head_kv * d), row_bytes(type_, cache.n_head_kv * d)
+    _check(hip().ds3_hip_rope_append(
+        _h(q), k, v, type_, *(strides or dense), _h(positions), slots, _h(table), _h(q_norm), _h(k_norm), eps, _h(q_out),
+        type_ if out_type is None else out_type, cache.k, cache.v, n_tokens, n_head, cache.n_head_kv, d,
+        d if rotary_dim is None else rotary_dim, interleaved, cache.n_blocks, cache.block_size), "rope_append")
+
+
+def kv_plan(new_lens: Buffer, kv_lens: Buffer, block_table: Buffer, free_blocks: Buffer, n_free: Buffer,
+            q_offsets: Buffer, positions: Buffer, slots: Buffer, status: Buffer, n_seq: int, max_blocks: int,
+            n_blocks: int, block_size: int, max_tokens: int, kv_lens_out: Buffer | None = None,
+            n_free_out: Buffer | None = None) -> None:
+    """A step's blocks, offsets, positions and slots from its requests' lengths (ds3_hip_kv_plan); without buffers of
+    their own the lengths and the count of free blocks are updated in place."""
+    _check(hip().ds3_hip_kv_plan(new_lens, kv_lens, kv_lens if kv_lens_out is None else kv_lens_out, block_table,
+                                 free_blocks, n_free, n_free if n_free_out is None else n_free_out, q_offsets, positions,
+                                 slots, status, n_seq, max_blocks, n_blocks, block_size, max_tokens), "kv_plan")
+
+
+def kv_release(done: Buffer, kv_lens: Buffer, block_table: Buffer, free_blocks: Buffer, n_free: Buffer, n_seq: int,
+               max_blocks: int, n_blocks: int, block_size: int) -> None:
+    """Requests with done != 0 give their blocks back (ds3_hip_kv_release)."""
+    _check(hip().ds3_hip_kv_release(done, kv_lens, block_table, free_blocks, n_free, n_seq, max_blocks, n_blocks,
+                                    block_size), "kv_release")
+
+
+def attention_paged(q: Buffer, cache: KvCache, block_table: Buffer, q_offsets: Buffer, kv_lens: Buffer, out: Buffer,
+                    n_tokens: int, n_seq: int, n_head: int, max_blocks: int, scale: float, type_: int = TYPE_F32,
+                    window: int = 0, row_stride: int | None = None, out_row_stride: int | None = None) -> None:
+    """Causal attention of each request's new tokens over its blocks of the cache (ds3_hip_attention_paged)."""
+    dense = row_bytes(type_, n_head * cache.head_dim)
+    _check(hip().ds3_hip_attention_paged(
+        q, type_, dense if row_stride is None else row_stride, cache.k, cache.v, block_table, q_offsets, kv_lens, out,
+        dense if out_row_stride is None else out_row_stride, n_tokens, n_seq, n_head, cache.n_head_kv, cache.head_dim,
+        cache.n_blocks, cache.block_size, max_blocks, scale, window), "attention_paged")
+
+
+def sample(logits: Buffer, uniform: Buffer, tokens: Buffer, n_rows: int, n_vocab: int, temperature: Buffer | None = None,
+           top_k: Buffer | None = None, top_p: Buffer | None = None, min_p: Buffer | None = None,
+           probs: Buffer | None = None, row_stride: int | None = None) -> None:
+    """One token a row, drawn by the given uniform numbers (ds3_hip_sample)."""
+    _check(hip().ds3_hip_sample(logits, 4 * n_vocab if row_stride is None else row_stride, uniform, _h(temperature),
+                                _h(top_k), _h(top_p), _h(min_p), tokens, _h(probs), n_rows, n_vocab), "sample")
+
+
 class Graph:
     """Calls made inside `with ds3.Graph() as gr:` are captured, not run;
     gr.launch() replays them (ds3_hip_graph_begin / _end / _launch)."""

@@ -1,0 +1,176 @@
+"""Attention of new tokens over a paged cache against its 64-bit form."""
+import numpy as np
+import pytest
+
+import _decode as D
+from _decode import F16, F32
+from qw3_amd import ds3
+
+pytestmark = pytest.mark.gpu
+
+
+def run(q, pages, new, lens, type_, window=0, scale=None, rows=None, pad=0, fill=3.0):
+    """The operator's rows [rows][heads][dim], with `pad` values behind each row."""
+    n, heads, dim = q.shape
+    rows = rows or n
+    wide = heads * dim + pad
+    host = np.full((rows, wide), 0.5, D.NP[type_])
+    host[:n, :heads * dim] = q.reshape(n, heads * dim)
+    out = ds3.Buffer.from_array(np.full((rows, wide), fill, D.NP[type_]))
+    offsets = np.concatenate(([0], np.cumsum(new)))
+    step = wide * host.itemsize
+    ds3.attention_paged(ds3.Buffer.from_array(host), pages.device(), D.ints(pages.table), D.ints(offsets), D.ints(lens), out,
+                        rows, len(new), heads, pages.max_blocks, dim ** -0.5 if scale is None else scale, type_, window,
+                        row_stride=step, out_row_stride=step)
+    got = out.read(D.NP[type_], (rows, wide))
+    assert np.all(got[:, heads * dim:] == fill) and np.all(got[n:] == fill)      # behind the rows, behind the last request
+    return got[:n, :heads * dim].reshape(q.shape)
+
+
+def check(seed, new, lens, heads, kv, dim, block, type_, window=0, scale=None, change=None, **more):
+    rng = np.random.default_rng(seed)
+    pages = D.Pages(rng, lens, block, kv, dim)
+    q = (1.5 * rng.standard_normal((sum(new), heads, dim))).astype(D.NP[type_])
+    if change:
+        change(pages, q)
+    got = run(q, pages, new, lens, type_, window, scale, **more)
+    want, tol = D.attention(q, pages, new, lens, dim ** -0.5 if scale is None else scale, window, type_)
+    tol = D.rounded_to(tol, want, type_)
+    bad = ~(np.abs(got.astype(np.float64) - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), float(np.nanmax(np.abs(got - want)[bad])), np.argwhere(bad)[:3].tolist())
+    return got
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("heads,kv,dim,block", [(32, 4, 128, 16), (4, 4, 64, 8), (7, 1, 80, 32), (6, 2, 256, 1),
+                                                (16, 1, 192, 128), (3, 3, 8, 4), (20, 4, 112, 2)])
+def test_one_token(hip_ready, type_, heads, kv, dim, block):
+    lens = [1, 2, 31, 64, 65, 200, 7]
+    check(dim, [1] * 7, lens, heads, kv, dim, block, type_)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("heads,kv,dim,block", [(8, 1, 128, 16), (2, 2, 64, 64), (5, 1, 96, 8), (4, 2, 256, 32),
+                                                (6, 2, 40, 1)])
+def test_chunks(hip_ready, type_, heads, kv, dim, block):
+    """Chunks behind cached tokens, whole prompts, single tokens and requests without tokens."""
+    new = [17, 1, 0, 40, 130, 1, 0]
+    lens = [60, 90, 33, 40, 131, 1, 0]
+    check(dim + 1, new, lens, heads, kv, dim, block, type_)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("window", [1, 5, 64, 100, 1000])
+def test_window(hip_ready, type_, window):
+    check(window, [1, 70, 3, 1], [300, 150, 3, 64], 4, 2, 64, 16, type_, window)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+def test_long_contexts(hip_ready, type_):
+    """Keys split over workgroups: one stream, few streams, one of them short."""
+    check(1, [1], [5000], 8, 1, 128, 16, type_)
+    check(2, [1, 1, 2], [3000, 9, 4100], 4, 2, 64, 32, type_)
+    check(3, [20], [2500], 2, 1, 128, 64, type_, window=2000)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+def test_rows_that_see_nothing(hip_ready, type_):
+    """More new tokens than length (positions below 0), and a request whose blocks all lie outside the cache."""
+    def change(pages, q):
+        pages.table[1] = [-1, 99, -2 ** 31, 2 ** 31 - 1][:pages.max_blocks]
+    got = check(4, [6, 2, 3], [4, 20, 30], 4, 2, 64, 8, type_, change=change)
+    assert not got[:2].any() and not got[6:8].any() and got[2:6].any()
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+def test_single_blocks_outside_the_cache(hip_ready, type_):
+    def change(pages, q):
+        pages.table[0, 1] = -1
+        pages.table[0, 3] = pages.n_blocks
+    check(5, [3, 1], [70, 90], 4, 1, 128, 16, type_, change=change)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+def test_values_that_are_not_finite_where_nothing_looks(hip_ready, type_):
+    """Rows behind the last position of a block and blocks of others: infinite and NaN."""
+    def change(pages, q):
+        n = 37
+        used = pages.table[0, :3]
+        junk = np.ones((pages.n_blocks, pages.block), bool)
+        pos = np.arange(n)
+        junk[used[pos // 16], pos % 16] = False
+        for a, bad in ((pages.k, np.nan), (pages.v, np.inf)):
+            a.transpose(0, 2, 1, 3)[junk] = bad
+            a.transpose(0, 2, 1, 3)[junk & (np.arange(pages.block) % 2 == 0)] = -bad
+    check(6, [1], [37], 4, 2, 64, 16, type_, change=change)
+    check(7, [20], [37], 4, 2, 64, 16, type_, change=change)
+
+
+def test_first_tokens_see_no_later_ones(hip_ready):
+    """Infinities and NaN at positions that a causal row does not see leave it as it is."""
+    for type_ in (F32, F16):
+        rng = np.random.default_rng(8)
+        pages = D.Pages(rng, [50], 16, 2, 64)
+        q = rng.standard_normal((50, 4, 64)).astype(D.NP[type_])
+        clean = run(q, pages, [50], [50], type_)
+        for a, bad in ((pages.k, np.nan), (pages.v, np.inf)):
+            a[pages.table[0, 30 // 16], :, 30 % 16] = bad
+        got = run(q, pages, [50], [50], type_)
+        assert np.array_equal(got[:30], clean[:30]) and not np.isfinite(got[30:]).any()
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+def test_extreme_scores(hip_ready, type_):
+    """Large and tiny q (F32: beyond F16's range), a zero and a negative scale."""
+    def large(pages, q):
+        q[:, ::2] *= 1000
+        if type_ == F32:
+            q[:, 1] *= 1e6
+            q[:, 3] *= 1e-9
+    check(9, [1, 18], [60, 40], 4, 2, 64, 8, type_, change=large, scale=0.01)
+    check(10, [1, 18], [60, 40], 4, 2, 64, 8, type_, scale=0.0)
+    check(11, [1, 18], [60, 40], 4, 2, 64, 8, type_, scale=-0.1)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+def test_padded_batch_and_strides(hip_ready, type_):
+    check(12, [1, 1, 0], [30, 50, 10], 4, 2, 64, 16, type_, rows=9, pad=16)
+    check(13, [30, 1], [30, 50], 4, 2, 64, 16, type_, rows=64, pad=8)
+
+
+def test_offsets_that_end_before_the_rows(hip_ready):
+    """A plan that was not carried out: nothing is written."""
+    pages = D.Pages(np.random.default_rng(0), [20, 20], 16, 2, 64)
+    for type_ in (F32, F16):
+        run(np.zeros((0, 4, 64), D.NP[type_]), pages, [0, 0], [20, 20], type_, rows=5)
+
+
+def test_same_result_again_and_in_a_graph(hip_ready):
+    rng = np.random.default_rng(14)
+    new, lens = [1, 40, 1], [700, 900, 5]
+    pages = D.Pages(rng, lens, 16, 2, 128)
+    cache, table, offsets, n = pages.device(), D.ints(pages.table), D.ints([0, 1, 41, 42]), D.ints(lens)
+    q = rng.standard_normal((42, 8, 128)).astype(np.float32)
+    qb, out = ds3.Buffer.from_array(q), ds3.Buffer.alloc(q.nbytes)
+
+    def call():
+        ds3.attention_paged(qb, cache, table, offsets, n, out, 42, 3, 8, pages.max_blocks, 0.1)
+    call()
+    want = out.read(np.float32, q.shape)
+    call()
+    assert np.array_equal(out.read(np.float32, q.shape), want)
+    with ds3.Graph() as graph:
+        call()
+    for shift in range(3):                            # new lengths, the same graph
+        lens2 = [x - 3 * shift for x in lens]
+        lens2[2] = 5
+        n.write(np.asarray(lens2, np.int32))
+        out.zero()
+        graph.launch()
+        got = out.read(np.float32, q.shape)
+        out.zero()
+        call()
+        assert np.array_equal(out.read(np.float32, q.shape), got)
+    n.write(np.asarray(lens, np.int32))
+    graph.launch()
+    assert np.array_equal(out.read(np.float32, q.shape), want)

@@ -1,0 +1,118 @@
+"""Sampling against its definition in whole numbers, row by row."""
+import numpy as np
+import pytest
+
+import _decode as D
+from qw3_amd import ds3
+
+pytestmark = pytest.mark.gpu
+
+TOP = np.float32(1 - 2.0 ** -24)                     # the largest number below 1
+
+
+def check(x, u, t=None, k=None, p=None, m=None, pad=0):
+    rows, vocab = x.shape
+    host = np.full((rows, vocab + pad), 100, np.float32)
+    host[:, :vocab] = x
+    tokens, probs = D.ints(np.full(rows, -5)), D.floats(np.full(rows, -5))
+    some = lambda v, f: None if v is None else f(v)                              # noqa: E731
+    ds3.sample(ds3.Buffer.from_array(host), D.floats(u), tokens, rows, vocab, temperature=some(t, D.floats),
+               top_k=some(k, D.ints), top_p=some(p, D.floats), min_p=some(m, D.floats), probs=probs,
+               row_stride=4 * (vocab + pad))
+    got, share = tokens.read(np.int32, rows), probs.read(np.float32, rows)
+    for r in range(rows):
+        of = lambda v, d: d if v is None else np.float32(v[r])                   # noqa: E731
+        want, prob = D.sample_row(x[r], float(np.float32(u[r])), of(t, 1.0), 0 if k is None else int(k[r]),
+                                  float(of(p, 1.0)), float(of(m, 0.0)))
+        assert got[r] == want, (r, got[r], want, x[r][got[r]], x[r][want])
+        # weights are off by 2^-45 each from the ratio's two sides, the quotient rounds to 32 bits
+        assert abs(share[r] - prob) <= prob * 2.0 ** -22 + 2.0 ** -60, (r, share[r], prob)
+    return got, share
+
+
+def logits(rng, rows, vocab, peak=6):
+    x = 2.5 * rng.standard_normal((rows, vocab))
+    at = rng.integers(0, vocab, (rows, 12))
+    np.put_along_axis(x, at, peak + 3 * np.abs(rng.standard_normal((rows, 12))), 1)
+    return x.astype(np.float32)
+
+
+SETTINGS = [dict(), dict(t=0.6, k=20, p=0.95), dict(t=1.3, p=0.8), dict(t=0.7, m=0.05), dict(t=1.0, k=1),
+            dict(t=0.9, k=300, p=0.9, m=0.01), dict(t=2.0, p=0.999), dict(t=0.05), dict(t=0.0), dict(t=5.0, k=5000)]
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 3, 31, 64, 1000, 4097, 32000])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_settings(hip_ready, vocab, rows):
+    rng = np.random.default_rng(vocab + rows)
+    x = logits(rng, rows, vocab)
+    for s in SETTINGS:
+        u = rng.random(rows).astype(np.float32)
+        u[0] = rng.choice(np.array([0.0, TOP, 0.5], np.float32))
+        check(x, u, **{n: np.full(rows, v) for n, v in s.items()})
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (3, 262144), (40, 32000), (300, 5000), (1100, 300)])
+def test_rows_with_settings_of_their_own(hip_ready, rows, vocab):
+    rng = np.random.default_rng(rows)
+    x = logits(rng, rows, vocab)
+    pick = [SETTINGS[i] for i in rng.integers(0, len(SETTINGS), rows)]
+    of = lambda n, d: np.array([s.get(n, d) for s in pick])                      # noqa: E731
+    check(x, rng.random(rows).astype(np.float32), of("t", 1.0), of("k", 0), of("p", 1.0), of("m", 0.0))
+
+
+@pytest.mark.parametrize("vocab", [5, 3000, 9000, 100000])
+def test_ties(hip_ready, vocab):
+    """Equal logits go by index: steps of a quarter, few values, all equal, zeros of both signs."""
+    rng = np.random.default_rng(vocab)
+    rows = np.stack([np.round(4 * logits(rng, 1, vocab)[0]) / 4, rng.integers(0, 3, vocab), np.full(vocab, 1.5),
+                     np.where(rng.random(vocab) < 0.5, 0.0, -0.0), np.full(vocab, -3e38)]).astype(np.float32)
+    n = len(rows)
+    for s in SETTINGS + [dict(k=vocab // 2 + 1, p=0.7), dict(k=vocab - 1), dict(p=0.5), dict(t=1e-3, p=0.3)]:
+        for u in (0.0, 0.3, TOP):
+            check(rows, np.full(n, u, np.float32), **{a: np.full(n, v) for a, v in s.items()})
+
+
+def test_rows_that_are_not_finite(hip_ready):
+    rng = np.random.default_rng(2)
+    x = logits(rng, 9, 500)
+    x[0] = -np.inf
+    x[1] = np.nan
+    x[2, ::2], x[2, 1::2] = -np.inf, np.nan
+    x[3, 77:80] = np.inf
+    x[4] = -np.inf
+    x[4, 123] = -50
+    x[5, :499] = np.nan
+    x[6, 10] = np.nan
+    x[7] = np.finfo(np.float32).min                   # a mask of the type's lowest value
+    x[7, [5, 9]] = 3
+    x[8, 100:] = np.finfo(np.float32).min
+    for s in SETTINGS:
+        got, share = check(x, rng.random(9).astype(np.float32), **{n: np.full(9, v) for n, v in s.items()})
+        assert got[:5].tolist() == [-1, -1, -1, 77, 123] and got[5] == 499 and share[:5].tolist() == [0, 0, 0, 1, 1]
+
+
+def test_settings_at_their_ends(hip_ready):
+    rng = np.random.default_rng(5)
+    x = logits(rng, 12, 2000)
+    u = np.array([0.0, TOP, 0.5, 1.0, 2.0, -1.0, np.nan, 0.9, 0.1, 0.7, 0.3, 0.6], np.float32)
+    held = np.where(np.isnan(u), 0, np.clip(u, 0, TOP)).astype(np.float32)
+    nan, inf = np.nan, np.inf
+    for s in (dict(t=[1, 1, inf, 1e-40, 1e30, -1, nan, 1, 0.5, 1, 1, 1]), dict(p=[0, 0, 1, 2, nan, -1, 1e-30, 0.5, 0, 1, inf, -inf]),
+              dict(m=[0, 1, 2, nan, -1, 1e-30, 0.5, 1, 0, inf, -inf, 0.1]),
+              dict(k=[-1, 0, 1, 2000, 2001, 2 ** 31 - 1, -2 ** 31, 1999, 2, 3, 5, 7])):
+        a, _ = check(x, held, **s)
+        some = {"t": "temperature", "k": "top_k", "p": "top_p", "m": "min_p"}
+        name, v = next(iter(s.items()))
+        tokens = ds3.Buffer.alloc(48)
+        ds3.sample(ds3.Buffer.from_array(x), D.floats(u), tokens, 12, 2000, **{some[name]: (D.ints if name == "k" else D.floats)(v)})
+        got = tokens.read(np.int32, 12)
+        # u outside 0 <= u < 1 is held to it
+        assert np.array_equal(got[np.isfinite(u) & (u < 1)], a[np.isfinite(u) & (u < 1)]) and np.array_equal(got[6], a[6])
+
+
+def test_strides_and_alignment(hip_ready):
+    rng = np.random.default_rng(7)
+    for pad in (1, 3, 64):
+        check(logits(rng, 4, 1001), rng.random(4).astype(np.float32), k=np.full(4, 40), pad=pad)
+        check(logits(rng, 4, 1001), rng.random(4).astype(np.float32), p=np.full(4, 0.9), pad=pad)

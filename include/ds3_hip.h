@@ -510,8 +510,10 @@ int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t *kv_lens, 
  * and sees positions 0 .. p, or with window != 0 the last `window` of those.
  * out = softmax(scale * q . k) . v by head; q head h reads kv head h / (n_head /
  * n_head_kv).  A token that sees nothing gets zeros: one at a position below 0, or
- * whose blocks all lie outside the cache.  Rows of out that belong to no request
- * are left as they were.  q and out are of `type`, rows of n_head heads.
+ * whose blocks all lie outside the cache.  A value of the cache that is infinite or
+ * NaN makes what it enters infinite or NaN (F32: NaN for an infinite v too) in the rows
+ * that see it, and in no others.  Rows of out that belong to no request are left as they
+ * were, as are those of a request whose rows do not lie within n_tokens.  q and out are of `type`, rows of n_head heads.
  *   F32: products to 22 bits of q and of the softmax's weights (two F16 parts each),
  *        against the cache's exact F16 values
  *   F16: q as it is, the softmax's weights rounded to F16

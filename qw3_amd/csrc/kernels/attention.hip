@@ -2,87 +2,551 @@
 //
 // Token j of a request with n cached and new tokens, m of them new, is at position
 // p = n - m + j.  Its output is sum_k w_k v_k / sum_k w_k over the keys k that it sees,
-// w_k = exp(s_k - max s), s_k = scale q . k_k, with the maximum and the sums carried
-// over the keys in one pass.
+// w_k = 2^(c (s_k - max s)), s_k = q . k_k, c = scale log2 e, with the maximum and the
+// sums carried over the keys in one pass.  The rows of a kv head are its tokens' q heads
+// side by side (row = token * group + head of the group): all share the keys.
+//
+// Both products run transposed on the matrix cores, S^T = K Q^T and O^T = V^T P^T: a
+// lane of the S^T result holds a row's weights for just those keys that it must hand
+// to the second product, so weights never cross lanes.  Weights carry a factor 2^8
+// (ATT_SHIFT), which cancels, so that small ones keep F16's precision.
+//
+// F32 rows are scaled by a power of two to about 2^14 and split into two F16 parts, as
+// are the weights: products of 22 bits with the cache's exact values.
 #include "common.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace ds3k {
 
-// The request of row t (below offsets[n_seq]).
-__device__ __forceinline__ int request_of(const int32_t *offsets, int n_seq, int t)
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float ATT_SHIFT = 8.0f;
+constexpr float ATT_LAG = 6.0f;              // a maximum may rise by 2^6 before sums are rescaled: weights stay below 2^14
+
+// ---------------------------------------------------------------------------
+// The split of the work.  A unit is one tile of rows (M of a request) with one run
+// of keys; runs are of `run` keys, chosen from all requests' lengths so that about
+// `target` units a kv head result, none shorter than `least`.  Every workgroup finds
+// its unit from the lengths by itself, in prefix sums over the requests.
+// ---------------------------------------------------------------------------
+
+struct Unit {
+    int seq, tile, chunk, run;
+    int first, m, kv;                        // the request's first row, new tokens, length
+    int n;                                   // positions that its blocks hold
+};
+
+constexpr int ATT_TPB = 256;
+
+__device__ __forceinline__ long long wave_sum(long long v)
 {
-    int lo = 0, hi = n_seq;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (offsets[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
+    return v;
 }
 
-// One wave a row and q head: a lane takes a key of each 64 for the scores, then
-// values of the head for the products.
-template <typename T>
-__global__ void __launch_bounds__(64) k_attn_rows(AttnArgs p)
+// Request i's tiles of M rows and the most keys that one of them sees.
+__device__ __forceinline__ void request_work(const AttnArgs &p, int M, int i, int &tiles, int &span, Unit &u)
 {
-    __shared__ float q_s[256];
-    const int t = blockIdx.x / p.n_head, h = blockIdx.x % p.n_head, g = h / (p.n_head / p.n_head_kv), lane = threadIdx.x;
-    if (t >= min(p.offsets[p.n_seq], p.n_tokens)) return;
-    const int i = request_of(p.offsets, p.n_seq, t);
-    const T *q = (const T *)((const uint8_t *)p.q + (uint64_t)t * p.q_stride) + (int64_t)h * p.head_dim;
-    for (int d = lane; d < p.head_dim; d += 64) q_s[d] = (float)q[d];
+    tiles = span = 0;
+    if (i >= p.n_seq) return;
+    const int group = p.n_head / p.n_head_kv, o0 = p.offsets[i], o1 = p.offsets[i + 1];
+    if (o0 < 0 || o1 <= o0 || o1 > p.n_tokens) return;
+    u.first = o0;
+    u.m = o1 - o0;
+    u.kv = p.lens[i];
+    u.n = (int)min((int64_t)max(u.kv, 0), (int64_t)p.max_blocks << p.log_block);
+    const long long rows = (long long)u.m * group;
+    if (rows < p.min_rows || rows > p.max_rows) return;
+    tiles = (int)((rows + M - 1) / M);
+    span = p.window ? (int)min((long long)u.n, (long long)p.window + M / group + 130) : u.n;
+    span = max(span, 1);
+}
+
+// The unit `id` of this workgroup's kv head; false: none.
+template <int TPB>
+__device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit &u)
+{
+    __shared__ long long part[2][TPB / 64];
+    __shared__ int found[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (p.n_seq == 1) {
+        int tiles, span;
+        request_work(p, M, 0, tiles, span, u);
+        u.seq = 0;
+        u.run = tiles >= p.target ? 1 << 30
+              : (int)min(((long long)tiles * span / (p.target - tiles) + p.least) / p.least * p.least, 1ll << 30);
+        const int chunks = (span + u.run - 1) / u.run;
+        if ((long long)id >= (long long)tiles * chunks) return false;
+        u.tile = id / chunks;
+        u.chunk = id - u.tile * chunks;
+        return true;
+    }
+    long long work = 0, all = 0;
+    for (int i0 = 0; i0 < p.n_seq; i0 += TPB) {
+        int tiles, span;
+        Unit r;
+        request_work(p, M, i0 + tid, tiles, span, r);
+        work += (long long)tiles * span;
+        all += tiles;
+    }
+    work = wave_sum(work);
+    all = wave_sum(all);
+    if (lane == 0) {
+        part[0][wave] = work;
+        part[1][wave] = all;
+    }
+    if (tid == 0) found[0] = -1;
     __syncthreads();
-    const int64_t n = min((int64_t)max(p.lens[i], 0), (int64_t)p.max_blocks << p.log_block);
-    const int64_t pos = (int64_t)p.lens[i] - p.offsets[i + 1] + t, last = min(pos, n - 1);
-    const int64_t first = p.window ? max(pos - p.window + 1, (int64_t)0) : 0;
-    float m = -INFINITY, sum = 0.0f, acc[4] = { 0, 0, 0, 0 };
-    for (int64_t k0 = first; k0 <= last; k0 += 64) {
-        const int64_t key = k0 + lane;
-        int64_t at = -1;                              // the key's row of the cache
-        if (key <= last) {
-            const int block = p.table[(int64_t)i * p.max_blocks + (key >> p.log_block)];
-            if (block >= 0 && block < p.n_blocks)
-                at = ((((int64_t)block * p.n_head_kv + g) << p.log_block) + (key & ((1 << p.log_block) - 1))) * p.head_dim;
-        }
-        float s = -INFINITY;
-        if (at >= 0) {
-            s = 0.0f;
-            for (int d = 0; d < p.head_dim; d++) s += q_s[d] * (float)p.k[at + d];
-            s *= p.scale;
-        }
-        float top = s;
-        for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
-        const float m2 = fmaxf(m, top);
-        if (m2 == -INFINITY) continue;
-        const float w = expf(s - m2), keep = expf(m - m2);
-        float add = w;
-        for (int d = 32; d > 0; d /= 2) add += __shfl_xor(add, d);
-        sum = sum * keep + add;
-        m = m2;
-#pragma unroll
-        for (int r = 0; r < 4; r++) acc[r] *= keep;
-        for (int j = 0; j < 64; j++) {
-            const float wj = __shfl(w, j);
-            const int64_t aj = __shfl(at, j);
-            if (aj < 0) continue;
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (lane + 64 * r < p.head_dim) acc[r] += wj * (float)p.v[aj + lane + 64 * r];
-        }
+    work = all = 0;
+    for (int w = 0; w < TPB / 64; w++) {
+        work += part[0][w];
+        all += part[1][w];
     }
-    T *out = (T *)((uint8_t *)p.out + (uint64_t)t * p.out_stride) + (int64_t)h * p.head_dim;
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-        if (lane + 64 * r < p.head_dim) out[lane + 64 * r] = (T)(sum == 0.0f ? 0.0f : acc[r] / sum);
+    __syncthreads();
+    const long long want = all >= p.target ? 1 << 30 : (work / (p.target - all) + p.least) / p.least * p.least;
+    u.run = (int)min(want, 1ll << 30);
+    long long before = 0;
+    for (int i0 = 0; i0 < p.n_seq && before <= id; i0 += TPB) {
+        int tiles, span;
+        Unit r;
+        request_work(p, M, i0 + tid, tiles, span, r);
+        const long long own = (long long)tiles * ((span + u.run - 1) / u.run);
+        long long sum = own;
+        for (int d = 1; d < 64; d *= 2) {
+            const long long o = __shfl_up(sum, d);
+            if (lane >= d) sum += o;
+        }
+        if (lane == 63) part[0][wave] = sum;
+        __syncthreads();
+        long long total = 0, mine = before + sum - own;
+        for (int w = 0; w < TPB / 64; w++) {
+            if (w < wave) mine += part[0][w];
+            total += part[0][w];
+        }
+        if (own > 0 && id >= mine && id < mine + own) {
+            found[0] = i0 + tid;
+            found[1] = (int)(id - mine);
+        }
+        before += total;
+        __syncthreads();
+    }
+    if (found[0] < 0) return false;
+    int tiles, span;
+    u.seq = found[0];
+    request_work(p, M, u.seq, tiles, span, u);
+    const int chunks = (span + u.run - 1) / u.run;
+    u.tile = found[1] / chunks;
+    u.chunk = found[1] - u.tile * chunks;
+    return true;
 }
 
-hipError_t launch_attention(const AttnArgs &p, int type, hipStream_t s)
+// ---------------------------------------------------------------------------
+// Parts
+// ---------------------------------------------------------------------------
+
+// v * 2^-e in two F16 parts, hi + lo, for |v| 2^-e below 2^15.
+__device__ __forceinline__ void split(float v, _Float16 &hi, _Float16 &lo)
 {
-    const dim3 grid((unsigned)p.n_tokens * p.n_head);
-    if (type == T_F32) hipLaunchKernelGGL(k_attn_rows<float>, grid, 64, 0, s, p);
-    else hipLaunchKernelGGL(k_attn_rows<_Float16>, grid, 64, 0, s, p);
+    hi = (_Float16)v;
+    lo = (_Float16)(v - (float)hi);
+}
+
+// Eight values of a row of q: F16 as they are, F32 scaled and in two parts.
+template <typename T>
+struct QFrag {
+    f16x8 hi, lo;
+};
+
+// The power of two that brings a row's largest magnitude to 2^13 .. 2^14 (1 where it is 0 or
+// not finite), as its exponent.
+__device__ __forceinline__ int row_exponent(float amax)
+{
+    const int e = (int)((__float_as_uint(amax) >> 23) & 255);
+    return e == 0 || e == 255 ? 0 : 13 + 127 - e;
+}
+
+__device__ __forceinline__ float mul_pow2(float v, int e) { return __builtin_ldexpf(v, e); }
+
+// 16 keys x 32 values: lane l holds key (or row) l % 16, values 8 (l / 16) + 0 .. 7.
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ bool finite_pair(int w)
+{
+    return (w & 0x7c00) != 0x7c00 && (w & 0x7c000000) != 0x7c000000;
+}
+
+// The row of a cache that holds position `key` (of kv head g): its first value's index, or -1.
+__device__ __forceinline__ int64_t cache_row(const AttnArgs &p, int block, int key, int g)
+{
+    return ((((int64_t)block * p.n_head_kv + g) << p.log_block) + (key & ((1 << p.log_block) - 1))) * p.head_dim;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: up to 16 a tile.  The four waves of a workgroup take keys 32 by 32 in
+// turn, straight from the cache to registers: bound by those reads.  For the first
+// product a lane reads 16 bytes of a key's row as the matrix operand wants them; for
+// the second it reads the values m DP/16 .. of eight keys, m = lane % 16, so that the
+// operand of output tile t is value t of each: an 8 x (DP / 16) transposition within
+// the lane.  The lane of the result then holds DP / 4 consecutive values of its row.
+// ---------------------------------------------------------------------------
+
+constexpr int ROWS_M = 16;
+
+template <int DP>
+struct RowsShared {
+    float o[4][ROWS_M][128 + 4];
+    float m[4][ROWS_M], l[4][ROWS_M];
+    int last;
+};
+
+template <typename T, int DP, bool PAD, bool TINY>
+__global__ void __launch_bounds__(ATT_TPB) k_attn_rows(AttnArgs p)
+{
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int NC = DP / 32;              // operands of a key's row
+    constexpr int NT = DP / 16;              // output tiles; values of a key that a lane reads for the second product
+    __shared__ RowsShared<DP> sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, h = lane >> 4;
+    const int g = blockIdx.x % p.n_head_kv, id = blockIdx.x / p.n_head_kv, group = p.n_head / p.n_head_kv;
+    Unit u;
+    if (!find_unit<ATT_TPB>(p, ROWS_M, id, u)) return;
+    const int row0 = u.tile * ROWS_M, rows = min(u.m * group - row0, ROWS_M);
+    // keys that any row sees, from a multiple of 32; those of this unit
+    const int64_t base = (int64_t)u.kv - u.m;                 // the first new token's position
+    const int j0 = row0 / group, j1 = (row0 + rows - 1) / group;
+    const int end = (int)max(min(base + j1 + 1, (int64_t)u.n), (int64_t)0);
+    const int start = p.window ? (int)max(base + j0 - p.window + 1, (int64_t)0) & ~31 : 0;
+    const int chunks = end > start ? (int)(((int64_t)end - start + u.run - 1) / u.run) : 1;
+    if (u.chunk >= chunks) return;
+    const int k0 = (int)min((int64_t)start + (int64_t)u.chunk * u.run, (int64_t)end),
+              k1 = (int)min((int64_t)k0 + u.run, (int64_t)end);
+
+    // this lane's row: its position, its first key, its q
+    const bool live = r < rows;
+    const int my_j = (row0 + (live ? r : 0)) / group, my_h = (row0 + (live ? r : 0)) % group;
+    const int pos = live ? (int)(base + my_j) : -1;
+    const int low = p.window ? pos - p.window + 1 : 0;        // (a window beyond int32 has no effect below 2^31 keys)
+    const T *q = (const T *)((const uint8_t *)p.q + (uint64_t)(u.first + my_j) * p.q_stride) +
+                 (int64_t)(g * group + my_h) * p.head_dim;
+    f16x8 qh[NC], ql[NC];
+    float c2 = p.scale;                       // |scale| log2 e, times the row's power of two
+    if constexpr (SPLIT) {
+        float v[NC][8], amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[c][e] = live && (!PAD || 32 * c + 8 * h < p.head_dim) ? q[32 * c + 8 * h + e] * p.q_sign : 0.0f;
+                amax = fmaxf(amax, fabsf(v[c][e]));
+            }
+        amax = fmaxf(amax, __shfl_xor(amax, 16));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int ex = row_exponent(amax);
+        c2 = mul_pow2(c2, -ex);
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                _Float16 a, b;
+                split(mul_pow2(v[c][e], ex), a, b);
+                qh[c][e] = a;
+                ql[c][e] = b;
+            }
+    } else {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            f16x8 v = { 0, 0, 0, 0, 0, 0, 0, 0 };
+            if (live && (!PAD || 32 * c + 8 * h < p.head_dim)) v = *(const f16x8 *)(q + 32 * c + 8 * h);
+            qh[c] = v * (_Float16)p.q_sign;
+        }
+    }
+
+    const int32_t *table = p.table + (int64_t)u.seq * p.max_blocks;
+    const int all_from = (int)max(p.window ? base + j1 - p.window + 1 : 0, (int64_t)0);      // keys that every row sees:
+    const int64_t all_to = base + j0;                                                        // from .. to
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = { 0, 0, 0, 0 };
+
+    for (int kb = k0 + 32 * wave; kb < k1; kb += 32 * (ATT_TPB / 64)) {
+        // where the keys lie: for the first product keys r and 16 + r, for the second 4 h .. 4 h + 3 and 16 + those
+        f16x8 kf[2][NC];
+        i32x4 vf[8][(NT + 7) / 8];
+        bool seen[8];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int key = kb + 16 * t + r;
+            const int block = key < k1 ? table[key >> p.log_block] : -1;
+            const bool ok = (unsigned)block < (unsigned)p.n_blocks;
+            const _Float16 *row = p.k + (ok ? cache_row(p, block, key, g) : 0);
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                f16x8 v = { 0, 0, 0, 0, 0, 0, 0, 0 };
+                if (!PAD || 32 * c + 8 * h < p.head_dim) v = *(const f16x8 *)(row + 32 * c + 8 * h);
+                kf[t][c] = v;
+            }
+        }
+        bool whole = true;                    // every key of the 32 is there
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            int block = -1;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int key = kb + 16 * t + 4 * h + e;
+                if (e == 0 || TINY) block = key < k1 ? table[key >> p.log_block] : -1;
+                const bool ok = key < k1 && (unsigned)block < (unsigned)p.n_blocks;
+                seen[4 * t + e] = ok;
+                whole &= ok;
+                const _Float16 *row = p.v + (ok ? cache_row(p, block, key, g) : 0);
+                if constexpr (NT == 4) {
+                    vf[4 * t + e][0] = { 0, 0, 0, 0 };
+                    if (!PAD || NT * r < p.head_dim) {
+                        const int2 w = *(const int2 *)(row + NT * r);
+                        vf[4 * t + e][0].x = w.x;
+                        vf[4 * t + e][0].y = w.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < NT / 8; x++) {
+                        vf[4 * t + e][x] = { 0, 0, 0, 0 };
+                        if (!PAD || NT * r + 8 * x < p.head_dim) vf[4 * t + e][x] = *(const i32x4 *)(row + NT * r + 8 * x);
+                    }
+                }
+            }
+        }
+
+        f32x4 s[2] = { { 0, 0, 0, 0 }, { 0, 0, 0, 0 } };
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                s[t] = mfma16(kf[t][c], qh[c], s[t]);
+                if constexpr (SPLIT) s[t] = mfma16(kf[t][c], ql[c], s[t]);
+            }
+
+        const bool plain = __all(whole) && kb >= all_from && kb + 31 <= all_to;
+        if (!plain) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int key = kb + 16 * (e / 4) + 4 * h + (e & 3);
+                if (!(seen[e] && key <= pos && key >= low)) s[e / 4][e & 3] = -INFINITY;
+                if (!seen[e]) {
+#pragma unroll
+                    for (int x = 0; x < (NT + 7) / 8; x++) vf[e][x] = { 0, 0, 0, 0 };
+                }
+            }
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * c2;
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // (the first keys always pass, as m is then -inf)
+        if (__any(top > m + ATT_LAG)) {
+            const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 1.0f : fast_exp2(m - m2);
+            m = m2;
+            l *= keep;
+#pragma unroll
+            for (int t = 0; t < NT; t++) acc[t] *= keep;
+        }
+        const float less = m == -INFINITY ? 0.0f : m - ATT_SHIFT;
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            w[e] = fast_exp2(__builtin_fmaf(s[e / 4][e & 3], c2, -less));
+            l += w[e];
+        }
+        f16x8 ph, pl;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            _Float16 a, b;
+            split(w[e], a, b);
+            ph[e] = a;
+            if constexpr (SPLIT) pl[e] = b;
+        }
+        // operand of output tile t: value t of the lane's eight keys
+        const auto operand = [&](int t) {
+            i32x4 a;
+            const int x = t / 8, d = t / 2 % 4;
+            const unsigned pick = t & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+            for (int e = 0; e < 4; e++) a[e] = __builtin_amdgcn_perm(vf[2 * e + 1][x][d], vf[2 * e][x][d], pick);
+            return a;
+        };
+        bool finite = true;
+        if (!plain && j1 > j0) {              // keys that some rows see and others do not
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+#pragma unroll
+                for (int x = 0; x < (NT + 7) / 8; x++)
+#pragma unroll
+                    for (int d = 0; d < (NT == 4 ? 2 : 4); d++) finite &= finite_pair(vf[e][x][d]);
+        }
+        if (__all(finite)) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const f16x8 a = __builtin_bit_cast(f16x8, operand(t));
+                acc[t] = mfma16(a, ph, acc[t]);
+                if constexpr (SPLIT) acc[t] = mfma16(a, pl, acc[t]);
+            }
+        } else {
+            // an infinity or NaN among them must not meet the weight 0: row by row, without the keys that the row does not see
+            for (int n = 0; n < rows; n++) {
+                const int to = __shfl(pos, n), from = __shfl(low, n);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    f16x8 a = __builtin_bit_cast(f16x8, operand(t));
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int key = kb + 16 * (e / 4) + 4 * h + (e & 3);
+                        if (key > to || key < from) a[e] = (_Float16)0.0f;
+                    }
+                    f32x4 o = mfma16(a, ph, acc[t]);
+                    if constexpr (SPLIT) o = mfma16(a, pl, o);
+                    if (r == n) acc[t] = o;
+                }
+            }
+        }
+    }
+
+    // the waves' sums, brought to one maximum
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (h == 0) {
+        sh.m[wave][r] = m;
+        sh.l[wave][r] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; w++) top = fmaxf(top, sh.m[w][r]);
+    const float part = m == -INFINITY ? 1.0f : fast_exp2(m - top);       // (of nothing, or of NaN)
+    // a unit's partial result: [rows][DP] sums, then each row's maximum and sum of weights
+    float *ws = p.partial + (int64_t)(g + (int64_t)id * p.n_head_kv) * (ROWS_M * (DP + 2));
+    constexpr int COLS = DP < 128 ? DP : 128;
+#pragma unroll
+    for (int c0 = 0; c0 < DP; c0 += COLS) {
+        if (c0) __syncthreads();
+        if (DP <= 128 || h * (DP / 4) / 128 == c0 / 128) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) sh.o[wave][r][(4 * h + i) * NT + t - c0] = acc[t][i] * part;
+        }
+        __syncthreads();
+        for (int x = tid; x < rows * COLS; x += ATT_TPB) {
+            const int n = x / COLS, d = x % COLS;
+            float o = 0.0f, top_n = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                o += sh.o[w][n][d];
+                top_n = fmaxf(top_n, sh.m[w][n]);
+            }
+#pragma unroll
+            for (int w = 0; w < 4; w++) sum += sh.m[w][n] == -INFINITY ? sh.l[w][n] : sh.l[w][n] * fast_exp2(sh.m[w][n] - top_n);
+            if (chunks == 1) {
+                if (c0 + d < p.head_dim) {
+                    const int j = (row0 + n) / group, a = (row0 + n) % group;
+                    T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) +
+                             (int64_t)(g * group + a) * p.head_dim;
+                    out[c0 + d] = (T)(sum == 0.0f ? 0.0f : o / sum);
+                }
+            } else {
+                ws[n * DP + c0 + d] = o;
+                if (c0 == 0 && d == 0) {
+                    ws[ROWS_M * DP + n] = top_n;
+                    ws[ROWS_M * DP + ROWS_M + n] = sum;
+                }
+            }
+        }
+    }
+    if (chunks == 1) return;
+
+    // the workgroup that ends last joins the tile's runs, in their order
+    __threadfence();
+    __syncthreads();
+    const int first_id = id - u.chunk;
+    if (tid == 0) {
+        int *ticket = p.tickets + first_id * p.n_head_kv + g;
+        const int old = atomicAdd(ticket, 1);
+        sh.last = old == chunks - 1;
+        if (old == chunks - 1) *ticket = 0;           // as the next launch expects it
+    }
+    __syncthreads();
+    if (!sh.last) return;
+    __threadfence();
+    const int64_t step = (int64_t)p.n_head_kv * (ROWS_M * (DP + 2));
+    const float *from = p.partial + (int64_t)(g + (int64_t)first_id * p.n_head_kv) * (ROWS_M * (DP + 2));
+    for (int x = tid; x < rows * DP; x += ATT_TPB) {
+        const int n = x / DP, d = x % DP;
+        if (d >= p.head_dim) continue;
+        float top_n = -INFINITY, o = 0.0f, sum = 0.0f;
+        for (int c = 0; c < chunks; c++) top_n = fmaxf(top_n, from[c * step + ROWS_M * DP + n]);
+        for (int c = 0; c < chunks; c++) {
+            const float mc = from[c * step + ROWS_M * DP + n], f = mc == -INFINITY ? 1.0f : fast_exp2(mc - top_n);
+            sum += f * from[c * step + ROWS_M * DP + ROWS_M + n];
+            o += f * from[c * step + n * DP + d];
+        }
+        const int j = (row0 + n) / group, a = (row0 + n) % group;
+        T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim;
+        out[d] = (T)(sum == 0.0f ? 0.0f : o / sum);
+    }
+}
+
+template <typename T, int DP>
+static void rows_launch(const AttnArgs &p, dim3 grid, hipStream_t s)
+{
+    const bool pad = p.head_dim != DP, tiny = p.log_block < 2;
+    if (tiny) hipLaunchKernelGGL((k_attn_rows<T, DP, true, true>), grid, ATT_TPB, 0, s, p);
+    else if (pad) hipLaunchKernelGGL((k_attn_rows<T, DP, true, false>), grid, ATT_TPB, 0, s, p);
+    else hipLaunchKernelGGL((k_attn_rows<T, DP, false, false>), grid, ATT_TPB, 0, s, p);
+}
+
+template <typename T>
+static void rows_dim(const AttnArgs &p, dim3 grid, hipStream_t s)
+{
+    if (p.head_dim <= 64) rows_launch<T, 64>(p, grid, s);
+    else if (p.head_dim <= 128) rows_launch<T, 128>(p, grid, s);
+    else rows_launch<T, 256>(p, grid, s);
+}
+
+static int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+// Units a kv head that the work is split into where there are fewer tiles.
+static int rows_target(const AttnArgs &p) { return std::max(1, ATT_MAX_UNITS / 2 / p.n_head_kv); }
+
+// Tiles of at most M rows that n_seq requests with n_tokens tokens in all can have.
+static int64_t most_tiles(const AttnArgs &p, int M)
+{
+    return (int64_t)p.n_tokens * (p.n_head / p.n_head_kv) / M + std::min(p.n_seq, p.n_tokens);
+}
+
+size_t attention_workspace(const AttnArgs &p)
+{
+    // units of split tiles: fewer than `target` tiles, and as many runs beyond one each
+    return (size_t)2 * rows_target(p) * p.n_head_kv * ROWS_M * (padded_dim(p.head_dim) + 2) * sizeof(float);
+}
+
+hipError_t launch_attention(AttnArgs p, int type, hipStream_t s)
+{
+    // S = q . k takes |scale|; its sign goes to q, and scale 0 makes q 0
+    p.q_sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
+    p.scale = p.scale == 0.0f ? 1.0f : std::fabs(p.scale) * 1.44269504088896340736f;
+    p.min_rows = 0;
+    p.max_rows = 0x7fffffff;
+    p.target = rows_target(p);
+    p.least = 128;
+    const int64_t units = (most_tiles(p, ROWS_M) + p.target) * p.n_head_kv;
+    if (units > 0x7fffff) return hipErrorInvalidValue;
+    if (type == T_F32) rows_dim<float>(p, dim3((unsigned)units), s);
+    else rows_dim<_Float16>(p, dim3((unsigned)units), s);
     return hipGetLastError();
 }
 

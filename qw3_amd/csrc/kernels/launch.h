@@ -348,8 +348,15 @@ struct AttnArgs {
     int n_blocks, log_block, max_blocks;
     float scale;
     int window;                          // 0: none
+    float *partial;                      // attention_workspace bytes
+    int *tickets;                        // ATT_MAX_UNITS, zero between launches
+    // the launcher's: requests of min_rows .. max_rows rows, units a kv head, keys a unit, q's factor
+    int min_rows, max_rows, target, least;
+    float q_sign;
 };
-hipError_t launch_attention(const AttnArgs &p, int type, hipStream_t s);
+constexpr int ATT_MAX_UNITS = 4096;
+size_t attention_workspace(const AttnArgs &p);
+hipError_t launch_attention(AttnArgs p, int type, hipStream_t s);
 
 // Sampling (sample.hip).
 struct SampleArgs {

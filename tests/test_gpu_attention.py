@@ -174,3 +174,32 @@ def test_same_result_again_and_in_a_graph(hip_ready):
     n.write(np.asarray(lens, np.int32))
     graph.launch()
     assert np.array_equal(out.read(np.float32, q.shape), want)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+def test_queries_that_are_not_finite(hip_ready, type_):
+    """NaN in one head's q makes that head NaN and nothing else."""
+    rng = np.random.default_rng(15)
+    for new, lens in (([1, 1], [40, 2000]), ([18, 2], [40, 700])):
+        pages = D.Pages(rng, lens, 16, 2, 64)
+        q = rng.standard_normal((sum(new), 4, 64)).astype(D.NP[type_])
+        clean = run(q, pages, new, lens, type_)
+        q[1, 2, 5] = np.nan
+        got = run(q, pages, new, lens, type_)
+        assert np.isnan(got[1, 2]).all()
+        got[1, 2] = clean[1, 2]
+        assert np.array_equal(got, clean)
+
+
+def test_groups_that_do_not_divide_tiles(hip_ready):
+    """20 heads a kv head: tiles begin inside a token; an infinity that only the later token sees."""
+    for type_ in (F32, F16):
+        rng = np.random.default_rng(16)
+        pages = D.Pages(rng, [33, 12], 4, 1, 64)
+        q = rng.standard_normal((5, 20, 64)).astype(D.NP[type_])
+        clean = run(q, pages, [3, 2], [33, 12], type_)
+        pages.v[pages.table[0, 8], :, 0, 7] = np.inf  # position 32, the third token's own
+        got = run(q, pages, [3, 2], [33, 12], type_)
+        assert np.array_equal(got[:2], clean[:2]) and not np.isfinite(got[2, :, 7]).any()
+        got[2, :, 7] = clean[2, :, 7]
+        assert np.array_equal(got, clean)

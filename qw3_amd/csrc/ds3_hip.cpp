@@ -76,7 +76,6 @@ struct State {
     int32_t *zero_idx = nullptr;     // device {0}
     int32_t *tickets = nullptr;      // kTickets router tickets (zero between launches)
     int router_mode = 0;             // ds3_hip_set_router_mode
-    int *attn_tickets = nullptr;     // ATT_MAX_UNITS attention tickets (zero between launches)
     unsigned long long *cert_stats = nullptr;   // device {certified, repaired} token counts
     float *one_f = nullptr;          // device {1.0f}
     int prefill_min = kDefaultPrefillMin;
@@ -452,14 +451,12 @@ extern "C" int ds3_hip_init(void)
         g.scratch_dev[g.device] = (uint8_t *)sp;
     }
     void *consts = nullptr;
-    const size_t tickets_at = 128 + (size_t)kTickets * 4 + 16, consts_bytes = tickets_at + (size_t)ATT_MAX_UNITS * 4;
-    if (hipMalloc(&consts, consts_bytes) != hipSuccess) return -1;
+    if (hipMalloc(&consts, 128 + (size_t)kTickets * 4 + 16) != hipSuccess) return -1;
     g.zero_idx = (int32_t *)consts;
     g.one_f = (float *)((uint8_t *)consts + 64);
     g.tickets = (int32_t *)((uint8_t *)consts + 128);   // router token-group tickets, kept at zero between launches
     g.cert_stats = (unsigned long long *)((uint8_t *)consts + 128 + (size_t)kTickets * 4);
-    g.attn_tickets = (int *)((uint8_t *)consts + tickets_at);
-    if (hipMemsetAsync(g.tickets, 0, consts_bytes - 128, g.stream) != hipSuccess ||
+    if (hipMemsetAsync(g.tickets, 0, (size_t)kTickets * 4 + 16, g.stream) != hipSuccess ||
         hipStreamSynchronize(g.stream) != hipSuccess)
         return -1;
     const int32_t zi = 0;
@@ -2837,7 +2834,6 @@ extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t
     p.max_blocks = (int)max_blocks;
     p.scale = scale;
     p.window = (int)window;
-    p.tickets = g.attn_tickets;
     p.partial = (float *)ws_get(attention_workspace(p));
     if (!p.partial) return -1;
     KScope ks("attention_paged");

@@ -37,6 +37,7 @@ constexpr float ATT_LAG = 6.0f;              // a maximum may rise by 2^6 before
 
 struct Unit {
     int seq, tile, chunk, run;
+    int whole;                               // the first unit of the tile, chunk 0
     int first, m, kv;                        // the request's first row, new tokens, length
     int n;                                   // positions that its blocks hold
 };
@@ -67,23 +68,31 @@ __device__ __forceinline__ void request_work(const AttnArgs &p, int M, int i, in
     span = max(span, 1);
 }
 
-// The unit `id` of this workgroup's kv head; false: none.
-template <int TPB>
+// Keys a unit: work / (target - tiles) or a little more, so that splitting adds at most target - tiles units.
+__device__ __forceinline__ int unit_run(const AttnArgs &p, long long work, long long tiles)
+{
+    if (tiles >= p.target) return 1 << 30;
+    const float want = (float)work / (float)(p.target - tiles) * (1.0f + 0x1p-20f);
+    return want >= 0x1p29f ? 1 << 30 : ((int)want + p.least) & -p.least;
+}
+
+// The unit `id` of this workgroup's kv head, or with TILES the tile `id` (its chunk 0); false: none.
+template <int TPB, bool TILES>
 __device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit &u)
 {
     __shared__ long long part[2][TPB / 64];
-    __shared__ int found[2];
+    __shared__ int found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (p.n_seq == 1) {
         int tiles, span;
         request_work(p, M, 0, tiles, span, u);
         u.seq = 0;
-        u.run = tiles >= p.target ? 1 << 30
-              : (int)min(((long long)tiles * span / (p.target - tiles) + p.least) / p.least * p.least, 1ll << 30);
+        u.run = unit_run(p, (long long)tiles * span, tiles);
         const int chunks = (span + u.run - 1) / u.run;
-        if ((long long)id >= (long long)tiles * chunks) return false;
-        u.tile = id / chunks;
-        u.chunk = id - u.tile * chunks;
+        if ((long long)id >= (long long)tiles * (TILES ? 1 : chunks)) return false;
+        u.tile = TILES ? id : id / chunks;
+        u.whole = u.tile * chunks;
+        u.chunk = TILES ? 0 : id - u.whole;
         return true;
     }
     long long work = 0, all = 0;
@@ -108,31 +117,43 @@ __device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit
         all += part[1][w];
     }
     __syncthreads();
-    const long long want = all >= p.target ? 1 << 30 : (work / (p.target - all) + p.least) / p.least * p.least;
-    u.run = (int)min(want, 1ll << 30);
-    long long before = 0;
+    u.run = unit_run(p, work, all);
+    long long before = 0, units_before = 0;           // of what `id` counts, and of units
     for (int i0 = 0; i0 < p.n_seq && before <= id; i0 += TPB) {
         int tiles, span;
         Unit r;
         request_work(p, M, i0 + tid, tiles, span, r);
-        const long long own = (long long)tiles * ((span + u.run - 1) / u.run);
-        long long sum = own;
+        const long long units = (long long)tiles * ((span + u.run - 1) / u.run);
+        long long sum = units, tile_sum = tiles;
         for (int d = 1; d < 64; d *= 2) {
-            const long long o = __shfl_up(sum, d);
-            if (lane >= d) sum += o;
+            const long long o = __shfl_up(sum, d), q = __shfl_up(tile_sum, d);
+            if (lane >= d) {
+                sum += o;
+                tile_sum += q;
+            }
         }
-        if (lane == 63) part[0][wave] = sum;
+        if (lane == 63) {
+            part[0][wave] = sum;
+            part[1][wave] = tile_sum;
+        }
         __syncthreads();
-        long long total = 0, mine = before + sum - own;
+        long long total = 0, tile_total = 0, at = units_before + sum - units, tile_at = before + tile_sum - tiles;
         for (int w = 0; w < TPB / 64; w++) {
-            if (w < wave) mine += part[0][w];
+            if (w < wave) {
+                at += part[0][w];
+                tile_at += part[1][w];
+            }
             total += part[0][w];
+            tile_total += part[1][w];
         }
-        if (own > 0 && id >= mine && id < mine + own) {
+        const long long first = TILES ? tile_at : at, own = TILES ? tiles : units;
+        if (own > 0 && id >= first && id < first + own) {
             found[0] = i0 + tid;
-            found[1] = (int)(id - mine);
+            found[1] = (int)(id - first);
+            found[2] = (int)at;
         }
-        before += total;
+        units_before += total;
+        before += TILES ? tile_total : total;
         __syncthreads();
     }
     if (found[0] < 0) return false;
@@ -140,9 +161,33 @@ __device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit
     u.seq = found[0];
     request_work(p, M, u.seq, tiles, span, u);
     const int chunks = (span + u.run - 1) / u.run;
-    u.tile = found[1] / chunks;
-    u.chunk = found[1] - u.tile * chunks;
+    u.tile = TILES ? found[1] : found[1] / chunks;
+    u.chunk = TILES ? 0 : found[1] - u.tile * chunks;
+    u.whole = found[2] + u.tile * chunks;
     return true;
+}
+
+// What a unit works on: rows of the tile, the keys that any of them sees from a multiple of 32 to an end, in how
+// many runs.
+struct Tile {
+    int row0, rows, j0, j1;                  // rows, and the tokens of the first and the last
+    int64_t base;                            // the position of the request's first new token
+    int start, end, chunks;
+};
+
+__device__ __forceinline__ Tile tile_of(const AttnArgs &p, int M, const Unit &u)
+{
+    Tile t;
+    const int group = p.n_head / p.n_head_kv;
+    t.row0 = u.tile * M;
+    t.rows = min(u.m * group - t.row0, M);
+    t.j0 = t.row0 / group;
+    t.j1 = (t.row0 + t.rows - 1) / group;
+    t.base = (int64_t)u.kv - u.m;
+    t.end = (int)max(min(t.base + t.j1 + 1, (int64_t)u.n), (int64_t)0);
+    t.start = p.window ? (int)max(t.base + t.j0 - p.window + 1, (int64_t)0) & ~31 : 0;
+    t.chunks = t.end > t.start ? (int)(((int64_t)t.end - t.start + u.run - 1) / u.run) : 1;
+    return t;
 }
 
 // ---------------------------------------------------------------------------
@@ -203,11 +248,10 @@ template <int DP>
 struct RowsShared {
     float o[4][ROWS_M][128 + 4];
     float m[4][ROWS_M], l[4][ROWS_M];
-    int last;
 };
 
 template <typename T, int DP, bool PAD, bool TINY>
-__global__ void __launch_bounds__(ATT_TPB) k_attn_rows(AttnArgs p)
+__global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnArgs p)
 {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NC = DP / 32;              // operands of a key's row
@@ -216,17 +260,13 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_rows(AttnArgs p)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, h = lane >> 4;
     const int g = blockIdx.x % p.n_head_kv, id = blockIdx.x / p.n_head_kv, group = p.n_head / p.n_head_kv;
     Unit u;
-    if (!find_unit<ATT_TPB>(p, ROWS_M, id, u)) return;
-    const int row0 = u.tile * ROWS_M, rows = min(u.m * group - row0, ROWS_M);
-    // keys that any row sees, from a multiple of 32; those of this unit
-    const int64_t base = (int64_t)u.kv - u.m;                 // the first new token's position
-    const int j0 = row0 / group, j1 = (row0 + rows - 1) / group;
-    const int end = (int)max(min(base + j1 + 1, (int64_t)u.n), (int64_t)0);
-    const int start = p.window ? (int)max(base + j0 - p.window + 1, (int64_t)0) & ~31 : 0;
-    const int chunks = end > start ? (int)(((int64_t)end - start + u.run - 1) / u.run) : 1;
-    if (u.chunk >= chunks) return;
-    const int k0 = (int)min((int64_t)start + (int64_t)u.chunk * u.run, (int64_t)end),
-              k1 = (int)min((int64_t)k0 + u.run, (int64_t)end);
+    if (!find_unit<ATT_TPB, false>(p, ROWS_M, id, u)) return;
+    const Tile tile = tile_of(p, ROWS_M, u);
+    if (u.chunk >= tile.chunks) return;
+    const int row0 = tile.row0, rows = tile.rows, j0 = tile.j0, j1 = tile.j1, chunks = tile.chunks;
+    const int64_t base = tile.base;
+    const int k0 = (int)min((int64_t)tile.start + (int64_t)u.chunk * u.run, (int64_t)tile.end),
+              k1 = (int)min((int64_t)k0 + u.run, (int64_t)tile.end);
 
     // this lane's row: its position, its first key, its q
     const bool live = r < rows;
@@ -276,17 +316,26 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_rows(AttnArgs p)
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = { 0, 0, 0, 0 };
 
-    for (int kb = k0 + 32 * wave; kb < k1; kb += 32 * (ATT_TPB / 64)) {
-        // where the keys lie: for the first product keys r and 16 + r, for the second 4 h .. 4 h + 3 and 16 + those
+    // Blocks of the keys of step kb: for the first product keys r and 16 + r, for the second 4 h .. 4 h + 3 and 16 + those
+    // (one entry each where a block holds at least four rows).  They are looked up one step ahead of the rows.
+    constexpr int NV = TINY ? 8 : 2;
+    int kblock[2], vblock[NV];
+    const auto look_up = [&](int kb) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) kblock[t] = table[min(kb + 16 * t + r, k1 - 1) >> p.log_block];
+#pragma unroll
+        for (int e = 0; e < NV; e++)
+            vblock[e] = table[min(TINY ? kb + 16 * (e / 4) + 4 * h + (e & 3) : kb + 16 * e + 4 * h, k1 - 1) >> p.log_block];
+    };
+    int kb = k0 + 32 * wave;
+    if (kb < k1) look_up(kb);
+    for (; kb < k1; kb += 32 * (ATT_TPB / 64)) {
         f16x8 kf[2][NC];
         i32x4 vf[8][(NT + 7) / 8];
         bool seen[8];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const int key = kb + 16 * t + r;
-            const int block = key < k1 ? table[key >> p.log_block] : -1;
-            const bool ok = (unsigned)block < (unsigned)p.n_blocks;
-            const _Float16 *row = p.k + (ok ? cache_row(p, block, key, g) : 0);
+            const _Float16 *row = p.k + ((unsigned)kblock[t] < (unsigned)p.n_blocks ? cache_row(p, kblock[t], kb + 16 * t + r, g) : 0);
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 f16x8 v = { 0, 0, 0, 0, 0, 0, 0, 0 };
@@ -295,33 +344,31 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_rows(AttnArgs p)
             }
         }
         bool whole = true;                    // every key of the 32 is there
+        const _Float16 *first_v = nullptr;
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            int block = -1;
+        for (int e = 0; e < 8; e++) {
+            const int key = kb + 16 * (e / 4) + 4 * h + (e & 3), block = vblock[TINY ? e : e / 4];
+            seen[e] = key < k1 && (unsigned)block < (unsigned)p.n_blocks;
+            whole &= seen[e];
+            if (TINY || e % 4 == 0)           // (the other three lie behind the first)
+                first_v = p.v + ((unsigned)block < (unsigned)p.n_blocks ? cache_row(p, block, key, g) : 0);
+            const _Float16 *row = first_v + (TINY ? 0 : (e % 4) * (PAD ? p.head_dim : DP));
+            if constexpr (NT == 4) {
+                vf[e][0] = { 0, 0, 0, 0 };
+                if (!PAD || NT * r < p.head_dim) {
+                    const int2 w = *(const int2 *)(row + NT * r);
+                    vf[e][0].x = w.x;
+                    vf[e][0].y = w.y;
+                }
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int key = kb + 16 * t + 4 * h + e;
-                if (e == 0 || TINY) block = key < k1 ? table[key >> p.log_block] : -1;
-                const bool ok = key < k1 && (unsigned)block < (unsigned)p.n_blocks;
-                seen[4 * t + e] = ok;
-                whole &= ok;
-                const _Float16 *row = p.v + (ok ? cache_row(p, block, key, g) : 0);
-                if constexpr (NT == 4) {
-                    vf[4 * t + e][0] = { 0, 0, 0, 0 };
-                    if (!PAD || NT * r < p.head_dim) {
-                        const int2 w = *(const int2 *)(row + NT * r);
-                        vf[4 * t + e][0].x = w.x;
-                        vf[4 * t + e][0].y = w.y;
-                    }
-                } else {
-#pragma unroll
-                    for (int x = 0; x < NT / 8; x++) {
-                        vf[4 * t + e][x] = { 0, 0, 0, 0 };
-                        if (!PAD || NT * r + 8 * x < p.head_dim) vf[4 * t + e][x] = *(const i32x4 *)(row + NT * r + 8 * x);
-                    }
+                for (int x = 0; x < NT / 8; x++) {
+                    vf[e][x] = { 0, 0, 0, 0 };
+                    if (!PAD || NT * r + 8 * x < p.head_dim) vf[e][x] = *(const i32x4 *)(row + NT * r + 8 * x);
                 }
             }
         }
+        look_up(kb + 32 * (ATT_TPB / 64));
 
         f32x4 s[2] = { { 0, 0, 0, 0 }, { 0, 0, 0, 0 } };
 #pragma unroll
@@ -372,10 +419,10 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_rows(AttnArgs p)
             if constexpr (SPLIT) pl[e] = b;
         }
         // operand of output tile t: value t of the lane's eight keys
-        const auto operand = [&](int t) {
+        const auto operand = [&](int t, unsigned odd = 0x07060302u, unsigned even = 0x05040100u) {
             i32x4 a;
             const int x = t / 8, d = t / 2 % 4;
-            const unsigned pick = t & 1 ? 0x07060302u : 0x05040100u;
+            const unsigned pick = t & 1 ? odd : even;
 #pragma unroll
             for (int e = 0; e < 4; e++) a[e] = __builtin_amdgcn_perm(vf[2 * e + 1][x][d], vf[2 * e][x][d], pick);
             return a;
@@ -400,9 +447,11 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_rows(AttnArgs p)
             // an infinity or NaN among them must not meet the weight 0: row by row, without the keys that the row does not see
             for (int n = 0; n < rows; n++) {
                 const int to = __shfl(pos, n), from = __shfl(low, n);
+                unsigned odd = 0x07060302u, even = 0x05040100u;
+                asm volatile("" : "+s"(odd), "+s"(even));     // the operands stay in the loop: there are no registers for all
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    f16x8 a = __builtin_bit_cast(f16x8, operand(t));
+                    f16x8 a = __builtin_bit_cast(f16x8, operand(t, odd, even));
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const int key = kb + 16 * (e / 4) + 4 * h + (e & 3);
@@ -467,60 +516,74 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_rows(AttnArgs p)
             }
         }
     }
-    if (chunks == 1) return;
+}
 
-    // the workgroup that ends last joins the tile's runs, in their order
-    __threadfence();
-    __syncthreads();
-    const int first_id = id - u.chunk;
-    if (tid == 0) {
-        int *ticket = p.tickets + first_id * p.n_head_kv + g;
-        const int old = atomicAdd(ticket, 1);
-        sh.last = old == chunks - 1;
-        if (old == chunks - 1) *ticket = 0;           // as the next launch expects it
-    }
-    __syncthreads();
-    if (!sh.last) return;
-    __threadfence();
-    const int64_t step = (int64_t)p.n_head_kv * (ROWS_M * (DP + 2));
-    const float *from = p.partial + (int64_t)(g + (int64_t)first_id * p.n_head_kv) * (ROWS_M * (DP + 2));
-    for (int x = tid; x < rows * DP; x += ATT_TPB) {
-        const int n = x / DP, d = x % DP;
-        if (d >= p.head_dim) continue;
-        float top_n = -INFINITY, o = 0.0f, sum = 0.0f;
-        for (int c = 0; c < chunks; c++) top_n = fmaxf(top_n, from[c * step + ROWS_M * DP + n]);
-        for (int c = 0; c < chunks; c++) {
-            const float mc = from[c * step + ROWS_M * DP + n], f = mc == -INFINITY ? 1.0f : fast_exp2(mc - top_n);
-            sum += f * from[c * step + ROWS_M * DP + ROWS_M + n];
-            o += f * from[c * step + n * DP + d];
+// ---------------------------------------------------------------------------
+// Tiles of several runs: a workgroup joins the partial results of JOIN_ROWS rows, [M][DP] sums and then every row's
+// maximum and sum of weights, unit after unit of a kv head.  A launch of its own: a device-wide release and acquire
+// in each unit of the split kernel, for the last of a tile to join it, writes back and invalidates its XCD's whole L2
+// and made 1,800 units of 64 streams wait for each other (614 us in place of 186).
+// ---------------------------------------------------------------------------
+
+constexpr int JOIN_ROWS = 4;
+
+template <typename T, int DP, int M>
+__global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
+{
+    constexpr int ITEMS = JOIN_ROWS * (DP / 4), PARTS = ATT_TPB / ITEMS;
+    __shared__ float factor[JOIN_ROWS][512];
+    __shared__ f32x4 sums[ATT_TPB];
+    const int tid = threadIdx.x, parts = (M + JOIN_ROWS - 1) / JOIN_ROWS, group = p.n_head / p.n_head_kv;
+    const int n0 = blockIdx.x % parts * JOIN_ROWS, g = blockIdx.x / parts % p.n_head_kv, id = blockIdx.x / parts / p.n_head_kv;
+    Unit u;
+    if (!find_unit<ATT_TPB, true>(p, M, id, u)) return;
+    const Tile tile = tile_of(p, M, u);
+    const int chunks = tile.chunks;
+    if (chunks == 1 || n0 >= tile.rows) return;
+    const int64_t step = (int64_t)p.n_head_kv * (M * (DP + 2));
+    const float *from = p.partial + (int64_t)(g + (int64_t)u.whole * p.n_head_kv) * (M * (DP + 2));
+    {
+        // each run's factor: 2^(its maximum - the largest) / sum of weights; a wave a row
+        const int lane = tid & 63, n = tid >> 6;
+        const float *f = from + M * DP + n0 + n;
+        float top = -INFINITY, sum = 0.0f;
+        for (int c = lane; c < chunks; c += 64) top = fmaxf(top, f[c * step]);
+        for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+        for (int c = lane; c < chunks; c += 64) {
+            const float m = f[c * step], x = m == -INFINITY ? 1.0f : fast_exp2(m - top);
+            factor[n][c] = x;
+            sum += x * f[c * step + M];
         }
-        const int j = (row0 + n) / group, a = (row0 + n) % group;
-        T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim;
-        out[d] = (T)(sum == 0.0f ? 0.0f : o / sum);
+        for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
+        const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int c = lane; c < chunks; c += 64) factor[n][c] *= by;
     }
-}
-
-template <typename T, int DP>
-static void rows_launch(const AttnArgs &p, dim3 grid, hipStream_t s)
-{
-    const bool pad = p.head_dim != DP, tiny = p.log_block < 2;
-    if (tiny) hipLaunchKernelGGL((k_attn_rows<T, DP, true, true>), grid, ATT_TPB, 0, s, p);
-    else if (pad) hipLaunchKernelGGL((k_attn_rows<T, DP, true, false>), grid, ATT_TPB, 0, s, p);
-    else hipLaunchKernelGGL((k_attn_rows<T, DP, false, false>), grid, ATT_TPB, 0, s, p);
-}
-
-template <typename T>
-static void rows_dim(const AttnArgs &p, dim3 grid, hipStream_t s)
-{
-    if (p.head_dim <= 64) rows_launch<T, 64>(p, grid, s);
-    else if (p.head_dim <= 128) rows_launch<T, 128>(p, grid, s);
-    else rows_launch<T, 256>(p, grid, s);
+    __syncthreads();
+    const int item = tid % ITEMS, part = tid / ITEMS, n = item / (DP / 4), d = item % (DP / 4) * 4;
+    const float *f = from + (int64_t)(n0 + n) * DP + d;
+    f32x4 o = { 0, 0, 0, 0 };
+    if (part < PARTS) {
+#pragma unroll 8
+        for (int c = part; c < chunks; c += PARTS) o += factor[n][c] * *(const f32x4 *)(f + c * step);
+    }
+    if constexpr (PARTS > 1) {
+        sums[tid] = o;
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int i = 1; i < PARTS; i++) o += sums[i * ITEMS + item];
+    }
+    if (n0 + n >= tile.rows || d >= p.head_dim) return;
+    const int j = (tile.row0 + n0 + n) / group, a = (tile.row0 + n0 + n) % group;
+    T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim + d;
+#pragma unroll
+    for (int i = 0; i < 4; i++) out[i] = (T)o[i];
 }
 
 static int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
 // Units a kv head that the work is split into where there are fewer tiles.
-static int rows_target(const AttnArgs &p) { return std::max(1, ATT_MAX_UNITS / 2 / p.n_head_kv); }
+static int rows_target(const AttnArgs &p) { return std::max(1, ATT_MAX_UNITS / p.n_head_kv); }
 
 // Tiles of at most M rows that n_seq requests with n_tokens tokens in all can have.
 static int64_t most_tiles(const AttnArgs &p, int M)
@@ -530,8 +593,39 @@ static int64_t most_tiles(const AttnArgs &p, int M)
 
 size_t attention_workspace(const AttnArgs &p)
 {
-    // units of split tiles: fewer than `target` tiles, and as many runs beyond one each
+    // split tiles are fewer than `target`, and so are their units; twice that where a unit ends at 2^30 keys
     return (size_t)2 * rows_target(p) * p.n_head_kv * ROWS_M * (padded_dim(p.head_dim) + 2) * sizeof(float);
+}
+
+template <typename T, int DP>
+static hipError_t rows_launch(AttnArgs p, hipStream_t s)
+{
+    p.min_rows = 0;
+    p.max_rows = 0x7fffffff;
+    p.target = rows_target(p);
+    // (at most 512 runs a tile, whatever the lengths)
+    p.least = 128;
+    const int64_t longest = (int64_t)p.max_blocks << p.log_block;
+    while (longest / p.least >= 512) p.least *= 2;
+    const int64_t tiles = most_tiles(p, ROWS_M), units = (tiles + p.target) * p.n_head_kv;
+    if (units > 0x7fffff) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)units);
+    if (p.log_block < 2) hipLaunchKernelGGL((k_attn_rows<T, DP, true, true>), grid, ATT_TPB, 0, s, p);
+    else if (p.head_dim != DP) hipLaunchKernelGGL((k_attn_rows<T, DP, true, false>), grid, ATT_TPB, 0, s, p);
+    else hipLaunchKernelGGL((k_attn_rows<T, DP, false, false>), grid, ATT_TPB, 0, s, p);
+    if (longest > p.least) {                  // only fewer than `target` tiles are split
+        const int64_t wgs = std::min<int64_t>(tiles, p.target) * p.n_head_kv * (ROWS_M / JOIN_ROWS);
+        hipLaunchKernelGGL((k_attn_join<T, DP, ROWS_M>), dim3((unsigned)wgs), ATT_TPB, 0, s, p);
+    }
+    return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t attention_dim(const AttnArgs &p, hipStream_t s)
+{
+    if (p.head_dim <= 64) return rows_launch<T, 64>(p, s);
+    if (p.head_dim <= 128) return rows_launch<T, 128>(p, s);
+    return rows_launch<T, 256>(p, s);
 }
 
 hipError_t launch_attention(AttnArgs p, int type, hipStream_t s)
@@ -539,15 +633,7 @@ hipError_t launch_attention(AttnArgs p, int type, hipStream_t s)
     // S = q . k takes |scale|; its sign goes to q, and scale 0 makes q 0
     p.q_sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
     p.scale = p.scale == 0.0f ? 1.0f : std::fabs(p.scale) * 1.44269504088896340736f;
-    p.min_rows = 0;
-    p.max_rows = 0x7fffffff;
-    p.target = rows_target(p);
-    p.least = 128;
-    const int64_t units = (most_tiles(p, ROWS_M) + p.target) * p.n_head_kv;
-    if (units > 0x7fffff) return hipErrorInvalidValue;
-    if (type == T_F32) rows_dim<float>(p, dim3((unsigned)units), s);
-    else rows_dim<_Float16>(p, dim3((unsigned)units), s);
-    return hipGetLastError();
+    return type == T_F32 ? attention_dim<float>(p, s) : attention_dim<_Float16>(p, s);
 }
 
 }  // namespace ds3k

@@ -349,12 +349,11 @@ struct AttnArgs {
     float scale;
     int window;                          // 0: none
     float *partial;                      // attention_workspace bytes
-    int *tickets;                        // ATT_MAX_UNITS, zero between launches
     // the launcher's: requests of min_rows .. max_rows rows, units a kv head, keys a unit, q's factor
     int min_rows, max_rows, target, least;
     float q_sign;
 };
-constexpr int ATT_MAX_UNITS = 4096;
+constexpr int ATT_MAX_UNITS = 2048;              // about as many units split tiles make, over all kv heads
 size_t attention_workspace(const AttnArgs &p);
 hipError_t launch_attention(AttnArgs p, int type, hipStream_t s);
 

@@ -43,6 +43,7 @@ struct Unit {
 };
 
 constexpr int ATT_TPB = 256;
+constexpr int ATT_FEW_ROWS = 64;             // requests of up to so many rows take tiles of 16
 
 __device__ __forceinline__ long long wave_sum(long long v)
 {
@@ -93,6 +94,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit
         u.tile = TILES ? id : id / chunks;
         u.whole = u.tile * chunks;
         u.chunk = TILES ? 0 : id - u.whole;
+        u.tile = tiles - 1 - u.tile;                  // (the last tiles, which see most keys, begin first)
         return true;
     }
     long long work = 0, all = 0;
@@ -164,6 +166,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit
     u.tile = TILES ? found[1] : found[1] / chunks;
     u.chunk = TILES ? 0 : found[1] - u.tile * chunks;
     u.whole = found[2] + u.tile * chunks;
+    u.tile = tiles - 1 - u.tile;
     return true;
 }
 
@@ -519,6 +522,297 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
 }
 
 // ---------------------------------------------------------------------------
+// Many rows: tiles of 32 a wave.  The workgroup stages KT keys at a time in LDS, twice (the next keys' loads run
+// beside the products); a wave multiplies them with its 32 rows on 32 x 32 x 16 matrix products.  Rows of both tiles
+// lie DP values apart in chunks of 16 bytes whose index is xored with bits of the key, so that eight lanes that read
+// one chunk of eight keys (k), and 32 that read 64 bytes of four keys (v), meet no bank twice.  V is transposed on its
+// way from LDS (ds_read_b64_tr_b16: a lane gets one value of four keys).
+// ---------------------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+template <int DP>
+struct TileShape {
+    static constexpr int WAVES = DP == 256 ? 4 : 8, M = 32 * WAVES, TPB = 64 * WAVES;
+    static constexpr int KT = DP == 256 ? 32 : 64;       // keys staged at a time
+};
+
+template <int DP>
+__device__ __forceinline__ int k_chunk(int key, int chunk) { return chunk ^ (key & 7); }
+template <int DP>
+__device__ __forceinline__ int v_chunk(int key, int chunk) { return chunk ^ (DP == 64 ? (key >> 1 & 1) << 2 : (key & 3) << 2); }
+
+template <typename T, int DP, bool PAD>
+__global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_tiles(AttnArgs p)
+{
+    using S = TileShape<DP>;
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int NC = DP / 16, NT = DP / 32, KT = S::KT, NS = KT / 32, CH = DP / 8;
+    constexpr int NL = KT * CH / S::TPB;      // chunks of each tile a thread stages
+    __shared__ __attribute__((aligned(1024))) _Float16 lk[2][KT * DP], lv[2][KT * DP];
+    __shared__ uint8_t flags[2][64];          // of each staged key: 1 there, 2 a value of v that is not finite
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, h = lane >> 5;
+    const int g = blockIdx.x % p.n_head_kv, id = blockIdx.x / p.n_head_kv, group = p.n_head / p.n_head_kv;
+    Unit u;
+    if (!find_unit<S::TPB, false>(p, S::M, id, u)) return;
+    const Tile tile = tile_of(p, S::M, u);
+    if (u.chunk >= tile.chunks) return;
+    const int64_t base = tile.base;
+    const int k0 = (int)min((int64_t)tile.start + (int64_t)u.chunk * u.run, (int64_t)tile.end),
+              k1 = (int)min((int64_t)k0 + u.run, (int64_t)tile.end);
+    const int32_t *table = p.table + (int64_t)u.seq * p.max_blocks;
+
+    // staging: the blocks of this thread's keys of step kb, then their chunks
+    int blocks[NL];
+    i32x4 sk[NL], sv[NL];
+    uint32_t there = 0;
+    const auto look_up = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) blocks[i] = table[min(kb + (tid + i * S::TPB) / CH, k1 - 1) >> p.log_block];
+    };
+    const auto load = [&](int kb) {
+        there = 0;
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int x = tid + i * S::TPB, key = kb + x / CH, c = x % CH;
+            sk[i] = { 0, 0, 0, 0 };
+            sv[i] = { 0, 0, 0, 0 };
+            if (key < k1 && (unsigned)blocks[i] < (unsigned)p.n_blocks) {
+                there |= 1u << i;
+                const int64_t at = cache_row(p, blocks[i], key, g) + 8 * c;
+                if (!PAD || 8 * c < p.head_dim) {
+                    sk[i] = *(const i32x4 *)(p.k + at);
+                    sv[i] = *(const i32x4 *)(p.v + at);
+                }
+            }
+        }
+    };
+    const auto store = [&](int buf, int kb) {
+        const bool edge = kb + KT - 1 > base + tile.j0 || p.window;       // some rows see keys that others do not
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int x = tid + i * S::TPB, key = x / CH, c = x % CH;
+            *(i32x4 *)&lk[buf][key * DP + 8 * k_chunk<DP>(key, c)] = sk[i];
+            *(i32x4 *)&lv[buf][key * DP + 8 * v_chunk<DP>(key, c)] = sv[i];
+            // (the CH lanes of a key lie in one wave)
+            bool bad = false;
+            if (edge) {
+#pragma unroll
+                for (int d = 0; d < 4; d++) bad |= !finite_pair(sv[i][d]);
+            }
+            const uint64_t any = __ballot(bad);
+            if (c == 0) flags[buf][key] = (there >> i & 1) | ((any >> (lane & ~(CH - 1)) & ((1ull << CH) - 1)) != 0 ? 2 : 0);
+        }
+    };
+
+    if (k0 < k1) {
+        look_up(k0);
+        load(k0);
+        look_up(k0 + KT);
+    }
+
+    // this lane's row
+    const int row = wave * 32 + r;
+    const bool live = row < tile.rows;
+    const int my_row = tile.row0 + (live ? row : 0), my_j = my_row / group, my_h = my_row % group;
+    const int pos = live ? (int)(base + my_j) : -1;
+    const int low = p.window ? pos - p.window + 1 : 0;
+    const T *q = (const T *)((const uint8_t *)p.q + (uint64_t)(u.first + my_j) * p.q_stride) +
+                 (int64_t)(g * group + my_h) * p.head_dim;
+    f16x8 qh[NC], ql[SPLIT ? NC : 1];
+    float c2 = p.scale;
+    if constexpr (SPLIT) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+            if (live && (!PAD || 16 * c + 8 * h < p.head_dim)) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(q[16 * c + 8 * h + e] * p.q_sign));
+            }
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int ex = row_exponent(amax);
+        c2 = mul_pow2(c2, -ex);
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = live && (!PAD || 16 * c + 8 * h < p.head_dim) ? q[16 * c + 8 * h + e] * p.q_sign : 0.0f;
+                _Float16 a, b;
+                split(mul_pow2(v, ex), a, b);
+                qh[c][e] = a;
+                ql[c][e] = b;
+            }
+    } else {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            f16x8 v = { 0, 0, 0, 0, 0, 0, 0, 0 };
+            if (live && (!PAD || 16 * c + 8 * h < p.head_dim)) v = *(const f16x8 *)(q + 16 * c + 8 * h);
+            qh[c] = v * (_Float16)p.q_sign;
+        }
+    }
+    // the wave's rows: positions from w_first to w_last; keys that all of them see end at w_first
+    const int w_rows = min(tile.rows - wave * 32, 32);
+    const int64_t w_first = base + (tile.row0 + wave * 32) / group, w_last = base + (tile.row0 + wave * 32 + w_rows - 1) / group;
+    const int64_t w_from = p.window ? w_last - p.window + 1 : 0, w_low = p.window ? w_first - p.window + 1 : 0;
+
+    float m = -INFINITY, l = 0.0f;
+    f32x16 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[t][i] = 0.0f;
+
+    const int k_row = r * DP, s16 = lane & 15;
+    const int v_row = (4 * h + (s16 >> 2)) * DP, v_in = 2 * (lane >> 4 & 1) + (s16 & 3) / 2, v_half = 4 * (s16 & 1);
+
+    if (k0 < k1) store(0, k0);
+    __syncthreads();
+    int buf = 0;
+    for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
+        const bool more = kb + KT < k1;
+        if (more) {
+            load(kb + KT);
+            look_up(kb + 2 * KT);
+        }
+        if (w_rows > 0 && kb <= w_last && kb + KT - 1 >= w_low) {
+            f32x16 s[NS];
+#pragma unroll
+            for (int n = 0; n < NS; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int n = 0; n < NS; n++) {
+                    const f16x8 a = *(const f16x8 *)&lk[buf][32 * n * DP + k_row + 8 * k_chunk<DP>(r, 2 * c + h)];
+                    s[n] = mfma32(a, qh[c], s[n]);
+                    if constexpr (SPLIT) s[n] = mfma32(a, ql[c], s[n]);
+                }
+            const int flag = lane < KT ? flags[buf][lane] : 1;
+            const uint64_t seen = __ballot(flag & 1), odd = __ballot(flag & 2);
+            const bool plain = ~seen == 0 && kb >= w_from && kb + KT - 1 <= w_first;
+            if (!plain) {
+#pragma unroll
+                for (int n = 0; n < NS; n++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int k = 32 * n + 8 * (i / 4) + 4 * h + (i & 3);
+                        if (!((seen >> k & 1) && kb + k <= pos && kb + k >= low)) s[n][i] = -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NS; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
+            top *= c2;
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > m + ATT_LAG)) {
+                const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 1.0f : fast_exp2(m - m2);
+                m = m2;
+                l *= keep;
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[t] *= keep;
+            }
+            const float less = m == -INFINITY ? 0.0f : m - ATT_SHIFT;
+            f16x8 ph[2 * NS], pl[SPLIT ? 2 * NS : 1];
+#pragma unroll
+            for (int n = 0; n < NS; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float w = fast_exp2(__builtin_fmaf(s[n][i], c2, -less));
+                    l += w;
+                    _Float16 a, b;
+                    split(w, a, b);
+                    ph[2 * n + i / 8][i % 8] = a;
+                    if constexpr (SPLIT) pl[2 * n + i / 8][i % 8] = b;
+                }
+            // operand t of 16 keys: a value of each of the keys 4 h .. + 3 and 8 + 4 h .. + 3
+            const auto operand = [&](int t, int k16) {
+                const int at = 16 * k16 * DP + v_row + 8 * ((4 * t + v_in) ^ (v_chunk<DP>(4 * h + (s16 >> 2), 0))) + v_half;
+                union {
+                    s16x4 part[2];
+                    f16x8 whole;
+                } a;
+                a.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at]);
+                a.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at + 8 * DP]);
+                return a.whole;
+            };
+            if (plain || odd == 0 || w_first == w_last) {
+#pragma unroll
+                for (int k16 = 0; k16 < 2 * NS; k16++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const f16x8 a = operand(t, k16);
+                        acc[t] = mfma32(a, ph[k16], acc[t]);
+                        if constexpr (SPLIT) acc[t] = mfma32(a, pl[k16], acc[t]);
+                    }
+            } else {
+                // an infinity or NaN must not meet the weight 0: row by row, without the keys that the row does not see
+#pragma unroll 1
+                for (int n = 0; n < w_rows; n++) {
+                    const int to = __shfl(pos, n), from = __shfl(low, n);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        f32x16 o = acc[t];
+#pragma unroll
+                        for (int k16 = 0; k16 < 2 * NS; k16++) {
+                            f16x8 a = operand(t, k16);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                const int key = kb + 16 * k16 + 8 * (e / 4) + 4 * h + (e & 3);
+                                if (key > to || key < from) a[e] = (_Float16)0.0f;
+                            }
+                            o = mfma32(a, ph[k16], o);
+                            if constexpr (SPLIT) o = mfma32(a, pl[k16], o);
+                        }
+                        if (r == n) acc[t] = o;
+                    }
+                }
+            }
+        }
+        if (more) store(buf ^ 1, kb + KT);
+        __syncthreads();
+    }
+
+    l += __shfl_xor(l, 32);
+    if (!live) return;
+    if (tile.chunks == 1) {
+        const float by = l == 0.0f ? 0.0f : 1.0f / l;
+        T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + my_j) * p.out_stride) + (int64_t)(g * group + my_h) * p.head_dim;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const int d = 32 * t + 8 * b + 4 * h;
+                if (PAD && d >= p.head_dim) continue;
+                typedef T vec4 __attribute__((ext_vector_type(4)));
+                vec4 v;
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] = (T)(acc[t][4 * b + j] * by);
+                *(vec4 *)(out + d) = v;
+            }
+    } else {
+        float *ws = p.partial + (int64_t)(g + (int64_t)id * p.n_head_kv) * (S::M * (DP + 2));
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const f32x4 v = { acc[t][4 * b], acc[t][4 * b + 1], acc[t][4 * b + 2], acc[t][4 * b + 3] };
+                *(f32x4 *)(ws + row * DP + 32 * t + 8 * b + 4 * h) = v;
+            }
+        if (h == 0) {
+            ws[S::M * DP + row] = m;
+            ws[S::M * DP + S::M + row] = l;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
 // Tiles of several runs: a workgroup joins the partial results of JOIN_ROWS rows, [M][DP] sums and then every row's
 // maximum and sum of weights, unit after unit of a kv head.  A launch of its own: a device-wide release and acquire
 // in each unit of the split kernel, for the last of a tile to join it, writes back and invalidates its XCD's whole L2
@@ -582,8 +876,9 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
 
 static int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
-// Units a kv head that the work is split into where there are fewer tiles.
-static int rows_target(const AttnArgs &p) { return std::max(1, ATT_MAX_UNITS / p.n_head_kv); }
+// Units a kv head that the work is split into where there are fewer tiles: several a compute unit of few rows, one of
+// many.
+static int target_units(const AttnArgs &p, bool many) { return std::max(1, (many ? 256 : 2048) / p.n_head_kv); }
 
 // Tiles of at most M rows that n_seq requests with n_tokens tokens in all can have.
 static int64_t most_tiles(const AttnArgs &p, int M)
@@ -594,38 +889,59 @@ static int64_t most_tiles(const AttnArgs &p, int M)
 size_t attention_workspace(const AttnArgs &p)
 {
     // split tiles are fewer than `target`, and so are their units; twice that where a unit ends at 2^30 keys
-    return (size_t)2 * rows_target(p) * p.n_head_kv * ROWS_M * (padded_dim(p.head_dim) + 2) * sizeof(float);
+    const int dp = padded_dim(p.head_dim), many = dp == 256 ? TileShape<256>::M : TileShape<128>::M;
+    const size_t units = std::max((size_t)target_units(p, false) * ROWS_M, (size_t)target_units(p, true) * many);
+    return 2 * units * p.n_head_kv * (dp + 2) * sizeof(float);
 }
 
-template <typename T, int DP>
-static hipError_t rows_launch(AttnArgs p, hipStream_t s)
+// The requests of min_rows .. max_rows rows, as tiles of at most 16 (MANY: TileShape::M).
+template <typename T, int DP, bool MANY>
+static hipError_t attention_rows(AttnArgs p, int min_rows, int max_rows, hipStream_t s)
 {
-    p.min_rows = 0;
-    p.max_rows = 0x7fffffff;
-    p.target = rows_target(p);
+    using S = TileShape<DP>;
+    constexpr int M = MANY ? S::M : ROWS_M, TPB = MANY ? S::TPB : ATT_TPB;
+    p.min_rows = min_rows;
+    p.max_rows = max_rows;
+    p.target = target_units(p, MANY);
     // (at most 512 runs a tile, whatever the lengths)
-    p.least = 128;
+    p.least = MANY ? 512 : 128;
     const int64_t longest = (int64_t)p.max_blocks << p.log_block;
     while (longest / p.least >= 512) p.least *= 2;
-    const int64_t tiles = most_tiles(p, ROWS_M), units = (tiles + p.target) * p.n_head_kv;
+    const int64_t tiles = most_tiles(p, M), units = (tiles + p.target) * p.n_head_kv;
     if (units > 0x7fffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)units);
-    if (p.log_block < 2) hipLaunchKernelGGL((k_attn_rows<T, DP, true, true>), grid, ATT_TPB, 0, s, p);
-    else if (p.head_dim != DP) hipLaunchKernelGGL((k_attn_rows<T, DP, true, false>), grid, ATT_TPB, 0, s, p);
-    else hipLaunchKernelGGL((k_attn_rows<T, DP, false, false>), grid, ATT_TPB, 0, s, p);
+    if constexpr (MANY) {
+        if (p.head_dim != DP) hipLaunchKernelGGL((k_attn_tiles<T, DP, true>), grid, TPB, 0, s, p);
+        else hipLaunchKernelGGL((k_attn_tiles<T, DP, false>), grid, TPB, 0, s, p);
+    } else if (p.log_block < 2) hipLaunchKernelGGL((k_attn_rows<T, DP, true, true>), grid, TPB, 0, s, p);
+    else if (p.head_dim != DP) hipLaunchKernelGGL((k_attn_rows<T, DP, true, false>), grid, TPB, 0, s, p);
+    else hipLaunchKernelGGL((k_attn_rows<T, DP, false, false>), grid, TPB, 0, s, p);
     if (longest > p.least) {                  // only fewer than `target` tiles are split
-        const int64_t wgs = std::min<int64_t>(tiles, p.target) * p.n_head_kv * (ROWS_M / JOIN_ROWS);
-        hipLaunchKernelGGL((k_attn_join<T, DP, ROWS_M>), dim3((unsigned)wgs), ATT_TPB, 0, s, p);
+        const int64_t wgs = std::min<int64_t>(tiles, p.target) * p.n_head_kv * (M / JOIN_ROWS);
+        hipLaunchKernelGGL((k_attn_join<T, DP, M>), dim3((unsigned)wgs), ATT_TPB, 0, s, p);
     }
     return hipGetLastError();
 }
 
-template <typename T>
+// Few rows and many rows are a launch each, the choice a request's own.  A step of single tokens (no more tokens
+// than requests) needs only the first, a single request only one of them.
+template <typename T, int DP>
 static hipError_t attention_dim(const AttnArgs &p, hipStream_t s)
 {
-    if (p.head_dim <= 64) return rows_launch<T, 64>(p, s);
-    if (p.head_dim <= 128) return rows_launch<T, 128>(p, s);
-    return rows_launch<T, 256>(p, s);
+    constexpr int FEW = ATT_FEW_ROWS;
+    const int64_t rows = (int64_t)p.n_tokens * (p.n_head / p.n_head_kv);
+    if (p.n_tokens <= p.n_seq || rows <= FEW) return attention_rows<T, DP, false>(p, 0, 0x7fffffff, s);
+    if (p.n_seq == 1) return attention_rows<T, DP, true>(p, 0, 0x7fffffff, s);
+    const hipError_t e = attention_rows<T, DP, true>(p, FEW + 1, 0x7fffffff, s);
+    return e != hipSuccess ? e : attention_rows<T, DP, false>(p, 0, FEW, s);
+}
+
+template <typename T>
+static hipError_t attention_type(const AttnArgs &p, hipStream_t s)
+{
+    if (p.head_dim <= 64) return attention_dim<T, 64>(p, s);
+    if (p.head_dim <= 128) return attention_dim<T, 128>(p, s);
+    return attention_dim<T, 256>(p, s);
 }
 
 hipError_t launch_attention(AttnArgs p, int type, hipStream_t s)
@@ -633,7 +949,7 @@ hipError_t launch_attention(AttnArgs p, int type, hipStream_t s)
     // S = q . k takes |scale|; its sign goes to q, and scale 0 makes q 0
     p.q_sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
     p.scale = p.scale == 0.0f ? 1.0f : std::fabs(p.scale) * 1.44269504088896340736f;
-    return type == T_F32 ? attention_dim<float>(p, s) : attention_dim<_Float16>(p, s);
+    return type == T_F32 ? attention_type<float>(p, s) : attention_type<_Float16>(p, s);
 }
 
 }  // namespace ds3k

@@ -353,7 +353,6 @@ struct AttnArgs {
     int min_rows, max_rows, target, least;
     float q_sign;
 };
-constexpr int ATT_MAX_UNITS = 2048;              // about as many units split tiles make, over all kv heads
 size_t attention_workspace(const AttnArgs &p);
 hipError_t launch_attention(AttnArgs p, int type, hipStream_t s);
 

@@ -225,9 +225,23 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __bu
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ __forceinline__ bool finite_pair(int w)
+// Two values of v, those that are not finite made 0; `bad` tells of one.
+__device__ __forceinline__ int finite_pair(int w, bool &bad)
 {
-    return (w & 0x7c00) != 0x7c00 && (w & 0x7c000000) != 0x7c000000;
+    const int keep = ((w & 0x7c00) != 0x7c00 ? 0xffff : 0) | ((w & 0x7c000000) != 0x7c000000 ? (int)0xffff0000 : 0);
+    bad |= keep != -1;
+    return w & keep;
+}
+
+// Four values of a row of v where they are not finite, else 0.
+__device__ __forceinline__ f32x4 odd_values(const _Float16 *v)
+{
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    const f16x4 x = *(const f16x4 *)v;
+    f32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = __builtin_fabsf((float)x[i]) < INFINITY ? 0.0f : (float)x[i];
+    return o;
 }
 
 // The row of a cache that holds position `key` (of kv head g): its first value's index, or -1.
@@ -421,50 +435,47 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
             ph[e] = a;
             if constexpr (SPLIT) pl[e] = b;
         }
-        // operand of output tile t: value t of the lane's eight keys
-        const auto operand = [&](int t, unsigned odd = 0x07060302u, unsigned even = 0x05040100u) {
-            i32x4 a;
-            const int x = t / 8, d = t / 2 % 4;
-            const unsigned pick = t & 1 ? odd : even;
+        if (!plain && j1 > j0) {
+            // Keys that some rows see and others do not: an infinity or NaN of theirs must not meet a weight 0.  It is
+            // left out of the product and added to the rows that see it.
+            uint32_t odd = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) a[e] = __builtin_amdgcn_perm(vf[2 * e + 1][x][d], vf[2 * e][x][d], pick);
-            return a;
-        };
-        bool finite = true;
-        if (!plain && j1 > j0) {              // keys that some rows see and others do not
-#pragma unroll
-            for (int e = 0; e < 8; e++)
+            for (int e = 0; e < 8; e++) {
+                bool bad = false;
 #pragma unroll
                 for (int x = 0; x < (NT + 7) / 8; x++)
 #pragma unroll
-                    for (int d = 0; d < (NT == 4 ? 2 : 4); d++) finite &= finite_pair(vf[e][x][d]);
-        }
-        if (__all(finite)) {
+                    for (int d = 0; d < (NT == 4 ? 2 : 4); d++) vf[e][x][d] = finite_pair(vf[e][x][d], bad);
+                const uint64_t any = __ballot(bad);
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const f16x8 a = __builtin_bit_cast(f16x8, operand(t));
-                acc[t] = mfma16(a, ph, acc[t]);
-                if constexpr (SPLIT) acc[t] = mfma16(a, pl, acc[t]);
+                for (int i = 0; i < 4; i++)
+                    if (any >> (16 * i) & 0xffff) odd |= 1u << (16 * (e / 4) + 4 * i + (e & 3));
             }
-        } else {
-            // an infinity or NaN among them must not meet the weight 0: row by row, without the keys that the row does not see
-            for (int n = 0; n < rows; n++) {
-                const int to = __shfl(pos, n), from = __shfl(low, n);
-                unsigned odd = 0x07060302u, even = 0x05040100u;
-                asm volatile("" : "+s"(odd), "+s"(even));     // the operands stay in the loop: there are no registers for all
+            for (; odd != 0; odd &= odd - 1) {
+                const int key = kb + __builtin_ctz(odd);
+                const _Float16 *row = p.v + cache_row(p, table[key >> p.log_block], key, g) + h * (DP / 4);
+                if (key > pos || key < low) continue;
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    f16x8 a = __builtin_bit_cast(f16x8, operand(t, odd, even));
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int key = kb + 16 * (e / 4) + 4 * h + (e & 3);
-                        if (key > to || key < from) a[e] = (_Float16)0.0f;
+                    for (int t = 0; t < NT; t += 4) {
+                        if (PAD && h * (DP / 4) + i * NT + t >= p.head_dim) continue;
+                        const f32x4 o = odd_values(row + i * NT + t);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) acc[t + j][i] += o[j];
                     }
-                    f32x4 o = mfma16(a, ph, acc[t]);
-                    if constexpr (SPLIT) o = mfma16(a, pl, o);
-                    if (r == n) acc[t] = o;
-                }
             }
+        }
+        // operand of output tile t: value t of the lane's eight keys
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            i32x4 a;
+            const unsigned pick = t & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                a[e] = __builtin_amdgcn_perm(vf[2 * e + 1][t / 8][t / 2 % 4], vf[2 * e][t / 8][t / 2 % 4], pick);
+            acc[t] = mfma16(__builtin_bit_cast(f16x8, a), ph, acc[t]);
+            if constexpr (SPLIT) acc[t] = mfma16(__builtin_bit_cast(f16x8, a), pl, acc[t]);
         }
     }
 
@@ -551,10 +562,10 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
 {
     using S = TileShape<DP>;
     constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int NC = DP / 16, NT = DP / 32, KT = S::KT, NS = KT / 32, CH = DP / 8;
+    constexpr int NC = DP / 16, NT = DP / 32, KT = S::KT, NS = SPLIT || DP == 256 ? 1 : 2, CH = DP / 8;
     constexpr int NL = KT * CH / S::TPB;      // chunks of each tile a thread stages
     __shared__ __attribute__((aligned(1024))) _Float16 lk[2][KT * DP], lv[2][KT * DP];
-    __shared__ uint8_t flags[2][64];          // of each staged key: 1 there, 2 a value of v that is not finite
+    __shared__ uint8_t flags[2][64];          // of each staged key: 1 there, 2 values of v left out that are not finite
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, h = lane >> 5;
     const int g = blockIdx.x % p.n_head_kv, id = blockIdx.x / p.n_head_kv, group = p.n_head / p.n_head_kv;
     Unit u;
@@ -592,19 +603,19 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
         }
     };
     const auto store = [&](int buf, int kb) {
-        const bool edge = kb + KT - 1 > base + tile.j0 || p.window;       // some rows see keys that others do not
+        // where some rows see keys that others do not, an infinity or NaN of v must not meet a weight 0: it is left out
+        const bool edge = kb + KT - 1 > base + tile.j0 || p.window;
 #pragma unroll
         for (int i = 0; i < NL; i++) {
             const int x = tid + i * S::TPB, key = x / CH, c = x % CH;
-            *(i32x4 *)&lk[buf][key * DP + 8 * k_chunk<DP>(key, c)] = sk[i];
-            *(i32x4 *)&lv[buf][key * DP + 8 * v_chunk<DP>(key, c)] = sv[i];
-            // (the CH lanes of a key lie in one wave)
             bool bad = false;
             if (edge) {
 #pragma unroll
-                for (int d = 0; d < 4; d++) bad |= !finite_pair(sv[i][d]);
+                for (int d = 0; d < 4; d++) sv[i][d] = finite_pair(sv[i][d], bad);
             }
-            const uint64_t any = __ballot(bad);
+            *(i32x4 *)&lk[buf][key * DP + 8 * k_chunk<DP>(key, c)] = sk[i];
+            *(i32x4 *)&lv[buf][key * DP + 8 * v_chunk<DP>(key, c)] = sv[i];
+            const uint64_t any = __ballot(bad);               // (the CH lanes of a key lie in one wave)
             if (c == 0) flags[buf][key] = (there >> i & 1) | ((any >> (lane & ~(CH - 1)) & ((1ull << CH) - 1)) != 0 ? 2 : 0);
         }
     };
@@ -679,100 +690,89 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
             look_up(kb + 2 * KT);
         }
         if (w_rows > 0 && kb <= w_last && kb + KT - 1 >= w_low) {
-            f32x16 s[NS];
-#pragma unroll
-            for (int n = 0; n < NS; n++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int n = 0; n < NS; n++) {
-                    const f16x8 a = *(const f16x8 *)&lk[buf][32 * n * DP + k_row + 8 * k_chunk<DP>(r, 2 * c + h)];
-                    s[n] = mfma32(a, qh[c], s[n]);
-                    if constexpr (SPLIT) s[n] = mfma32(a, ql[c], s[n]);
-                }
             const int flag = lane < KT ? flags[buf][lane] : 1;
-            const uint64_t seen = __ballot(flag & 1), odd = __ballot(flag & 2);
-            const bool plain = ~seen == 0 && kb >= w_from && kb + KT - 1 <= w_first;
-            if (!plain) {
+            const uint64_t there_all = __ballot(flag & 1);
+            uint64_t odd = __ballot(flag & 2);
+            for (; odd != 0; odd &= odd - 1) {
+                const int key = kb + __builtin_ctzll(odd);
+                const _Float16 *v = p.v + cache_row(p, table[key >> p.log_block], key, g) + 4 * h;
+                if (key > pos || key < low) continue;
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        if (PAD && 32 * t + 8 * b + 4 * h >= p.head_dim) continue;
+                        const f32x4 o = odd_values(v + 32 * t + 8 * b);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) acc[t][4 * b + j] += o[j];
+                    }
+            }
+#pragma unroll
+            for (int sub = 0; sub < KT; sub += 32 * NS) {
+                f32x16 s[NS];
+#pragma unroll
+                for (int n = 0; n < NS; n++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int n = 0; n < NS; n++) {
+                        const f16x8 a = *(const f16x8 *)&lk[buf][(sub + 32 * n) * DP + k_row + 8 * k_chunk<DP>(r, 2 * c + h)];
+                        s[n] = mfma32(a, qh[c], s[n]);
+                        if constexpr (SPLIT) s[n] = mfma32(a, ql[c], s[n]);
+                    }
+                if (~there_all != 0 || kb < w_from || kb + KT - 1 > w_first) {
+#pragma unroll
+                    for (int n = 0; n < NS; n++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int k = sub + 32 * n + 8 * (i / 4) + 4 * h + (i & 3);
+                            if (!((there_all >> k & 1) && kb + k <= pos && kb + k >= low)) s[n][i] = -INFINITY;
+                        }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NS; n++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
+                top *= c2;
+                top = fmaxf(top, __shfl_xor(top, 32));
+                if (__any(top > m + ATT_LAG)) {
+                    const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 1.0f : fast_exp2(m - m2);
+                    m = m2;
+                    l *= keep;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) acc[t] *= keep;
+                }
+                const float less = m == -INFINITY ? 0.0f : m - ATT_SHIFT;
+                f16x8 ph[2 * NS], pl[SPLIT ? 2 * NS : 1];
 #pragma unroll
                 for (int n = 0; n < NS; n++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const int k = 32 * n + 8 * (i / 4) + 4 * h + (i & 3);
-                        if (!((seen >> k & 1) && kb + k <= pos && kb + k >= low)) s[n][i] = -INFINITY;
+                        const float w = fast_exp2(__builtin_fmaf(s[n][i], c2, -less));
+                        l += w;
+                        _Float16 a, b;
+                        split(w, a, b);
+                        ph[2 * n + i / 8][i % 8] = a;
+                        if constexpr (SPLIT) pl[2 * n + i / 8][i % 8] = b;
                     }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < NS; n++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
-            top *= c2;
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > m + ATT_LAG)) {
-                const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 1.0f : fast_exp2(m - m2);
-                m = m2;
-                l *= keep;
-#pragma unroll
-                for (int t = 0; t < NT; t++) acc[t] *= keep;
-            }
-            const float less = m == -INFINITY ? 0.0f : m - ATT_SHIFT;
-            f16x8 ph[2 * NS], pl[SPLIT ? 2 * NS : 1];
-#pragma unroll
-            for (int n = 0; n < NS; n++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float w = fast_exp2(__builtin_fmaf(s[n][i], c2, -less));
-                    l += w;
-                    _Float16 a, b;
-                    split(w, a, b);
-                    ph[2 * n + i / 8][i % 8] = a;
-                    if constexpr (SPLIT) pl[2 * n + i / 8][i % 8] = b;
-                }
-            // operand t of 16 keys: a value of each of the keys 4 h .. + 3 and 8 + 4 h .. + 3
-            const auto operand = [&](int t, int k16) {
-                const int at = 16 * k16 * DP + v_row + 8 * ((4 * t + v_in) ^ (v_chunk<DP>(4 * h + (s16 >> 2), 0))) + v_half;
-                union {
-                    s16x4 part[2];
-                    f16x8 whole;
-                } a;
-                a.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at]);
-                a.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at + 8 * DP]);
-                return a.whole;
-            };
-            if (plain || odd == 0 || w_first == w_last) {
 #pragma unroll
                 for (int k16 = 0; k16 < 2 * NS; k16++)
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        const f16x8 a = operand(t, k16);
-                        acc[t] = mfma32(a, ph[k16], acc[t]);
-                        if constexpr (SPLIT) acc[t] = mfma32(a, pl[k16], acc[t]);
+                        // a value of each of the keys 4 h .. + 3 and 8 + 4 h .. + 3 of 16
+                        const int at = (sub + 16 * k16) * DP + v_row + 8 * ((4 * t + v_in) ^ v_chunk<DP>(4 * h + (s16 >> 2), 0)) + v_half;
+                        union {
+                            s16x4 part[2];
+                            f16x8 whole;
+                        } a;
+                        a.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at]);
+                        a.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at + 8 * DP]);
+                        acc[t] = mfma32(a.whole, ph[k16], acc[t]);
+                        if constexpr (SPLIT) acc[t] = mfma32(a.whole, pl[k16], acc[t]);
                     }
-            } else {
-                // an infinity or NaN must not meet the weight 0: row by row, without the keys that the row does not see
-#pragma unroll 1
-                for (int n = 0; n < w_rows; n++) {
-                    const int to = __shfl(pos, n), from = __shfl(low, n);
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        f32x16 o = acc[t];
-#pragma unroll
-                        for (int k16 = 0; k16 < 2 * NS; k16++) {
-                            f16x8 a = operand(t, k16);
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                const int key = kb + 16 * k16 + 8 * (e / 4) + 4 * h + (e & 3);
-                                if (key > to || key < from) a[e] = (_Float16)0.0f;
-                            }
-                            o = mfma32(a, ph[k16], o);
-                            if constexpr (SPLIT) o = mfma32(a, pl[k16], o);
-                        }
-                        if (r == n) acc[t] = o;
-                    }
-                }
             }
         }
         if (more) store(buf ^ 1, kb + KT);

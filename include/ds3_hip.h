@@ -538,8 +538,10 @@ int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint
  * temperature 0 or less, or a logit of +inf: the first token, share 1.  A row of nothing but
  * -inf and NaN: token -1, share 0.  The settings are one F32 (top_k: int32) a row;
  * NULL: temperature 1, all tokens.
- * Weights are summed as whole numbers of 2^-44 of the first's, so a token does not
- * depend on the order of sums.  n_vocab is at most 2^18. */
+ * Weights are summed in 64 bits (where only their bins decide, as whole numbers of
+ * 2^-44 of the first's), in an order that the sizes fix: the same call gives the
+ * same token.  n_vocab is at most 2^18.  It uses the library's workspace: before a
+ * capture the call is made once. */
 int ds3_hip_sample(const ds3_hip_buffer_t *logits, uint64_t row_stride, const ds3_hip_buffer_t *uniform,
                    const ds3_hip_buffer_t *temperature, const ds3_hip_buffer_t *top_k, const ds3_hip_buffer_t *top_p,
                    const ds3_hip_buffer_t *min_p, ds3_hip_buffer_t *tokens, ds3_hip_buffer_t *probs, uint32_t n_rows,

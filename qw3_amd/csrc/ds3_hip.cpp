@@ -2864,8 +2864,9 @@ extern "C" int ds3_hip_sample(const ds3_hip_buffer_t *logits, uint64_t row_strid
         !apart(what, { out[0], out[1] }, { in[0], in[1], in[2], in[3], in[4], in[5] }) || !ensure_init())
         return -1;
     const auto fp = [](const ds3_hip_buffer_t *b) { return b ? fptr(b) : nullptr; };
-    const SampleArgs p{ fp(logits), row_stride, fp(uniform), fp(temperature), fp(top_p), fp(min_p),
-                        (const int32_t *)dptr(top_k), (int32_t *)dptr(tokens), fp(probs), (int)n_rows, (int)n_vocab };
+    SampleArgs p{ fp(logits), row_stride, fp(uniform), fp(temperature), fp(top_p), fp(min_p), (const int32_t *)dptr(top_k),
+                  (int32_t *)dptr(tokens), fp(probs), (int)n_rows, (int)n_vocab, nullptr, 0 };
+    if (const size_t bytes = sample_workspace(p); bytes != 0 && !(p.part = (SamplePart *)ws_get(bytes))) return -1;
     KScope ks("sample");
     return finish(launch_sample(p, g.stream), what);
 }

@@ -356,7 +356,14 @@ struct AttnArgs {
 size_t attention_workspace(const AttnArgs &p);
 hipError_t launch_attention(AttnArgs p, int type, hipStream_t s);
 
-// Sampling (sample.hip).
+// Sampling (sample.hip).  A part of a row hands on its best token, its largest ones and the others' weights.
+struct SamplePart {
+    unsigned long long best;
+    double rest;                         // of weights relative to ref
+    float ref;
+    int n;                               // above 1024: more than the list holds
+    unsigned long long list[1024];
+};
 struct SampleArgs {
     const float *logits;
     uint64_t stride;                     // bytes between rows
@@ -365,7 +372,10 @@ struct SampleArgs {
     int32_t *tokens;
     float *probs;
     int n_rows, n_vocab;
+    SamplePart *part;                    // sample_workspace bytes
+    int parts;                           // the launcher's
 };
-hipError_t launch_sample(const SampleArgs &p, hipStream_t s);
+size_t sample_workspace(const SampleArgs &a);
+hipError_t launch_sample(SampleArgs a, hipStream_t s);
 
 }  // namespace ds3k

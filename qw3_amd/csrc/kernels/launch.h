@@ -356,13 +356,15 @@ struct AttnArgs {
 size_t attention_workspace(const AttnArgs &p);
 hipError_t launch_attention(AttnArgs p, int type, hipStream_t s);
 
-// Sampling (sample.hip).  A part of a row hands on its best token, its largest ones and the others' weights.
+// Sampling (sample.hip).  A part of a row hands on its best token, its largest ones, which are all up to `bound`,
+// and the others' weights by bins, relative to ref's.
 struct SamplePart {
     unsigned long long best;
-    double rest;                         // of weights relative to ref
+    uint32_t bound;
     float ref;
     int n;                               // above 1024: more than the list holds
     unsigned long long list[1024];
+    unsigned long long weight[2048];
 };
 struct SampleArgs {
     const float *logits;

@@ -7,17 +7,19 @@
 // and where they do not decide, the weights of all are summed by bins and only the bins
 // that a border lies in are resolved.
 //
-//   collect  each thread's first logits stay in registers; the k-th smallest of the
-//            threads' best bounds the row's k-th logit from below, so what lies under
-//            it is passed over, in registers and in the rest of the row that streams by.
-//            Without top-k the passed weights are summed in 64 bits, in an order that
-//            the sizes fix.
+//   collect  from the threads' best ones of the first 32,768 logits follows a bound that
+//            at least k of the row's reach, so what lies under it is passed over as the
+//            row streams by.  Without top-k the weights of what is passed are summed by bins
+//            of (max - x) / T, as whole numbers of 2^-44: exact in any order of atomics.
 //   finish   the collected tokens sorted, their weights summed along; every border and
 //            the draw are looked for there.
-//   borders  where they lie below the collected ones (a flat row, a large top-k): the
-//            weights as whole numbers of 2^-44 of the first's, whose sums do not depend
-//            on the order of atomics.
+//   below    where one lies below the collected ones (a flat row), its bin's tokens are
+//            gathered and sorted.
+//   borders  a top-k of thousands, thousands of equal logits: counts and weights by bins
+//            of the whole row, the bins of borders narrowed by digits until they can be
+//            sorted.
 //
+// All sums but the bins' are in 64-bit floating point, in an order that the sizes fix.
 // Few rows are collected by several workgroups each (k_sample_part) and finished by one.
 #include "common.h"
 
@@ -28,7 +30,8 @@ namespace ds3k {
 constexpr int SMP_TPB = 1024;
 constexpr int SMP_BINS = 2048;               // bins of 1 / 64 over 32, the last of all beyond
 constexpr int SMP_LIST = 4096;               // tokens sorted at once
-constexpr int SMP_HELD = 8;                  // groups of four logits that a thread holds
+constexpr int SMP_HALF = SMP_LIST / 2;       // of them where a second list lies behind the first
+constexpr int SMP_FIRST = 8 * SMP_TPB;        // groups of four logits from which `collect` takes its bound
 constexpr int SMP_TOP_K = 512;               // top_k up to which `collect` decides
 constexpr int SMP_OPEN = 256;                // tokens that it looks for without top_k
 constexpr double SMP_ONE = 0x1p44;           // the first token's weight in whole numbers
@@ -50,6 +53,30 @@ __device__ __forceinline__ float token_value(u64 token) { return key_value((uint
 __device__ __forceinline__ u64 token_of(float x, int i) { return (u64)order_key(x) << 32 | (uint32_t)i; }
 __device__ __forceinline__ bool counts(float v) { return v > -INFINITY; }      // neither -inf nor NaN
 
+// exp(y), y <= 0: reduced by multiples of ln 2 in two parts (Cody and Waite), Taylor's series to the twelfth power
+// on -0.35 .. 0.35 (its rest is 2e-16).  The library's function costs three times as many instructions, 54 in place of
+// EXP_US us a row of 151,936.
+__device__ __forceinline__ double exp_below(double y)
+{
+    y = fmax(y, -800.0);
+    const double n = rint(y * 1.4426950408889634074);
+    const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, y));
+    double e = 1.0 / 479001600.0;
+    e = fma(e, r, 1.0 / 39916800.0);
+    e = fma(e, r, 1.0 / 3628800.0);
+    e = fma(e, r, 1.0 / 362880.0);
+    e = fma(e, r, 1.0 / 40320.0);
+    e = fma(e, r, 1.0 / 5040.0);
+    e = fma(e, r, 1.0 / 720.0);
+    e = fma(e, r, 1.0 / 120.0);
+    e = fma(e, r, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    return __builtin_ldexp(e, (int)n);
+}
+
 struct SampleShared {
     u64 weight[SMP_BINS];                    // by bin
     uint32_t count[SMP_BINS];
@@ -57,6 +84,7 @@ struct SampleShared {
     u64 wave_w[SMP_TPB / 64];
     double wave_d[SMP_TPB / 64];
     uint32_t wave_c[SMP_TPB / 64];
+    uint32_t shown[7 * (SMP_TPB / 64)];
     u64 best;
     uint32_t n;                              // tokens pushed, those beyond the list too
     int bin;
@@ -84,57 +112,36 @@ __device__ __forceinline__ Draw settings(const SampleArgs &a, int r)
 }
 
 // Inclusive sums over the workgroup, and those of all.
-__device__ __forceinline__ void scan2(SampleShared &sh, u64 &w, uint32_t &c, u64 &w_all, uint32_t &c_all)
+template <typename T>
+__device__ __forceinline__ T scan(T *waves, T &v)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll 1
     for (int d = 1; d < 64; d *= 2) {
-        const u64 a = __shfl_up(w, d);
-        const uint32_t b = __shfl_up(c, d);
-        if (lane >= d) {
-            w += a;
-            c += b;
-        }
-    }
-    __syncthreads();
-    if (lane == 63) {
-        sh.wave_w[wave] = w;
-        sh.wave_c[wave] = c;
-    }
-    __syncthreads();
-    w_all = 0;
-    c_all = 0;
-    u64 before_w = 0;
-    uint32_t before_c = 0;
-    for (int i = 0; i < SMP_TPB / 64; i++) {
-        if (i == wave) {
-            before_w = w_all;
-            before_c = c_all;
-        }
-        w_all += sh.wave_w[i];
-        c_all += sh.wave_c[i];
-    }
-    w += before_w;
-    c += before_c;
-}
-
-__device__ __forceinline__ double scan_f64(SampleShared &sh, double &v)
-{
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int d = 1; d < 64; d *= 2) {
-        const double a = __shfl_up(v, d);
+        const T a = __shfl_up(v, d);
         if (lane >= d) v += a;
     }
     __syncthreads();
-    if (lane == 63) sh.wave_d[wave] = v;
+    if (lane == 63) waves[wave] = v;
     __syncthreads();
-    double all = 0.0, before = 0.0;
-    for (int i = 0; i < SMP_TPB / 64; i++) {
-        if (i == wave) before = all;
-        all += sh.wave_d[i];
+    T sums = lane < SMP_TPB / 64 ? waves[lane] : T(0);
+#pragma unroll 1
+    for (int d = 1; d < SMP_TPB / 64; d *= 2) {
+        const T a = __shfl_up(sums, d);
+        if (lane >= d) sums += a;
     }
-    v += before;
-    return all;
+    const T before = __shfl(sums, max(wave - 1, 0));
+    if (wave > 0) v += before;
+    return __shfl(sums, SMP_TPB / 64 - 1);
 }
+
+__device__ __forceinline__ void scan2(SampleShared &sh, u64 &w, uint32_t &c, u64 &w_all, uint32_t &c_all)
+{
+    w_all = scan(sh.wave_w, w);
+    c_all = scan(sh.wave_c, c);
+}
+
+__device__ __forceinline__ double scan_f64(SampleShared &sh, double &v) { return scan(sh.wave_d, v); }
 
 // A row, read in groups of four that start on multiples of 16 bytes: group q holds logits 4 q - shift .. + 3.
 struct Row {
@@ -169,19 +176,22 @@ struct Row {
         const double b = depth(v) * 64.0;
         return b < SMP_BINS - 1 ? (int)b : SMP_BINS - 1;
     }
-    __device__ double weight(float v) const { return exp(-depth(v)); }
+    __device__ double weight(float v) const { return exp_below(-depth(v)); }
     __device__ u64 units(float v) const { return (u64)__double2ll_rn(weight(v) * SMP_ONE); }
+    // the same bins for every part of a row: v lies in step(v) of 1 / 64 each
+    __device__ double step(float v) const { return floor((double)v * inv_t * 64.0); }
 
-    // f(value, index) of every logit of groups [q0, q1), four groups a thread in flight
-    template <typename F>
-    __device__ void each(int q0, int q1, F f) const
+    // f(value, index) of every logit of groups [q0, q1), AT groups a thread in flight
+    template <int AT = 2, typename F>
+    __device__ __forceinline__ void each(int q0, int q1, F f) const
     {
-        for (int q = q0 + threadIdx.x; q < q1; q += 4 * SMP_TPB) {
-            float4 v[4];
+#pragma unroll 1
+        for (int q = q0 + threadIdx.x; q < q1; q += AT * SMP_TPB) {
+            float4 v[AT];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = q + i * SMP_TPB < q1 ? load(q + i * SMP_TPB) : float4{ NAN, NAN, NAN, NAN };
+            for (int i = 0; i < AT; i++) v[i] = q + i * SMP_TPB < q1 ? load(q + i * SMP_TPB) : float4{ NAN, NAN, NAN, NAN };
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < AT; i++) {
                 const int g = q + i * SMP_TPB;
                 f(v[i].x, index(g, 0));
                 f(v[i].y, index(g, 1));
@@ -209,9 +219,8 @@ __device__ __forceinline__ bool count_border(SampleShared &sh, uint32_t least)
     __syncthreads();
     const int b = 2 * threadIdx.x;
     const uint32_t x = sh.count[b], y = sh.count[b + 1];
-    u64 w = 0, w_all;
-    uint32_t c = x + y, all;
-    scan2(sh, w, c, w_all, all);
+    uint32_t c = x + y;
+    const uint32_t all = scan(sh.wave_c, c);
     if (c >= least && c - x - y < least) {
         const bool first = c - y >= least;
         sh.bin = b + (first ? 0 : 1);
@@ -222,18 +231,39 @@ __device__ __forceinline__ bool count_border(SampleShared &sh, uint32_t least)
     return all >= least;
 }
 
-// A key that at least `least` of the threads' keys do not pass (22 bits of it decided; 0xffffffff: fewer
-// threads have one).  Threads without a key give 0xffffffff.
-__device__ uint32_t key_bound(SampleShared &sh, uint32_t key, int least)
+// A key that at least `least` of the threads' keys do not pass (0xffffffff: fewer threads have one).  Every wave sorts
+// its keys and shows its best, its second, fourth, ... 64th; for each shown key the shown ones up to it tell how many
+// there are at least.
+__device__ __forceinline__ uint32_t key_bound(SampleShared &sh, uint32_t key, int least)
 {
-    clear_bins(sh);
-    if (key != 0xffffffffu) atomicAdd(&sh.count[key >> 21], 1u);
-    if (!count_border(sh, (uint32_t)least)) return 0xffffffffu;
-    const uint32_t high = (uint32_t)sh.bin, before = (uint32_t)sh.found[1];
-    clear_bins(sh);
-    if (key != 0xffffffffu && key >> 21 == high) atomicAdd(&sh.count[key >> 10 & 2047], 1u);
-    count_border(sh, (uint32_t)least - before);
-    return high << 21 | (uint32_t)sh.bin << 10 | 1023u;
+    constexpr int SHOWN = 7, ALL = SHOWN * (SMP_TPB / 64);
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 2; k <= 64; k *= 2)
+#pragma unroll
+        for (int j = k / 2; j > 0; j /= 2) {
+            const uint32_t o = __shfl_xor(key, j);
+            key = ((lane & j) == 0) == ((lane & k) == 0) ? min(key, o) : max(key, o);
+        }
+    __syncthreads();
+    if ((lane & (lane + 1)) == 0) sh.shown[(threadIdx.x >> 6) * SHOWN + __popc(lane)] = key;
+    __syncthreads();
+    uint32_t bound = 0xffffffffu;
+    const uint32_t k0 = sh.shown[lane], k1 = lane + 64 < ALL ? sh.shown[lane + 64] : 0xffffffffu;
+    int n0 = 0, n1 = 0;
+#pragma unroll 1
+    for (int w = 0; w < ALL; w += SHOWN)
+#pragma unroll
+        for (int i = 0; i < SHOWN; i++) {    // a wave's i-th shown key brings 2^i keys in place of 2^(i - 1)
+            const uint32_t s = sh.shown[w + i];
+            const int more = i == 0 ? 1 : 1 << (i - 1);
+            n0 += s <= k0 ? more : 0;
+            n1 += s <= k1 ? more : 0;
+        }
+    if (n0 >= least) bound = k0;
+    if (n1 >= least) bound = min(bound, k1);
+    for (int d = 32; d > 0; d /= 2) bound = min(bound, __shfl_xor(bound, d));
+    return bound;
 }
 
 __device__ __forceinline__ void push(SampleShared &sh, u64 token)
@@ -254,29 +284,28 @@ __device__ __forceinline__ u64 best_of(SampleShared &sh, u64 best)
     return sh.best;
 }
 
-// One pass over groups [q0, q1): sh.list gets (sh.n tells how many, perhaps more than fit) at least the `least`
-// best tokens, or all; returns the best.  with_rest: sum of the other tokens' weights relative to `ref`, a logit.
-__device__ u64 collect(SampleShared &sh, const Row &row, int q0, int q1, int least, bool with_rest, double inv_t, double &rest,
-                       float &ref)
+// What lies under the collected tokens: none of key `bound` or less.
+struct Passed {
+    uint32_t bound;
+    float ref;                               // weights are relative to this logit's
+};
+
+// One pass over groups [q0, q1): sh.list gets (sh.n tells how many, perhaps more than fit) the tokens up to a bound,
+// at least the `least` best or all; returns the best.  by_bins: the other tokens' weights in sh.weight, by steps below
+// that of `ref`.
+__device__ __forceinline__ u64 collect(SampleShared &sh, const Row &row, int q0, int q1, int least, bool by_bins, Passed &passed)
 {
-    float4 held[SMP_HELD];
-#pragma unroll
-    for (int i = 0; i < SMP_HELD; i++) {
-        const int q = q0 + threadIdx.x + i * SMP_TPB;
-        held[i] = q < q1 ? row.load(q) : float4{ NAN, NAN, NAN, NAN };
-    }
-    float most = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < SMP_HELD; i++) most = fmaxf(fmaxf(fmaxf(most, held[i].x), fmaxf(held[i].y, held[i].z)), held[i].w);
-    const uint32_t mine = counts(most) ? order_key(most) : 0xffffffffu;
     if (threadIdx.x == 0) sh.n = 0;
-    // (the first of the best keys serves as reference: any of them would, near the row's largest)
+    for (int b = threadIdx.x; b < SMP_BINS; b += SMP_TPB) sh.weight[b] = 0;
+    float most = -INFINITY;
+    row.each<4>(q0, min(q1, q0 + SMP_FIRST), [&](float v, int) { most = fmaxf(most, v); });
+    const uint32_t mine = counts(most) ? order_key(most) : 0xffffffffu;
     const uint32_t bound = key_bound(sh, mine, least);
+    // (a logit near the largest; none that is passed lies above it)
     const u64 first = best_of(sh, (u64)mine << 32);
-    ref = first >> 32 == 0xffffffffu ? 0.0f : token_value(first);
+    const float ref = first >> 32 == 0xffffffffu ? 0.0f : token_value(first);
     u64 best = ~0ull;
-    double sum = 0.0;
-    const double at = (double)ref;
+    const double at = (double)ref, top_step = row.step(ref);
     const auto take = [&](float v, int i) {
         if (!counts(v)) return;
         const uint32_t key = order_key(v);
@@ -284,58 +313,53 @@ __device__ u64 collect(SampleShared &sh, const Row &row, int q0, int q1, int lea
             const u64 token = (u64)key << 32 | (uint32_t)i;
             best = min(best, token);
             push(sh, token);
-        } else if (with_rest) sum += exp(((double)v - at) * inv_t);
+        } else if (by_bins) {
+            const double b = top_step - row.step(v);
+            if (b < SMP_BINS)                // (beyond, weights are below 2^-46)
+                atomicAdd(&sh.weight[(int)b], (u64)__double2ll_rn(exp_below(((double)v - at) * row.inv_t) * SMP_ONE));
+        }
     };
-#pragma unroll
-    for (int i = 0; i < SMP_HELD; i++) {
-        const int q = q0 + threadIdx.x + i * SMP_TPB;
-        take(held[i].x, row.index(q, 0));
-        take(held[i].y, row.index(q, 1));
-        take(held[i].z, row.index(q, 2));
-        take(held[i].w, row.index(q, 3));
-    }
-    row.each(q0 + SMP_HELD * SMP_TPB, q1, take);
+    row.each(q0, q1, take);
     best = best_of(sh, best);
-    if (with_rest) rest = scan_f64(sh, sum);
-    __syncthreads();
+    passed = { bound, ref };
     return best;
 }
 
-// Tokens of sh.list[0 .. n) in order.
-__device__ void sort_list(SampleShared &sh, int n)
+// list[0 .. n) in order; it has room for the next power of two.
+__device__ __forceinline__ void sort_list(u64 *list, int n)
 {
     const int tid = threadIdx.x;
     int size = 64;
     while (size < n) size *= 2;
     __syncthreads();
-    for (int i = n + tid; i < size; i += SMP_TPB) sh.list[i] = ~0ull;
+    for (int i = n + tid; i < size; i += SMP_TPB) list[i] = ~0ull;
     __syncthreads();
     if (size <= SMP_TPB) {
         // a token a thread: steps of up to 32 within the wave
-        u64 v = tid < size ? sh.list[tid] : ~0ull;
+        u64 v = tid < size ? list[tid] : ~0ull;
         for (int k = 2; k <= size; k *= 2)
             for (int j = k / 2; j > 0; j /= 2) {
                 u64 o;
                 if (j >= 64) {
                     __syncthreads();
-                    if (tid < size) sh.list[tid] = v;
+                    if (tid < size) list[tid] = v;
                     __syncthreads();
-                    o = tid < size ? sh.list[tid ^ j] : v;
+                    o = tid < size ? list[tid ^ j] : v;
                 } else o = __shfl_xor(v, j);
                 const bool low = (tid & j) == 0, up = (tid & k) == 0;
                 v = (low == up) == (o < v) ? o : v;
             }
         __syncthreads();
-        if (tid < size) sh.list[tid] = v;
+        if (tid < size) list[tid] = v;
     } else {
         for (int k = 2; k <= size; k *= 2)
             for (int j = k / 2; j > 0; j /= 2) {
                 for (int i = tid; i < size / 2; i += SMP_TPB) {
                     const int a = 2 * i - (i & (j - 1)), b = a + j;      // the pairs whose bit j differs
-                    const u64 x = sh.list[a], y = sh.list[b];
+                    const u64 x = list[a], y = list[b];
                     if ((x > y) == ((a & k) == 0)) {
-                        sh.list[a] = y;
-                        sh.list[b] = x;
+                        list[a] = y;
+                        list[b] = x;
                     }
                 }
                 __syncthreads();
@@ -352,10 +376,10 @@ __device__ __forceinline__ void answer(const SampleArgs &a, int r, int token, fl
 
 // The draw from sh.list[0 .. n), n > 0: with top_k at least the k best tokens of the row, else its best n, the others'
 // weights summing to `rest` of the first's.  False: they do not decide.
-__device__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, int n, double rest)
+__device__ __forceinline__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, int &n, double rest, double &listed)
 {
     const int tid = threadIdx.x;
-    if (d.k > 0 && n > d.k + 64) {
+    if (d.k > 0 && n > SMP_TPB && n > d.k + 64) {
         // only the k best need sorting: a bound for them by counts, the others dropped
         u64 held[SMP_LIST / SMP_TPB];
         uint32_t high = 0, before = 0;
@@ -385,7 +409,7 @@ __device__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw 
         __syncthreads();
         n = (int)sh.n;
     }
-    sort_list(sh, n);
+    sort_list(sh.list, n);
     if (d.k > 0) n = min(n, d.k);
     // weights, and their sums up to and with each
     constexpr int BLOCKS = SMP_LIST / SMP_TPB;
@@ -403,6 +427,7 @@ __device__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw 
         }
     }
     const bool complete = d.k > 0 || rest == 0.0;
+    listed = mass;
     if (!complete) mass += rest;
     constexpr int NONE = 0x7fffffff;
     __syncthreads();
@@ -411,20 +436,12 @@ __device__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw 
         sh.n = NONE;                         // the drawn token's place
     }
     __syncthreads();
-    if (d.p < 1.0f) {
-        const double least = (double)fmaxf(d.p, 0.0f) * mass;
+    if (d.p < 1.0f || d.m > 0.0f) {
+        const double least = d.p < 1.0f ? (double)fmaxf(d.p, 0.0f) * mass : INFINITY;
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
             const int i = b * SMP_TPB + tid;
             if (i < n && upto[b] >= least) atomicMin(&sh.bin, i + 1);
-        }
-        __syncthreads();
-        if (sh.bin == NONE && !complete) return false;
-    }
-    if (d.m > 0.0f) {
-#pragma unroll
-        for (int b = 0; b < BLOCKS; b++) {
-            const int i = b * SMP_TPB + tid;
             if (i > 0 && i < n && own[b] < (double)d.m) atomicMin(&sh.bin, i);
         }
         __syncthreads();
@@ -452,7 +469,187 @@ __device__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw 
 }
 
 // ---------------------------------------------------------------------------
-// Borders below the collected tokens.
+// A border below the collected tokens, without top_k.
+// ---------------------------------------------------------------------------
+
+// The smallest key in [lo, hi] whose value fails `f`, or hi + 1: f holds up to some key and not beyond.
+template <typename F>
+__device__ __forceinline__ u64 first_key(uint32_t lo, uint32_t hi, F f)
+{
+    u64 a = lo, b = (u64)hi + 1;
+    while (a < b) {
+        const u64 mid = (a + b) / 2;
+        if (f(key_value((uint32_t)mid))) a = mid + 1;
+        else b = mid;
+    }
+    return a;
+}
+
+struct Below {
+    double listed;                           // weight of the collected tokens
+    double w[2], upto;                       // of this thread's two bins, and of all up to and with them
+    double step;                             // the first bin's
+    uint32_t bound;                          // keys above it
+};
+
+// The token below at which the weights, with `listed`, pass `least` (or the last one), and the weights up to and with it.
+__device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, const Below &b, double least, u64 &token, double &mass)
+{
+    const int tid = threadIdx.x;
+    u64 *list = sh.list + SMP_HALF;
+    __syncthreads();
+    if (tid == 0) sh.bin = 0x7fffffff;
+    __syncthreads();
+    const double upto_first = b.upto - b.w[1];
+    const int mine = upto_first >= least && b.w[0] > 0.0 ? 2 * tid : b.upto >= least && b.w[1] > 0.0 ? 2 * tid + 1 : 0x7fffffff;
+    if (mine != 0x7fffffff) atomicMin(&sh.bin, mine);
+    __syncthreads();
+    if (sh.bin == 0x7fffffff) {              // rounding: the last bin with a weight
+        __syncthreads();
+        if (tid == 0) sh.bin = -1;
+        __syncthreads();
+        if (b.w[0] > 0.0 || b.w[1] > 0.0) atomicMax(&sh.bin, b.w[1] > 0.0 ? 2 * tid + 1 : 2 * tid);
+        __syncthreads();
+    }
+    const int bin = sh.bin;
+    if (tid == bin / 2) sh.mass = bin & 1 ? b.upto - b.w[1] : upto_first - b.w[0];
+    __syncthreads();
+    double before = sh.mass;                 // of everything above the bin
+    // its keys
+    const auto depth = [&](float v) { return b.step - row.step(v); };
+    uint32_t lo = (uint32_t)first_key(b.bound + 1, 0xff7fffffu, [&](float v) { return depth(v) < bin; }),
+             hi = (uint32_t)(first_key(lo, 0xff7fffffu, [&](float v) { return depth(v) <= bin; }) - 1);
+    uint32_t i0 = 0, i1 = (uint32_t)row.n;   // where one key is left: its indices
+    int n;
+    for (;;) {
+        __syncthreads();
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        row.each(0, row.groups, [&](float v, int i) {
+            if (!counts(v)) return;
+            const uint32_t key = order_key(v);
+            if (key < lo || key > hi || (uint32_t)i < i0 || (uint32_t)i >= i1) return;
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < SMP_HALF) list[at] = (u64)key << 32 | (uint32_t)i;
+        });
+        __syncthreads();
+        n = (int)sh.n;
+        if (n <= SMP_HALF) break;
+        // too many: their weights by 2048 slices of the keys, then of the indices
+        const bool by_key = lo < hi;
+        const uint32_t span = by_key ? hi - lo : i1 - i0 - 1;
+        const int shift = max(0, 21 - __builtin_clz(span | 1));
+        clear_bins(sh);
+        row.each(0, row.groups, [&](float v, int i) {
+            if (!counts(v)) return;
+            const uint32_t key = order_key(v);
+            if (key < lo || key > hi || (uint32_t)i < i0 || (uint32_t)i >= i1) return;
+            atomicAdd(&sh.weight[(by_key ? key - lo : (uint32_t)i - i0) >> shift], row.units(v));
+        });
+        __syncthreads();
+        const u64 x = sh.weight[2 * tid], y = sh.weight[2 * tid + 1];
+        u64 w = x + y, w_all;
+        uint32_t c = 0, c_all;
+        scan2(sh, w, c, w_all, c_all);
+        __syncthreads();
+        if (tid == 0) sh.bin = 0x7fffffff;
+        __syncthreads();
+        const auto reaches = [&](u64 units) { return before + (double)units / SMP_ONE >= least; };
+        const int at = x > 0 && reaches(w - y) ? 2 * tid : y > 0 && reaches(w) ? 2 * tid + 1 : 0x7fffffff;
+        if (at != 0x7fffffff) atomicMin(&sh.bin, at);
+        __syncthreads();
+        if (sh.bin == 0x7fffffff) {
+            __syncthreads();
+            if (tid == 0) sh.bin = 0;
+            __syncthreads();
+            if (x > 0 || y > 0) atomicMax(&sh.bin, y > 0 ? 2 * tid + 1 : 2 * tid);
+            __syncthreads();
+        }
+        const uint32_t slice = (uint32_t)sh.bin;
+        if (tid == (int)slice / 2) sh.found[0] = slice & 1 ? w - y : w - y - x;
+        __syncthreads();
+        before += (double)sh.found[0] / SMP_ONE;
+        if (by_key) {
+            hi = min(hi, lo + ((slice + 1) << shift) - 1);
+            lo += slice << shift;
+        } else {
+            i1 = min(i1, i0 + ((slice + 1) << shift));
+            i0 += slice << shift;
+        }
+    }
+    sort_list(list, n);
+    // (n <= SMP_HALF: two tokens a thread)
+    __syncthreads();
+    if (tid == 0) sh.n = (uint32_t)max(n - 1, 0);
+    double upto[SMP_HALF / SMP_TPB];
+#pragma unroll
+    for (int j = 0; j < SMP_HALF / SMP_TPB; j++) {
+        const int i = j * SMP_TPB + tid;
+        double w = i < n ? row.weight(token_value(list[i])) : 0.0;
+        const double all = scan_f64(sh, w);
+        upto[j] = before + w;
+        before += all;
+        if (i < n && upto[j] >= least) atomicMin(&sh.n, (uint32_t)i);
+    }
+    __syncthreads();
+    const int at = (int)sh.n;
+#pragma unroll
+    for (int j = 0; j < SMP_HALF / SMP_TPB; j++)
+        if (j * SMP_TPB + tid == at) {
+            sh.found[0] = list[at];
+            sh.mass = upto[j];
+        }
+    __syncthreads();
+    token = sh.found[0];
+    mass = sh.mass;
+    __syncthreads();
+}
+
+// The draw where the sorted list [0 .. n), n <= SMP_HALF, does not decide.
+__device__ __forceinline__ void draw_below(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, int n, const Below &b)
+{
+    const int tid = threadIdx.x;
+    double w = b.w[0] + b.w[1], mass = b.listed + scan_f64(sh, w), kept = mass;
+    u64 token;
+    if (d.p < 1.0f) border_below(sh, row, b, (double)d.p * mass, token, kept);
+    if (d.m > 0.0f) {
+        // the weights of at least min_p are a run of the order's start
+        double sum = 0.0;
+        row.each(0, row.groups, [&](float v, int) {
+            if (!counts(v) || order_key(v) <= b.bound) return;
+            const double x = row.weight(v);
+            if (x >= (double)d.m) sum += x;
+        });
+        kept = fmin(kept, b.listed + scan_f64(sh, sum));
+    }
+    const double target = (double)d.u * kept;
+    if (target < b.listed) {
+        __syncthreads();
+        if (tid == 0) sh.n = (uint32_t)n - 1;
+        double before = 0.0, own[SMP_HALF / SMP_TPB];
+#pragma unroll
+        for (int j = 0; j < SMP_HALF / SMP_TPB; j++) {
+            const int i = j * SMP_TPB + tid;
+            own[j] = i < n ? row.weight(token_value(sh.list[i])) : 0.0;
+            double x = own[j];
+            const double all = scan_f64(sh, x);
+            if (i < n && before + x > target) atomicMin(&sh.n, (uint32_t)i);
+            before += all;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < SMP_HALF / SMP_TPB; j++)
+            if (j * SMP_TPB + tid == (int)sh.n) answer(a, r, (int)(uint32_t)sh.list[sh.n], (float)(own[j] / kept));
+        return;
+    }
+    // past the target: at least the next larger number; within what is kept
+    double upto;
+    border_below(sh, row, b, fmin(nextafter(target, INFINITY), kept), token, upto);
+    if (tid == 0) answer(a, r, (int)(uint32_t)token, (float)(row.weight(token_value(token)) / kept));
+}
+
+// ---------------------------------------------------------------------------
+// Borders of the whole row.
 // ---------------------------------------------------------------------------
 
 // What a border is looked for by: the first token in order whose inclusive count or weight reaches `least`.
@@ -465,7 +662,7 @@ struct Border {
 };
 
 // The token of bin `bin` at which the inclusive sum, from (w0, c0) before the bin, reaches `least`.
-__device__ Border resolve(SampleShared &sh, const Row &row, int bin, u64 w0, uint32_t c0, int by, u64 least)
+__device__ __forceinline__ Border resolve(SampleShared &sh, const Row &row, int bin, u64 w0, uint32_t c0, int by, u64 least)
 {
     // the bin's tokens are narrowed by digits of key << 32 | index until they can be sorted
     u64 prefix = 0, mask = 0;
@@ -516,7 +713,7 @@ __device__ Border resolve(SampleShared &sh, const Row &row, int bin, u64 w0, uin
         w0 = sh.found[1];
         c0 = (uint32_t)sh.found[2];
     }
-    sort_list(sh, n);
+    sort_list(sh.list, n);
     for (int i0 = 0; i0 < n; i0 += SMP_TPB) {
         const int i = i0 + threadIdx.x;
         const u64 own = i < n ? row.units(token_value(sh.list[i])) : 0;
@@ -540,7 +737,7 @@ __device__ Border resolve(SampleShared &sh, const Row &row, int bin, u64 w0, uin
 }
 
 // The whole row's draw.  row.top and row.inv_t are set.
-__device__ void draw_by_borders(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row)
+__device__ __forceinline__ void draw_by_borders(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row)
 {
     const int tid = threadIdx.x;
     const bool by_count = d.k > 0;
@@ -601,7 +798,7 @@ __device__ void draw_by_borders(SampleShared &sh, const SampleArgs &a, int r, co
 }
 
 // A top_k beyond `collect`: if the k best fit the list they are gathered by counts of keys, and decide.
-__device__ bool draw_large_k(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row)
+__device__ __forceinline__ bool draw_large_k(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row)
 {
     if (d.k > SMP_LIST - 512) return false;
     uint32_t high = 0, before = 0, upto = 0;
@@ -629,7 +826,9 @@ __device__ bool draw_large_k(SampleShared &sh, const SampleArgs &a, int r, const
         if (counts(v) && order_key(v) <= bound) push(sh, token_of(v, i));
     });
     __syncthreads();
-    return finish(sh, a, r, d, row, (int)sh.n, 0.0);
+    int n = (int)sh.n;
+    double listed;
+    return finish(sh, a, r, d, row, n, 0.0, listed);
 }
 
 // What the best token decides by itself.
@@ -649,24 +848,35 @@ __device__ __forceinline__ int looked_for(const Draw &d)
 __global__ void __launch_bounds__(SMP_TPB) k_sample(SampleArgs a)
 {
     __shared__ SampleShared sh;
-    const int r = blockIdx.x;
+    const int r = blockIdx.x, tid = threadIdx.x;
     const Draw d = settings(a, r);
     Row row;
     row.bind(a, r);
-    const bool rest_too = d.k == 0 && d.t > 0.0f;
     row.inv_t = 1.0 / (double)d.t;
-    double rest = 0.0;
-    float ref;
-    const u64 best = collect(sh, row, 0, row.groups, looked_for(d), rest_too, row.inv_t, rest, ref);
+    Passed passed;
+    const u64 best = collect(sh, row, 0, row.groups, looked_for(d), d.k == 0 && d.t > 0.0f, passed);
     if (first_decides(a, r, d, best)) return;
     row.top = (double)token_value(best);
-    const uint32_t n = sh.n;
-    __syncthreads();
+    int n = (int)sh.n;
     if (d.k > SMP_TOP_K) {
         if (draw_large_k(sh, a, r, d, row)) return;
     } else if (n <= SMP_LIST) {
-        if (rest > 0.0) rest *= exp(((double)ref - row.top) * row.inv_t);
-        if (finish(sh, a, r, d, row, (int)n, rest)) return;
+        Below b = { 0.0, { 0.0, 0.0 }, 0.0, row.step(passed.ref), passed.bound };
+        double rest = 0.0;
+        if (d.k == 0) {
+            const double unit = exp_below(((double)passed.ref - row.top) * row.inv_t) / SMP_ONE;
+            b.w[0] = (double)sh.weight[2 * tid] * unit;
+            b.w[1] = (double)sh.weight[2 * tid + 1] * unit;
+            b.upto = b.w[0] + b.w[1];
+            rest = scan_f64(sh, b.upto);
+        }
+        __syncthreads();
+        if (finish(sh, a, r, d, row, n, rest, b.listed)) return;
+        if (n <= SMP_HALF) {
+            b.upto += b.listed;
+            draw_below(sh, a, r, d, row, n, b);
+            return;
+        }
     }
     draw_by_borders(sh, a, r, d, row);
 }
@@ -679,20 +889,22 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample_part(SampleArgs a)
     const Draw d = settings(a, r);
     Row row;
     row.bind(a, r);
-    const bool rest_too = d.k == 0 && d.t > 0.0f;
-    double rest = 0.0;
-    float ref;
+    row.inv_t = 1.0 / (double)d.t;
+    Passed passed;
+    const bool by_bins = d.k == 0 && d.t > 0.0f;
     const u64 best = collect(sh, row, (int)((int64_t)row.groups * part / a.parts), (int)((int64_t)row.groups * (part + 1) / a.parts),
-                             looked_for(d), rest_too, 1.0 / (double)d.t, rest, ref);
+                             looked_for(d), by_bins, passed);
     SamplePart *out = a.part + blockIdx.x;
     const int n = (int)min(sh.n, (uint32_t)PART_LIST);
     if (threadIdx.x == 0) {
         out->best = best;
         out->n = (int)min(sh.n, (uint32_t)PART_LIST + 1);
-        out->rest = rest;
-        out->ref = ref;
+        out->bound = passed.bound;
+        out->ref = passed.ref;
     }
     for (int i = threadIdx.x; i < n; i += SMP_TPB) out->list[i] = sh.list[i];
+    if (by_bins)
+        for (int i = threadIdx.x; i < SMP_BINS; i += SMP_TPB) out->weight[i] = sh.weight[i];
 }
 
 __global__ void __launch_bounds__(SMP_TPB) k_sample_join(SampleArgs a)
@@ -704,17 +916,20 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample_join(SampleArgs a)
     row.bind(a, r);
     row.inv_t = 1.0 / (double)d.t;
     const SamplePart *in = a.part + (int64_t)r * a.parts;
-    // every token of the parts in a register, a part's list beside the others'
+    // every token of the parts in a register
     u64 held[PART_MOST], best = ~0ull;
-    uint32_t mine = 0xffffffffu;
+    uint32_t mine = 0xffffffffu, passed = 0xffffffffu;       // the least bound of the parts: all tokens up to it are here
     bool fits = true;
-    double rest = 0.0;
 #pragma unroll
     for (int i = 0; i < PART_MOST; i++) {
         const int n = i < a.parts ? in[i].n : 0;
         fits &= n <= PART_LIST;
-        held[i] = tid < n && n <= PART_LIST ? in[i].list[tid] : ~0ull;
-        if (i < a.parts) best = min(best, in[i].best);
+        const int at = (tid - 64 * i) & (SMP_TPB - 1);        // (so that few tokens a part lie in different threads)
+        held[i] = at < n && n <= PART_LIST ? in[i].list[at] : ~0ull;
+        if (i < a.parts) {
+            best = min(best, in[i].best);
+            passed = min(passed, in[i].bound);
+        }
         mine = min(mine, (uint32_t)(held[i] >> 32));
     }
     if (first_decides(a, r, d, best)) return;
@@ -723,24 +938,44 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample_join(SampleArgs a)
         if (draw_large_k(sh, a, r, d, row)) return;
     } else if (fits) {
         if (tid == 0) sh.n = 0;
-        const uint32_t bound = key_bound(sh, mine, looked_for(d));
-        double sum = 0.0;
+        for (int i = tid; i < SMP_BINS; i += SMP_TPB) sh.weight[i] = 0;
+        uint32_t bound = key_bound(sh, mine, looked_for(d));
+        if (d.k == 0) bound = min(bound, passed);
+        Below b = { 0.0, { 0.0, 0.0 }, 0.0, row.step((float)row.top), bound };
 #pragma unroll
         for (int i = 0; i < PART_MOST; i++) {
             if (held[i] == ~0ull) continue;
+            const float v = token_value(held[i]);
             if ((uint32_t)(held[i] >> 32) <= bound) push(sh, held[i]);
-            else if (d.k == 0) sum += row.weight(token_value(held[i]));
+            else if (d.k == 0 && b.step - row.step(v) < SMP_BINS) atomicAdd(&sh.weight[(int)(b.step - row.step(v))], row.units(v));
         }
+        __syncthreads();
+        double rest = 0.0;
         if (d.k == 0) {
-            rest = scan_f64(sh, sum);
+            for (int i = 0; i < 2; i++) b.w[i] = (double)sh.weight[2 * tid + i] / SMP_ONE;
+            for (int i = 0; i < a.parts; i++) {
+                // a part's bins begin at its own reference, so many below the largest logit's
+                const double behind = b.step - row.step(in[i].ref), unit = exp_below(((double)in[i].ref - row.top) * row.inv_t) / SMP_ONE;
+                if (in[i].best == ~0ull || !(behind < SMP_BINS)) continue;
 #pragma unroll
-            for (int i = 0; i < PART_MOST; i++)
-                if (i < a.parts && in[i].rest > 0.0) rest += in[i].rest * exp(((double)in[i].ref - row.top) * row.inv_t);
+                for (int j = 0; j < 2; j++) {
+                    const int at = 2 * tid + j - (int)behind;
+                    if (at >= 0) b.w[j] += (double)in[i].weight[at] * unit;
+                }
+            }
+            b.upto = b.w[0] + b.w[1];
+            rest = scan_f64(sh, b.upto);
         }
+        int n = (int)sh.n;
         __syncthreads();
-        const uint32_t n = sh.n;
-        __syncthreads();
-        if (n <= SMP_LIST && finish(sh, a, r, d, row, (int)n, rest)) return;
+        if (n <= SMP_LIST) {
+            if (finish(sh, a, r, d, row, n, rest, b.listed)) return;
+            if (n <= SMP_HALF) {
+                b.upto += b.listed;
+                draw_below(sh, a, r, d, row, n, b);
+                return;
+            }
+        }
     }
     draw_by_borders(sh, a, r, d, row);
 }

@@ -22,13 +22,14 @@
 // All sums but the bins' are in 64-bit floating point, in an order that the sizes fix.
 // Few rows are collected by several workgroups each (k_sample_part) and finished by one.
 #include "common.h"
+#include "lanes.h"
 
 #include <algorithm>
 
 namespace ds3k {
 
 constexpr int SMP_TPB = 1024;
-constexpr int SMP_BINS = 2048;               // bins of 1 / 64 over 32, the last of all beyond
+constexpr int SMP_BINS = 2048;               // bins of 1 / 64 over 32 (the whole row's), or of 1 / 32 of an octave over 64
 constexpr int SMP_LIST = 4096;               // tokens sorted at once
 constexpr int SMP_HALF = SMP_LIST / 2;       // of them where a second list lies behind the first
 constexpr int SMP_FIRST = 8 * SMP_TPB;        // groups of four logits from which `collect` takes its bound
@@ -55,7 +56,7 @@ __device__ __forceinline__ bool counts(float v) { return v > -INFINITY; }      /
 
 // exp(y), y <= 0: reduced by multiples of ln 2 in two parts (Cody and Waite), Taylor's series to the twelfth power
 // on -0.35 .. 0.35 (its rest is 2e-16).  The library's function costs three times as many instructions, 54 in place of
-// EXP_US us a row of 151,936.
+// ? of 151,936.
 __device__ __forceinline__ double exp_below(double y)
 {
     y = fmax(y, -800.0);
@@ -77,6 +78,21 @@ __device__ __forceinline__ double exp_below(double y)
     return __builtin_ldexp(e, (int)n);
 }
 
+// 2^(f / 32) in whole numbers of 2^-44, 0 <= f < 1: Taylor's series to the fifth power (its rest is 1.4e-13), made whole
+// by adding 2^52.  Bins of weights hold these, so that the octaves' powers come in once a bin.
+__device__ __forceinline__ unsigned long long part_of_step(double f)
+{
+    constexpr double a = 0.021660849392498290;        // ln 2 / 32
+    double e = a * a * a * a * a / 120;
+    e = fma(e, f, a * a * a * a / 24);
+    e = fma(e, f, a * a * a / 6);
+    e = fma(e, f, a * a / 2);
+    e = fma(e, f, a);
+    e = fma(e, f, 1.0);
+    const double whole = fma(e, 0x1p44, 0x1p52);
+    return __builtin_bit_cast(unsigned long long, whole) & 0x000fffffffffffffull;
+}
+
 struct SampleShared {
     u64 weight[SMP_BINS];                    // by bin
     uint32_t count[SMP_BINS];
@@ -85,7 +101,6 @@ struct SampleShared {
     double wave_d[SMP_TPB / 64];
     uint32_t wave_c[SMP_TPB / 64];
     uint32_t shown[7 * (SMP_TPB / 64)];
-    u64 best;
     uint32_t n;                              // tokens pushed, those beyond the list too
     int bin;
     u64 found[4];
@@ -116,23 +131,15 @@ template <typename T>
 __device__ __forceinline__ T scan(T *waves, T &v)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 1
-    for (int d = 1; d < 64; d *= 2) {
-        const T a = __shfl_up(v, d);
-        if (lane >= d) v += a;
-    }
+    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) waves[wave] = v;
     __syncthreads();
-    T sums = lane < SMP_TPB / 64 ? waves[lane] : T(0);
-#pragma unroll 1
-    for (int d = 1; d < SMP_TPB / 64; d *= 2) {
-        const T a = __shfl_up(sums, d);
-        if (lane >= d) sums += a;
-    }
-    const T before = __shfl(sums, max(wave - 1, 0));
-    if (wave > 0) v += before;
-    return __shfl(sums, SMP_TPB / 64 - 1);
+    const T sums = row_scan(waves[lane & (SMP_TPB / 64 - 1)]);
+    const int before = __builtin_amdgcn_readfirstlane(max(wave - 1, 0));
+    const T base = lane_of(sums, before);
+    if (wave > 0) v += base;
+    return lane_of(sums, SMP_TPB / 64 - 1);
 }
 
 __device__ __forceinline__ void scan2(SampleShared &sh, u64 &w, uint32_t &c, u64 &w_all, uint32_t &c_all)
@@ -145,6 +152,7 @@ __device__ __forceinline__ double scan_f64(SampleShared &sh, double &v) { return
 
 // A row, read in groups of four that start on multiples of 16 bytes: group q holds logits 4 q - shift .. + 3.
 struct Row {
+    static constexpr double STEPS = 32 * 1.4426950408889634074;
     const float *x;
     int n, shift, groups;
     double top, inv_t;                       // the largest logit, 1 / temperature
@@ -178,8 +186,9 @@ struct Row {
     }
     __device__ double weight(float v) const { return exp_below(-depth(v)); }
     __device__ u64 units(float v) const { return (u64)__double2ll_rn(weight(v) * SMP_ONE); }
-    // the same bins for every part of a row: v lies in step(v) of 1 / 64 each
-    __device__ double step(float v) const { return floor((double)v * inv_t * 64.0); }
+    // v / T in steps of 1 / 32 of an octave, a grid that the parts of a row have in common
+    __device__ double steps(float v) const { return (double)v * (inv_t * STEPS); }
+    __device__ double step(float v) const { return floor(steps(v)); }
 
     // f(value, index) of every logit of groups [q0, q1), AT groups a thread in flight
     template <int AT = 2, typename F>
@@ -231,39 +240,24 @@ __device__ __forceinline__ bool count_border(SampleShared &sh, uint32_t least)
     return all >= least;
 }
 
-// A key that at least `least` of the threads' keys do not pass (0xffffffff: fewer threads have one).  Every wave sorts
-// its keys and shows its best, its second, fourth, ... 64th; for each shown key the shown ones up to it tell how many
-// there are at least.
+// A key that at least `least` of the threads' keys do not pass (0xffffffff: none is found).  Every wave sorts its keys
+// and shows its best, its second, fourth, ... 64th; as many waves' 2^j-th as it takes bound so many keys, and the best
+// such bound over j is taken.
 __device__ __forceinline__ uint32_t key_bound(SampleShared &sh, uint32_t key, int least)
 {
-    constexpr int SHOWN = 7, ALL = SHOWN * (SMP_TPB / 64);
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int k = 2; k <= 64; k *= 2)
-#pragma unroll
-        for (int j = k / 2; j > 0; j /= 2) {
-            const uint32_t o = __shfl_xor(key, j);
-            key = ((lane & j) == 0) == ((lane & k) == 0) ? min(key, o) : max(key, o);
-        }
+    constexpr int WAVES = SMP_TPB / 64;
+    static_assert(WAVES == 16, "rows of 16 lanes");
+    const int lane = threadIdx.x & 63, row = lane >> 4;
+    key = sort_lanes<64>(key);
     __syncthreads();
-    if ((lane & (lane + 1)) == 0) sh.shown[(threadIdx.x >> 6) * SHOWN + __popc(lane)] = key;
+    if ((lane & (lane + 1)) == 0) sh.shown[__popc(lane) * WAVES + (threadIdx.x >> 6)] = key;
     __syncthreads();
-    uint32_t bound = 0xffffffffu;
-    const uint32_t k0 = sh.shown[lane], k1 = lane + 64 < ALL ? sh.shown[lane + 64] : 0xffffffffu;
-    int n0 = 0, n1 = 0;
-#pragma unroll 1
-    for (int w = 0; w < ALL; w += SHOWN)
-#pragma unroll
-        for (int i = 0; i < SHOWN; i++) {    // a wave's i-th shown key brings 2^i keys in place of 2^(i - 1)
-            const uint32_t s = sh.shown[w + i];
-            const int more = i == 0 ? 1 : 1 << (i - 1);
-            n0 += s <= k0 ? more : 0;
-            n1 += s <= k1 ? more : 0;
-        }
-    if (n0 >= least) bound = k0;
-    if (n1 >= least) bound = min(bound, k1);
-    for (int d = 32; d > 0; d /= 2) bound = min(bound, __shfl_xor(bound, d));
-    return bound;
+    // rows of 16 lanes sort the waves' keys of one rank: ranks 1 .. 8, then 16 .. 64
+    const uint32_t a = sort_lanes<16>(sh.shown[lane]), b = sort_lanes<16>(row < 3 ? sh.shown[64 + lane] : 0xffffffffu);
+    const int need_a = (least + (1 << row) - 1) >> row, need_b = (least + (16 << row) - 1) >> (4 + row);
+    uint32_t bound = (lane & 15) == need_a - 1 ? a : 0xffffffffu;
+    if (row < 3 && (lane & 15) == need_b - 1) bound = min(bound, b);
+    return lanes_join<32>(bound, [](uint32_t x, uint32_t y) { return min(x, y); });
 }
 
 __device__ __forceinline__ void push(SampleShared &sh, u64 token)
@@ -275,13 +269,12 @@ __device__ __forceinline__ void push(SampleShared &sh, u64 token)
 // The best token of each thread, of all.
 __device__ __forceinline__ u64 best_of(SampleShared &sh, u64 best)
 {
-    for (int d = 32; d > 0; d /= 2) best = min(best, (u64)__shfl_xor(best, d));
+    const auto least = [](u64 x, u64 y) { return x < y ? x : y; };
+    best = lanes_join<32>(best, least);
     __syncthreads();
-    if (threadIdx.x == 0) sh.best = ~0ull;
+    if ((threadIdx.x & 63) == 0) sh.wave_w[threadIdx.x >> 6] = best;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) atomicMin(&sh.best, best);
-    __syncthreads();
-    return sh.best;
+    return lanes_join<8>(sh.wave_w[threadIdx.x & 15], least);
 }
 
 // What lies under the collected tokens: none of key `bound` or less.
@@ -305,7 +298,7 @@ __device__ __forceinline__ u64 collect(SampleShared &sh, const Row &row, int q0,
     const u64 first = best_of(sh, (u64)mine << 32);
     const float ref = first >> 32 == 0xffffffffu ? 0.0f : token_value(first);
     u64 best = ~0ull;
-    const double at = (double)ref, top_step = row.step(ref);
+    const double top_step = row.step(ref);
     const auto take = [&](float v, int i) {
         if (!counts(v)) return;
         const uint32_t key = order_key(v);
@@ -314,9 +307,9 @@ __device__ __forceinline__ u64 collect(SampleShared &sh, const Row &row, int q0,
             best = min(best, token);
             push(sh, token);
         } else if (by_bins) {
-            const double b = top_step - row.step(v);
-            if (b < SMP_BINS)                // (beyond, weights are below 2^-46)
-                atomicAdd(&sh.weight[(int)b], (u64)__double2ll_rn(exp_below(((double)v - at) * row.inv_t) * SMP_ONE));
+            const double x = row.steps(v), s = floor(x), b = top_step - s;
+            // (beyond the bins, weights are below 2^-63)
+            if (b < SMP_BINS) atomicAdd(&sh.weight[(int)b], part_of_step(x - s));
         }
     };
     row.each(q0, q1, take);
@@ -337,18 +330,27 @@ __device__ __forceinline__ void sort_list(u64 *list, int n)
     if (size <= SMP_TPB) {
         // a token a thread: steps of up to 32 within the wave
         u64 v = tid < size ? list[tid] : ~0ull;
-        for (int k = 2; k <= size; k *= 2)
-            for (int j = k / 2; j > 0; j /= 2) {
-                u64 o;
-                if (j >= 64) {
+        if (size == 64) v = sort_lanes<64>(v);
+        else {
+            v = sort_merge<1>(v, 2);
+            v = sort_merge<2>(v, 4);
+            v = sort_merge<4>(v, 8);
+            v = sort_merge<8>(v, 16);
+            v = sort_merge<16>(v, 32);
+            v = sort_merge<32>(v, 64);
+#pragma unroll 1
+            for (int k = 128; k <= size; k *= 2) {
+#pragma unroll 1
+                for (int j = k / 2; j > 32; j /= 2) {
                     __syncthreads();
                     if (tid < size) list[tid] = v;
                     __syncthreads();
-                    o = tid < size ? list[tid ^ j] : v;
-                } else o = __shfl_xor(v, j);
-                const bool low = (tid & j) == 0, up = (tid & k) == 0;
-                v = (low == up) == (o < v) ? o : v;
+                    const u64 o = tid < size ? list[tid ^ j] : v;
+                    v = ((tid & j) == 0) == ((tid & k) == 0) ? min(v, o) : max(v, o);
+                }
+                v = sort_merge<32>(v, k);
             }
+        }
         __syncthreads();
         if (tid < size) list[tid] = v;
     } else {
@@ -483,6 +485,12 @@ __device__ __forceinline__ u64 first_key(uint32_t lo, uint32_t hi, F f)
         else b = mid;
     }
     return a;
+}
+
+// The weight of a bin's whole numbers of part_of_step.
+__device__ __forceinline__ double bin_weight(const Row &row, double step, u64 units)
+{
+    return units == 0 ? 0.0 : (double)units / SMP_ONE * exp_below((step - row.steps((float)row.top)) * (1.0 / 32 * 0.6931471805599453));
 }
 
 struct Below {
@@ -864,9 +872,8 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample(SampleArgs a)
         Below b = { 0.0, { 0.0, 0.0 }, 0.0, row.step(passed.ref), passed.bound };
         double rest = 0.0;
         if (d.k == 0) {
-            const double unit = exp_below(((double)passed.ref - row.top) * row.inv_t) / SMP_ONE;
-            b.w[0] = (double)sh.weight[2 * tid] * unit;
-            b.w[1] = (double)sh.weight[2 * tid + 1] * unit;
+#pragma unroll
+            for (int i = 0; i < 2; i++) b.w[i] = bin_weight(row, b.step - (2 * tid + i), sh.weight[2 * tid + i]);
             b.upto = b.w[0] + b.w[1];
             rest = scan_f64(sh, b.upto);
         }
@@ -902,67 +909,73 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample_part(SampleArgs a)
         out->bound = passed.bound;
         out->ref = passed.ref;
     }
-    for (int i = threadIdx.x; i < n; i += SMP_TPB) out->list[i] = sh.list[i];
+    if (threadIdx.x < n) out->list[threadIdx.x] = sh.list[threadIdx.x];
     if (by_bins)
         for (int i = threadIdx.x; i < SMP_BINS; i += SMP_TPB) out->weight[i] = sh.weight[i];
 }
 
 __global__ void __launch_bounds__(SMP_TPB) k_sample_join(SampleArgs a)
 {
+    static_assert(PART_MOST <= SMP_TPB / 64 && PART_LIST == 16 * 64, "a wave holds a part's tokens");
     __shared__ SampleShared sh;
-    const int r = blockIdx.x, tid = threadIdx.x;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const SamplePart *in = a.part + (int64_t)r * a.parts, *own = in + min(wave, a.parts - 1);
     const Draw d = settings(a, r);
+    // a wave holds a part's tokens; the first 64 places are read before their number is known
+    u64 held[PART_LIST / 64], best = own->best;
+    uint32_t passed = own->bound;                     // the least bound of the parts: all tokens up to it are here
+    const int count = wave < a.parts ? __builtin_amdgcn_readfirstlane(own->n) : 0;
+    held[0] = own->list[lane];
+    if (lane >= count) held[0] = ~0ull;
+    bool fits = count <= PART_LIST;
+    uint32_t mine = (uint32_t)(held[0] >> 32);
+#pragma unroll
+    for (int i = 1; i < PART_LIST / 64; i++) {
+        held[i] = ~0ull;
+        if (64 * i < count) {
+            if (64 * i + lane < count && fits) held[i] = own->list[64 * i + lane];
+            mine = min(mine, (uint32_t)(held[i] >> 32));
+        }
+    }
     Row row;
     row.bind(a, r);
     row.inv_t = 1.0 / (double)d.t;
-    const SamplePart *in = a.part + (int64_t)r * a.parts;
-    // every token of the parts in a register
-    u64 held[PART_MOST], best = ~0ull;
-    uint32_t mine = 0xffffffffu, passed = 0xffffffffu;       // the least bound of the parts: all tokens up to it are here
-    bool fits = true;
-#pragma unroll
-    for (int i = 0; i < PART_MOST; i++) {
-        const int n = i < a.parts ? in[i].n : 0;
-        fits &= n <= PART_LIST;
-        const int at = (tid - 64 * i) & (SMP_TPB - 1);        // (so that few tokens a part lie in different threads)
-        held[i] = at < n && n <= PART_LIST ? in[i].list[at] : ~0ull;
-        if (i < a.parts) {
-            best = min(best, in[i].best);
-            passed = min(passed, in[i].bound);
-        }
-        mine = min(mine, (uint32_t)(held[i] >> 32));
-    }
+    best = best_of(sh, best);
     if (first_decides(a, r, d, best)) return;
     row.top = (double)token_value(best);
     if (d.k > SMP_TOP_K) {
         if (draw_large_k(sh, a, r, d, row)) return;
-    } else if (fits) {
+    } else if (__syncthreads_and(fits)) {
         if (tid == 0) sh.n = 0;
         for (int i = tid; i < SMP_BINS; i += SMP_TPB) sh.weight[i] = 0;
         uint32_t bound = key_bound(sh, mine, looked_for(d));
-        if (d.k == 0) bound = min(bound, passed);
+        if (d.k == 0) bound = min(bound, (uint32_t)best_of(sh, passed));
         Below b = { 0.0, { 0.0, 0.0 }, 0.0, row.step((float)row.top), bound };
 #pragma unroll
-        for (int i = 0; i < PART_MOST; i++) {
+        for (int i = 0; i < PART_LIST / 64; i++) {
+            if (64 * i >= count) break;
             if (held[i] == ~0ull) continue;
-            const float v = token_value(held[i]);
             if ((uint32_t)(held[i] >> 32) <= bound) push(sh, held[i]);
-            else if (d.k == 0 && b.step - row.step(v) < SMP_BINS) atomicAdd(&sh.weight[(int)(b.step - row.step(v))], row.units(v));
+            else if (d.k == 0) {
+                const double x = row.steps(token_value(held[i])), s = floor(x);
+                if (b.step - s < SMP_BINS) atomicAdd(&sh.weight[(int)(b.step - s)], part_of_step(x - s));
+            }
         }
         __syncthreads();
         double rest = 0.0;
         if (d.k == 0) {
-            for (int i = 0; i < 2; i++) b.w[i] = (double)sh.weight[2 * tid + i] / SMP_ONE;
+            u64 units[2] = { sh.weight[2 * tid], sh.weight[2 * tid + 1] };
             for (int i = 0; i < a.parts; i++) {
                 // a part's bins begin at its own reference, so many below the largest logit's
-                const double behind = b.step - row.step(in[i].ref), unit = exp_below(((double)in[i].ref - row.top) * row.inv_t) / SMP_ONE;
+                const double behind = b.step - row.step(in[i].ref);
                 if (in[i].best == ~0ull || !(behind < SMP_BINS)) continue;
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     const int at = 2 * tid + j - (int)behind;
-                    if (at >= 0) b.w[j] += (double)in[i].weight[at] * unit;
+                    if (at >= 0) units[j] += in[i].weight[at];
                 }
             }
+            for (int i = 0; i < 2; i++) b.w[i] = bin_weight(row, b.step - (2 * tid + i), units[i]);
             b.upto = b.w[0] + b.w[1];
             rest = scan_f64(sh, b.upto);
         }

@@ -112,24 +112,24 @@ __device__ __forceinline__ double lane_of(double v, int lane)
     return __builtin_bit_cast(double, lane_of(__builtin_bit_cast(unsigned long long, v), lane));
 }
 
-// One step of a bitonic sort of 64 lanes: the pairs J apart, ascending where lane & K is 0.
+// One step of a bitonic sort: the pairs J apart, ascending where threadIdx.x & k is 0, or the other way round.
 template <int J, typename T>
-__device__ __forceinline__ T sort_step(T v, int k)
+__device__ __forceinline__ T sort_step(T v, int k, bool down = false)
 {
     const T o = lane_xor<J>(v);
-    return ((threadIdx.x & J) == 0) == ((threadIdx.x & k) == 0) ? (o < v ? o : v) : (o < v ? v : o);
+    return ((threadIdx.x & J) == 0) == (((threadIdx.x & k) == 0) != down) ? (o < v ? o : v) : (o < v ? v : o);
 }
 
-// Merges runs of K / 2 (ascending and descending in turn) into runs of K, from pairs J apart on; k: as in sort_step.
+// Merges, from pairs J apart on, two runs of 2 J values in all into one; k, down: as in sort_step.
 template <int J, typename T>
-__device__ __forceinline__ T sort_merge(T v, int k)
+__device__ __forceinline__ T sort_merge(T v, int k, bool down = false)
 {
-    v = sort_step<J>(v, k);
-    if constexpr (J > 1) v = sort_merge<J / 2>(v, k);
+    v = sort_step<J>(v, k, down);
+    if constexpr (J > 1) v = sort_merge<J / 2>(v, k, down);
     return v;
 }
 
-// The lanes' values ascending over UPTO lanes (16 or 64); k past that: over the lanes & k alternately.
+// The lanes' values ascending over UPTO lanes each (16 or 64).
 template <int UPTO, typename T>
 __device__ __forceinline__ T sort_lanes(T v)
 {

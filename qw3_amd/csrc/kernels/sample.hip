@@ -25,6 +25,7 @@
 #include "lanes.h"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace ds3k {
 
@@ -34,7 +35,7 @@ constexpr int SMP_LIST = 4096;               // tokens sorted at once
 constexpr int SMP_HALF = SMP_LIST / 2;       // of them where a second list lies behind the first
 constexpr int SMP_FIRST = 8 * SMP_TPB;        // groups of four logits from which `collect` takes its bound
 constexpr int SMP_TOP_K = 512;               // top_k up to which `collect` decides
-constexpr int SMP_OPEN = 256;                // tokens that it looks for without top_k
+constexpr int SMP_OPEN = 64;                 // tokens that it looks for without top_k
 constexpr double SMP_ONE = 0x1p44;           // the first token's weight in whole numbers
 
 constexpr int PART_LIST = 1024;              // tokens that a part of a row hands on
@@ -78,19 +79,14 @@ __device__ __forceinline__ double exp_below(double y)
     return __builtin_ldexp(e, (int)n);
 }
 
-// 2^(f / 32) in whole numbers of 2^-44, 0 <= f < 1: Taylor's series to the fifth power (its rest is 1.4e-13), made whole
-// by adding 2^52.  Bins of weights hold these, so that the octaves' powers come in once a bin.
-__device__ __forceinline__ unsigned long long part_of_step(double f)
+// 2^(f / 32) in whole numbers of 2^-32, 0 <= f < 1: 1 and Taylor's series to the fourth power in 32 bits (off by 2e-9, a
+// rounding that changes its sign from logit to logit).  Bins of weights hold these; the octaves' powers come in once a bin.
+constexpr double STEP_ONE = 0x1p32;
+__device__ __forceinline__ unsigned long long part_of_step(float f)
 {
-    constexpr double a = 0.021660849392498290;        // ln 2 / 32
-    double e = a * a * a * a * a / 120;
-    e = fma(e, f, a * a * a * a / 24);
-    e = fma(e, f, a * a * a / 6);
-    e = fma(e, f, a * a / 2);
-    e = fma(e, f, a);
-    e = fma(e, f, 1.0);
-    const double whole = fma(e, 0x1p44, 0x1p52);
-    return __builtin_bit_cast(unsigned long long, whole) & 0x000fffffffffffffull;
+    constexpr float a = 0.021660849392498290f;        // ln 2 / 32
+    const float e = f * fmaf(f, fmaf(f, fmaf(f, a * a * a * a / 24, a * a * a / 6), a * a / 2), a);
+    return 0x100000000ull + (uint32_t)fmaf(e, 0x1p32f, 0.5f);
 }
 
 struct SampleShared {
@@ -152,7 +148,6 @@ __device__ __forceinline__ double scan_f64(SampleShared &sh, double &v) { return
 
 // A row, read in groups of four that start on multiples of 16 bytes: group q holds logits 4 q - shift .. + 3.
 struct Row {
-    static constexpr double STEPS = 32 * 1.4426950408889634074;
     const float *x;
     int n, shift, groups;
     double top, inv_t;                       // the largest logit, 1 / temperature
@@ -186,9 +181,34 @@ struct Row {
     }
     __device__ double weight(float v) const { return exp_below(-depth(v)); }
     __device__ u64 units(float v) const { return (u64)__double2ll_rn(weight(v) * SMP_ONE); }
-    // v / T in steps of 1 / 32 of an octave, a grid that the parts of a row have in common
-    __device__ double steps(float v) const { return (double)v * (inv_t * STEPS); }
-    __device__ double step(float v) const { return floor(steps(v)); }
+    // v / T in steps of 1 / 32 of an octave, as whole + more + part: a grid that the parts of a row have in common.  The
+    // product of 48 bits (two factors, the first product's rounding by an fma) keeps the part to 2^-25 where steps are
+    // many; 64-bit instructions for it took three times as long.
+    float c_hi, c_lo;
+    struct Steps {
+        float whole, more, part;
+    };
+    __device__ void set_temperature(float t)
+    {
+        inv_t = 1.0 / (double)t;
+        const double c = inv_t * (32 * 1.4426950408889634074);
+        c_hi = (float)c;
+        c_lo = (float)(c - (double)c_hi);
+    }
+    __device__ Steps steps(float v) const
+    {
+        const float hi = v * c_hi, lo = fmaf(v, c_lo, fmaf(v, c_hi, -hi));
+        Steps s;
+        s.whole = floorf(hi);
+        const float f = (hi - s.whole) + lo;
+        s.more = floorf(f);
+        s.part = f - s.more;
+        return s;
+    }
+    // steps of b below a (NaN where one is not finite)
+    static __device__ float below(const Steps &a, const Steps &b) { return (a.whole - b.whole) + (a.more - b.more); }
+    // whether steps tell logits near v apart
+    __device__ bool graded(float v) const { return c_hi < 1e30f && fabsf(v * c_hi) < 1e30f; }
 
     // f(value, index) of every logit of groups [q0, q1), AT groups a thread in flight
     template <int AT = 2, typename F>
@@ -298,75 +318,115 @@ __device__ __forceinline__ u64 collect(SampleShared &sh, const Row &row, int q0,
     const u64 first = best_of(sh, (u64)mine << 32);
     const float ref = first >> 32 == 0xffffffffu ? 0.0f : token_value(first);
     u64 best = ~0ull;
-    const double top_step = row.step(ref);
-    const auto take = [&](float v, int i) {
-        if (!counts(v)) return;
-        const uint32_t key = order_key(v);
-        if (key <= bound) {
-            const u64 token = (u64)key << 32 | (uint32_t)i;
-            best = min(best, token);
-            push(sh, token);
-        } else if (by_bins) {
-            const double x = row.steps(v), s = floor(x), b = top_step - s;
-            // (beyond the bins, weights are below 2^-63)
-            if (b < SMP_BINS) atomicAdd(&sh.weight[(int)b], part_of_step(x - s));
+    // two groups a thread at a time, the next two on their way: one comparison tells that none of their logits is collected
+    const Row::Steps top = row.steps(ref);
+    const float least_value = bound == 0xffffffffu ? -FLT_MAX : key_value(bound);
+    const auto group = [&](int q) { return q < q1 ? row.load(q) : float4{ NAN, NAN, NAN, NAN }; };
+    float4 x = group(q0 + threadIdx.x), y = group(q0 + threadIdx.x + SMP_TPB);
+#pragma unroll 1
+    for (int q = q0 + threadIdx.x; q < q1; q += 2 * SMP_TPB) {
+        const float v[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
+        x = group(q + 2 * SMP_TPB);
+        y = group(q + 3 * SMP_TPB);
+        float largest = v[0];
+#pragma unroll
+        for (int j = 1; j < 8; j++) largest = fmaxf(largest, v[j]);
+        if (largest >= least_value) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (v[j] >= least_value) {
+                    const u64 token = token_of(v[j], row.index(q + j / 4 * SMP_TPB, j & 3));
+                    best = min(best, token);
+                    push(sh, token);
+                }
         }
-    };
-    row.each(q0, q1, take);
+        if (by_bins) {
+            u64 units[8];
+            float bin[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const Row::Steps s = row.steps(v[j]);
+                // (beyond the bins, weights are below 2^-63; -inf and NaN are no bin's)
+                bin[j] = v[j] < least_value ? Row::below(top, s) : INFINITY;
+                units[j] = part_of_step(s.part);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (bin[j] < SMP_BINS) atomicAdd(&sh.weight[(int)bin[j]], units[j]);
+        }
+    }
     best = best_of(sh, best);
     passed = { bound, ref };
     return best;
 }
 
-// list[0 .. n) in order; it has room for the next power of two.
-__device__ __forceinline__ void sort_list(u64 *list, int n)
+// list[0 .. size) in order, E tokens a thread (places tid, tid + SMP_TPB, ...): steps of up to 32 within the wave, of up to
+// 512 through the list, larger ones within the thread.
+template <int E>
+__device__ __forceinline__ void sort_places(u64 *list, int size)
 {
     const int tid = threadIdx.x;
-    int size = 64;
-    while (size < n) size *= 2;
-    __syncthreads();
-    for (int i = n + tid; i < size; i += SMP_TPB) list[i] = ~0ull;
-    __syncthreads();
-    if (size <= SMP_TPB) {
-        // a token a thread: steps of up to 32 within the wave
-        u64 v = tid < size ? list[tid] : ~0ull;
-        if (size == 64) v = sort_lanes<64>(v);
-        else {
-            v = sort_merge<1>(v, 2);
-            v = sort_merge<2>(v, 4);
-            v = sort_merge<4>(v, 8);
-            v = sort_merge<8>(v, 16);
-            v = sort_merge<16>(v, 32);
-            v = sort_merge<32>(v, 64);
+    u64 v[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        v[e] = E > 1 || tid < size ? list[tid + e * SMP_TPB] : ~0ull;
+        v[e] = sort_merge<1>(v[e], 2);
+        v[e] = sort_merge<2>(v[e], 4);
+        v[e] = sort_merge<4>(v[e], 8);
+        v[e] = sort_merge<8>(v[e], 16);
+        v[e] = sort_merge<16>(v[e], 32);
+        v[e] = sort_merge<32>(v[e], 64);
+    }
 #pragma unroll 1
-            for (int k = 128; k <= size; k *= 2) {
-#pragma unroll 1
-                for (int j = k / 2; j > 32; j /= 2) {
-                    __syncthreads();
-                    if (tid < size) list[tid] = v;
-                    __syncthreads();
-                    const u64 o = tid < size ? list[tid ^ j] : v;
-                    v = ((tid & j) == 0) == ((tid & k) == 0) ? min(v, o) : max(v, o);
+    for (int k = 128; k <= size; k *= 2) {
+        if constexpr (E > 1) {
+#pragma unroll
+            for (int j = E / 2; j > 0; j /= 2)
+                if (j * SMP_TPB < k) {
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if ((e & j) == 0) {
+                            const bool up = (e * SMP_TPB & k) == 0;
+                            const u64 x = v[e], y = v[e + j];
+                            v[e] = up == (x < y) ? x : y;
+                            v[e + j] = up == (x < y) ? y : x;
+                        }
                 }
-                v = sort_merge<32>(v, k);
+        }
+#pragma unroll 1
+        for (int j = min(k, SMP_TPB) / 2; j > 32; j /= 2) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (E > 1 || tid < size) list[tid + e * SMP_TPB] = v[e];
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const u64 o = E > 1 || tid < size ? list[(tid ^ j) + e * SMP_TPB] : v[e];
+                v[e] = ((tid & j) == 0) == ((tid + e * SMP_TPB & k) == 0) ? min(v[e], o) : max(v[e], o);
             }
         }
-        __syncthreads();
-        if (tid < size) list[tid] = v;
-    } else {
-        for (int k = 2; k <= size; k *= 2)
-            for (int j = k / 2; j > 0; j /= 2) {
-                for (int i = tid; i < size / 2; i += SMP_TPB) {
-                    const int a = 2 * i - (i & (j - 1)), b = a + j;      // the pairs whose bit j differs
-                    const u64 x = list[a], y = list[b];
-                    if ((x > y) == ((a & k) == 0)) {
-                        list[a] = y;
-                        list[b] = x;
-                    }
-                }
-                __syncthreads();
-            }
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = sort_merge<32>(v[e], k < SMP_TPB ? k : 0, (tid + e * SMP_TPB & k) != 0 && k >= SMP_TPB);
     }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (E > 1 || tid < size) list[tid + e * SMP_TPB] = v[e];
+}
+
+// list[0 .. n) in order; MOST: the places that it has.
+template <int MOST>
+__device__ __forceinline__ void sort_list(u64 *list, int n)
+{
+    int size = 64;
+    while (size < n) size *= 2;
+    if (size > SMP_TPB) size = MOST;
+    __syncthreads();
+    for (int i = n + threadIdx.x; i < size; i += SMP_TPB) list[i] = ~0ull;
+    __syncthreads();
+    if (size <= SMP_TPB) sort_places<1>(list, size);
+    else sort_places<MOST / SMP_TPB>(list, size);
     __syncthreads();
 }
 
@@ -411,7 +471,7 @@ __device__ __forceinline__ bool finish(SampleShared &sh, const SampleArgs &a, in
         __syncthreads();
         n = (int)sh.n;
     }
-    sort_list(sh.list, n);
+    sort_list<SMP_LIST>(sh.list, n);
     if (d.k > 0) n = min(n, d.k);
     // weights, and their sums up to and with each
     constexpr int BLOCKS = SMP_LIST / SMP_TPB;
@@ -487,16 +547,18 @@ __device__ __forceinline__ u64 first_key(uint32_t lo, uint32_t hi, F f)
     return a;
 }
 
-// The weight of a bin's whole numbers of part_of_step.
-__device__ __forceinline__ double bin_weight(const Row &row, double step, u64 units)
+// The weight of a bin's whole numbers of part_of_step, `bin` steps below those of `top`.
+__device__ __forceinline__ double bin_weight(const Row &row, const Row::Steps &top, int bin, u64 units)
 {
-    return units == 0 ? 0.0 : (double)units / SMP_ONE * exp_below((step - row.steps((float)row.top)) * (1.0 / 32 * 0.6931471805599453));
+    if (units == 0) return 0.0;
+    const double x = (double)top.whole + (double)top.more - bin - row.top * row.inv_t * (32 * 1.4426950408889634074);
+    return (double)units / STEP_ONE * exp_below(x * (1.0 / 32 * 0.6931471805599453));
 }
 
 struct Below {
     double listed;                           // weight of the collected tokens
     double w[2], upto;                       // of this thread's two bins, and of all up to and with them
-    double step;                             // the first bin's
+    Row::Steps top;                          // the first bin's
     uint32_t bound;                          // keys above it
 };
 
@@ -524,7 +586,7 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
     __syncthreads();
     double before = sh.mass;                 // of everything above the bin
     // its keys
-    const auto depth = [&](float v) { return b.step - row.step(v); };
+    const auto depth = [&](float v) { return Row::below(b.top, row.steps(v)); };
     uint32_t lo = (uint32_t)first_key(b.bound + 1, 0xff7fffffu, [&](float v) { return depth(v) < bin; }),
              hi = (uint32_t)(first_key(lo, 0xff7fffffu, [&](float v) { return depth(v) <= bin; }) - 1);
     uint32_t i0 = 0, i1 = (uint32_t)row.n;   // where one key is left: its indices
@@ -533,7 +595,7 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
         __syncthreads();
         if (tid == 0) sh.n = 0;
         __syncthreads();
-        row.each(0, row.groups, [&](float v, int i) {
+        row.each<8>(0, row.groups, [&](float v, int i) {
             if (!counts(v)) return;
             const uint32_t key = order_key(v);
             if (key < lo || key > hi || (uint32_t)i < i0 || (uint32_t)i >= i1) return;
@@ -585,7 +647,7 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
             i0 += slice << shift;
         }
     }
-    sort_list(list, n);
+    sort_list<SMP_HALF>(list, n);
     // (n <= SMP_HALF: two tokens a thread)
     __syncthreads();
     if (tid == 0) sh.n = (uint32_t)max(n - 1, 0);
@@ -721,7 +783,7 @@ __device__ __forceinline__ Border resolve(SampleShared &sh, const Row &row, int 
         w0 = sh.found[1];
         c0 = (uint32_t)sh.found[2];
     }
-    sort_list(sh.list, n);
+    sort_list<SMP_LIST>(sh.list, n);
     for (int i0 = 0; i0 < n; i0 += SMP_TPB) {
         const int i = i0 + threadIdx.x;
         const u64 own = i < n ? row.units(token_value(sh.list[i])) : 0;
@@ -805,33 +867,27 @@ __device__ __forceinline__ void draw_by_borders(SampleShared &sh, const SampleAr
     if (tid == 0) answer(a, r, (int)(uint32_t)drawn.token, (float)(row.weight(token_value(drawn.token)) * SMP_ONE / (double)mass));
 }
 
-// A top_k beyond `collect`: if the k best fit the list they are gathered by counts of keys, and decide.
-__device__ __forceinline__ bool draw_large_k(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row)
+// A top_k beyond `collect`, which has looked for the SMP_TOP_K best, at least as many up to `bound`: their depth below
+// the largest logit, three times over, divided into bins, shows by counts where the k-th lies (bins of keys would
+// be few and their counters fought over).  Where the k best fit the list they are gathered and decide.
+__device__ __forceinline__ bool draw_large_k(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, uint32_t bound)
 {
-    if (d.k > SMP_LIST - 512) return false;
-    uint32_t high = 0, before = 0, upto = 0;
-    for (int step = 0; step < 2; step++) {
-        clear_bins(sh);
-        row.each(0, row.groups, [&](float v, int) {
-            if (!counts(v)) return;
-            const uint32_t key = order_key(v);
-            if (step == 0) atomicAdd(&sh.count[key >> 21], 1u);
-            else if (key >> 21 == high) atomicAdd(&sh.count[key >> 10 & 2047], 1u);
-        });
-        if (!count_border(sh, (uint32_t)d.k - before)) return false;      // fewer than k tokens count
-        upto = before + (uint32_t)sh.found[1] + (uint32_t)sh.found[2];
-        if (step == 0) {
-            high = (uint32_t)sh.bin;
-            before = (uint32_t)sh.found[1];
-        }
-    }
-    if (upto > SMP_LIST) return false;
-    const uint32_t bound = high << 21 | (uint32_t)sh.bin << 10 | 1023u;
+    const float top = (float)row.top, depth = 3.0f * (top - key_value(bound)), scale = (float)SMP_BINS / depth;
+    if (d.k > SMP_LIST - 512 || bound == 0xffffffffu || !(depth > 0.0f && depth < INFINITY && scale < INFINITY)) return false;
+    const auto bin = [&](float v) { return (top - v) * scale; };          // (rises as v falls)
+    clear_bins(sh);
+    row.each<8>(0, row.groups, [&](float v, int) {
+        const float b = bin(v);
+        if (b < SMP_BINS) atomicAdd(&sh.count[(int)b], 1u);
+    });
+    if (!count_border(sh, (uint32_t)d.k)) return false;                   // it lies deeper
+    if (sh.found[1] + sh.found[2] > SMP_LIST) return false;
+    const float last = (float)(sh.bin + 1);
     __syncthreads();
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
-    row.each(0, row.groups, [&](float v, int i) {
-        if (counts(v) && order_key(v) <= bound) push(sh, token_of(v, i));
+    row.each<8>(0, row.groups, [&](float v, int i) {
+        if (bin(v) < last) push(sh, token_of(v, i));
     });
     __syncthreads();
     int n = (int)sh.n;
@@ -850,7 +906,7 @@ __device__ __forceinline__ bool first_decides(const SampleArgs &a, int r, const 
 __device__ __forceinline__ int looked_for(const Draw &d)
 {
     if (!(d.t > 0.0f)) return 1;
-    return d.k > 0 && d.k <= SMP_TOP_K ? d.k : d.k > 0 ? 1 : SMP_OPEN;
+    return d.k > 0 ? min(d.k, SMP_TOP_K) : SMP_OPEN;
 }
 
 __global__ void __launch_bounds__(SMP_TPB) k_sample(SampleArgs a)
@@ -860,20 +916,20 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample(SampleArgs a)
     const Draw d = settings(a, r);
     Row row;
     row.bind(a, r);
-    row.inv_t = 1.0 / (double)d.t;
+    row.set_temperature(d.t);
     Passed passed;
     const u64 best = collect(sh, row, 0, row.groups, looked_for(d), d.k == 0 && d.t > 0.0f, passed);
     if (first_decides(a, r, d, best)) return;
     row.top = (double)token_value(best);
     int n = (int)sh.n;
     if (d.k > SMP_TOP_K) {
-        if (draw_large_k(sh, a, r, d, row)) return;
-    } else if (n <= SMP_LIST) {
-        Below b = { 0.0, { 0.0, 0.0 }, 0.0, row.step(passed.ref), passed.bound };
+        if (draw_large_k(sh, a, r, d, row, passed.bound)) return;
+    } else if (n <= SMP_LIST && (d.k > 0 || row.graded((float)row.top))) {
+        Below b = { 0.0, { 0.0, 0.0 }, 0.0, row.steps(passed.ref), passed.bound };
         double rest = 0.0;
         if (d.k == 0) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) b.w[i] = bin_weight(row, b.step - (2 * tid + i), sh.weight[2 * tid + i]);
+            for (int i = 0; i < 2; i++) b.w[i] = bin_weight(row, b.top, 2 * tid + i, sh.weight[2 * tid + i]);
             b.upto = b.w[0] + b.w[1];
             rest = scan_f64(sh, b.upto);
         }
@@ -896,7 +952,7 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample_part(SampleArgs a)
     const Draw d = settings(a, r);
     Row row;
     row.bind(a, r);
-    row.inv_t = 1.0 / (double)d.t;
+    row.set_temperature(d.t);
     Passed passed;
     const bool by_bins = d.k == 0 && d.t > 0.0f;
     const u64 best = collect(sh, row, (int)((int64_t)row.groups * part / a.parts), (int)((int64_t)row.groups * (part + 1) / a.parts),
@@ -922,7 +978,8 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample_join(SampleArgs a)
     const SamplePart *in = a.part + (int64_t)r * a.parts, *own = in + min(wave, a.parts - 1);
     const Draw d = settings(a, r);
     // a wave holds a part's tokens; the first 64 places are read before their number is known
-    u64 held[PART_LIST / 64], best = own->best;
+    const u64 own_best = own->best;
+    u64 held[PART_LIST / 64];
     uint32_t passed = own->bound;                     // the least bound of the parts: all tokens up to it are here
     const int count = wave < a.parts ? __builtin_amdgcn_readfirstlane(own->n) : 0;
     held[0] = own->list[lane];
@@ -939,43 +996,45 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample_join(SampleArgs a)
     }
     Row row;
     row.bind(a, r);
-    row.inv_t = 1.0 / (double)d.t;
-    best = best_of(sh, best);
+    row.set_temperature(d.t);
+    const u64 best = best_of(sh, own_best);
     if (first_decides(a, r, d, best)) return;
     row.top = (double)token_value(best);
     if (d.k > SMP_TOP_K) {
-        if (draw_large_k(sh, a, r, d, row)) return;
-    } else if (__syncthreads_and(fits)) {
+        if (draw_large_k(sh, a, r, d, row, (uint32_t)best_of(sh, passed))) return;
+    } else if (__syncthreads_and(fits && (d.k > 0 || row.graded((float)row.top)))) {
         if (tid == 0) sh.n = 0;
         for (int i = tid; i < SMP_BINS; i += SMP_TPB) sh.weight[i] = 0;
         uint32_t bound = key_bound(sh, mine, looked_for(d));
         if (d.k == 0) bound = min(bound, (uint32_t)best_of(sh, passed));
-        Below b = { 0.0, { 0.0, 0.0 }, 0.0, row.step((float)row.top), bound };
+        Below b = { 0.0, { 0.0, 0.0 }, 0.0, row.steps((float)row.top), bound };
 #pragma unroll
         for (int i = 0; i < PART_LIST / 64; i++) {
-            if (64 * i >= count) break;
             if (held[i] == ~0ull) continue;
             if ((uint32_t)(held[i] >> 32) <= bound) push(sh, held[i]);
             else if (d.k == 0) {
-                const double x = row.steps(token_value(held[i])), s = floor(x);
-                if (b.step - s < SMP_BINS) atomicAdd(&sh.weight[(int)(b.step - s)], part_of_step(x - s));
+                const Row::Steps s = row.steps(token_value(held[i]));
+                const float bin = Row::below(b.top, s);
+                if (bin < SMP_BINS) atomicAdd(&sh.weight[(int)bin], part_of_step(s.part));
             }
         }
         __syncthreads();
         double rest = 0.0;
         if (d.k == 0) {
             u64 units[2] = { sh.weight[2 * tid], sh.weight[2 * tid + 1] };
+            // a part's bins begin at its own reference, so many below the largest logit's
+            const float behind = Row::below(b.top, row.steps(own->ref));
+            if (lane == 0) sh.shown[wave] = own_best != ~0ull && behind < SMP_BINS ? (uint32_t)(int)behind : (uint32_t)SMP_BINS;
+            __syncthreads();
+#pragma unroll 4
             for (int i = 0; i < a.parts; i++) {
-                // a part's bins begin at its own reference, so many below the largest logit's
-                const double behind = b.step - row.step(in[i].ref);
-                if (in[i].best == ~0ull || !(behind < SMP_BINS)) continue;
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const int at = 2 * tid + j - (int)behind;
+                    const int at = 2 * tid + j - (int)sh.shown[i];
                     if (at >= 0) units[j] += in[i].weight[at];
                 }
             }
-            for (int i = 0; i < 2; i++) b.w[i] = bin_weight(row, b.step - (2 * tid + i), units[i]);
+            for (int i = 0; i < 2; i++) b.w[i] = bin_weight(row, b.top, 2 * tid + i, units[i]);
             b.upto = b.w[0] + b.w[1];
             rest = scan_f64(sh, b.upto);
         }

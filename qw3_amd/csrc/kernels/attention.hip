@@ -14,6 +14,7 @@
 // F32 rows are scaled by a power of two to about 2^14 and split into two F16 parts, as
 // are the weights: products of 22 bits with the cache's exact values.
 #include "common.h"
+#include "lanes.h"
 
 #include <algorithm>
 #include <cmath>
@@ -47,8 +48,7 @@ constexpr int ATT_FEW_ROWS = 64;             // requests of up to so many rows t
 
 __device__ __forceinline__ long long wave_sum(long long v)
 {
-    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
-    return v;
+    return lanes_join<32>(v, [](long long x, long long y) { return x + y; });
 }
 
 // Request i's tiles of M rows and the most keys that one of them sees.
@@ -126,14 +126,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit
         Unit r;
         request_work(p, M, i0 + tid, tiles, span, r);
         const long long units = (long long)tiles * ((span + u.run - 1) / u.run);
-        long long sum = units, tile_sum = tiles;
-        for (int d = 1; d < 64; d *= 2) {
-            const long long o = __shfl_up(sum, d), q = __shfl_up(tile_sum, d);
-            if (lane >= d) {
-                sum += o;
-                tile_sum += q;
-            }
-        }
+        const long long sum = wave_scan(units), tile_sum = wave_scan((long long)tiles);
         if (lane == 63) {
             part[0][wave] = sum;
             part[1][wave] = tile_sum;
@@ -285,6 +278,21 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
     const int k0 = (int)min((int64_t)tile.start + (int64_t)u.chunk * u.run, (int64_t)tile.end),
               k1 = (int)min((int64_t)k0 + u.run, (int64_t)tile.end);
 
+    const int32_t *table = p.table + (int64_t)u.seq * p.max_blocks;
+    // Blocks of the keys of step kb: for the first product keys r and 16 + r, for the second 4 h .. 4 h + 3 and 16 + those
+    // (one entry each where a block holds at least four rows).  They are looked up one step ahead of the rows.
+    constexpr int NV = TINY ? 8 : 2;
+    int kblock[2], vblock[NV];
+    const auto look_up = [&](int kb) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) kblock[t] = table[min(kb + 16 * t + r, k1 - 1) >> p.log_block];
+#pragma unroll
+        for (int e = 0; e < NV; e++)
+            vblock[e] = table[min(TINY ? kb + 16 * (e / 4) + 4 * h + (e & 3) : kb + 16 * e + 4 * h, k1 - 1) >> p.log_block];
+    };
+    int kb = k0 + 32 * wave;
+    if (kb < k1) look_up(kb);
+
     // this lane's row: its position, its first key, its q
     const bool live = r < rows;
     const int my_j = (row0 + (live ? r : 0)) / group, my_h = (row0 + (live ? r : 0)) % group;
@@ -303,8 +311,8 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
                 v[c][e] = live && (!PAD || 32 * c + 8 * h < p.head_dim) ? q[32 * c + 8 * h + e] * p.q_sign : 0.0f;
                 amax = fmaxf(amax, fabsf(v[c][e]));
             }
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        amax = fmaxf(amax, lane_xor<16>(amax));
+        amax = fmaxf(amax, lane_xor<32>(amax));
         const int ex = row_exponent(amax);
         c2 = mul_pow2(c2, -ex);
 #pragma unroll
@@ -325,7 +333,6 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
         }
     }
 
-    const int32_t *table = p.table + (int64_t)u.seq * p.max_blocks;
     const int all_from = (int)max(p.window ? base + j1 - p.window + 1 : 0, (int64_t)0);      // keys that every row sees:
     const int64_t all_to = base + j0;                                                        // from .. to
     float m = -INFINITY, l = 0.0f;
@@ -333,19 +340,6 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = { 0, 0, 0, 0 };
 
-    // Blocks of the keys of step kb: for the first product keys r and 16 + r, for the second 4 h .. 4 h + 3 and 16 + those
-    // (one entry each where a block holds at least four rows).  They are looked up one step ahead of the rows.
-    constexpr int NV = TINY ? 8 : 2;
-    int kblock[2], vblock[NV];
-    const auto look_up = [&](int kb) {
-#pragma unroll
-        for (int t = 0; t < 2; t++) kblock[t] = table[min(kb + 16 * t + r, k1 - 1) >> p.log_block];
-#pragma unroll
-        for (int e = 0; e < NV; e++)
-            vblock[e] = table[min(TINY ? kb + 16 * (e / 4) + 4 * h + (e & 3) : kb + 16 * e + 4 * h, k1 - 1) >> p.log_block];
-    };
-    int kb = k0 + 32 * wave;
-    if (kb < k1) look_up(kb);
     for (; kb < k1; kb += 32 * (ATT_TPB / 64)) {
         f16x8 kf[2][NC];
         i32x4 vf[8][(NT + 7) / 8];
@@ -410,8 +404,8 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
         }
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * c2;
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = fmaxf(top, lane_xor<16>(top));
+        top = fmaxf(top, lane_xor<32>(top));
         // (the first keys always pass, as m is then -inf)
         if (__any(top > m + ATT_LAG)) {
             const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 1.0f : fast_exp2(m - m2);
@@ -480,8 +474,8 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
     }
 
     // the waves' sums, brought to one maximum
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    l += lane_xor<16>(l);
+    l += lane_xor<32>(l);
     if (h == 0) {
         sh.m[wave][r] = m;
         sh.l[wave][r] = l;
@@ -644,7 +638,7 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
 #pragma unroll
                 for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(q[16 * c + 8 * h + e] * p.q_sign));
             }
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        amax = fmaxf(amax, lane_xor<32>(amax));
         const int ex = row_exponent(amax);
         c2 = mul_pow2(c2, -ex);
 #pragma unroll
@@ -737,7 +731,7 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
 #pragma unroll
                     for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
                 top *= c2;
-                top = fmaxf(top, __shfl_xor(top, 32));
+                top = fmaxf(top, lane_xor<32>(top));
                 if (__any(top > m + ATT_LAG)) {
                     const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 1.0f : fast_exp2(m - m2);
                     m = m2;
@@ -779,7 +773,7 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
         __syncthreads();
     }
 
-    l += __shfl_xor(l, 32);
+    l += lane_xor<32>(l);
     if (!live) return;
     if (tile.chunks == 1) {
         const float by = l == 0.0f ? 0.0f : 1.0f / l;
@@ -819,7 +813,8 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
 // and made 1,800 units of 64 streams wait for each other (614 us in place of 186).
 // ---------------------------------------------------------------------------
 
-constexpr int JOIN_ROWS = 4;
+constexpr int JOIN_ROWS = 4;                 // at a time
+constexpr int JOIN_PART(int M) { return M == ROWS_M ? JOIN_ROWS : 32; }      // rows a workgroup
 
 template <typename T, int DP, int M>
 __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
@@ -827,51 +822,50 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
     constexpr int ITEMS = JOIN_ROWS * (DP / 4), PARTS = ATT_TPB / ITEMS;
     __shared__ float factor[JOIN_ROWS][512];
     __shared__ f32x4 sums[ATT_TPB];
-    const int tid = threadIdx.x, parts = (M + JOIN_ROWS - 1) / JOIN_ROWS, group = p.n_head / p.n_head_kv;
-    const int n0 = blockIdx.x % parts * JOIN_ROWS, g = blockIdx.x / parts % p.n_head_kv, id = blockIdx.x / parts / p.n_head_kv;
+    const int tid = threadIdx.x, parts = M / JOIN_PART(M), group = p.n_head / p.n_head_kv;
+    const int from_row = blockIdx.x % parts * JOIN_PART(M), g = blockIdx.x / parts % p.n_head_kv, id = blockIdx.x / parts / p.n_head_kv;
     Unit u;
     if (!find_unit<ATT_TPB, true>(p, M, id, u)) return;
     const Tile tile = tile_of(p, M, u);
     const int chunks = tile.chunks;
-    if (chunks == 1 || n0 >= tile.rows) return;
+    if (chunks == 1) return;
     const int64_t step = (int64_t)p.n_head_kv * (M * (DP + 2));
     const float *from = p.partial + (int64_t)(g + (int64_t)u.whole * p.n_head_kv) * (M * (DP + 2));
-    {
-        // each run's factor: 2^(its maximum - the largest) / sum of weights; a wave a row
-        const int lane = tid & 63, n = tid >> 6;
-        const float *f = from + M * DP + n0 + n;
-        float top = -INFINITY, sum = 0.0f;
-        for (int c = lane; c < chunks; c += 64) top = fmaxf(top, f[c * step]);
-        for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
-        for (int c = lane; c < chunks; c += 64) {
-            const float m = f[c * step], x = m == -INFINITY ? 1.0f : fast_exp2(m - top);
-            factor[n][c] = x;
-            sum += x * f[c * step + M];
+    for (int n0 = from_row; n0 < min(tile.rows, from_row + JOIN_PART(M)); n0 += JOIN_ROWS) {
+        {
+            // each run's factor: 2^(its maximum - the largest) / sum of weights; a wave a row
+            const int lane = tid & 63, n = tid >> 6;
+            const float *f = from + M * DP + n0 + n;
+            float top = -INFINITY, sum = 0.0f;
+            for (int c = lane; c < chunks; c += 64) top = fmaxf(top, f[c * step]);
+            top = lanes_join<32>(top, [](float x, float y) { return fmaxf(x, y); });
+            for (int c = lane; c < chunks; c += 64) {
+                const float m = f[c * step], x = m == -INFINITY ? 1.0f : fast_exp2(m - top);
+                factor[n][c] = x;
+                sum += x * f[c * step + M];
+            }
+            sum = lanes_join<32>(sum, [](float x, float y) { return x + y; });
+            const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+            for (int c = lane; c < chunks; c += 64) factor[n][c] *= by;
         }
-        for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-        const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-        for (int c = lane; c < chunks; c += 64) factor[n][c] *= by;
-    }
-    __syncthreads();
-    const int item = tid % ITEMS, part = tid / ITEMS, n = item / (DP / 4), d = item % (DP / 4) * 4;
-    const float *f = from + (int64_t)(n0 + n) * DP + d;
-    f32x4 o = { 0, 0, 0, 0 };
-    if (part < PARTS) {
+        __syncthreads();
+        const int item = tid % ITEMS, part = tid / ITEMS, n = item / (DP / 4), d = item % (DP / 4) * 4;
+        const float *f = from + (int64_t)(n0 + n) * DP + d;
+        f32x4 o = { 0, 0, 0, 0 };
 #pragma unroll 8
         for (int c = part; c < chunks; c += PARTS) o += factor[n][c] * *(const f32x4 *)(f + c * step);
-    }
-    if constexpr (PARTS > 1) {
-        sums[tid] = o;
+        if constexpr (PARTS > 1) sums[tid] = o;
         __syncthreads();
-        if (part != 0) return;
+        if (part == 0 && n0 + n < tile.rows && d < p.head_dim) {
 #pragma unroll
-        for (int i = 1; i < PARTS; i++) o += sums[i * ITEMS + item];
+            for (int i = 1; i < PARTS; i++) o += sums[i * ITEMS + item];
+            const int j = (tile.row0 + n0 + n) / group, a = (tile.row0 + n0 + n) % group;
+            T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim + d;
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[i] = (T)o[i];
+        }
+        __syncthreads();
     }
-    if (n0 + n >= tile.rows || d >= p.head_dim) return;
-    const int j = (tile.row0 + n0 + n) / group, a = (tile.row0 + n0 + n) % group;
-    T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim + d;
-#pragma unroll
-    for (int i = 0; i < 4; i++) out[i] = (T)o[i];
 }
 
 static int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -907,7 +901,12 @@ static hipError_t attention_rows(AttnArgs p, int min_rows, int max_rows, hipStre
     p.least = MANY ? 512 : 128;
     const int64_t longest = (int64_t)p.max_blocks << p.log_block;
     while (longest / p.least >= 512) p.least *= 2;
-    const int64_t tiles = most_tiles(p, M), units = (tiles + p.target) * p.n_head_kv;
+    // Tiles at most; units: `target` or as many as there are tiles (a unit ends at 2^30 keys), and no more than the runs
+    // that the longest request could have.
+    int64_t tiles = most_tiles(p, M);
+    if (max_rows < 0x7fffffff) tiles = std::min<int64_t>(tiles, (int64_t)p.n_seq * ((max_rows + M - 1) / M));
+    const int64_t runs = (longest + p.least - 1) / p.least,
+                  units = std::min(std::max<int64_t>(tiles, p.target) * (longest > 1 << 30 ? 2 : 1), tiles * runs) * p.n_head_kv;
     if (units > 0x7fffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)units);
     if constexpr (MANY) {
@@ -917,7 +916,7 @@ static hipError_t attention_rows(AttnArgs p, int min_rows, int max_rows, hipStre
     else if (p.head_dim != DP) hipLaunchKernelGGL((k_attn_rows<T, DP, true, false>), grid, TPB, 0, s, p);
     else hipLaunchKernelGGL((k_attn_rows<T, DP, false, false>), grid, TPB, 0, s, p);
     if (longest > p.least) {                  // only fewer than `target` tiles are split
-        const int64_t wgs = std::min<int64_t>(tiles, p.target) * p.n_head_kv * (M / JOIN_ROWS);
+        const int64_t wgs = std::min<int64_t>(tiles, p.target) * p.n_head_kv * (M / JOIN_PART(M));
         hipLaunchKernelGGL((k_attn_join<T, DP, M>), dim3((unsigned)wgs), ATT_TPB, 0, s, p);
     }
     return hipGetLastError();

@@ -77,9 +77,12 @@ __device__ __forceinline__ int unit_run(const AttnArgs &p, long long work, long 
     return want >= 0x1p29f ? 1 << 30 : ((int)want + p.least) & -p.least;
 }
 
+// A value that every lane of the wave has, in a scalar register: what follows from it branches.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // The unit `id` of this workgroup's kv head, or with TILES the tile `id` (its chunk 0); false: none.
 template <int TPB, bool TILES>
-__device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit &u)
+__device__ __forceinline__ bool search_unit(const AttnArgs &p, int M, int id, Unit &u)
 {
     __shared__ long long part[2][TPB / 64];
     __shared__ int found[3];
@@ -163,6 +166,16 @@ __device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit
     return true;
 }
 
+template <int TPB, bool TILES>
+__device__ __forceinline__ bool find_unit(const AttnArgs &p, int M, int id, Unit &u)
+{
+    Unit v;
+    const bool is = search_unit<TPB, TILES>(p, M, id, v);
+    u = { uniform(v.seq), uniform(v.tile), uniform(v.chunk), uniform(v.run), uniform(v.whole), uniform(v.first), uniform(v.m),
+          uniform(v.kv), uniform(v.n) };
+    return is;
+}
+
 // What a unit works on: rows of the tile, the keys that any of them sees from a multiple of 32 to an end, in how
 // many runs.
 struct Tile {
@@ -237,6 +250,53 @@ __device__ __forceinline__ f32x4 odd_values(const _Float16 *v)
     return o;
 }
 
+// A lane's row of q, NC chunks of eight values STEP apart, as F16 parts with the row's power of two taken out of `c2`;
+// STEP / 8 lanes share a row.  Every load is made, of columns that are there: a branch around each
+// would wait for it (41,000 cycles of a unit's 130,000).
+template <typename T, bool PAD, int NC, int STEP>
+__device__ __forceinline__ void load_q(const AttnArgs &p, const T *q, bool live, int h, f16x8 *hi, f16x8 *lo, float &c2)
+{
+    if constexpr (sizeof(T) == 4) {
+        f32x4 x[2 * NC];
+#pragma unroll
+        for (int c = 0; c < 2 * NC; c++) {
+            const int at = STEP * (c / 2) + 8 * h;
+            x[c] = *(const f32x4 *)(q + (PAD && at >= p.head_dim ? 0 : at) + 4 * (c & 1));
+        }
+        float amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2 * NC; c++) {
+            const bool in = live && (!PAD || STEP * (c / 2) + 8 * h < p.head_dim);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[c][e] = in ? x[c][e] * p.q_sign : 0.0f;
+                amax = fmaxf(amax, fabsf(x[c][e]));
+            }
+        }
+        if constexpr (STEP == 32) amax = fmaxf(amax, lane_xor<16>(amax));
+        amax = fmaxf(amax, lane_xor<32>(amax));
+        const int ex = row_exponent(amax);
+        c2 = mul_pow2(c2, -ex);
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                _Float16 a, b;
+                split(mul_pow2(x[2 * c + e / 4][e & 3], ex), a, b);
+                hi[c][e] = a;
+                lo[c][e] = b;
+            }
+    } else {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const bool in = !PAD || STEP * c + 8 * h < p.head_dim;
+            f16x8 v = *(const f16x8 *)(q + (in ? STEP * c + 8 * h : 0));
+            if (!live || !in) v = f16x8{ 0, 0, 0, 0, 0, 0, 0, 0 };
+            hi[c] = v * (_Float16)p.q_sign;
+        }
+    }
+}
+
 // The row of a cache that holds position `key` (of kv head g): its first value's index, or -1.
 __device__ __forceinline__ int64_t cache_row(const AttnArgs &p, int block, int key, int g)
 {
@@ -267,7 +327,7 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
     constexpr int NC = DP / 32;              // operands of a key's row
     constexpr int NT = DP / 16;              // output tiles; values of a key that a lane reads for the second product
     __shared__ RowsShared<DP> sh;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, h = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, h = lane >> 4;
     const int g = blockIdx.x % p.n_head_kv, id = blockIdx.x / p.n_head_kv, group = p.n_head / p.n_head_kv;
     Unit u;
     if (!find_unit<ATT_TPB, false>(p, ROWS_M, id, u)) return;
@@ -302,36 +362,7 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
                  (int64_t)(g * group + my_h) * p.head_dim;
     f16x8 qh[NC], ql[NC];
     float c2 = p.scale;                       // |scale| log2 e, times the row's power of two
-    if constexpr (SPLIT) {
-        float v[NC][8], amax = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[c][e] = live && (!PAD || 32 * c + 8 * h < p.head_dim) ? q[32 * c + 8 * h + e] * p.q_sign : 0.0f;
-                amax = fmaxf(amax, fabsf(v[c][e]));
-            }
-        amax = fmaxf(amax, lane_xor<16>(amax));
-        amax = fmaxf(amax, lane_xor<32>(amax));
-        const int ex = row_exponent(amax);
-        c2 = mul_pow2(c2, -ex);
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                _Float16 a, b;
-                split(mul_pow2(v[c][e], ex), a, b);
-                qh[c][e] = a;
-                ql[c][e] = b;
-            }
-    } else {
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            f16x8 v = { 0, 0, 0, 0, 0, 0, 0, 0 };
-            if (live && (!PAD || 32 * c + 8 * h < p.head_dim)) v = *(const f16x8 *)(q + 32 * c + 8 * h);
-            qh[c] = v * (_Float16)p.q_sign;
-        }
-    }
+    load_q<T, PAD, NC, 32>(p, q, live, h, qh, ql, c2);
 
     const int all_from = (int)max(p.window ? base + j1 - p.window + 1 : 0, (int64_t)0);      // keys that every row sees:
     const int64_t all_to = base + j0;                                                        // from .. to
@@ -527,11 +558,17 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: tiles of 32 a wave.  The workgroup stages KT keys at a time in LDS, twice (the next keys' loads run
-// beside the products); a wave multiplies them with its 32 rows on 32 x 32 x 16 matrix products.  Rows of both tiles
-// lie DP values apart in chunks of 16 bytes whose index is xored with bits of the key, so that eight lanes that read
-// one chunk of eight keys (k), and 32 that read 64 bytes of four keys (v), meet no bank twice.  V is transposed on its
-// way from LDS (ds_read_b64_tr_b16: a lane gets one value of four keys).
+// Many rows: tiles of 32 a wave.  The workgroup stages KT keys at a time in LDS, twice; a wave multiplies them with its
+// 32 rows on 32 x 32 x 16 matrix products.  Rows of both tiles lie DP values apart in chunks of 16 bytes whose index is
+// xored with bits of the key, so that eight lanes that read one chunk of eight keys (k), and 32 that read 64 bytes of
+// four keys (v), meet no bank twice.  V is transposed on its way from LDS (ds_read_b64_tr_b16: a lane gets one value of
+// four keys).
+//
+// A step's K is of one tile, its V of the tile before: weights come from scores already there, and one barrier a step,
+// between weights and the products, is enough.  Waves drift apart by most of a step, so that one's weights (vector units)
+// and staging run beside the other's products on its SIMD.  Two chunks of 4096 and 2582 tokens on up to 12,288 cached,
+// F16, 32 heads over 4 of 128: 1610 us, 862 TFLOP/s, where a large product reaches 1176.  With a second barrier after the
+// products 1734; with four waves half a step behind the others and two barriers, so that they always take turns, 1756.
 // ---------------------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -540,27 +577,55 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-template <int DP>
+template <typename T, int DP>
 struct TileShape {
     static constexpr int WAVES = DP == 256 ? 4 : 8, M = 32 * WAVES, TPB = 64 * WAVES;
-    static constexpr int KT = DP == 256 ? 32 : 64;       // keys staged at a time
+    static constexpr int KT = DP == 256 || (DP == 128 && sizeof(T) == 4) ? 32 : 64;     // keys staged at a time
 };
 
+// Where a chunk of a key's row lies: the rows' starts are 256 bytes (all banks) apart, 128 for DP 64.
 template <int DP>
-__device__ __forceinline__ int k_chunk(int key, int chunk) { return chunk ^ (key & 7); }
+__device__ __forceinline__ int k_chunk(int key, int chunk) { return chunk ^ (DP == 64 ? key >> 1 & 7 : key & 15); }
 template <int DP>
-__device__ __forceinline__ int v_chunk(int key, int chunk) { return chunk ^ (DP == 64 ? (key >> 1 & 1) << 2 : (key & 3) << 2); }
-
-template <typename T, int DP, bool PAD>
-__global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_tiles(AttnArgs p)
+__device__ __forceinline__ int v_chunk(int key, int chunk)
 {
-    using S = TileShape<DP>;
+    return chunk ^ (DP == 64 ? (key >> 1 & 1) << 2 | (key >> 2 & 1) << 1 : (key & 3) << 2 | (key >> 2 & 1) << 1);
+}
+
+// N operands from LDS, read(i), and their products, use(i, operand): four operands ahead, in an order that the compiler
+// keeps (by itself it reads each right before its product and waits).
+template <int N, typename R, typename F>
+__device__ __forceinline__ void stream_operands(R read, F use)
+{
+    constexpr int AT = 4;
+    static_assert(N % AT == 0, "whole groups");
+    f16x8 a[2][AT];
+#pragma unroll
+    for (int i = 0; i < AT; i++) a[0][i] = read(i);
+#pragma unroll
+    for (int g = 0; g < N / AT; g++) {
+        if (g + 1 < N / AT) {
+#pragma unroll
+            for (int i = 0; i < AT; i++) a[(g + 1) & 1][i] = read((g + 1) * AT + i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < AT; i++) use(g * AT + i, a[g & 1][i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// TINY: blocks of fewer keys than a wave reads at once (64 / CH).
+template <typename T, int DP, bool PAD, bool TINY>
+__global__ void __launch_bounds__((TileShape<T, DP>::TPB), DP == 256 ? 1 : 2) k_attn_tiles(AttnArgs p)
+{
+    using S = TileShape<T, DP>;
     constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int NC = DP / 16, NT = DP / 32, KT = S::KT, NS = SPLIT || DP == 256 ? 1 : 2, CH = DP / 8;
+    constexpr int NC = DP / 16, NT = DP / 32, KT = S::KT, NS = KT / 32, CH = DP / 8;
     constexpr int NL = KT * CH / S::TPB;      // chunks of each tile a thread stages
     __shared__ __attribute__((aligned(1024))) _Float16 lk[2][KT * DP], lv[2][KT * DP];
-    __shared__ uint8_t flags[2][64];          // of each staged key: 1 there, 2 values of v left out that are not finite
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, h = lane >> 5;
+    __shared__ uint8_t odd[2][64];            // of staged keys: values of v were left out that are not finite
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 31, h = lane >> 5;
     const int g = blockIdx.x % p.n_head_kv, id = blockIdx.x / p.n_head_kv, group = p.n_head / p.n_head_kv;
     Unit u;
     if (!find_unit<S::TPB, false>(p, S::M, id, u)) return;
@@ -569,55 +634,80 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
     const int64_t base = tile.base;
     const int k0 = (int)min((int64_t)tile.start + (int64_t)u.chunk * u.run, (int64_t)tile.end),
               k1 = (int)min((int64_t)k0 + u.run, (int64_t)tile.end);
+    const int steps = (k1 - k0 + KT - 1) / KT;
     const int32_t *table = p.table + (int64_t)u.seq * p.max_blocks;
 
-    // staging: the blocks of this thread's keys of step kb, then their chunks
-    int blocks[NL];
+    // Staging of pair n: v of step n and k of step n + 1, from the blocks of both.  A wave's lanes read chunks of 64 / CH
+    // keys at a time, which lie in one block: its place is found in scalar registers, a lane adds its own offset (with
+    // places by lane, staging took 2,300 cycles of a step's 5,300).
+    // Every load is made, of a row of the cache in any case: a branch around one would wait for those before it.  What is
+    // not there becomes 0 on its way into LDS.
+    constexpr int KW = 64 / CH;
+    int block[NL];                            // of the step after a pair's
+    int64_t at_k[NL], at_v[NL];               // v of a step lies where k did
+    bool has_k[NL], has_v[NL];
     i32x4 sk[NL], sv[NL];
-    uint32_t there = 0;
-    const auto look_up = [&](int kb) {
+    const bool lane_in = !PAD || 8 * (lane % CH) < p.head_dim;
+    const int lane_key = lane / CH, lane_at = (TINY ? 0 : lane_key * p.head_dim) + (lane_in ? 8 * (lane % CH) : 0);
+    const int64_t block_stride = (int64_t)p.n_head_kv * p.head_dim << p.log_block, head_at = (int64_t)g * p.head_dim << p.log_block;
+    const _Float16 *head_k = p.k + head_at, *head_v = p.v + head_at;
+    const auto first_key = [&](int n, int i) { return k0 + n * KT + i * (S::TPB / CH) + wave * KW; };
+    const auto look_up = [&](int n) {
 #pragma unroll
-        for (int i = 0; i < NL; i++) blocks[i] = table[min(kb + (tid + i * S::TPB) / CH, k1 - 1) >> p.log_block];
+        for (int i = 0; i < NL; i++) block[i] = table[min(first_key(n, i) + (TINY ? lane_key : 0), k1 - 1) >> p.log_block];
     };
-    const auto load = [&](int kb) {
-        there = 0;
+    const auto load = [&](int n, bool with_v) {
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int x = tid + i * S::TPB, key = kb + x / CH, c = x % CH;
-            sk[i] = { 0, 0, 0, 0 };
-            sv[i] = { 0, 0, 0, 0 };
-            if (key < k1 && (unsigned)blocks[i] < (unsigned)p.n_blocks) {
-                there |= 1u << i;
-                const int64_t at = cache_row(p, blocks[i], key, g) + 8 * c;
-                if (!PAD || 8 * c < p.head_dim) {
-                    sk[i] = *(const i32x4 *)(p.k + at);
-                    sv[i] = *(const i32x4 *)(p.v + at);
-                }
-            }
+            at_v[i] = at_k[i];
+            has_v[i] = has_k[i];
+            const int b = TINY ? block[i] : uniform(block[i]), key = first_key(n + 1, i) + (TINY ? lane_key : 0);
+            const bool ok = (unsigned)b < (unsigned)p.n_blocks;
+            at_k[i] = (ok ? b : 0) * block_stride + (key & ((1 << p.log_block) - 1)) * p.head_dim;
+            has_k[i] = ok && first_key(n + 1, i) + lane_key < k1 && lane_in;
         }
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            if (with_v) sv[i] = *(const i32x4 *)(head_v + at_v[i] + lane_at);
+            sk[i] = *(const i32x4 *)(head_k + at_k[i] + lane_at);
+        }
+        look_up(n + 2);
     };
-    const auto store = [&](int buf, int kb) {
-        // where some rows see keys that others do not, an infinity or NaN of v must not meet a weight 0: it is left out
-        const bool edge = kb + KT - 1 > base + tile.j0 || p.window;
+    // Steps from which on some rows see keys that others do not: there an infinity or NaN of v must not meet a weight 0
+    // and is left out.
+    const auto floor_step = [&](int64_t key) { return (int)min(max((key - k0) >> (KT == 64 ? 6 : 5), (int64_t)-2), (int64_t)0x7ffffff0); };
+    const int edge = p.window ? 0 : max(floor_step(base + tile.j0 - KT + 1) + 1, 0);
+    const auto store = [&](int n, bool with_v) {
 #pragma unroll
         for (int i = 0; i < NL; i++) {
             const int x = tid + i * S::TPB, key = x / CH, c = x % CH;
-            bool bad = false;
-            if (edge) {
+            if (!__all(has_k[i] && (has_v[i] || !with_v))) {
+#pragma unroll
+                for (int d = 0; d < 4; d++) {
+                    if (!has_k[i]) sk[i][d] = 0;
+                    if (!has_v[i]) sv[i][d] = 0;
+                }
+            }
+            *(i32x4 *)&lk[(n + 1) & 1][key * DP + 8 * k_chunk<DP>(key, c)] = sk[i];
+            if (!with_v) continue;
+            if (n >= edge) {
+                bool bad = false;
 #pragma unroll
                 for (int d = 0; d < 4; d++) sv[i][d] = finite_pair(sv[i][d], bad);
+                const uint64_t any = __ballot(bad);           // (the CH lanes of a key lie in one wave)
+                if (c == 0) odd[n & 1][key] = (any >> (lane & ~(CH - 1)) & ((1ull << CH) - 1)) != 0;
             }
-            *(i32x4 *)&lk[buf][key * DP + 8 * k_chunk<DP>(key, c)] = sk[i];
-            *(i32x4 *)&lv[buf][key * DP + 8 * v_chunk<DP>(key, c)] = sv[i];
-            const uint64_t any = __ballot(bad);               // (the CH lanes of a key lie in one wave)
-            if (c == 0) flags[buf][key] = (there >> i & 1) | ((any >> (lane & ~(CH - 1)) & ((1ull << CH) - 1)) != 0 ? 2 : 0);
+            *(i32x4 *)&lv[n & 1][key * DP + 8 * v_chunk<DP>(key, c)] = sv[i];
         }
     };
+    // whether the keys of a step are there, a lane each (of 64 or 32), looked up a step ahead
+    int key_block = 0;
+    const auto look_up_key = [&](int n) { key_block = table[min(k0 + n * KT + (lane & (KT - 1)), k1 - 1) >> p.log_block]; };
 
-    if (k0 < k1) {
-        look_up(k0);
-        load(k0);
-        look_up(k0 + KT);
+    if (steps > 0) {
+        look_up(0);
+        look_up_key(0);
+        load(-1, false);
     }
 
     // this lane's row
@@ -630,38 +720,10 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
                  (int64_t)(g * group + my_h) * p.head_dim;
     f16x8 qh[NC], ql[SPLIT ? NC : 1];
     float c2 = p.scale;
-    if constexpr (SPLIT) {
-        float amax = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-            if (live && (!PAD || 16 * c + 8 * h < p.head_dim)) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(q[16 * c + 8 * h + e] * p.q_sign));
-            }
-        amax = fmaxf(amax, lane_xor<32>(amax));
-        const int ex = row_exponent(amax);
-        c2 = mul_pow2(c2, -ex);
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = live && (!PAD || 16 * c + 8 * h < p.head_dim) ? q[16 * c + 8 * h + e] * p.q_sign : 0.0f;
-                _Float16 a, b;
-                split(mul_pow2(v, ex), a, b);
-                qh[c][e] = a;
-                ql[c][e] = b;
-            }
-    } else {
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            f16x8 v = { 0, 0, 0, 0, 0, 0, 0, 0 };
-            if (live && (!PAD || 16 * c + 8 * h < p.head_dim)) v = *(const f16x8 *)(q + 16 * c + 8 * h);
-            qh[c] = v * (_Float16)p.q_sign;
-        }
-    }
+    load_q<T, PAD, NC, 16>(p, q, live, h, qh, ql, c2);
     // the wave's rows: positions from w_first to w_last; keys that all of them see end at w_first
     const int w_rows = min(tile.rows - wave * 32, 32);
-    const int64_t w_first = base + (tile.row0 + wave * 32) / group, w_last = base + (tile.row0 + wave * 32 + w_rows - 1) / group;
+    const int64_t w_first = base + (tile.row0 + wave * 32) / group, w_last = base + (tile.row0 + wave * 32 + max(w_rows, 1) - 1) / group;
     const int64_t w_from = p.window ? w_last - p.window + 1 : 0, w_low = p.window ? w_first - p.window + 1 : 0;
 
     float m = -INFINITY, l = 0.0f;
@@ -674,103 +736,120 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
     const int k_row = r * DP, s16 = lane & 15;
     const int v_row = (4 * h + (s16 >> 2)) * DP, v_in = 2 * (lane >> 4 & 1) + (s16 & 3) / 2, v_half = 4 * (s16 & 1);
 
-    if (k0 < k1) store(0, k0);
-    __syncthreads();
-    int buf = 0;
-    for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
-        const bool more = kb + KT < k1;
-        if (more) {
-            load(kb + KT);
-            look_up(kb + 2 * KT);
-        }
-        if (w_rows > 0 && kb <= w_last && kb + KT - 1 >= w_low) {
-            const int flag = lane < KT ? flags[buf][lane] : 1;
-            const uint64_t there_all = __ballot(flag & 1);
-            uint64_t odd = __ballot(flag & 2);
-            for (; odd != 0; odd &= odd - 1) {
-                const int key = kb + __builtin_ctzll(odd);
-                const _Float16 *v = p.v + cache_row(p, table[key >> p.log_block], key, g) + 4 * h;
-                if (key > pos || key < low) continue;
+    // the steps that any of them sees, and those of which all see all
+    const int work_from = floor_step(w_low), work_to = w_rows > 0 ? floor_step(w_last) : -1;
+    const int all_from = floor_step(w_from + KT - 1), all_to = floor_step(w_first - KT + 1);
+    const auto at_work = [&](int n) { return n >= work_from && n <= work_to; };
+    f32x16 s[NS];
+    f16x8 ph[2 * NS], pl[SPLIT ? 2 * NS : 1];
+    const auto scores = [&](int n) {          // S^T of step n
+        if (!at_work(n)) return;
+        const int buf = n & 1;
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+        for (int t = 0; t < NS; t++)
 #pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        if (PAD && 32 * t + 8 * b + 4 * h >= p.head_dim) continue;
-                        const f32x4 o = odd_values(v + 32 * t + 8 * b);
+            for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+        stream_operands<NC * NS>(
+            [&](int i) { return *(const f16x8 *)&lk[buf][32 * (i % NS) * DP + k_row + 8 * k_chunk<DP>(r, 2 * (i / NS) + h)]; },
+            [&](int i, f16x8 a) {
+                s[i % NS] = mfma32(a, qh[i / NS], s[i % NS]);
+                if constexpr (SPLIT) s[i % NS] = mfma32(a, ql[i / NS], s[i % NS]);
+            });
+    };
+    const auto weights = [&](int n) {         // of step n, from its scores
+        if (!at_work(n)) return;
+        const int kb = k0 + n * KT;
+        const uint64_t seen = __ballot((unsigned)key_block < (unsigned)p.n_blocks && kb + (lane & (KT - 1)) < k1);
+        if (~seen != 0 || n < all_from || n > all_to) {
+            const uint64_t mine = seen >> (4 * h);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) acc[t][4 * b + j] += o[j];
-                    }
-            }
+            for (int t = 0; t < NS; t++)
 #pragma unroll
-            for (int sub = 0; sub < KT; sub += 32 * NS) {
-                f32x16 s[NS];
-#pragma unroll
-                for (int n = 0; n < NS; n++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
-#pragma unroll
-                for (int c = 0; c < NC; c++)
-#pragma unroll
-                    for (int n = 0; n < NS; n++) {
-                        const f16x8 a = *(const f16x8 *)&lk[buf][(sub + 32 * n) * DP + k_row + 8 * k_chunk<DP>(r, 2 * c + h)];
-                        s[n] = mfma32(a, qh[c], s[n]);
-                        if constexpr (SPLIT) s[n] = mfma32(a, ql[c], s[n]);
-                    }
-                if (~there_all != 0 || kb < w_from || kb + KT - 1 > w_first) {
-#pragma unroll
-                    for (int n = 0; n < NS; n++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int k = sub + 32 * n + 8 * (i / 4) + 4 * h + (i & 3);
-                            if (!((there_all >> k & 1) && kb + k <= pos && kb + k >= low)) s[n][i] = -INFINITY;
-                        }
+                for (int i = 0; i < 16; i++) {
+                    const int k = 32 * t + 8 * (i / 4) + (i & 3);
+                    if (!((mine >> k & 1) && kb + k + 4 * h <= pos && kb + k + 4 * h >= low)) s[t][i] = -INFINITY;
                 }
-                float top = -INFINITY;
-#pragma unroll
-                for (int n = 0; n < NS; n++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
-                top *= c2;
-                top = fmaxf(top, lane_xor<32>(top));
-                if (__any(top > m + ATT_LAG)) {
-                    const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 1.0f : fast_exp2(m - m2);
-                    m = m2;
-                    l *= keep;
-#pragma unroll
-                    for (int t = 0; t < NT; t++) acc[t] *= keep;
-                }
-                const float less = m == -INFINITY ? 0.0f : m - ATT_SHIFT;
-                f16x8 ph[2 * NS], pl[SPLIT ? 2 * NS : 1];
-#pragma unroll
-                for (int n = 0; n < NS; n++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float w = fast_exp2(__builtin_fmaf(s[n][i], c2, -less));
-                        l += w;
-                        _Float16 a, b;
-                        split(w, a, b);
-                        ph[2 * n + i / 8][i % 8] = a;
-                        if constexpr (SPLIT) pl[2 * n + i / 8][i % 8] = b;
-                    }
-#pragma unroll
-                for (int k16 = 0; k16 < 2 * NS; k16++)
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        // a value of each of the keys 4 h .. + 3 and 8 + 4 h .. + 3 of 16
-                        const int at = (sub + 16 * k16) * DP + v_row + 8 * ((4 * t + v_in) ^ v_chunk<DP>(4 * h + (s16 >> 2), 0)) + v_half;
-                        union {
-                            s16x4 part[2];
-                            f16x8 whole;
-                        } a;
-                        a.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at]);
-                        a.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at + 8 * DP]);
-                        acc[t] = mfma32(a.whole, ph[k16], acc[t]);
-                        if constexpr (SPLIT) acc[t] = mfma32(a.whole, pl[k16], acc[t]);
-                    }
-            }
         }
-        if (more) store(buf ^ 1, kb + KT);
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < NS; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[t][i]);
+        top *= c2;
+        top = fmaxf(top, lane_xor<32>(top));
+        if (__any(top > m + ATT_LAG)) {
+            const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 1.0f : fast_exp2(m - m2);
+            m = m2;
+            l *= keep;
+#pragma unroll
+            for (int t = 0; t < NT; t++) acc[t] *= keep;
+        }
+        const float less = m == -INFINITY ? 0.0f : m - ATT_SHIFT;
+#pragma unroll
+        for (int t = 0; t < NS; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float w = fast_exp2(__builtin_fmaf(s[t][i], c2, -less));
+                l += w;
+                _Float16 a, b;
+                split(w, a, b);
+                ph[2 * t + i / 8][i % 8] = a;
+                if constexpr (SPLIT) pl[2 * t + i / 8][i % 8] = b;
+            }
+    };
+    const auto values = [&](int n) {          // O^T += V^T P^T of step n
+        if (!at_work(n)) return;
+        const int kb = k0 + n * KT, buf = n & 1;
+        uint64_t left_out = n >= edge ? __ballot(lane < KT ? odd[buf][lane] : 0) : 0;
+        for (; left_out != 0; left_out &= left_out - 1) {
+            const int key = kb + __builtin_ctzll(left_out);
+            const _Float16 *v = p.v + cache_row(p, table[key >> p.log_block], key, g) + 4 * h;
+            if (key > pos || key < low) continue;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    if (PAD && 32 * t + 8 * b + 4 * h >= p.head_dim) continue;
+                    const f32x4 o = odd_values(v + 32 * t + 8 * b);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[t][4 * b + j] += o[j];
+                }
+        }
+        stream_operands<2 * NS * NT>(
+            [&](int i) {
+                // of 16 keys a value of each of 4 h .. + 3 and 8 + 4 h .. + 3
+                const int k16 = i / NT, t = i % NT,
+                          at = 16 * k16 * DP + v_row + 8 * ((4 * t + v_in) ^ v_chunk<DP>(4 * h + (s16 >> 2), 0)) + v_half;
+                union {
+                    s16x4 part[2];
+                    f16x8 whole;
+                } a;
+                a.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at]);
+                a.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)&lv[buf][at + 8 * DP]);
+                return a.whole;
+            },
+            [&](int i, f16x8 a) {
+                acc[i % NT] = mfma32(a, ph[i / NT], acc[i % NT]);
+                if constexpr (SPLIT) acc[i % NT] = mfma32(a, pl[i / NT], acc[i % NT]);
+            });
+    };
+
+    // A step's one barrier: before it all have stored pair n (v of n, k of n + 1), after it they read it.  The places of
+    // pair n + 1 were last read before it.
+    if (steps > 0) {
+        store(-1, false);
+        load(0, true);
         __syncthreads();
+        scores(0);
+        for (int n = 0; n < steps; n++) {
+            store(n, true);                  // (keys past the last are zeros)
+            load(n + 1, true);
+            weights(n);
+            look_up_key(n + 1);
+            __syncthreads();
+            values(n);
+            if (n + 1 < steps) scores(n + 1);
+        }
     }
 
     l += lane_xor<32>(l);
@@ -807,31 +886,38 @@ __global__ void __launch_bounds__(TileShape<DP>::TPB, DP == 256 ? 1 : 2) k_attn_
 }
 
 // ---------------------------------------------------------------------------
-// Tiles of several runs: a workgroup joins the partial results of JOIN_ROWS rows, [M][DP] sums and then every row's
-// maximum and sum of weights, unit after unit of a kv head.  A launch of its own: a device-wide release and acquire
-// in each unit of the split kernel, for the last of a tile to join it, writes back and invalidates its XCD's whole L2
-// and made 1,800 units of 64 streams wait for each other (614 us in place of 186).
+// Tiles of several runs: a workgroup joins the partial results of some rows, [M][DP] sums and then every row's maximum
+// and sum of weights, unit after unit of a kv head.  A launch of its own: a device-wide release and acquire in each unit
+// of the split kernel, for the last of a tile to join it, writes back and invalidates its XCD's whole L2 and made 1,800
+// units of 64 streams wait for each other (614 us in place of 186).
+//
+// Small tiles have up to 512 runs, which lanes share out: four rows a workgroup, their factors by a wave each, then
+// 16-byte pieces of rows, ATT_TPB in all.  Large ones have few: a thread takes a piece of one row and all its runs, which
+// needs neither LDS nor a barrier.
 // ---------------------------------------------------------------------------
 
-constexpr int JOIN_ROWS = 4;                 // at a time
-constexpr int JOIN_PART(int M) { return M == ROWS_M ? JOIN_ROWS : 32; }      // rows a workgroup
+constexpr int JOIN_ROWS(int M, int DP) { return M == ROWS_M ? 4 : ATT_TPB / (DP / 4); }      // rows a workgroup
 
 template <typename T, int DP, int M>
 __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
 {
-    constexpr int ITEMS = JOIN_ROWS * (DP / 4), PARTS = ATT_TPB / ITEMS;
-    __shared__ float factor[JOIN_ROWS][512];
-    __shared__ f32x4 sums[ATT_TPB];
-    const int tid = threadIdx.x, parts = M / JOIN_PART(M), group = p.n_head / p.n_head_kv;
-    const int from_row = blockIdx.x % parts * JOIN_PART(M), g = blockIdx.x / parts % p.n_head_kv, id = blockIdx.x / parts / p.n_head_kv;
+    constexpr int ROWS = JOIN_ROWS(M, DP), parts = M / ROWS;
+    const int tid = threadIdx.x, group = p.n_head / p.n_head_kv;
+    const int n0 = blockIdx.x % parts * ROWS, g = blockIdx.x / parts % p.n_head_kv, id = blockIdx.x / parts / p.n_head_kv;
     Unit u;
     if (!find_unit<ATT_TPB, true>(p, M, id, u)) return;
     const Tile tile = tile_of(p, M, u);
     const int chunks = tile.chunks;
-    if (chunks == 1) return;
+    if (chunks == 1 || n0 >= tile.rows) return;
     const int64_t step = (int64_t)p.n_head_kv * (M * (DP + 2));
     const float *from = p.partial + (int64_t)(g + (int64_t)u.whole * p.n_head_kv) * (M * (DP + 2));
-    for (int n0 = from_row; n0 < min(tile.rows, from_row + JOIN_PART(M)); n0 += JOIN_ROWS) {
+    constexpr int ITEMS = ROWS * (DP / 4), PARTS = ATT_TPB / ITEMS;
+    const int item = tid % ITEMS, part = tid / ITEMS, n = item / (DP / 4), d = item % (DP / 4) * 4;
+    const float *f = from + (int64_t)(n0 + n) * DP + d;
+    f32x4 o = { 0, 0, 0, 0 };
+    if constexpr (M == ROWS_M) {
+        __shared__ float factor[ROWS][512];
+        __shared__ f32x4 sums[ATT_TPB];
         {
             // each run's factor: 2^(its maximum - the largest) / sum of weights; a wave a row
             const int lane = tid & 63, n = tid >> 6;
@@ -849,22 +935,34 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
             for (int c = lane; c < chunks; c += 64) factor[n][c] *= by;
         }
         __syncthreads();
-        const int item = tid % ITEMS, part = tid / ITEMS, n = item / (DP / 4), d = item % (DP / 4) * 4;
-        const float *f = from + (int64_t)(n0 + n) * DP + d;
-        f32x4 o = { 0, 0, 0, 0 };
 #pragma unroll 8
         for (int c = part; c < chunks; c += PARTS) o += factor[n][c] * *(const f32x4 *)(f + c * step);
-        if constexpr (PARTS > 1) sums[tid] = o;
-        __syncthreads();
-        if (part == 0 && n0 + n < tile.rows && d < p.head_dim) {
+        if constexpr (PARTS > 1) {
+            sums[tid] = o;
+            __syncthreads();
+            if (part == 0) {
 #pragma unroll
-            for (int i = 1; i < PARTS; i++) o += sums[i * ITEMS + item];
-            const int j = (tile.row0 + n0 + n) / group, a = (tile.row0 + n0 + n) % group;
-            T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim + d;
-#pragma unroll
-            for (int i = 0; i < 4; i++) out[i] = (T)o[i];
+                for (int i = 1; i < PARTS; i++) o += sums[i * ITEMS + item];
+            }
         }
-        __syncthreads();
+    } else {
+        const float *w = from + M * DP + n0 + n;
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < chunks; c++) top = fmaxf(top, w[c * step]);
+#pragma unroll 4
+        for (int c = 0; c < chunks; c++) {
+            const float m = w[c * step], x = m == -INFINITY ? 1.0f : fast_exp2(m - top);
+            sum += x * w[c * step + M];
+            o += x * *(const f32x4 *)(f + c * step);
+        }
+        o *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    }
+    if (part == 0 && n0 + n < tile.rows && d < p.head_dim) {
+        const int j = (tile.row0 + n0 + n) / group, a = (tile.row0 + n0 + n) % group;
+        T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim + d;
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = (T)o[i];
     }
 }
 
@@ -883,7 +981,7 @@ static int64_t most_tiles(const AttnArgs &p, int M)
 size_t attention_workspace(const AttnArgs &p)
 {
     // split tiles are fewer than `target`, and so are their units; twice that where a unit ends at 2^30 keys
-    const int dp = padded_dim(p.head_dim), many = dp == 256 ? TileShape<256>::M : TileShape<128>::M;
+    const int dp = padded_dim(p.head_dim), many = dp == 256 ? TileShape<float, 256>::M : TileShape<float, 128>::M;
     const size_t units = std::max((size_t)target_units(p, false) * ROWS_M, (size_t)target_units(p, true) * many);
     return 2 * units * p.n_head_kv * (dp + 2) * sizeof(float);
 }
@@ -892,7 +990,7 @@ size_t attention_workspace(const AttnArgs &p)
 template <typename T, int DP, bool MANY>
 static hipError_t attention_rows(AttnArgs p, int min_rows, int max_rows, hipStream_t s)
 {
-    using S = TileShape<DP>;
+    using S = TileShape<T, DP>;
     constexpr int M = MANY ? S::M : ROWS_M, TPB = MANY ? S::TPB : ATT_TPB;
     p.min_rows = min_rows;
     p.max_rows = max_rows;
@@ -910,13 +1008,14 @@ static hipError_t attention_rows(AttnArgs p, int min_rows, int max_rows, hipStre
     if (units > 0x7fffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)units);
     if constexpr (MANY) {
-        if (p.head_dim != DP) hipLaunchKernelGGL((k_attn_tiles<T, DP, true>), grid, TPB, 0, s, p);
-        else hipLaunchKernelGGL((k_attn_tiles<T, DP, false>), grid, TPB, 0, s, p);
+        if (1 << p.log_block < 512 / DP) hipLaunchKernelGGL((k_attn_tiles<T, DP, true, true>), grid, TPB, 0, s, p);
+        else if (p.head_dim != DP) hipLaunchKernelGGL((k_attn_tiles<T, DP, true, false>), grid, TPB, 0, s, p);
+        else hipLaunchKernelGGL((k_attn_tiles<T, DP, false, false>), grid, TPB, 0, s, p);
     } else if (p.log_block < 2) hipLaunchKernelGGL((k_attn_rows<T, DP, true, true>), grid, TPB, 0, s, p);
     else if (p.head_dim != DP) hipLaunchKernelGGL((k_attn_rows<T, DP, true, false>), grid, TPB, 0, s, p);
     else hipLaunchKernelGGL((k_attn_rows<T, DP, false, false>), grid, TPB, 0, s, p);
     if (longest > p.least) {                  // only fewer than `target` tiles are split
-        const int64_t wgs = std::min<int64_t>(tiles, p.target) * p.n_head_kv * (M / JOIN_PART(M));
+        const int64_t wgs = std::min<int64_t>(tiles, p.target) * p.n_head_kv * (M / JOIN_ROWS(M, DP));
         hipLaunchKernelGGL((k_attn_join<T, DP, M>), dim3((unsigned)wgs), ATT_TPB, 0, s, p);
     }
     return hipGetLastError();

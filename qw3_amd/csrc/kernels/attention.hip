@@ -100,6 +100,23 @@ __device__ __forceinline__ bool search_unit(const AttnArgs &p, int M, int id, Un
         u.tile = tiles - 1 - u.tile;                  // (the last tiles, which see most keys, begin first)
         return true;
     }
+    if (p.n_seq <= 64) {                              // every wave by itself: neither LDS nor a barrier
+        int tiles, span;
+        request_work(p, M, lane, tiles, span, u);
+        u.run = unit_run(p, wave_sum((long long)tiles * span), wave_sum((long long)tiles));
+        const long long units = (long long)tiles * ((span + u.run - 1) / u.run);
+        const long long at = wave_scan(units) - units, first = TILES ? wave_scan((long long)tiles) - tiles : at;
+        const uint64_t here = __ballot(id >= first && id < first + (TILES ? tiles : units));
+        if (here == 0) return false;
+        const int i = __builtin_ctzll(here), of = (int)(id - first), chunks = (span + u.run - 1) / u.run;
+        u.seq = i;
+        u.tile = TILES ? of : of / max(chunks, 1);
+        u.chunk = TILES ? 0 : of - u.tile * chunks;
+        u.whole = (int)at + u.tile * chunks;
+        u.tile = tiles - 1 - u.tile;
+        for (int *v : { &u.tile, &u.chunk, &u.whole, &u.first, &u.m, &u.kv, &u.n }) *v = __builtin_amdgcn_readlane(*v, i);
+        return true;
+    }
     long long work = 0, all = 0;
     for (int i0 = 0; i0 < p.n_seq; i0 += TPB) {
         int tiles, span;
@@ -896,7 +913,7 @@ __global__ void __launch_bounds__((TileShape<T, DP>::TPB), DP == 256 ? 1 : 2) k_
 // needs neither LDS nor a barrier.
 // ---------------------------------------------------------------------------
 
-constexpr int JOIN_ROWS(int M, int DP) { return M == ROWS_M ? 4 : ATT_TPB / (DP / 4); }      // rows a workgroup
+constexpr int JOIN_ROWS(int M, int DP) { return M == ROWS_M ? 4 : 32; }      // rows a workgroup
 
 template <typename T, int DP, int M>
 __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
@@ -911,10 +928,15 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
     if (chunks == 1 || n0 >= tile.rows) return;
     const int64_t step = (int64_t)p.n_head_kv * (M * (DP + 2));
     const float *from = p.partial + (int64_t)(g + (int64_t)u.whole * p.n_head_kv) * (M * (DP + 2));
-    constexpr int ITEMS = ROWS * (DP / 4), PARTS = ATT_TPB / ITEMS;
-    const int item = tid % ITEMS, part = tid / ITEMS, n = item / (DP / 4), d = item % (DP / 4) * 4;
-    const float *f = from + (int64_t)(n0 + n) * DP + d;
-    f32x4 o = { 0, 0, 0, 0 };
+    constexpr int ITEMS = ROWS * (DP / 4) < ATT_TPB ? ROWS * (DP / 4) : ATT_TPB, PARTS = ATT_TPB / ITEMS, AT = ITEMS / (DP / 4);
+    const int item = tid % ITEMS, part = tid / ITEMS, d = item % (DP / 4) * 4;
+    const auto put = [&](int n, f32x4 o) {
+        if (n >= tile.rows || d >= p.head_dim) return;
+        const int j = (tile.row0 + n) / group, a = (tile.row0 + n) % group;
+        T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim + d;
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = (T)o[i];
+    };
     if constexpr (M == ROWS_M) {
         __shared__ float factor[ROWS][512];
         __shared__ f32x4 sums[ATT_TPB];
@@ -935,6 +957,9 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
             for (int c = lane; c < chunks; c += 64) factor[n][c] *= by;
         }
         __syncthreads();
+        const int n = item / (DP / 4);
+        const float *f = from + (int64_t)(n0 + n) * DP + d;
+        f32x4 o = { 0, 0, 0, 0 };
 #pragma unroll 8
         for (int c = part; c < chunks; c += PARTS) o += factor[n][c] * *(const f32x4 *)(f + c * step);
         if constexpr (PARTS > 1) {
@@ -945,24 +970,32 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_join(AttnArgs p)
                 for (int i = 1; i < PARTS; i++) o += sums[i * ITEMS + item];
             }
         }
+        if (part == 0) put(n0 + n, o);
     } else {
-        const float *w = from + M * DP + n0 + n;
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-        for (int c = 0; c < chunks; c++) top = fmaxf(top, w[c * step]);
-#pragma unroll 4
-        for (int c = 0; c < chunks; c++) {
-            const float m = w[c * step], x = m == -INFINITY ? 1.0f : fast_exp2(m - top);
-            sum += x * w[c * step + M];
-            o += x * *(const f32x4 *)(f + c * step);
-        }
-        o *= sum == 0.0f ? 0.0f : 1.0f / sum;
-    }
-    if (part == 0 && n0 + n < tile.rows && d < p.head_dim) {
-        const int j = (tile.row0 + n0 + n) / group, a = (tile.row0 + n0 + n) % group;
-        T *out = (T *)((uint8_t *)p.out + (uint64_t)(u.first + j) * p.out_stride) + (int64_t)(g * group + a) * p.head_dim + d;
+        constexpr int EACH = ROWS / AT;
+        const float *w = from + M * DP + n0 + item / (DP / 4), *f = from + (int64_t)(n0 + item / (DP / 4)) * DP + d;
+        float top[EACH], sum[EACH];
+        f32x4 o[EACH];
 #pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = (T)o[i];
+        for (int i = 0; i < EACH; i++) {
+            top[i] = -INFINITY;
+            sum[i] = 0.0f;
+            o[i] = f32x4{ 0, 0, 0, 0 };
+        }
+        for (int c = 0; c < chunks; c++) {
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const float m = w[c * step + i * AT], l = w[c * step + M + i * AT], high = fmaxf(top[i], m);
+                const f32x4 v = *(const f32x4 *)(f + c * step + i * AT * DP);
+                const float x = m == -INFINITY ? 1.0f : fast_exp2(m - high);
+                const float y = top[i] == -INFINITY ? 1.0f : fast_exp2(top[i] - high);
+                top[i] = high;
+                sum[i] = sum[i] * y + x * l;
+                o[i] = o[i] * y + x * v;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; i++) put(n0 + item / (DP / 4) + i * AT, o[i] * (sum[i] == 0.0f ? 0.0f : 1.0f / sum[i]));
     }
 }
 

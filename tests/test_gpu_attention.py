@@ -203,3 +203,51 @@ def test_groups_that_do_not_divide_tiles(hip_ready):
         assert np.array_equal(got[:2], clean[:2]) and not np.isfinite(got[2, :, 7]).any()
         got[2, :, 7] = clean[2, :, 7]
         assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("n_seq", [64, 65, 300, 700])
+def test_many_requests(hip_ready, type_, n_seq):
+    """Requests beyond a wave's and a workgroup's, of few and many rows, some without tokens."""
+    rng = np.random.default_rng(n_seq)
+    new = rng.choice([0, 1, 1, 1, 2], n_seq)
+    new[[3, n_seq // 2, n_seq - 1]] = 33, 70, 40
+    lens = new + rng.integers(0, 40, n_seq)
+    lens[n_seq // 2] = 1200
+    check(n_seq, new.tolist(), lens.tolist(), 4, 1, 64, 16, type_)
+    one = np.ones(n_seq, int)
+    check(n_seq + 1, one.tolist(), (one + rng.integers(0, 300, n_seq) * (np.arange(n_seq) % 50 == 7)).tolist(), 2, 2, 64, 8, type_)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("heads,kv,dim,block", [(2, 1, 128, 2), (2, 1, 64, 4), (2, 2, 256, 1), (1, 1, 24, 2), (3, 1, 128, 1),
+                                                (2, 1, 136, 4), (1, 1, 104, 8)])
+def test_chunks_of_small_blocks(hip_ready, type_, heads, kv, dim, block):
+    """Blocks of fewer keys than are read at once, and the head sizes that fill no whole tile, over several steps."""
+    check(dim + block, [90, 150], [90, 230], heads, kv, dim, block, type_)
+    check(dim + block + 1, [100], [700], heads, kv, dim, block, type_, window=150)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+def test_chunks_split_over_their_keys(hip_ready, type_):
+    """Tiles of many rows whose keys are split, with blocks that lie outside the cache and rows that see nothing."""
+    def change(pages, q):
+        pages.table[0, 10:50] = -1
+        pages.table[1, :200] = pages.n_blocks
+    check(20, [40, 35], [1700, 3000], 4, 2, 64, 8, type_, change=change)
+    got = check(21, [80], [60], 2, 1, 128, 16, type_)
+    assert not got[:20].any() and got[20:].any()
+
+
+def test_requests_that_pass_the_rows(hip_ready):
+    """A request whose rows end behind n_tokens, or whose offsets fall, is left out; others are not."""
+    rng = np.random.default_rng(22)
+    for type_ in (F32, F16):
+        pages = D.Pages(rng, [30, 40, 9, 12], 16, 2, 64)
+        q = rng.standard_normal((12, 4, 64)).astype(D.NP[type_])
+        want = run(q[:3], pages, [3], [30], type_)
+        out = ds3.Buffer.from_array(np.full(q.shape, 7, D.NP[type_]))
+        ds3.attention_paged(ds3.Buffer.from_array(q), pages.device(), D.ints(pages.table), D.ints([0, 3, 13, 2, -1]),
+                            D.ints([30, 40, 9, 12]), out, 12, 4, 4, pages.max_blocks, 64 ** -0.5, type_)
+        got = out.read(D.NP[type_], q.shape)
+        assert np.array_equal(got[:3], want) and np.all(got[3:] == 7)

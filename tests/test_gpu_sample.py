@@ -116,3 +116,68 @@ def test_strides_and_alignment(hip_ready):
     for pad in (1, 3, 64):
         check(logits(rng, 4, 1001), rng.random(4).astype(np.float32), k=np.full(4, 40), pad=pad)
         check(logits(rng, 4, 1001), rng.random(4).astype(np.float32), p=np.full(4, 0.9), pad=pad)
+
+
+@pytest.mark.parametrize("vocab", [6000, 120000])
+def test_large_top_k_with_ties(hip_ready, vocab):
+    """More tokens kept than a list holds, borders within values that many tokens share."""
+    rng = np.random.default_rng(vocab)
+    x = (np.round(logits(rng, 8, vocab) * 4) / 4).astype(np.float32)
+    k = np.array([513, 600, 1000, 2000, 4000, 5999, vocab, 700])
+    for p in (1.0, 0.9):
+        check(x, rng.random(8), t=np.full(8, 1.5), k=k, p=np.full(8, p))
+
+
+@pytest.mark.parametrize("rows", [1, 4, 260])
+def test_rows_of_few_finite_logits(hip_ready, rows):
+    """Minus infinity nearly everywhere: one token, three, a run at either end."""
+    rng, vocab = np.random.default_rng(rows), 70000 if rows < 100 else 9000
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    for r in range(rows):
+        at = [[rng.integers(vocab)], rng.integers(0, vocab, 3), range(40), range(vocab - 40, vocab)][r % 4]
+        x[r, list(at)] = rng.standard_normal(len(at))
+    check(x, rng.random(rows), t=np.full(rows, 0.8))
+    check(x, rng.random(rows), t=np.full(rows, 0.8), k=np.full(rows, 20), p=np.full(rows, 0.9))
+
+
+def test_few_rows_draw_as_many_rows_do(hip_ready):
+    """A row's token does not depend on how many rows the call has."""
+    rng = np.random.default_rng(7)
+    for vocab in (5000, 60000):
+        x = logits(rng, 3, vocab)
+        for s in ({}, dict(k=20, p=0.95), dict(k=1500), dict(m=0.001, p=0.999)):
+            u = rng.random(3).astype(np.float32)
+            full = {key: np.full(3, value) for key, value in s.items()}
+            one = [check(x[i:i + 1], u[i:i + 1], **{key: v[:1] for key, v in full.items()}) for i in range(3)]
+            many = 300
+            wide = np.broadcast_to(x[:, None], (3, many // 3, vocab)).reshape(many, vocab)
+            tokens, probs = D.ints([0] * many), D.floats([0] * many)
+            of = {"k": ("top_k", D.ints), "p": ("top_p", D.floats), "m": ("min_p", D.floats)}
+            ds3.sample(ds3.Buffer.from_array(np.ascontiguousarray(wide)), D.floats(np.repeat(u, many // 3)), tokens, many,
+                       vocab, probs=probs, **{of[key][0]: of[key][1](np.full(many, value)) for key, value in s.items()})
+            got, share = tokens.read(np.int32, many).reshape(3, -1), probs.read(np.float32, many).reshape(3, -1)
+            for i in range(3):
+                assert (got[i] == one[i][0][0]).all() and (share[i] == one[i][1][0]).all()
+
+
+def test_graph_of_draws(hip_ready):
+    """One row and many, replayed with new numbers: the eager call's tokens."""
+    rng = np.random.default_rng(8)
+    for rows, vocab in ((1, 151936), (70, 20000)):
+        logit, u = ds3.Buffer.from_array(logits(rng, rows, vocab)), D.floats([0] * rows)
+        tokens, k, p = D.ints([0] * rows), D.ints([50] * rows), D.floats([0.9] * rows)
+
+        def call():
+            ds3.sample(logit, u, tokens, rows, vocab, top_k=k, top_p=p)
+        call()
+        with ds3.Graph() as graph:
+            call()
+        for _ in range(4):
+            u.write(rng.random(rows).astype(np.float32))
+            logit.write(logits(rng, rows, vocab))
+            graph.launch()
+            got = tokens.read(np.int32, rows)
+            tokens.write(np.full(rows, -9, np.int32))
+            call()
+            assert np.array_equal(tokens.read(np.int32, rows), got)
+        graph.close()                                 # (while nothing is captured)

@@ -512,8 +512,9 @@ int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t *kv_lens, 
  * n_head_kv).  A token that sees nothing gets zeros: one at a position below 0, or
  * whose blocks all lie outside the cache.  A value of the cache that is infinite or
  * NaN makes what it enters infinite or NaN (F32: NaN for an infinite v too) in the rows
- * that see it, and in no others.  Rows of out that belong to no request are left as they
- * were, as are those of a request whose rows do not lie within n_tokens.  q and out are of `type`, rows of n_head heads.
+ * that see it, and in no others.  Rows of out that belong to no request are left as
+ * they were, as are those of a request whose rows do not lie within n_tokens.  q and
+ * out are of `type`, rows of n_head heads.
  *   F32: products to 22 bits of q and of the softmax's weights (two F16 parts each),
  *        against the cache's exact F16 values
  *   F16: q as it is, the softmax's weights rounded to F16
@@ -538,9 +539,10 @@ int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint
  * temperature 0 or less, or a logit of +inf: the first token, share 1.  A row of nothing but
  * -inf and NaN: token -1, share 0.  The settings are one F32 (top_k: int32) a row;
  * NULL: temperature 1, all tokens.
- * Weights are summed in 64 bits (where only their bins decide, as whole numbers of
- * 2^-44 of the first's), in an order that the sizes fix: the same call gives the
- * same token.  n_vocab is at most 2^18.  It uses the library's workspace: before a
+ * Weights are summed in 64 bits, where only sums of many small ones matter each to
+ * 2^-28 of itself, in an order that the sizes fix: the same call gives the same token.
+ * (One with another number of rows does but where a sum meets u, top_p or min_p to
+ * within 2^-28.)  n_vocab is at most 2^18.  It uses the library's workspace: before a
  * capture the call is made once. */
 int ds3_hip_sample(const ds3_hip_buffer_t *logits, uint64_t row_stride, const ds3_hip_buffer_t *uniform,
                    const ds3_hip_buffer_t *temperature, const ds3_hip_buffer_t *top_k, const ds3_hip_buffer_t *top_p,

@@ -5,8 +5,9 @@
  * Include this instead of ds3_metal.h: every ds3_metal_* name the MoE path
  * uses maps onto its ds3_hip_* counterpart, ds3_metal_buffer_t onto
  * ds3_hip_buffer_t.  ds3_type_t values pass unchanged (same GGUF ids).
- * Entry points outside the MoE path (attention, RoPE, RMSNorm, dense F32
- * matmul) are not provided by this backend.
+ * Entry points outside the MoE path (attention, RoPE, dense F32 matmul) have no
+ * counterparts of the same names; ds3_hip.h has operators of its own for attention
+ * and rotary positions.
  */
 #ifndef DS3_METAL_COMPAT_H
 #define DS3_METAL_COMPAT_H

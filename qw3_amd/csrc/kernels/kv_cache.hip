@@ -11,13 +11,14 @@ namespace ds3k {
 // Rotary positions.  Pair j of a head turns by position * theta_j; the table holds
 // theta_j / (2 pi), so the product's whole part is dropped in 64 bits (32 lose the
 // angle of far positions) and sine and cosine are taken of the remaining half turn
-// in 32.  They depend on the token and the pair alone: a group of lanes holds V
-// pairs a lane of one token and walks over some of its heads, those of a token's groups
-// side by side.
+// in 32.  They depend on the token and the pair alone: a workgroup computes those of its
+// tokens into LDS, then a group of lanes holds V pairs a lane of one token and walks over
+// some of its heads, those of a token's groups side by side.
 // Bound by memory: 4096 tokens of 32 + 4 + 4 heads of 128 from F32 to F16 with norms
-// 22 us for 126 MB, 5.6 TB/s (part of it from the last-level cache); 4001 tokens of 64
-// heads, F16 to F16, 33 us for 131 MB, 4.0 TB/s, where a copy moves 4.6.  With runs of heads
-// a group 23 and 36; with four heads a group 25 and 33, with eight 22 and 34; the next
+// 22 us for 126 MB, 5.7 TB/s (part of it from the last-level cache); 4001 tokens of 64
+// heads, F16 to F16, 31 us for 131 MB, 4.2 TB/s, where a copy moves 4.6.  With angles in
+// every group by itself 22 and 33 (the vector units are busy 78 % of the second), runs of
+// heads a group besides 23 and 36; two heads a group 27 and 32, eight 22 and 31; the next
 // head's loads ahead of this one's work 23 and 35; loads that pass the caches by 26 and
 // 42.  One token: 3.6 us, the launch.
 // ---------------------------------------------------------------------------
@@ -91,29 +92,38 @@ template <typename TI, typename TO, int V, bool INTER>
 __global__ void __launch_bounds__(ROPE_TPB) k_rope(RopeArgs p)
 {
     constexpr int NU = 4 / V;
-    const int lane = threadIdx.x & (p.lanes - 1);
-    const int64_t group = ((int64_t)blockIdx.x * ROPE_TPB + threadIdx.x) / p.lanes;
-    const int64_t t = group / p.chunks;
-    if (t >= p.n_tokens) return;
-    const int heads = p.n_head + 2 * p.n_head_kv;
-    const int h0 = (int)(group - t * p.chunks);
-    const int half = p.rotary / 2, units = p.head_dim / (2 * V), turning = half / V;
+    __shared__ float2 angle[4 * ROPE_TPB];            // cosine and sine: (ROPE_TPB / lanes) tokens of half <= 4 lanes pairs
+    const int lane = threadIdx.x & (p.lanes - 1), half = p.rotary / 2;
+    const int groups = ROPE_TPB / p.lanes, tokens = max(groups >> p.log_chunks, 1);
+    const int64_t group = (int64_t)blockIdx.x * groups + threadIdx.x / p.lanes;
+    const int64_t t = group >> p.log_chunks, t0 = (int64_t)blockIdx.x * groups >> p.log_chunks;
+    if (half > 0) {
+        const float m = (float)p.table[half];
+        for (int i = threadIdx.x; i < tokens * half; i += ROPE_TPB) {
+            const int of = tokens == 1 ? 0 : i / half;
+            if (t0 + of >= p.n_tokens) break;
+            const double turn = (double)p.positions[t0 + of] * p.table[i - of * half];
+            float s, c;
+            sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
+            angle[i] = make_float2(m * c, m * s);
+        }
+        __syncthreads();
+    }
+    const int heads = p.n_head + 2 * p.n_head_kv, chunks = 1 << p.log_chunks;
+    const int h0 = (int)(group & (chunks - 1));
+    if (t >= p.n_tokens || h0 >= heads) return;
+    const int units = p.head_dim / (2 * V), turning = half / V;
 
     float c[NU][V], s[NU][V];
-    if (turning > 0 && h0 < p.n_head + p.n_head_kv) {
-        const double pos = (double)p.positions[t];
-        const float m = (float)p.table[half];
 #pragma unroll
-        for (int u = 0; u < NU; u++) {
-            const int unit = lane + u * p.lanes;
-            if (unit < turning) {
+    for (int u = 0; u < NU; u++) {
+        const int unit = lane + u * p.lanes;
+        if (unit < turning) {
 #pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const double turn = pos * p.table[unit * V + i];
-                    sincospif(2.0f * (float)(turn - rint(turn)), &s[u][i], &c[u][i]);
-                    s[u][i] *= m;
-                    c[u][i] *= m;
-                }
+            for (int i = 0; i < V; i++) {
+                const float2 cs = angle[(int)(t - t0) * half + unit * V + i];
+                c[u][i] = cs.x;
+                s[u][i] = cs.y;
             }
         }
     }
@@ -125,7 +135,7 @@ __global__ void __launch_bounds__(ROPE_TPB) k_rope(RopeArgs p)
            : (((slot >> p.log_block) * p.n_head_kv << p.log_block) + (slot & ((1 << p.log_block) - 1))) * p.head_dim;
     }
 
-    for (int h = h0; h < heads; h += p.chunks) {
+    for (int h = h0; h < heads; h += chunks) {
         const int kind = h < p.n_head ? 0 : h < p.n_head + p.n_head_kv ? 1 : 2;
         const int g = h - (kind == 0 ? 0 : kind == 1 ? p.n_head : p.n_head + p.n_head_kv);
         if (kind != 0 && at < 0) continue;
@@ -207,11 +217,12 @@ hipError_t launch_rope(RopeArgs p, int in_type, int out_type, bool inter, hipStr
     p.lanes = 1;
     while (p.lanes < std::min(units, WAVE)) p.lanes *= 2;
     const int heads = p.n_head + 2 * p.n_head_kv;
-    // one head a group of lanes until the card is full, then up to five: angles cost more than a head does
+    // one head a group of lanes until the card is full, then up to five
     const int64_t groups = p.n_tokens * heads, full = (int64_t)device_cu_count() * 8 * (ROPE_TPB / p.lanes);
     const int per = (int)std::clamp<int64_t>(groups / full, 1, 5);
-    p.chunks = (heads + per - 1) / per;
-    const int64_t n = p.n_tokens * p.chunks * p.lanes;
+    p.log_chunks = 0;
+    while ((1 << p.log_chunks) * per < heads) p.log_chunks++;
+    const int64_t n = (p.n_tokens << p.log_chunks) * p.lanes;
     const int64_t wgs = (n + ROPE_TPB - 1) / ROPE_TPB;
     if (wgs > 0xffffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)wgs);

@@ -316,7 +316,7 @@ struct RopeArgs {
     void *k_cache, *v_cache;     // F16 [blocks][n_head_kv][block][head_dim]
     int64_t n_slots, n_tokens;
     int log_block, n_head, n_head_kv, head_dim, rotary;
-    int lanes, chunks;           // lanes a head; groups of them a token
+    int lanes, log_chunks;       // lanes a head; groups of them a token (a power of two)
 };
 hipError_t launch_rope(RopeArgs p, int in_type, int out_type, bool inter, hipStream_t s);
 

@@ -147,3 +147,33 @@ def test_no_tokens(hip_ready):
     table, b = ds3.rope_table(8, 1e4), ds3.Buffer.alloc(64)
     ds3.rope(b, D.ints([0]), table, ds3.Buffer.alloc(64), 0, 1, 8)
     ds3.rope_append(None, b, b, None, D.ints([0]), ds3.KvCache.alloc(1, 1, 1, 8), None, 0, 0)
+
+
+@pytest.mark.parametrize("tokens,heads,dim,rotary", [(301, 1, 8, 8), (301, 1, 8, 6), (1025, 2, 16, 2), (77, 1, 512, 510),
+                                                     (77, 3, 512, 508), (40, 20, 264, 264), (600, 1, 40, 20), (3, 130, 64, 60)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_rope_of_tokens_that_share_a_workgroup(hip_ready, tokens, heads, dim, rotary, inter):
+    """Many tokens of few lanes, few of many, more groups of lanes than a workgroup's a token."""
+    rng = np.random.default_rng(tokens + dim + rotary)
+    x = rng.standard_normal((tokens, heads, dim)).astype(np.float32)
+    pos = rng.integers(0, 1 << 17, tokens).astype(np.int32)
+    theta, m = D.frequencies(rotary, *TABLES["linear"])
+    out = ds3.Buffer.alloc(x.nbytes)
+    ds3.rope(ds3.Buffer.from_array(x), D.ints(pos), ds3.rope_table(rotary, *TABLES["linear"]), out, tokens, heads, dim, rotary,
+             interleaved=inter)
+    want, tol = D.rope(x, pos, theta, m, interleaved=inter)
+    check(out.read(np.float32, x.shape), want, tol, F32)
+
+
+def test_append_in_place(hip_ready):
+    """q_out may be q itself."""
+    rng = np.random.default_rng(10)
+    for tokens in (1, 70):
+        q, k = rng.standard_normal((tokens, 6, 64)).astype(np.float32), rng.standard_normal((tokens, 2, 64)).astype(np.float32)
+        cache, table = ds3.KvCache.alloc(20, 4, 2, 64), ds3.rope_table(48, 1e4)
+        pos, slots, kb = D.ints(rng.integers(0, 9999, tokens)), D.ints(rng.permutation(80)[:tokens]), ds3.Buffer.from_array(k)
+        same, out = ds3.Buffer.from_array(q), ds3.Buffer.alloc(q.nbytes)
+        for b in (out, same):
+            ds3.rope_append(ds3.Buffer.from_array(q) if b is out else b, kb, kb, pos, slots, cache, b, tokens, 6, table=table,
+                            rotary_dim=48, q_norm=D.floats(np.linspace(0.5, 1.5, 64)))
+        assert np.array_equal(same.read(np.float32, q.shape), out.read(np.float32, q.shape))

@@ -518,7 +518,9 @@ int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t *kv_lens, 
  *   F32: products to 22 bits of q and of the softmax's weights (two F16 parts each),
  *        against the cache's exact F16 values
  *   F16: q as it is, the softmax's weights rounded to F16
- * Sums and the softmax are F32.  head_dim is a multiple of 8 up to 256.
+ * Sums and the softmax are F32.  head_dim is a multiple of 8 up to 256, max_blocks *
+ * block_size at most 2^31 - 2^16.  Requests' rows do not overlap (of those that do it is
+ * not defined which are written).
  * It uses the library's workspace: before a capture the call is made once. */
 int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint64_t q_row_stride,
                             const ds3_hip_buffer_t *k_cache, const ds3_hip_buffer_t *v_cache,

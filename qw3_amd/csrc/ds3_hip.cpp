@@ -2791,7 +2791,7 @@ extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t
     int log_block = 0;
     if (!float_type_ok(what, type) || !head_counts_ok(what, n_head, n_head_kv, head_dim, 256) ||
         !pages_ok(what, n_blocks, block_size, &log_block) || !size_in(what, "n_seq", n_seq, 1, 1u << 20) ||
-        !size_in(what, "max_blocks", max_blocks, 1, 0x7fffffffu >> log_block) ||
+        !size_in(what, "max_blocks", max_blocks, 1, 0x7fff0000u >> log_block) ||       // (keys are looked up ahead)
         !size_in(what, "n_tokens", n_tokens, 0, 1u << 20) || !size_in(what, "window", window, 0, 0x7fffffffu))
         return -1;
     if (!std::isfinite(scale)) {

@@ -117,3 +117,11 @@ def test_table_during_a_capture(lib, capfd):                                    
         assert "rope_table is not allowed during graph capture" in capfd.readouterr().err
     finally:
         lib.ds3_hip_debug_simulate_capture(0)
+
+
+def test_positions_near_the_end_of_int32(lib, capfd):                            # noqa: F811
+    """Attention reads up to a few hundred keys ahead: its positions end 2^16 before 2^31."""
+    huge = buf(1 << 40, 1 << 44)
+    for block, most in ((1, 0x7fff0000), (16, 0x7fff000), (1 << 16, 0x7fff)):
+        args = changed(ATTN, a4=huge, a15=1, a16=block)
+        refused(lib, capfd, "attention_paged", changed(args, a17=most + 1), "max_blocks")

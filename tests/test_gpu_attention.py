@@ -251,3 +251,26 @@ def test_requests_that_pass_the_rows(hip_ready):
                             D.ints([30, 40, 9, 12]), out, 12, 4, 4, pages.max_blocks, 64 ** -0.5, type_)
         got = out.read(D.NP[type_], q.shape)
         assert np.array_equal(got[:3], want) and np.all(got[3:] == 7)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("heads,kv,dim,new,lens,window", [
+    (4, 2, 64, [100], [130], 40), (8, 1, 128, [90], [1500], 700), (4, 1, 256, [70], [300], 33),       # tiles of many rows
+    (4, 2, 64, [7], [60], 5), (16, 1, 128, [2], [1300], 600), (6, 2, 80, [9, 20], [40, 900], 16)])    # of few
+def test_window_over_values_that_are_not_finite(hip_ready, type_, heads, kv, dim, new, lens, window):
+    """Rows whose window does not reach a NaN key and an infinite value are what they are without them."""
+    rng = np.random.default_rng(dim + window)
+    pages = D.Pages(rng, lens, 8, kv, dim)
+    q = rng.standard_normal((sum(new), heads, dim)).astype(D.NP[type_])
+    want, tol = D.attention(q, pages, new, lens, dim ** -0.5, window, type_)
+    tol = D.rounded_to(tol, want, type_)
+    at = [n - m + m // 2 - window // 2 for m, n in zip(new, lens)]               # half of the rows see it
+    for i, p in enumerate(at):
+        pages.k[pages.table[i, p // 8], :, p % 8, 1] = np.nan
+        pages.v[pages.table[i, p // 8], :, p % 8] = np.inf
+    got = run(q, pages, new, lens, type_, window)
+    pos = np.concatenate([np.arange(n - m, n) for m, n in zip(new, lens)])
+    bad = np.repeat(at, new)
+    sees = (bad <= pos) & (bad > pos - window)
+    assert sees.any() and not np.isfinite(got[sees]).any()
+    assert (np.abs(got[~sees].astype(np.float64) - want[~sees]) <= tol[~sees]).all()

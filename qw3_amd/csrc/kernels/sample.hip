@@ -26,11 +26,12 @@
 // and finished by one (k_sample_join).  What bounds it: the passes over a row by one
 // compute unit (a pass of 256 rows of 151,936 takes 30 us, 5.2 TB/s) and the chains of
 // sorting, summing and looking up behind them (10 us), which no other row hides as a call
-// waits for its slowest.  256 rows of 151,936 by setting: temperature 0 33 us, top-k 20
-// with top-p 42, top-k 200 52, min-p 63, temperature 0.3 alone 63, 1 alone 95 (every
-// logit's weight goes into a bin: LDS atomics), top-p 0.9 at temperature 1 131 (the
-// border lies below the collected: a second and third pass), top-k 2000 132; settings
-// drawn from all of these 131.  One row: 10 us, 19, 26, 33, 32, 32, 69, 88.
+// waits for its slowest.  256 rows of 151,936 by setting: temperature 0 32 us, top-k 20
+// with top-p 42, top-k 200 52, min-p 63, temperature 0.3 alone 63, 1 alone 89 (every
+// logit's weight goes into a bin: some 25 vector instructions a logit, LDS atomics), top-p
+// 0.9 at temperature 1 121 (the border lies below the collected: a second pass for each
+// border), top-k 2000 132; settings drawn from all of these 125.  One row: 10 us, 15, 26,
+// 32, 32, 32, 60, 87.
 #include "common.h"
 #include "lanes.h"
 
@@ -626,8 +627,10 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
         __syncthreads();
         if (tid == 0) sh.n = 0;
         __syncthreads();
+        // (by values first: with keys for every logit a pass took 22 us of one row in place of 17)
+        const float high = key_value(lo), low = key_value(hi);
         row.each<8>(0, row.groups, [&](float v, int i) {
-            if (!counts(v)) return;
+            if (!(v >= low && v <= high)) return;
             const uint32_t key = order_key(v);
             if (key < lo || key > hi || (uint32_t)i < i0 || (uint32_t)i >= i1) return;
             const uint32_t at = atomicAdd(&sh.n, 1u);

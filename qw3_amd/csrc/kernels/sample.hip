@@ -26,12 +26,12 @@
 // and finished by one (k_sample_join).  What bounds it: the passes over a row by one
 // compute unit (a pass of 256 rows of 151,936 takes 30 us, 5.2 TB/s) and the chains of
 // sorting, summing and looking up behind them (10 us), which no other row hides as a call
-// waits for its slowest.  256 rows of 151,936 by setting: temperature 0 32 us, top-k 20
-// with top-p 42, top-k 200 52, min-p 63, temperature 0.3 alone 63, 1 alone 89 (every
+// waits for its slowest.  256 rows of 151,936 by setting: temperature 0 33 us, top-k 20
+// with top-p 42, top-k 200 50, min-p 61, temperature 0.3 alone 62, 1 alone 87 (every
 // logit's weight goes into a bin: some 25 vector instructions a logit, LDS atomics), top-p
-// 0.9 at temperature 1 121 (the border lies below the collected: a second pass for each
-// border), top-k 2000 132; settings drawn from all of these 125.  One row: 10 us, 15, 26,
-// 32, 32, 32, 60, 87.
+// 0.9 at temperature 1 115 (the border lies below the collected: a second pass for each
+// border), top-k 2000 110 (a pass that counts, one that gathers, the sort).  One row: 10
+// us, 15, 24, 32, 31, 31, 58, 66.
 #include "common.h"
 #include "lanes.h"
 
@@ -370,6 +370,15 @@ __device__ __forceinline__ u64 collect(SampleShared &sh, const Row &row, int q0,
     return best;
 }
 
+// *least gets the smallest place that holds: a wave's places rise from lane to lane, so its first lane's will do (where
+// thousands hold, an atomic of each took 6 us).
+template <typename U>
+__device__ __forceinline__ void first_place(U *least, bool holds, int place)
+{
+    const uint64_t those = __ballot(holds);
+    if (holds && (those & ((1ull << (threadIdx.x & 63)) - 1)) == 0) atomicMin(least, (U)place);
+}
+
 // list[0 .. size) in order, E tokens a thread (places tid, tid + SMP_TPB, ...): steps of up to 32 within the wave, of up to
 // 512 through the list, larger ones within the thread.
 template <int E>
@@ -431,12 +440,13 @@ __device__ __forceinline__ void sort_list(u64 *list, int n)
 {
     int size = 64;
     while (size < n) size *= 2;
-    if (size > SMP_TPB) size = MOST;
+    if (size > SMP_TPB) size = size <= SMP_HALF ? SMP_HALF : MOST;
     __syncthreads();
     for (int i = n + threadIdx.x; i < size; i += SMP_TPB) list[i] = ~0ull;
     __syncthreads();
     if (size <= SMP_TPB) sort_places<1>(list, size);
-    else sort_places<MOST / SMP_TPB>(list, size);
+    else if (MOST == SMP_HALF || size <= SMP_HALF) sort_places<SMP_HALF / SMP_TPB>(list, SMP_HALF);
+    else sort_places<MOST / SMP_TPB>(list, MOST);
     __syncthreads();
 }
 
@@ -535,8 +545,8 @@ __device__ __forceinline__ bool finish(SampleShared &sh, const SampleArgs &a, in
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
             const int i = b * SMP_TPB + tid;
-            if (i < n && upto[b] >= least) atomicMin(&sh.bin, i + 1);
-            if (i > 0 && i < n && own[b] < (double)d.m) atomicMin(&sh.bin, i);
+            first_place(&sh.bin, i < n && upto[b] >= least, i + 1);
+            first_place(&sh.bin, i > 0 && i < n && own[b] < (double)d.m, i);
         }
         __syncthreads();
         if (sh.bin == NONE && !complete) return false;
@@ -551,7 +561,7 @@ __device__ __forceinline__ bool finish(SampleShared &sh, const SampleArgs &a, in
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) {
         const int i = b * SMP_TPB + tid;
-        if (i < kept && upto[b] > target) atomicMin(&sh.n, (uint32_t)i);
+        first_place(&sh.n, i < kept && upto[b] > target, i);
     }
     __syncthreads();
     if (sh.n == NONE && open) return false;
@@ -604,7 +614,7 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
     __syncthreads();
     const double upto_first = b.upto - b.w[1];
     const int mine = upto_first >= least && b.w[0] > 0.0 ? 2 * tid : b.upto >= least && b.w[1] > 0.0 ? 2 * tid + 1 : 0x7fffffff;
-    if (mine != 0x7fffffff) atomicMin(&sh.bin, mine);
+    first_place(&sh.bin, mine != 0x7fffffff, mine);
     __syncthreads();
     if (sh.bin == 0x7fffffff) {              // rounding: the last bin with a weight
         __syncthreads();
@@ -660,7 +670,7 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
         __syncthreads();
         const auto reaches = [&](u64 units) { return before + (double)units / SMP_ONE >= least; };
         const int at = x > 0 && reaches(w - y) ? 2 * tid : y > 0 && reaches(w) ? 2 * tid + 1 : 0x7fffffff;
-        if (at != 0x7fffffff) atomicMin(&sh.bin, at);
+        first_place(&sh.bin, at != 0x7fffffff, at);
         __syncthreads();
         if (sh.bin == 0x7fffffff) {
             __syncthreads();
@@ -693,7 +703,7 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
         const double all = scan_f64(sh, w);
         upto[j] = before + w;
         before += all;
-        if (i < n && upto[j] >= least) atomicMin(&sh.n, (uint32_t)i);
+        first_place(&sh.n, i < n && upto[j] >= least, i);
     }
     __syncthreads();
     const int at = (int)sh.n;
@@ -737,7 +747,7 @@ __device__ __forceinline__ void draw_below(SampleShared &sh, const SampleArgs &a
             own[j] = i < n ? row.weight(token_value(sh.list[i])) : 0.0;
             double x = own[j];
             const double all = scan_f64(sh, x);
-            if (i < n && before + x > target) atomicMin(&sh.n, (uint32_t)i);
+            first_place(&sh.n, i < n && before + x > target, i);
             before += all;
         }
         __syncthreads();
@@ -920,7 +930,7 @@ __device__ __forceinline__ bool draw_large_k(SampleShared &sh, const SampleArgs 
     __syncthreads();
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
-    row.each<8>(0, row.groups, [&](float v, int i) {
+    row.each<2>(0, row.groups, [&](float v, int i) {
         if (bin(v) < last) push(sh, token_of(v, i));
     });
     __syncthreads();

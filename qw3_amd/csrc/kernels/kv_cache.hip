@@ -2,6 +2,7 @@
 // with the heads' norms, the writing of new tokens' k and v, and the plan of a
 // step's blocks, positions and slots from the requests' lengths.
 #include "common.h"
+#include "lanes.h"
 
 #include <algorithm>
 
@@ -239,9 +240,9 @@ hipError_t launch_rope(RopeArgs p, int in_type, int out_type, bool inter, hipStr
 // (two prefix sums) and decides; then every token finds its request by bisection of
 // the offsets.  A new block's first position is a new token's, so that token enters
 // the block in the table and nothing is written twice.
-// Bound by latency: lengths, sums and the decision are a chain of 5 us at any size; up to
-// 2048 rows the same workgroup writes them (8 requests: 5 us in all), more are a second
-// launch of 5 us (1000 requests, 25,000 rows).
+// Bound by latency: lengths, sums and the decision are a chain of 4 us at any size (5 with
+// sums by LDS exchanges); up to 2048 rows the same workgroup writes them (8 requests: 4 us
+// in all), more are a second launch of 4 us (1000 requests, 25,000 rows).
 // ---------------------------------------------------------------------------
 
 constexpr int PLAN_TPB = 1024;
@@ -254,13 +255,8 @@ struct PlanSums {
 __device__ __forceinline__ PlanSums plan_scan(PlanSums v, PlanSums *waves, PlanSums &total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int d = 1; d < 64; d *= 2) {
-        const long long a = __shfl_up(v.tokens, d), b = __shfl_up(v.blocks, d);
-        if (lane >= d) {
-            v.tokens += a;
-            v.blocks += b;
-        }
-    }
+    v.tokens = wave_scan(v.tokens);
+    v.blocks = wave_scan(v.blocks);
     __syncthreads();
     if (lane == 63) waves[wave] = v;
     __syncthreads();
@@ -279,21 +275,21 @@ __device__ __forceinline__ PlanSums plan_scan(PlanSums v, PlanSums *waves, PlanS
 
 __device__ __forceinline__ int sat32(long long v) { return (int)min(v, 0x7fffffffll); }
 
-// Rows [row0, row1) in steps of `step`: position, slot, and the table's new entries.
-__device__ __forceinline__ void plan_rows(const PlanArgs &p, int64_t row0, int64_t row1, int step)
+// Rows [row0, row1) in steps of `step`, `total` of which belong to requests: position, slot, and the table's new entries.
+template <typename O>
+__device__ __forceinline__ void plan_rows(const PlanArgs &p, O offsets, int total, int n_free, int64_t row0, int64_t row1, int step)
 {
-    const int total = p.offsets[p.n_seq], n_free = p.head[0];
     for (int64_t t = row0; t < row1; t += step) {
         int position = 0, slot = -1;
         if (t < total) {
-            int lo = 0, hi = p.n_seq;                 // offsets[lo] <= t < offsets[hi]
+            int lo = 0, hi = p.n_seq;                 // offsets(lo) <= t < offsets(hi)
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (p.offsets[mid] <= t) lo = mid;
+                if (offsets(mid) <= t) lo = mid;
                 else hi = mid;
             }
             const int cached = p.cached[lo];
-            position = cached + (int)(t - p.offsets[lo]);
+            position = cached + (int)(t - offsets(lo));
             const int had = (int)(((int64_t)cached + (1 << p.log_block) - 1) >> p.log_block), at = position >> p.log_block;
             int32_t *entry = p.table + (int64_t)lo * p.max_blocks + at;
             int block;
@@ -307,6 +303,8 @@ __device__ __forceinline__ void plan_rows(const PlanArgs &p, int64_t row0, int64
         p.slots[t] = slot;
     }
 }
+
+constexpr int PLAN_HELD = 4096;              // requests whose offsets are bisected in LDS
 
 template <bool ROWS>
 __global__ void __launch_bounds__(PLAN_TPB) k_kv_plan(PlanArgs p)
@@ -356,14 +354,21 @@ __global__ void __launch_bounds__(PLAN_TPB) k_kv_plan(PlanArgs p)
     }
     if constexpr (ROWS) {
         __syncthreads();
-        plan_rows(p, threadIdx.x, p.max_tokens, PLAN_TPB);
+        const int total = done ? (int)sum.tokens : 0;
+        plan_rows(p, [&](int i) { return p.offsets[i]; }, total, n_free, threadIdx.x, p.max_tokens, PLAN_TPB);
     }
 }
 
 __global__ void __launch_bounds__(256) k_kv_plan_rows(PlanArgs p)
 {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    plan_rows(p, t, min((int64_t)p.max_tokens, t + 1), 1);
+    __shared__ int held[PLAN_HELD];
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, end = min((int64_t)p.max_tokens, t + 1);
+    const int total = p.offsets[p.n_seq], n_free = p.head[0];
+    if (p.n_seq <= PLAN_HELD) {              // (in memory each step of the bisection is a round trip: 5.6 us in place of 4.7 for 1000)
+        for (int i = threadIdx.x; i < p.n_seq; i += 256) held[i] = p.offsets[i];
+        __syncthreads();
+        plan_rows(p, [&](int i) { return held[i]; }, total, n_free, t, end, 1);
+    } else plan_rows(p, [&](int i) { return p.offsets[i]; }, total, n_free, t, end, 1);
 }
 
 hipError_t launch_kv_plan(const PlanArgs &p, hipStream_t s)

@@ -465,10 +465,11 @@ int ds3_hip_rope(const ds3_hip_buffer_t *x, ds3_hip_type_t x_type, uint64_t x_ro
  * normalised (q_norm, k_norm, optional) and rotated as in ds3_hip_rope, and the
  * cache's v rows = v, k and v at slots[t] (int32; a slot outside the cache: the
  * row is not written).  q, k, v are rows of `type`, their strides in bytes (of one
- * packed buffer: views); q_out is dense, or q itself (of one type and dense).  table may be NULL: no rotation,
- * positions (then unused) may be NULL too.  q and q_out may be NULL: k and v only.
- * The slots of a call differ; of rows with one slot it is not defined which is
- * kept.  Values beyond F16's range become infinite in the cache. */
+ * packed buffer: views); q_out is dense, or q itself where that is dense and of its
+ * type.  table may be NULL: no rotation, positions (then unused) may be NULL too.  q
+ * and q_out may be NULL: k and v only.  The slots of a call differ; of rows with one
+ * slot it is not defined which is kept.  Values beyond F16's range become infinite in
+ * the cache. */
 int ds3_hip_rope_append(const ds3_hip_buffer_t *q, const ds3_hip_buffer_t *k, const ds3_hip_buffer_t *v,
                         ds3_hip_type_t type, uint64_t q_row_stride, uint64_t k_row_stride, uint64_t v_row_stride,
                         const ds3_hip_buffer_t *positions, const ds3_hip_buffer_t *slots,

@@ -1105,11 +1105,13 @@ static hipError_t attention_dim(const AttnArgs &p, hipStream_t s)
     const bool only_few = p.n_tokens <= p.n_seq || rows <= FEW, only_many = !only_few && p.n_seq == 1;
     AttnArgs many = p, few = p;
     int many_wgs = 0, few_wgs = 0, many_join = 0, few_join = 0;
-    if (!only_few && !attention_split<T, DP, true>(many, only_many ? 0 : FEW + 1, 0x7fffffff, many_wgs, many_join)) return hipErrorInvalidValue;
-    if (!only_many && !attention_split<T, DP, false>(few, 0, only_few ? 0x7fffffff : FEW, few_wgs, few_join)) return hipErrorInvalidValue;
+    if ((!only_few && !attention_split<T, DP, true>(many, only_many ? 0 : FEW + 1, 0x7fffffff, many_wgs, many_join)) ||
+        (!only_many && !attention_split<T, DP, false>(few, 0, only_few ? 0x7fffffff : FEW, few_wgs, few_join)))
+        return hipErrorInvalidValue;
     if (many_wgs > 0) attention_tiles<T, DP>(many, many_wgs, s);
     if (few_wgs > 0) attention_few<T, DP>(few, few_wgs, s);
-    if (many_join > 0 && few_join > 0) hipLaunchKernelGGL((k_attn_join_both<T, DP, M>), dim3(many_join + few_join), ATT_TPB, 0, s, many, few, many_join);
+    if (many_join > 0 && few_join > 0)
+        hipLaunchKernelGGL((k_attn_join_both<T, DP, M>), dim3(many_join + few_join), ATT_TPB, 0, s, many, few, many_join);
     else if (many_join > 0) hipLaunchKernelGGL((k_attn_join<T, DP, M>), dim3(many_join), ATT_TPB, 0, s, many);
     else if (few_join > 0) hipLaunchKernelGGL((k_attn_join<T, DP, ROWS_M>), dim3(few_join), ATT_TPB, 0, s, few);
     return hipGetLastError();

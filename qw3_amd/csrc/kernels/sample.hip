@@ -476,7 +476,8 @@ __device__ __forceinline__ void finish_few(const u64 *list, const SampleArgs &a,
 
 // The draw from sh.list[0 .. n), n > 0: with top_k at least the k best tokens of the row, else its best n, the others'
 // weights summing to `rest` of the first's.  False: they do not decide.
-__device__ __forceinline__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, int &n, double rest, double &listed)
+__device__ __forceinline__ bool finish(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, int &n,
+                                       double rest, double &listed)
 {
     const int tid = threadIdx.x;
     if (d.k > 0 && n <= 64) {
@@ -495,7 +496,8 @@ __device__ __forceinline__ bool finish(SampleShared &sh, const SampleArgs &a, in
 #pragma unroll
             for (int i = 0; i < SMP_LIST / SMP_TPB; i++) {
                 const uint32_t key = (uint32_t)(held[i] >> 32);
-                if (held[i] != ~0ull && (step == 0 || key >> 21 == high)) atomicAdd(&sh.count[step == 0 ? key >> 21 : key >> 10 & 2047], 1u);
+                if (held[i] != ~0ull && (step == 0 || key >> 21 == high))
+                    atomicAdd(&sh.count[step == 0 ? key >> 21 : key >> 10 & 2047], 1u);
             }
             count_border(sh, (uint32_t)d.k - before);
             if (step == 0) {
@@ -720,7 +722,8 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
 }
 
 // The draw where the sorted list [0 .. n), n <= SMP_HALF, does not decide.
-__device__ __forceinline__ void draw_below(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, int n, const Below &b)
+__device__ __forceinline__ void draw_below(SampleShared &sh, const SampleArgs &a, int r, const Draw &d, const Row &row, int n,
+                                           const Below &b)
 {
     const int tid = threadIdx.x;
     double w = b.w[0] + b.w[1], mass = b.listed + scan_f64(sh, w), kept = mass;

@@ -1069,9 +1069,12 @@ __global__ void __launch_bounds__(SMP_TPB) k_sample_join(SampleArgs a)
         double rest = 0.0;
         if (d.k == 0) {
             u64 units[2] = { sh.weight[2 * tid], sh.weight[2 * tid + 1] };
-            // a part's bins begin at its own reference, so many below the largest logit's
+            // a part's bins begin at its own reference, so many below the largest logit's; a part without a bound has
+            // passed nothing, and its reference may be no logit of the row
             const float behind = Row::below(b.top, row.steps(own->ref));
-            if (lane == 0) sh.shown[wave] = own_best != ~0ull && behind < SMP_BINS ? (uint32_t)(int)behind : (uint32_t)SMP_BINS;
+            if (lane == 0)
+                sh.shown[wave] = passed != 0xffffffffu && behind >= 0.0f && behind < SMP_BINS ? (uint32_t)(int)behind
+                                                                                             : (uint32_t)SMP_BINS;
             __syncthreads();
 #pragma unroll 4
             for (int i = 0; i < a.parts; i++) {

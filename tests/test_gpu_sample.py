@@ -181,3 +181,21 @@ def test_graph_of_draws(hip_ready):
             call()
             assert np.array_equal(tokens.read(np.int32, rows), got)
         graph.close()                                 # (while nothing is captured)
+
+
+@pytest.mark.parametrize("rows,vocab", [(64, 151936), (40, 262144)])
+def test_parts_that_begin_with_masked_logits(hip_ready, rows, vocab):
+    """A part of a row of more than 32,768 logits, all of them masked but a few at its end, which are negative or lie
+    below those of parts that are not masked."""
+    rng = np.random.default_rng(rows)
+    parts = 256 // rows
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    ends = [vocab * (i + 1) // parts for i in range(parts)]
+    for r in range(rows):
+        for i, end in enumerate(ends):
+            at = rng.integers(end - 4900, end - 100, 30)
+            x[r, at] = [-30, -0.5, 4, -3][r % 4] + rng.standard_normal(len(at))
+            if r % 8 >= 4 and i == r % parts:             # one part in full
+                x[r, end - vocab // parts + 8:end - 8] = 2 * rng.standard_normal(vocab // parts - 16) - 20 * (r % 3)
+    for s in (dict(), dict(t=0.3), dict(t=1e-4), dict(p=0.9), dict(m=0.1, t=2.0)):
+        check(x, rng.random(rows).astype(np.float32), **{n: np.full(rows, v) for n, v in s.items()})

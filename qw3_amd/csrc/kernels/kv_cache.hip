@@ -312,6 +312,7 @@ __global__ void __launch_bounds__(PLAN_TPB) k_kv_plan(PlanArgs p)
     __shared__ PlanSums waves[PLAN_TPB / 64];
     __shared__ int too_long;
     if (threadIdx.x == 0) too_long = 0;
+    __syncthreads();                                  // (before any wave counts)
     const int n_free = min(max(*p.n_free, 0), p.n_blocks);
     PlanSums sum = { 0, 0 };
     for (int i0 = 0; i0 < p.n_seq; i0 += PLAN_TPB) {  // prefix sums, kept where they are looked up

@@ -120,3 +120,16 @@ def test_tables_that_name_no_block(hip_ready):
                 kv_lens_out=ds3.Buffer.alloc(8), n_free_out=ds3.Buffer.alloc(4))
     assert slots.read(np.int32, 8).tolist() == [-1, -1, -1, -1, -1, -1, -1, -1]
     assert pos.read(np.int32, 8).tolist() == [6, 7, 1, 2, 0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("n_seq", [64, 1024, 3000])
+def test_requests_too_long_in_every_wave(hip_ready, n_seq):
+    """One request longer than its table row, in any wave, refuses the plan; the count of such requests is exact."""
+    s = State(n_seq + 1, n_seq, 4, 8 * n_seq, 6)
+    assert s.step([1] * n_seq, n_seq)
+    for at in [*range(0, n_seq, 61), n_seq - 1]:
+        new = np.zeros(n_seq, int)
+        new[at] = 24                                  # 25 tokens of at most 24
+        assert not s.step(new, 4096)
+    assert not s.step([24] * n_seq, 24 * n_seq)
+    assert s.step([23] + [0] * (n_seq - 1), 4096)

@@ -402,6 +402,8 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
 
     const int all_from = (int)max(p.window ? base + j1 - p.window + 1 : 0, (int64_t)0);      // keys that every row sees:
     const int64_t all_to = base + j0;                                                        // from .. to
+    // Rows of one token all see the same keys: what lies before its window (the first key is a multiple of 32) is no key.
+    const int lone_from = j0 == j1 ? all_from : 0;
     float m = -INFINITY, l = 0.0f;
     f32x4 acc[NT];
 #pragma unroll
@@ -463,7 +465,7 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
             for (int e = 0; e < 8; e++) {
                 const int key = kb + 16 * (e / 4) + 4 * h + (e & 3);
                 if (!(seen[e] && key <= pos && key >= low)) s[e / 4][e & 3] = -INFINITY;
-                if (!seen[e]) {
+                if (!seen[e] || key < lone_from) {
 #pragma unroll
                     for (int x = 0; x < (NT + 7) / 8; x++) vf[e][x] = { 0, 0, 0, 0 };
                 }

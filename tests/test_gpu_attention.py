@@ -274,3 +274,24 @@ def test_window_over_values_that_are_not_finite(hip_ready, type_, heads, kv, dim
     sees = (bad <= pos) & (bad > pos - window)
     assert sees.any() and not np.isfinite(got[sees]).any()
     assert (np.abs(got[~sees].astype(np.float64) - want[~sees]) <= tol[~sees]).all()
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("heads,kv,dim,block", [(2, 2, 64, 16), (4, 1, 128, 16), (16, 1, 64, 2), (32, 2, 256, 1), (6, 1, 40, 8)])
+@pytest.mark.parametrize("new,lens,window", [([1], [1000], 100), ([1], [3000], 2050), ([1] * 3, [40, 70, 500], 33),
+                                             ([1] * 70, [90] * 70, 5), ([2], [75], 1), ([3], [400], 70)])
+def test_values_just_before_a_window(hip_ready, type_, heads, kv, dim, block, new, lens, window):
+    """NaN and infinities at the keys before each request's first one that is seen leave every row as it is."""
+    rng = np.random.default_rng(dim + window)
+    pages = D.Pages(rng, lens, block, kv, dim)
+    q = rng.standard_normal((sum(new), heads, dim)).astype(D.NP[type_])
+    want, tol = D.attention(q, pages, new, lens, dim ** -0.5, window, type_)
+    for i, (m, n) in enumerate(zip(new, lens)):
+        first = n - m - window + 1                    # of the first new token; later ones see less
+        for p in {first - 1, first & ~31, max(first - 17, 0)}:
+            if 0 <= p < first:
+                at = pages.table[i, p // block], slice(None), p % block
+                pages.k[at], pages.v[at] = np.nan, [np.inf, -np.inf, np.nan][i % 3]
+    got = run(q, pages, new, lens, type_, window)
+    assert np.isfinite(got).all()
+    assert (np.abs(got.astype(np.float64) - want) <= D.rounded_to(tol, want, type_)).all()

@@ -614,6 +614,16 @@ int ds3_hip_debug_product_plan(ds3_hip_type_t type, uint32_t M, uint32_t N, uint
  * Launches nothing and needs no device; -1 for sizes that no product takes. */
 int ds3_hip_debug_mx_plan(uint32_t n_rows, uint32_t n_group, uint32_t N, uint32_t K, bool gate_up, int64_t *plan);
 
+/* No ds3_metal.h counterpart (a test hook): how ds3_hip_attention_paged splits a
+ * call, from offsets and lengths in host memory.  split = of tiles of many rows
+ * (requests of more than 64), then of few: { keys a unit, tiles, units (a tile and
+ * a run of its keys), units launched, tiles whose units are joined, units that the
+ * workspace holds }, each of one kv head; zeros where none are launched.
+ * Launches nothing and needs no device; -1 for calls that are refused. */
+int ds3_hip_debug_attention_split(const int32_t *q_offsets, const int32_t *kv_lens, uint32_t n_tokens, uint32_t n_seq,
+                                  uint32_t n_head, uint32_t n_head_kv, uint32_t head_dim, uint32_t block_size,
+                                  uint32_t max_blocks, uint32_t window, int64_t *split);
+
 /* No ds3_metal.h counterpart: the row count of A from which
  * ds3_hip_matmul_quantized_batch takes its fp16 MFMA path (see there).  0
  * restores the default (64).  Returns the previous value. */

@@ -2778,6 +2778,29 @@ extern "C" int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t
     return finish(launch_kv_release(p, g.stream), what);
 }
 
+// The sizes of a call, put into p.
+static bool attention_sizes_ok(const char *what, uint32_t n_tokens, uint32_t n_seq, uint32_t n_head, uint32_t n_head_kv,
+                               uint32_t head_dim, uint32_t n_blocks, uint32_t block_size, uint32_t max_blocks,
+                               uint32_t window, AttnArgs &p)
+{
+    int log_block = 0;
+    if (!head_counts_ok(what, n_head, n_head_kv, head_dim, 256) || !pages_ok(what, n_blocks, block_size, &log_block) ||
+        !size_in(what, "n_seq", n_seq, 1, 1u << 20) ||
+        !size_in(what, "max_blocks", max_blocks, 1, 0x7fff0000u >> log_block) ||       // (keys are looked up ahead)
+        !size_in(what, "n_tokens", n_tokens, 0, 1u << 20) || !size_in(what, "window", window, 0, 0x7fffffffu))
+        return false;
+    p.n_tokens = (int)n_tokens;
+    p.n_seq = (int)n_seq;
+    p.n_head = (int)n_head;
+    p.n_head_kv = (int)n_head_kv;
+    p.head_dim = (int)head_dim;
+    p.n_blocks = (int)n_blocks;
+    p.log_block = log_block;
+    p.max_blocks = (int)max_blocks;
+    p.window = (int)window;
+    return true;
+}
+
 extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint64_t q_row_stride,
                                        const ds3_hip_buffer_t *k_cache, const ds3_hip_buffer_t *v_cache,
                                        const ds3_hip_buffer_t *block_table, const ds3_hip_buffer_t *q_offsets,
@@ -2788,11 +2811,9 @@ extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t
 {
     const char *what = "attention_paged";
     if (!q || !k_cache || !v_cache || !block_table || !q_offsets || !kv_lens || !out) return -1;
-    int log_block = 0;
-    if (!float_type_ok(what, type) || !head_counts_ok(what, n_head, n_head_kv, head_dim, 256) ||
-        !pages_ok(what, n_blocks, block_size, &log_block) || !size_in(what, "n_seq", n_seq, 1, 1u << 20) ||
-        !size_in(what, "max_blocks", max_blocks, 1, 0x7fff0000u >> log_block) ||       // (keys are looked up ahead)
-        !size_in(what, "n_tokens", n_tokens, 0, 1u << 20) || !size_in(what, "window", window, 0, 0x7fffffffu))
+    AttnArgs p{};
+    if (!float_type_ok(what, type) ||
+        !attention_sizes_ok(what, n_tokens, n_seq, n_head, n_head_kv, head_dim, n_blocks, block_size, max_blocks, window, p))
         return -1;
     if (!std::isfinite(scale)) {
         fprintf(stderr, "ds3_hip: %s: scale is not finite\n", what);
@@ -2814,7 +2835,6 @@ extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t
                  { block_table, t_b, "block_table" }, { q_offsets, s_b + 4, "q_offsets" }, { kv_lens, s_b, "kv_lens" } }) ||
         !ensure_init())
         return -1;
-    AttnArgs p{};
     p.q = dptr(q);
     p.out = dptr(out);
     p.q_stride = q_row_stride;
@@ -2824,20 +2844,30 @@ extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t
     p.table = (const int32_t *)dptr(block_table);
     p.offsets = (const int32_t *)dptr(q_offsets);
     p.lens = (const int32_t *)dptr(kv_lens);
-    p.n_tokens = (int)n_tokens;
-    p.n_seq = (int)n_seq;
-    p.n_head = (int)n_head;
-    p.n_head_kv = (int)n_head_kv;
-    p.head_dim = (int)head_dim;
-    p.n_blocks = (int)n_blocks;
-    p.log_block = log_block;
-    p.max_blocks = (int)max_blocks;
     p.scale = scale;
-    p.window = (int)window;
     p.partial = (float *)ws_get(attention_workspace(p));
     if (!p.partial) return -1;
     KScope ks("attention_paged");
     return finish(launch_attention(p, type, g.stream), what);
+}
+
+extern "C" int ds3_hip_debug_attention_split(const int32_t *q_offsets, const int32_t *kv_lens, uint32_t n_tokens,
+                                             uint32_t n_seq, uint32_t n_head, uint32_t n_head_kv, uint32_t head_dim,
+                                             uint32_t block_size, uint32_t max_blocks, uint32_t window, int64_t *split)
+{
+    AttnArgs p{};
+    AttnUnits of[2];
+    if (!q_offsets || !kv_lens || !split ||
+        !attention_sizes_ok("attention_split", n_tokens, n_seq, n_head, n_head_kv, head_dim, 1, block_size, max_blocks, window, p))
+        return -1;
+    p.offsets = q_offsets;
+    p.lens = kv_lens;
+    if (!attention_units(p, of)) return -1;
+    for (const AttnUnits &u : of) {
+        const int64_t v[6] = { u.run, u.tiles, u.units, u.grid, u.joined, u.partial };
+        split = std::copy(v, v + 6, split);
+    }
+    return 0;
 }
 
 extern "C" int ds3_hip_sample(const ds3_hip_buffer_t *logits, uint64_t row_stride, const ds3_hip_buffer_t *uniform,

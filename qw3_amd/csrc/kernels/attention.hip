@@ -45,6 +45,7 @@ struct Unit {
 
 constexpr int ATT_TPB = 256;
 constexpr int ATT_FEW_ROWS = 64;             // requests of up to so many rows take tiles of 16
+constexpr int ATT_WHOLE = 0x7fff0000;        // a run that holds any request's keys
 
 __device__ __forceinline__ long long wave_sum(long long v)
 {
@@ -52,7 +53,7 @@ __device__ __forceinline__ long long wave_sum(long long v)
 }
 
 // Request i's tiles of M rows and the most keys that one of them sees.
-__device__ __forceinline__ void request_work(const AttnArgs &p, int M, int i, int &tiles, int &span, Unit &u)
+__host__ __device__ __forceinline__ void request_work(const AttnArgs &p, int M, int i, int &tiles, int &span, Unit &u)
 {
     tiles = span = 0;
     if (i >= p.n_seq) return;
@@ -61,28 +62,30 @@ __device__ __forceinline__ void request_work(const AttnArgs &p, int M, int i, in
     u.first = o0;
     u.m = o1 - o0;
     u.kv = p.lens[i];
-    u.n = (int)min((int64_t)max(u.kv, 0), (int64_t)p.max_blocks << p.log_block);
+    u.n = (int)std::min((int64_t)std::max(u.kv, 0), (int64_t)p.max_blocks << p.log_block);
     const long long rows = (long long)u.m * group;
     if (rows < p.min_rows || rows > p.max_rows) return;
     tiles = (int)((rows + M - 1) / M);
-    span = p.window ? (int)min((long long)u.n, (long long)p.window + M / group + 130) : u.n;
-    span = max(span, 1);
+    span = p.window ? (int)std::min((long long)u.n, (long long)p.window + M / group + 130) : u.n;
+    span = std::max(span, 1);
 }
 
 // Keys a unit: work / (target - tiles) or a little more, so that splitting adds at most target - tiles units.
-__device__ __forceinline__ int whole_runs(const AttnArgs &p, int M, float want)
+__host__ __device__ __forceinline__ int whole_runs(const AttnArgs &p, int M, float want)
 {
     const int grain = M == 16 ? 128 : 64;             // keys that a workgroup takes at a time
-    return want >= 0x1p29f ? 1 << 30 : max(((int)want + grain) & -grain, p.least);
+    return want >= 0x1p30f ? ATT_WHOLE : std::max(((int)want + grain) & -grain, p.least);
 }
-__device__ __forceinline__ int unit_run(const AttnArgs &p, int M, long long work, long long tiles)
+// (span and run up to ATT_WHOLE: their sum passes 2^31)
+__host__ __device__ __forceinline__ int runs_of(int span, int run) { return (int)(((unsigned)span + (unsigned)run - 1) / (unsigned)run); }
+__host__ __device__ __forceinline__ int unit_run(const AttnArgs &p, int M, long long work, long long tiles)
 {
-    if (tiles >= p.target) return 1 << 30;
+    if (tiles >= p.target) return ATT_WHOLE;
     return whole_runs(p, M, (float)work / (float)(p.target - tiles) * (1.0f + 0x1p-20f));
 }
 // Runs that fill `target` units if no tile's last run were short: shorter ones, to be taken where the units that result
 // are no more than `target` (one chunk of 512 tokens: 16 tiles in four runs each rather than three, 45 us to 38).
-__device__ __forceinline__ int tight_run(const AttnArgs &p, int M, long long work)
+__host__ __device__ __forceinline__ int tight_run(const AttnArgs &p, int M, long long work)
 {
     return whole_runs(p, M, (float)work / (float)p.target * (1.0f + 0x1p-20f));
 }
@@ -103,8 +106,8 @@ __device__ __forceinline__ bool search_unit(const AttnArgs &p, int M, int id, Un
         u.seq = 0;
         u.run = unit_run(p, M, (long long)tiles * span, tiles);
         const int tight = tight_run(p, M, (long long)tiles * span);
-        if (tight < u.run && (long long)tiles * ((span + tight - 1) / tight) <= p.target) u.run = tight;
-        const int chunks = (span + u.run - 1) / u.run;
+        if (tight < u.run && (long long)tiles * (runs_of(span, tight)) <= p.target) u.run = tight;
+        const int chunks = runs_of(span, u.run);
         if ((long long)id >= (long long)tiles * (TILES ? 1 : chunks)) return false;
         u.tile = TILES ? id : id / chunks;
         u.whole = u.tile * chunks;
@@ -118,12 +121,12 @@ __device__ __forceinline__ bool search_unit(const AttnArgs &p, int M, int id, Un
         const long long work = wave_sum((long long)tiles * span);
         u.run = unit_run(p, M, work, wave_sum((long long)tiles));
         const int tight = tight_run(p, M, work);
-        if (tight < u.run && wave_sum((long long)tiles * ((span + tight - 1) / tight)) <= p.target) u.run = tight;
-        const long long units = (long long)tiles * ((span + u.run - 1) / u.run);
+        if (tight < u.run && wave_sum((long long)tiles * (runs_of(span, tight))) <= p.target) u.run = tight;
+        const long long units = (long long)tiles * runs_of(span, u.run);
         const long long at = wave_scan(units) - units, first = TILES ? wave_scan((long long)tiles) - tiles : at;
         const uint64_t here = __ballot(id >= first && id < first + (TILES ? tiles : units));
         if (here == 0) return false;
-        const int i = __builtin_ctzll(here), of = (int)(id - first), chunks = (span + u.run - 1) / u.run;
+        const int i = __builtin_ctzll(here), of = (int)(id - first), chunks = runs_of(span, u.run);
         u.seq = i;
         u.tile = TILES ? of : of / max(chunks, 1);
         u.chunk = TILES ? 0 : of - u.tile * chunks;
@@ -160,7 +163,7 @@ __device__ __forceinline__ bool search_unit(const AttnArgs &p, int M, int id, Un
         int tiles, span;
         Unit r;
         request_work(p, M, i0 + tid, tiles, span, r);
-        const long long units = (long long)tiles * ((span + u.run - 1) / u.run);
+        const long long units = (long long)tiles * runs_of(span, u.run);
         const long long sum = wave_scan(units), tile_sum = wave_scan((long long)tiles);
         if (lane == 63) {
             part[0][wave] = sum;
@@ -190,7 +193,7 @@ __device__ __forceinline__ bool search_unit(const AttnArgs &p, int M, int id, Un
     int tiles, span;
     u.seq = found[0];
     request_work(p, M, u.seq, tiles, span, u);
-    const int chunks = (span + u.run - 1) / u.run;
+    const int chunks = runs_of(span, u.run);
     u.tile = TILES ? found[1] : found[1] / chunks;
     u.chunk = TILES ? 0 : found[1] - u.tile * chunks;
     u.whole = found[2] + u.tile * chunks;
@@ -227,7 +230,7 @@ __device__ __forceinline__ Tile tile_of(const AttnArgs &p, int M, const Unit &u)
     t.base = (int64_t)u.kv - u.m;
     t.end = (int)max(min(t.base + t.j1 + 1, (int64_t)u.n), (int64_t)0);
     t.start = p.window ? (int)max(t.base + t.j0 - p.window + 1, (int64_t)0) & ~31 : 0;
-    t.chunks = t.end > t.start ? (int)(((int64_t)t.end - t.start + u.run - 1) / u.run) : 1;
+    t.chunks = t.end > t.start ? runs_of(t.end - t.start, u.run) : 1;
     return t;
 }
 
@@ -935,12 +938,12 @@ __global__ void __launch_bounds__((TileShape<T, DP>::TPB), DP == 256 ? 1 : 2) k_
 // MB, 3.6 TB/s).
 // ---------------------------------------------------------------------------
 
-constexpr int JOIN_ROWS(int M, int DP) { return M == ROWS_M ? 4 : 32; }      // rows a workgroup
+constexpr int rows_joined(int M) { return M == ROWS_M ? 4 : 32; }       // rows a workgroup
 
 template <typename T, int DP, int M>
 __device__ __forceinline__ void join_rows(const AttnArgs &p, int block)
 {
-    constexpr int ROWS = JOIN_ROWS(M, DP), parts = M / ROWS;
+    constexpr int ROWS = rows_joined(M), parts = M / ROWS;
     const int tid = threadIdx.x, group = p.n_head / p.n_head_kv;
     const int n0 = block % parts * ROWS, g = block / parts % p.n_head_kv, id = block / parts / p.n_head_kv;
     Unit u;
@@ -1034,6 +1037,13 @@ __global__ void __launch_bounds__(ATT_TPB) k_attn_join_both(AttnArgs many, AttnA
 
 static int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
+// Rows of a tile of many rows.
+static int tile_rows(const AttnArgs &p)
+{
+    static_assert(TileShape<float, 64>::M == TileShape<float, 128>::M, "one size up to heads of 128");
+    return padded_dim(p.head_dim) == 256 ? TileShape<float, 256>::M : TileShape<float, 128>::M;
+}
+
 // Units a kv head that the work is split into where there are fewer tiles: several a compute unit of few rows, one of
 // many.
 static int target_units(const AttnArgs &p, bool many) { return std::max(1, (many ? 256 : 2048) / p.n_head_kv); }
@@ -1044,39 +1054,87 @@ static int64_t most_tiles(const AttnArgs &p, int M)
     return (int64_t)p.n_tokens * (p.n_head / p.n_head_kv) / M + std::min(p.n_seq, p.n_tokens);
 }
 
-// Values of the partial results of split tiles.  They are fewer than `target`, and so are their units; twice that where a
-// unit ends at 2^30 keys.
+// Values of the partial results of split tiles, whose units are at most `target` in all.
 static size_t partial_values(const AttnArgs &p, bool many)
 {
-    const int dp = padded_dim(p.head_dim), rows = !many ? ROWS_M : dp == 256 ? TileShape<float, 256>::M : TileShape<float, 128>::M;
-    return (size_t)2 * target_units(p, many) * rows * p.n_head_kv * (dp + 2);
+    const int rows = many ? tile_rows(p) : ROWS_M;
+    return (size_t)target_units(p, many) * rows * p.n_head_kv * (padded_dim(p.head_dim) + 2);
 }
 
 size_t attention_workspace(const AttnArgs &p) { return (partial_values(p, false) + partial_values(p, true)) * sizeof(float); }
 
-// The split of the requests of min_rows .. max_rows rows into tiles of at most 16 (MANY: TileShape::M): `p` is set up for
+// The split of the requests of min_rows .. max_rows rows into tiles of at most 16 (many: TileShape::M): `p` is set up for
 // it; workgroups of the products and of the join (0: no tile is split).
-template <typename T, int DP, bool MANY>
-static bool attention_split(AttnArgs &p, int min_rows, int max_rows, int &wgs, int &join_wgs)
+static bool attention_split(AttnArgs &p, bool many, int min_rows, int max_rows, int &wgs, int &join_wgs)
 {
-    constexpr int M = MANY ? TileShape<T, DP>::M : ROWS_M;
+    const int M = many ? tile_rows(p) : ROWS_M;
     p.min_rows = min_rows;
     p.max_rows = max_rows;
-    p.target = target_units(p, MANY);
-    if (!MANY) p.partial += partial_values(p, true);
+    p.target = target_units(p, many);
+    if (!many) p.partial += partial_values(p, true);
     // (at most 512 runs a tile, whatever the lengths)
-    p.least = MANY ? 256 : 128;
+    p.least = many ? 256 : 128;
     const int64_t longest = (int64_t)p.max_blocks << p.log_block;
     while (longest / p.least >= 512) p.least *= 2;
-    // Tiles at most; units: `target` or as many as there are tiles (a unit ends at 2^30 keys), and no more than the runs
-    // that the longest request could have.
+    // Tiles at most; units: `target` or as many as there are tiles, and no more than the runs that the longest request
+    // could have.
     int64_t tiles = most_tiles(p, M);
     if (max_rows < 0x7fffffff) tiles = std::min<int64_t>(tiles, (int64_t)p.n_seq * ((max_rows + M - 1) / M));
     const int64_t runs = (longest + p.least - 1) / p.least,
-                  units = std::min(std::max<int64_t>(tiles, p.target) * (longest > 1 << 30 ? 2 : 1), tiles * runs) * p.n_head_kv;
+                  units = std::min(std::max<int64_t>(tiles, p.target), tiles * runs) * p.n_head_kv;
     if (units > 0x7fffff) return false;
     wgs = (int)units;                         // (only fewer than `target` tiles are split)
-    join_wgs = longest > p.least ? (int)(std::min<int64_t>(tiles, p.target) * p.n_head_kv * (M / JOIN_ROWS(M, DP))) : 0;
+    join_wgs = longest > p.least ? (int)(std::min<int64_t>(tiles, p.target) * p.n_head_kv * (M / rows_joined(M))) : 0;
+    return true;
+}
+
+// A call's tiles of many rows and of few, each with a set of arguments, workgroups of its own (0: none are launched).  A
+// step of single tokens (no more tokens than requests) needs only the second, a single request only one of them.
+struct AttnLaunch {
+    AttnArgs many, few;
+    int many_wgs, few_wgs, many_join, few_join;
+};
+
+static bool attention_launch(const AttnArgs &p, AttnLaunch &l)
+{
+    const int64_t rows = (int64_t)p.n_tokens * (p.n_head / p.n_head_kv);
+    const bool only_few = p.n_tokens <= p.n_seq || rows <= ATT_FEW_ROWS, only_many = !only_few && p.n_seq == 1;
+    l = { p, p, 0, 0, 0, 0 };
+    return (only_few || attention_split(l.many, true, only_many ? 0 : ATT_FEW_ROWS + 1, 0x7fffffff, l.many_wgs, l.many_join)) &&
+           (only_many || attention_split(l.few, false, 0, only_few ? 0x7fffffff : ATT_FEW_ROWS, l.few_wgs, l.few_join));
+}
+
+bool attention_units(const AttnArgs &p, AttnUnits out[2])
+{
+    AttnLaunch l;
+    if (!attention_launch(p, l)) return false;
+    for (int k = 0; k < 2; k++) {
+        const AttnArgs &a = k == 0 ? l.many : l.few;
+        const int M = k == 0 ? tile_rows(p) : ROWS_M, wgs = k == 0 ? l.many_wgs : l.few_wgs, join = k == 0 ? l.many_join : l.few_join;
+        AttnUnits &o = out[k];
+        o = {};
+        if (wgs == 0) continue;
+        const auto sum = [&](auto f) {
+            int64_t n = 0;
+            for (int i = 0; i < p.n_seq; i++) {
+                int tiles, span;
+                Unit u;
+                request_work(a, M, i, tiles, span, u);
+                n += tiles * (int64_t)f(span);
+            }
+            return n;
+        };
+        const int64_t work = sum([](int span) { return span; });
+        o.tiles = sum([](int) { return 1; });
+        int run = unit_run(a, M, work, o.tiles);
+        const int tight = tight_run(a, M, work);
+        if (p.n_seq <= 64 && tight < run && sum([&](int span) { return runs_of(span, tight); }) <= a.target) run = tight;
+        o.run = run;
+        o.units = sum([&](int span) { return runs_of(span, run); });
+        o.grid = wgs / p.n_head_kv;
+        o.joined = join / (p.n_head_kv * (M / rows_joined(M)));
+        o.partial = (int64_t)(partial_values(p, k == 0) / ((size_t)M * p.n_head_kv * (padded_dim(p.head_dim) + 2)));
+    }
     return true;
 }
 
@@ -1097,25 +1155,19 @@ static void attention_few(const AttnArgs &p, int wgs, hipStream_t s)
     else hipLaunchKernelGGL((k_attn_rows<T, DP, false, false>), dim3(wgs), ATT_TPB, 0, s, p);
 }
 
-// Few rows and many rows are a launch each, the choice a request's own, and one joins both.  A step of single tokens (no
-// more tokens than requests) needs only the first, a single request only one of them.
+// Few rows and many rows are a launch each, the choice a request's own, and one joins both.
 template <typename T, int DP>
 static hipError_t attention_dim(const AttnArgs &p, hipStream_t s)
 {
-    constexpr int FEW = ATT_FEW_ROWS, M = TileShape<T, DP>::M;
-    const int64_t rows = (int64_t)p.n_tokens * (p.n_head / p.n_head_kv);
-    const bool only_few = p.n_tokens <= p.n_seq || rows <= FEW, only_many = !only_few && p.n_seq == 1;
-    AttnArgs many = p, few = p;
-    int many_wgs = 0, few_wgs = 0, many_join = 0, few_join = 0;
-    if ((!only_few && !attention_split<T, DP, true>(many, only_many ? 0 : FEW + 1, 0x7fffffff, many_wgs, many_join)) ||
-        (!only_many && !attention_split<T, DP, false>(few, 0, only_few ? 0x7fffffff : FEW, few_wgs, few_join)))
-        return hipErrorInvalidValue;
-    if (many_wgs > 0) attention_tiles<T, DP>(many, many_wgs, s);
-    if (few_wgs > 0) attention_few<T, DP>(few, few_wgs, s);
-    if (many_join > 0 && few_join > 0)
-        hipLaunchKernelGGL((k_attn_join_both<T, DP, M>), dim3(many_join + few_join), ATT_TPB, 0, s, many, few, many_join);
-    else if (many_join > 0) hipLaunchKernelGGL((k_attn_join<T, DP, M>), dim3(many_join), ATT_TPB, 0, s, many);
-    else if (few_join > 0) hipLaunchKernelGGL((k_attn_join<T, DP, ROWS_M>), dim3(few_join), ATT_TPB, 0, s, few);
+    constexpr int M = TileShape<T, DP>::M;
+    AttnLaunch l;
+    if (!attention_launch(p, l)) return hipErrorInvalidValue;
+    if (l.many_wgs > 0) attention_tiles<T, DP>(l.many, l.many_wgs, s);
+    if (l.few_wgs > 0) attention_few<T, DP>(l.few, l.few_wgs, s);
+    if (l.many_join > 0 && l.few_join > 0)
+        hipLaunchKernelGGL((k_attn_join_both<T, DP, M>), dim3(l.many_join + l.few_join), ATT_TPB, 0, s, l.many, l.few, l.many_join);
+    else if (l.many_join > 0) hipLaunchKernelGGL((k_attn_join<T, DP, M>), dim3(l.many_join), ATT_TPB, 0, s, l.many);
+    else if (l.few_join > 0) hipLaunchKernelGGL((k_attn_join<T, DP, ROWS_M>), dim3(l.few_join), ATT_TPB, 0, s, l.few);
     return hipGetLastError();
 }
 

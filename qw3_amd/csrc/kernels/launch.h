@@ -354,6 +354,13 @@ struct AttnArgs {
     float q_sign;
 };
 size_t attention_workspace(const AttnArgs &p);
+// A call's split as its kernels find it, of tiles of many rows and of few, offsets and lens being host memory: tiles and
+// units of a kv head, keys a unit; units that are launched, tiles that are joined and units that the workspace holds.
+// False: more than a launch has.
+struct AttnUnits {
+    int64_t run, tiles, units, grid, joined, partial;
+};
+bool attention_units(const AttnArgs &p, AttnUnits out[2]);
 hipError_t launch_attention(AttnArgs p, int type, hipStream_t s);
 
 // Sampling (sample.hip).  A part of a row hands on its best token, its largest ones, which are all up to `bound`,

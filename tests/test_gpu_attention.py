@@ -295,3 +295,27 @@ def test_values_just_before_a_window(hip_ready, type_, heads, kv, dim, block, ne
     got = run(q, pages, new, lens, type_, window)
     assert np.isfinite(got).all()
     assert (np.abs(got.astype(np.float64) - want) <= D.rounded_to(tol, want, type_)).all()
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("short,n", [(0, 2 ** 31 - 2 ** 16), (0, 2 ** 30 + 5), (1, 2 ** 31 - 2 ** 16 - 3), (70, 2 ** 31 - 2 ** 22 + 7)])
+def test_lengths_near_2_31(hip_ready, type_, short, n):
+    """One request of nearly 2^31 keys, its blocks shared, beside short ones.  k is 0, so every key has the same weight, a
+    power of two; v is 1 in one block and 3 in the other.  Sums of a run are whole multiples of that weight below 2^24,
+    so only those over at most 512 runs round, and the quotient: 520 half steps of 2^-24."""
+    block, dim = 1 << 16, 8
+    rng = np.random.default_rng(short)
+    lens = [n] + [5] * short
+    of = rng.integers(0, 2, 0x7fff).astype(np.int32)
+    pages = D.Pages(rng, [1], 1, 1, dim)
+    pages.block, pages.n_blocks, pages.max_blocks = block, 2, 0x7fff
+    pages.k, pages.v = np.zeros((2, 1, block, dim), np.float16), np.ones((2, 1, block, dim), np.float16)
+    pages.v[1] = 3
+    pages.table = np.zeros((len(lens), 0x7fff), np.int32)
+    pages.table[0], pages.table[1:, 0] = of, 1
+    q = rng.standard_normal((len(lens), 1, dim)).astype(D.NP[type_])
+    got = run(q, pages, [1] * len(lens), lens, type_)
+    keys = np.minimum(np.maximum(n - block * np.arange(0x7fff), 0), block)      # of each block
+    want = float((keys * (1 + 2 * of.astype(np.int64))).sum()) / n
+    assert np.abs(got[0].astype(np.float64) - want).max() <= want * (520 * 2.0 ** -24 + D.HALF_STEP[type_])
+    assert np.all(got[1:] == 3)

@@ -128,7 +128,7 @@ __device__ __forceinline__ Draw settings(const SampleArgs &a, int r)
     d.k = a.top_k ? max(a.top_k[r], 0) : 0;
     if (d.k >= a.n_vocab) d.k = 0;           // (all)
     const float u = a.uniform[r];
-    d.u = u > 0.0f ? u : 0.0f;
+    d.u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;       // (the largest number below 1)
     return d;
 }
 
@@ -651,7 +651,8 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
         __syncthreads();
         n = (int)sh.n;
         if (n <= SMP_HALF) break;
-        // too many: their weights by 2048 slices of the keys, then of the indices
+        // too many: their weights, at least a unit each so that a slice of tokens is not empty, by 2048 slices of the keys,
+        // then of the indices
         const bool by_key = lo < hi;
         const uint32_t span = by_key ? hi - lo : i1 - i0 - 1;
         const int shift = max(0, 21 - __builtin_clz(span | 1));
@@ -660,7 +661,7 @@ __device__ __forceinline__ void border_below(SampleShared &sh, const Row &row, c
             if (!counts(v)) return;
             const uint32_t key = order_key(v);
             if (key < lo || key > hi || (uint32_t)i < i0 || (uint32_t)i >= i1) return;
-            atomicAdd(&sh.weight[(by_key ? key - lo : (uint32_t)i - i0) >> shift], row.units(v));
+            atomicAdd(&sh.weight[(by_key ? key - lo : (uint32_t)i - i0) >> shift], max(row.units(v), 1ull));
         });
         __syncthreads();
         const u64 x = sh.weight[2 * tid], y = sh.weight[2 * tid + 1];

@@ -199,3 +199,26 @@ def test_parts_that_begin_with_masked_logits(hip_ready, rows, vocab):
                 x[r, end - vocab // parts + 8:end - 8] = 2 * rng.standard_normal(vocab // parts - 16) - 20 * (r % 3)
     for s in (dict(), dict(t=0.3), dict(t=1e-4), dict(p=0.9), dict(m=0.1, t=2.0)):
         check(x, rng.random(rows).astype(np.float32), **{n: np.full(rows, v) for n, v in s.items()})
+
+
+def test_numbers_beyond_their_range(hip_ready):
+    """u of 1 and more draws what the largest number below 1 does: no token of weight 0, whatever masks the row."""
+    rng = np.random.default_rng(11)
+    lowest = np.finfo(np.float32).min
+    for rows, vocab in ((6, 2000), (6, 40000), (300, 9000)):
+        x = logits(rng, rows, vocab)
+        x[1, 50:] = lowest
+        x[2, ::2] = lowest
+        x[3] = np.where(np.arange(vocab) % 7 == 0, x[3], -90)                    # a tail of small, equal weights
+        x[4] = np.where(np.arange(vocab) < 5, x[4], x[4] - 60)
+        x[5:] = x[5:] if rows == 6 else np.where(rng.random((rows - 5, vocab)) < 0.01, x[5:], lowest)
+        high = np.resize(np.array([1, 2, np.inf, 1e30, 1.0000001], np.float32), rows)
+        for s in SETTINGS + [dict(t=1e-3), dict(t=30.0)]:
+            s = {n: np.full(rows, v) for n, v in s.items()}
+            want, _ = check(x, np.full(rows, TOP), **s)
+            tokens = D.ints([-5] * rows)
+            some = {"t": ("temperature", D.floats), "k": ("top_k", D.ints), "p": ("top_p", D.floats), "m": ("min_p", D.floats)}
+            for u in (high, high[::-1].copy()):
+                ds3.sample(ds3.Buffer.from_array(x), D.floats(u), tokens, rows, vocab, **{some[n][0]: some[n][1](v) for n, v in s.items()})
+                got = tokens.read(np.int32, rows)
+                assert np.array_equal(got, want), np.argwhere(got != want)

@@ -520,7 +520,7 @@ int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t *kv_lens, 
  *        against the cache's exact F16 values
  *   F16: q as it is, the softmax's weights rounded to F16
  * Sums and the softmax are F32.  head_dim is a multiple of 8 up to 256, max_blocks *
- * block_size at most 2^31 - 2^16.  Requests' rows do not overlap (of those that do it is
+ * block_size at most 2^31 - 2^16, scale's magnitude at most 2^127.  Requests' rows do not overlap (of those that do it is
  * not defined which are written).
  * It uses the library's workspace: before a capture the call is made once. */
 int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint64_t q_row_stride,

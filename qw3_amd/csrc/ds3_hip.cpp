@@ -2815,8 +2815,8 @@ extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t
     if (!float_type_ok(what, type) ||
         !attention_sizes_ok(what, n_tokens, n_seq, n_head, n_head_kv, head_dim, n_blocks, block_size, max_blocks, window, p))
         return -1;
-    if (!std::isfinite(scale)) {
-        fprintf(stderr, "ds3_hip: %s: scale is not finite\n", what);
+    if (!(std::fabs(scale) <= 0x1p127f)) {            // (times log2 e it is finite)
+        fprintf(stderr, "ds3_hip: %s: scale=%g is not within 2^127\n", what, scale);
         return -1;
     }
     if (n_tokens == 0) return 0;

@@ -17,6 +17,7 @@
 #include "lanes.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace ds3k {
@@ -251,15 +252,23 @@ struct QFrag {
     f16x8 hi, lo;
 };
 
-// The power of two that brings a row's largest magnitude to 2^13 .. 2^14 (1 where it is 0 or
-// not finite), as its exponent.
+// The power of two that brings a row's largest magnitude to 2^13 .. 2^14 (below it where that is no normal number; 1 where
+// it is not finite), as its exponent.
 __device__ __forceinline__ int row_exponent(float amax)
 {
     const int e = (int)((__float_as_uint(amax) >> 23) & 255);
-    return e == 0 || e == 255 ? 0 : 13 + 127 - e;
+    return e == 255 ? 0 : 13 + 127 - max(e, 1);
 }
 
 __device__ __forceinline__ float mul_pow2(float v, int e) { return __builtin_ldexpf(v, e); }
+
+// A row's power of two, held so that the scale (not 0) without it stays above 2^-123: masked scores are -inf and must not
+// meet a 0.  Where it is held, the scale comes to less than 2^-98 and scores are below 2^39: all weights are alike,
+// whatever bits of q are lost.
+__device__ __forceinline__ int held_exponent(int e, float scale)
+{
+    return min(e, 100 + (int)(__float_as_uint(scale) >> 23) - 127);
+}
 
 // 16 keys x 32 values: lane l holds key (or row) l % 16, values 8 (l / 16) + 0 .. 7.
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -310,8 +319,8 @@ __device__ __forceinline__ void load_q(const AttnArgs &p, const T *q, bool live,
         }
         if constexpr (STEP == 32) amax = fmaxf(amax, lane_xor<16>(amax));
         amax = fmaxf(amax, lane_xor<32>(amax));
-        const int ex = row_exponent(amax);
-        c2 = mul_pow2(c2, -ex);
+        const int ex = held_exponent(row_exponent(amax), c2);
+        c2 = fminf(mul_pow2(c2, -ex), FLT_MAX);
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll

@@ -125,3 +125,8 @@ def test_positions_near_the_end_of_int32(lib, capfd):                           
     for block, most in ((1, 0x7fff0000), (16, 0x7fff000), (1 << 16, 0x7fff)):
         args = changed(ATTN, a4=huge, a15=1, a16=block)
         refused(lib, capfd, "attention_paged", changed(args, a17=most + 1), "max_blocks")
+
+
+def test_scales_beyond_2_127(lib, capfd):                                        # noqa: F811
+    for bad in (2.0 ** 127 * 1.001, -3e38, float("-inf")):
+        refused(lib, capfd, "attention_paged", changed(ATTN, a18=bad), "scale")

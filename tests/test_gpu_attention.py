@@ -319,3 +319,25 @@ def test_lengths_near_2_31(hip_ready, type_, short, n):
     want = float((keys * (1 + 2 * of.astype(np.int64))).sum()) / n
     assert np.abs(got[0].astype(np.float64) - want).max() <= want * (520 * 2.0 ** -24 + D.HALF_STEP[type_])
     assert np.all(got[1:] == 3)
+
+
+@pytest.mark.parametrize("type_", [F32, F16])
+@pytest.mark.parametrize("new,lens,window", [([1, 1], [60, 700], 0), ([1], [50], 20), ([20, 40], [33, 300], 0), ([70], [100], 30)])
+def test_scales_and_queries_at_the_ends_of_their_range(hip_ready, type_, new, lens, window):
+    """Scales that are no normal numbers, q next to them, and products of a tiny q with a large scale: masked keys stay
+    masked, and scores of 0 stay 0."""
+    def times(f):
+        def change(pages, q):
+            q[...] = q.astype(np.float64) * f
+        return change
+
+    def zero(pages, q):
+        pages.k[...] = 0
+        if type_ == F32:
+            q *= 1e30
+    cases = [(1e-42, None), (-1e-45, None), (2.0 ** 127, zero), (-1e30, zero)]
+    if type_ == F32:
+        cases += [(1e-4, times(2e-38)), (1e-4, times(1e-40)), (1e-42, times(1e-40)), (1e-44, times(1e30)), (0.1, times(0)),
+                  (1e38, times(1e-38)), (1e37, times(1e-37)), (1e38, times(0))]
+    for i, (scale, change) in enumerate(cases):
+        check(100 + i, new, lens, 4, 2, 64, 8, type_, window, scale=scale, change=change)

@@ -520,8 +520,11 @@ int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t *kv_lens, 
  *        against the cache's exact F16 values
  *   F16: q as it is, the softmax's weights rounded to F16
  * Sums and the softmax are F32.  head_dim is a multiple of 8 up to 256, max_blocks *
- * block_size at most 2^31 - 2^16, scale's magnitude at most 2^127.  Requests' rows do not overlap (of those that do it is
- * not defined which are written).
+ * block_size at most 2^31 - 2^16, scale's magnitude at most 2^127.  A call has at most
+ * 2^23 - 1 tiles over all kv heads, counted as one a request and one for every 16 rows
+ * (tokens times n_head / n_head_kv; 256 where a request has more than 64, 128 for heads
+ * above 128): 2^20 requests of one token at seven kv heads, say.  Requests' rows do not
+ * overlap (of those that do it is not defined which are written).
  * It uses the library's workspace: before a capture the call is made once. */
 int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint64_t q_row_stride,
                             const ds3_hip_buffer_t *k_cache, const ds3_hip_buffer_t *v_cache,

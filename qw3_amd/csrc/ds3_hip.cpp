@@ -2798,7 +2798,10 @@ static bool attention_sizes_ok(const char *what, uint32_t n_tokens, uint32_t n_s
     p.log_block = log_block;
     p.max_blocks = (int)max_blocks;
     p.window = (int)window;
-    return true;
+    if (attention_fits(p)) return true;
+    fprintf(stderr, "ds3_hip: %s: %u tokens of %u heads, %u kv heads, in %u requests are more than 2^23 - 1 tiles\n", what,
+            n_tokens, n_head, n_head_kv, n_seq);
+    return false;
 }
 
 extern "C" int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint64_t q_row_stride,

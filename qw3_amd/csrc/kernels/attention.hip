@@ -1113,6 +1113,12 @@ static bool attention_launch(const AttnArgs &p, AttnLaunch &l)
            (only_many || attention_split(l.few, false, 0, only_few ? 0x7fffffff : ATT_FEW_ROWS, l.few_wgs, l.few_join));
 }
 
+bool attention_fits(const AttnArgs &p)
+{
+    AttnLaunch l;
+    return attention_launch(p, l);
+}
+
 bool attention_units(const AttnArgs &p, AttnUnits out[2])
 {
     AttnLaunch l;

@@ -353,10 +353,11 @@ struct AttnArgs {
     int min_rows, max_rows, target, least;
     float q_sign;
 };
+bool attention_fits(const AttnArgs &p);              // its tiles' workgroups fit a launch
 size_t attention_workspace(const AttnArgs &p);
 // A call's split as its kernels find it, of tiles of many rows and of few, offsets and lens being host memory: tiles and
 // units of a kv head, keys a unit; units that are launched, tiles that are joined and units that the workspace holds.
-// False: more than a launch has.
+// False: not attention_fits.
 struct AttnUnits {
     int64_t run, tiles, units, grid, joined, partial;
 };

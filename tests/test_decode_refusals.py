@@ -130,3 +130,12 @@ def test_positions_near_the_end_of_int32(lib, capfd):                           
 def test_scales_beyond_2_127(lib, capfd):                                        # noqa: F811
     for bad in (2.0 ** 127 * 1.001, -3e38, float("-inf")):
         refused(lib, capfd, "attention_paged", changed(ATTN, a18=bad), "scale")
+
+
+def test_tiles_beyond_a_launch(lib, capfd):                                      # noqa: F811
+    """2^23 workgroups of 256 or 512 threads are more than a launch has."""
+    far = [buf(1 << 42, (i + 1) << 44) for i in range(7)]
+    for heads, kv, tokens, seqs in ((8, 8, 1 << 20, 1 << 20), (1 << 16, 1 << 16, 1 << 15, 1), (1 << 16, 1, 1 << 20, 1)):
+        stride = heads * 8 * 4
+        args = [far[0], F32, stride, *far[1:6], far[6], stride, tokens, seqs, heads, kv, 8, 5, 16, 4, 0.125, 0]
+        refused(lib, capfd, "attention_paged", args, "more than 2^23 - 1 tiles")

@@ -455,7 +455,10 @@ int ds3_hip_rope_table(ds3_hip_buffer_t *table, uint32_t rotary_dim, double base
  * eps) * norm, in F32.  The first rotary_dim values of a head turn: value i with
  * value i + rotary_dim / 2, or interleaved, 2 i with 2 i + 1; the rest are copied
  * (normalised).  Angles are reduced in 64 bits.  out may be x itself (one type,
- * one stride).  head_dim is a multiple of 8 up to 512, rotary_dim even. */
+ * one stride).  head_dim is a multiple of 8 up to 512, rotary_dim even.  Calls of more
+ * than 2^24 - 1 workgroups are refused: 256 lanes each, a head's lanes its values / 8
+ * (rotary_dim a multiple of 8; / 4 or / 2 else) up to a power of two, at most 64, for
+ * up to five of its token's heads. */
 int ds3_hip_rope(const ds3_hip_buffer_t *x, ds3_hip_type_t x_type, uint64_t x_row_stride,
                  const ds3_hip_buffer_t *positions, const ds3_hip_buffer_t *table, const ds3_hip_buffer_t *norm,
                  float eps, ds3_hip_buffer_t *out, ds3_hip_type_t out_type, uint64_t out_row_stride, uint32_t n_tokens,

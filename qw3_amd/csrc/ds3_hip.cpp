@@ -2538,6 +2538,21 @@ bool head_counts_ok(const char *what, uint32_t n_head, uint32_t n_head_kv, uint3
     return true;
 }
 
+bool rope_fits_ok(const char *what, uint32_t n_tokens, uint32_t n_head, uint32_t n_head_kv, uint32_t head_dim,
+                  uint32_t rotary_dim)
+{
+    RopeArgs p{};
+    p.n_tokens = n_tokens;
+    p.n_head = (int)n_head;
+    p.n_head_kv = (int)n_head_kv;
+    p.head_dim = (int)head_dim;
+    p.rotary = (int)rotary_dim;
+    if (rope_fits(p)) return true;
+    fprintf(stderr, "ds3_hip: %s: %u tokens of %u and %u heads of %u are more than 2^24 - 1 workgroups\n", what, n_tokens,
+            n_head, 2 * n_head_kv, head_dim);
+    return false;
+}
+
 bool rotary_ok(const char *what, uint32_t rotary_dim, uint32_t most)
 {
     if (rotary_dim != 0 && rotary_dim % 2 == 0 && rotary_dim <= most) return true;
@@ -2601,7 +2616,8 @@ extern "C" int ds3_hip_rope(const ds3_hip_buffer_t *x, ds3_hip_type_t x_type, ui
     const char *what = "rope";
     if (!x || !positions || !table || !out) return -1;
     if (!float_type_ok(what, x_type) || !float_type_ok(what, out_type) || !head_counts_ok(what, n_head, 1, head_dim, 512) ||
-        !rotary_ok(what, rotary_dim, head_dim) || !mx_sizes_ok(what, { n_tokens }))
+        !rotary_ok(what, rotary_dim, head_dim) || !mx_sizes_ok(what, { n_tokens }) ||
+        !rope_fits_ok(what, n_tokens, n_head, 0, head_dim, rotary_dim))
         return -1;
     if (n_tokens == 0) return 0;
     const size_t p_b = (size_t)n_tokens * 4, t_b = ((size_t)rotary_dim / 2 + 1) * 8, w_b = (size_t)head_dim * 4;
@@ -2655,7 +2671,8 @@ extern "C" int ds3_hip_rope_append(const ds3_hip_buffer_t *q, const ds3_hip_buff
     if (!float_type_ok(what, type) || (q && !float_type_ok(what, q_out_type)) ||
         !head_counts_ok(what, q ? n_head : n_head_kv, n_head_kv, head_dim, 512) ||
         (table && !rotary_ok(what, rotary_dim, head_dim)) || !mx_sizes_ok(what, { n_tokens }) ||
-        !pages_ok(what, n_blocks, block_size, &log_block))
+        !pages_ok(what, n_blocks, block_size, &log_block) ||
+        !rope_fits_ok(what, n_tokens, q ? n_head : 0, n_head_kv, head_dim, table ? rotary_dim : 0))
         return -1;
     if (n_tokens == 0) return 0;
     const size_t i_b = (size_t)n_tokens * 4, t_b = table ? ((size_t)rotary_dim / 2 + 1) * 8 : 0, w_b = (size_t)head_dim * 4,

@@ -211,20 +211,39 @@ static void rope_width(const RopeArgs &p, bool inter, int v, dim3 grid, hipStrea
     else rope_launch<TI, TO, 1>(p, inter, grid, s);
 }
 
+constexpr int ROPE_HEADS = 5;                // that a group of lanes takes at most
+
+static int rope_pairs(const RopeArgs &p) { return p.rotary % 8 == 0 ? 4 : p.rotary % 4 == 0 ? 2 : 1; }
+
+static int rope_lanes(const RopeArgs &p)
+{
+    int lanes = 1;
+    while (lanes < std::min(p.head_dim / (2 * rope_pairs(p)), WAVE)) lanes *= 2;
+    return lanes;
+}
+
+// Workgroups of groups that take `per` heads each or a few less; p.lanes is set.
+static int64_t rope_split(RopeArgs &p, int per)
+{
+    p.log_chunks = 0;
+    while ((1 << p.log_chunks) * per < p.n_head + 2 * p.n_head_kv) p.log_chunks++;
+    return ((p.n_tokens << p.log_chunks) * p.lanes + ROPE_TPB - 1) / ROPE_TPB;
+}
+
+bool rope_fits(RopeArgs p)
+{
+    p.lanes = rope_lanes(p);
+    return rope_split(p, ROPE_HEADS) <= 0xffffff;
+}
+
 hipError_t launch_rope(RopeArgs p, int in_type, int out_type, bool inter, hipStream_t s)
 {
-    const int v = p.rotary % 8 == 0 ? 4 : p.rotary % 4 == 0 ? 2 : 1;
-    const int units = p.head_dim / (2 * v);
-    p.lanes = 1;
-    while (p.lanes < std::min(units, WAVE)) p.lanes *= 2;
-    const int heads = p.n_head + 2 * p.n_head_kv;
+    const int v = rope_pairs(p);
+    p.lanes = rope_lanes(p);
     // one head a group of lanes until the card is full, then up to five
-    const int64_t groups = p.n_tokens * heads, full = (int64_t)device_cu_count() * 8 * (ROPE_TPB / p.lanes);
-    const int per = (int)std::clamp<int64_t>(groups / full, 1, 5);
-    p.log_chunks = 0;
-    while ((1 << p.log_chunks) * per < heads) p.log_chunks++;
-    const int64_t n = (p.n_tokens << p.log_chunks) * p.lanes;
-    const int64_t wgs = (n + ROPE_TPB - 1) / ROPE_TPB;
+    const int64_t groups = p.n_tokens * (p.n_head + 2 * p.n_head_kv),
+                  full = (int64_t)device_cu_count() * 8 * (ROPE_TPB / p.lanes);
+    const int64_t wgs = rope_split(p, (int)std::clamp<int64_t>(groups / full, 1, ROPE_HEADS));
     if (wgs > 0xffffff) return hipErrorInvalidValue;
     const dim3 grid((unsigned)wgs);
     if (in_type == T_F32) {

@@ -318,6 +318,7 @@ struct RopeArgs {
     int log_block, n_head, n_head_kv, head_dim, rotary;
     int lanes, log_chunks;       // lanes a head; groups of them a token (a power of two)
 };
+bool rope_fits(RopeArgs p);              // its workgroups fit a launch
 hipError_t launch_rope(RopeArgs p, int in_type, int out_type, bool inter, hipStream_t s);
 
 // The plan of a step (ds3_hip_kv_plan) with its scratch: n_free as it was, and of

@@ -139,3 +139,15 @@ def test_tiles_beyond_a_launch(lib, capfd):                                     
         stride = heads * 8 * 4
         args = [far[0], F32, stride, *far[1:6], far[6], stride, tokens, seqs, heads, kv, 8, 5, 16, 4, 0.125, 0]
         refused(lib, capfd, "attention_paged", args, "more than 2^23 - 1 tiles")
+
+
+def test_heads_beyond_a_launch(lib, capfd):                                      # noqa: F811
+    """2^24 workgroups of 256 threads are more than a launch has: here 2^26 groups of 64 lanes."""
+    far = [buf(1 << 45, (i + 1) << 46) for i in range(11)]
+    for tokens, heads, dim in ((1 << 26, 5, 512), (1 << 25, 6, 264), (1 << 12, 1 << 16, 512), (1 << 31, 1, 512)):
+        row = heads * dim * 4
+        args = [far[0], F32, row, far[1], far[2], far[3], 1e-6, far[4], F32, row, tokens, heads, dim, 64, False]
+        refused(lib, capfd, "rope", args, "out of range" if tokens >> 31 else "more than 2^24 - 1 workgroups")
+    args = [far[0], far[1], far[2], F32, 2048, 2048, 2048, far[3], far[4], far[5], far[6], far[7], 1e-6, far[8], F32, far[9],
+            far[10], 1 << 26, 1, 1, 512, 64, False, 5, 16]
+    refused(lib, capfd, "rope_append", args, "more than 2^24 - 1 workgroups")

@@ -193,7 +193,9 @@ struct Row {
     __device__ u64 units(float v) const { return (u64)__double2ll_rn(weight(v) * SMP_ONE); }
     // v / T in steps of 1 / 32 of an octave, as whole + more + part: a grid that the parts of a row have in common.  The
     // product of 48 bits (two factors, the first product's rounding by an fma) keeps the part to 2^-25 where steps are
-    // many; 64-bit instructions for it took three times as long.
+    // many; 64-bit instructions for it took three times as long.  hi is the rounded product wherever it stands: taken into
+    // an fma, hi - whole would count its rounding twice (weights off by 0.3 % at v / T of 5e4) and the whole steps would
+    // not fall with v.
     float c_hi, c_lo;
     struct Steps {
         float whole, more, part;
@@ -207,6 +209,7 @@ struct Row {
     }
     __device__ Steps steps(float v) const
     {
+#pragma clang fp contract(off)
         const float hi = v * c_hi, lo = fmaf(v, c_lo, fmaf(v, c_hi, -hi));
         Steps s;
         s.whole = floorf(hi);

@@ -222,3 +222,14 @@ def test_numbers_beyond_their_range(hip_ready):
                 ds3.sample(ds3.Buffer.from_array(x), D.floats(u), tokens, rows, vocab, **{some[n][0]: some[n][1](v) for n, v in s.items()})
                 got = tokens.read(np.int32, rows)
                 assert np.array_equal(got, want), np.argwhere(got != want)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 60000), (20, 20000), (300, 5000)])
+def test_many_steps_of_temperature(hip_ready, rows, vocab):
+    """Logits far from 0 in units of the temperature: their weights are as exact as those of others."""
+    rng = np.random.default_rng(vocab)
+    for centre, t in ((-50, 1e-3), (50, 1e-3), (-50, 0.3), (1000, 0.05), (-2e4, 2.0), (30, 1.0)):
+        x = (centre + t * logits(rng, rows, vocab, peak=3)).astype(np.float32)
+        for s in (dict(), dict(p=0.9), dict(p=0.99999), dict(m=1e-3)):
+            s = {"t": t, **s}
+            check(x, rng.random(rows).astype(np.float32), **{n: np.full(rows, v) for n, v in s.items()})

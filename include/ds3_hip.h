@@ -493,8 +493,10 @@ int ds3_hip_rope_append(const ds3_hip_buffer_t *q, const ds3_hip_buffer_t *k, co
  *   max_blocks blocks }.
  * A plan that lacks blocks, has such a request or more than max_tokens tokens is
  * not carried out: lengths, table and n_free stay, every offset is 0, every slot
- * -1.  Each of them is then safe to run the layer's calls on, which do nothing.
- * free_blocks holds n_blocks entries; n_free is held to 0 .. n_blocks. */
+ * -1.  Each of them is then safe to run the layer's calls on, which do nothing (status
+ * tells the blocks that it would have taken).  free_blocks holds n_blocks entries;
+ * n_free is held to 0 .. n_blocks.
+ * It uses the library's workspace: before a capture the call is made once. */
 int ds3_hip_kv_plan(const ds3_hip_buffer_t *new_lens, const ds3_hip_buffer_t *kv_lens, ds3_hip_buffer_t *kv_lens_out,
                     ds3_hip_buffer_t *block_table, const ds3_hip_buffer_t *free_blocks, const ds3_hip_buffer_t *n_free,
                     ds3_hip_buffer_t *n_free_out, ds3_hip_buffer_t *q_offsets, ds3_hip_buffer_t *positions,
@@ -516,7 +518,8 @@ int ds3_hip_kv_release(const ds3_hip_buffer_t *done, ds3_hip_buffer_t *kv_lens, 
  * n_head_kv).  A token that sees nothing gets zeros: one at a position below 0, or
  * whose blocks all lie outside the cache.  A value of the cache that is infinite or
  * NaN makes what it enters infinite or NaN (F32: NaN for an infinite v too) in the rows
- * that see it, and in no others.  Rows of out that belong to no request are left as
+ * that see it, and in no others; an infinite k whose score is -inf may leave its key
+ * without weight instead.  Rows of out that belong to no request are left as
  * they were, as are those of a request whose rows do not lie within n_tokens.  q and
  * out are of `type`, rows of n_head heads.
  *   F32: products to 22 bits of q and of the softmax's weights (two F16 parts each),

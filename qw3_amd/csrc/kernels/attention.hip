@@ -246,12 +246,6 @@ __device__ __forceinline__ void split(float v, _Float16 &hi, _Float16 &lo)
     lo = (_Float16)(v - (float)hi);
 }
 
-// Eight values of a row of q: F16 as they are, F32 scaled and in two parts.
-template <typename T>
-struct QFrag {
-    f16x8 hi, lo;
-};
-
 // The power of two that brings a row's largest magnitude to 2^13 .. 2^14 (below it where that is no normal number; 1 where
 // it is not finite), as its exponent.
 __device__ __forceinline__ int row_exponent(float amax)
@@ -341,7 +335,7 @@ __device__ __forceinline__ void load_q(const AttnArgs &p, const T *q, bool live,
     }
 }
 
-// The row of a cache that holds position `key` (of kv head g): its first value's index, or -1.
+// The row of a cache that holds position `key` (of kv head g) in `block`: its first value's index.
 __device__ __forceinline__ int64_t cache_row(const AttnArgs &p, int block, int key, int g)
 {
     return ((((int64_t)block * p.n_head_kv + g) << p.log_block) + (key & ((1 << p.log_block) - 1))) * p.head_dim;
@@ -355,14 +349,14 @@ __device__ __forceinline__ int64_t cache_row(const AttnArgs &p, int block, int k
 // operand of output tile t is value t of each: an 8 x (DP / 16) transposition within
 // the lane.  The lane of the result then holds DP / 4 consecutive values of its row.
 // LDS would only pass on what one wave alone reads.  64 streams with 433,032 keys in all, F16, 32 heads over 4 of 128:
-// 164 us, 5.4 TB/s (a copy on this card moves 4.6, reads alone more), and 10 of the join.  One stream on 4097 keys,
-// F32: 8 us, of which the reads are 2: launch, the chain from lengths over the table to the keys, sums over four waves;
-// and 4 of the join (one launch for both ends each unit in a device-wide fence).
+// 167 us, 5.3 TB/s (a copy on this card moves 4.6, reads alone more), and 10 of the join; F32 1 % longer.  One stream on
+// 4097 keys, F32: 8 us, of which the reads are 2: launch, the chain from lengths over the table to the keys, sums over
+// four waves; and 5 of the join (one launch for both ends each unit in a device-wide fence).  Heads between 64, 128 and
+// 256 take the next one's products and time: 64 streams on up to 4096 keys 59 us at 80, 62 at 128, 131 at 136, 140 at 256.
 // ---------------------------------------------------------------------------
 
 constexpr int ROWS_M = 16;
 
-template <int DP>
 struct RowsShared {
     float o[4][ROWS_M][128 + 4];
     float m[4][ROWS_M], l[4][ROWS_M];
@@ -374,7 +368,7 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NC = DP / 32;              // operands of a key's row
     constexpr int NT = DP / 16;              // output tiles; values of a key that a lane reads for the second product
-    __shared__ RowsShared<DP> sh;
+    __shared__ RowsShared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), r = lane & 15, h = lane >> 4;
     const int g = blockIdx.x % p.n_head_kv, id = blockIdx.x / p.n_head_kv, group = p.n_head / p.n_head_kv;
     Unit u;
@@ -617,8 +611,9 @@ __global__ void __launch_bounds__(ATT_TPB, DP == 256 ? 1 : 2) k_attn_rows(AttnAr
 // A step's K is of one tile, its V of the tile before: weights come from scores already there, and one barrier a step,
 // between weights and the products, is enough.  Waves drift apart by most of a step, so that one's weights (vector units)
 // and staging run beside the other's products on its SIMD.  Two chunks of 4096 and 2582 tokens on up to 12,288 cached,
-// F16, 32 heads over 4 of 128: 1610 us, 862 TFLOP/s, where a large product reaches 1176.  With a second barrier after the
-// products 1734; with four waves half a step behind the others and two barriers, so that they always take turns, 1756.
+// F16, 32 heads over 4 of 128: 1610 us, 862 TFLOP/s, where a large product reaches 1176 (F32 2820, twice the products; the
+// first 30 launches on an idle card 1700, single ones more).  With a second barrier after the products 1734; with four
+// waves half a step behind the others and two barriers, so that they always take turns, 1756.
 // ---------------------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));

@@ -301,8 +301,8 @@ struct MxPlan {
 MxPlan mx_product_plan(const MxProduct &p, bool gate_up);
 
 // Rotary positions and the writing of k and v (kv_cache.hip).  Kinds: 0 q, 1 k, 2 v;
-// without a cache n_head_kv is 0, without q n_head is.  `lanes`, `per` and `chunks`
-// are the launcher's.
+// without a cache n_head_kv is 0, without q n_head is.  `lanes` and `log_chunks` are
+// the launcher's.
 struct RopeArgs {
     const void *x[3];            // rows of heads, stride[] bytes apart
     uint64_t stride[3];

@@ -27,11 +27,11 @@
 // compute unit (a pass of 256 rows of 151,936 takes 30 us, 5.2 TB/s) and the chains of
 // sorting, summing and looking up behind them (10 us), which no other row hides as a call
 // waits for its slowest.  256 rows of 151,936 by setting: temperature 0 33 us, top-k 20
-// with top-p 42, top-k 200 50, min-p 61, temperature 0.3 alone 62, 1 alone 87 (every
+// with top-p 42, top-k 200 50, min-p 61, temperature 0.3 alone 60, 1 alone 87 (every
 // logit's weight goes into a bin: some 25 vector instructions a logit, LDS atomics), top-p
 // 0.9 at temperature 1 115 (the border lies below the collected: a second pass for each
-// border), top-k 2000 110 (a pass that counts, one that gathers, the sort).  One row: 10
-// us, 15, 24, 32, 31, 31, 58, 66.
+// border), top-k 2000 109 (a pass that counts, one that gathers, the sort).  One row: 10
+// us, 15, 24, 32, 31, 31, 57, 65.
 #include "common.h"
 #include "lanes.h"
 

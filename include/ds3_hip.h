@@ -426,8 +426,9 @@ int ds3_hip_moe_block_mx(ds3_hip_buffer_t *hidden, const ds3_hip_buffer_t *delta
  * What device buffers hold cannot be refused by the host: slots and block ids
  * outside the cache are passed over (not written, not read), and each entry point
  * says what other values do.
- * Buffers: int32 and F32 ones start on multiples of 4 bytes, heads and caches on
- * multiples of 16 (of 8 where they hold fewer than 16 bytes a head half). */
+ * Buffers: int32 ones, logits and settings start on multiples of 4 bytes, tables of
+ * angles on multiples of 8, heads, caches and norms on multiples of 16; rows of heads lie
+ * a multiple of 16 bytes apart. */
 
 /* Angles of rotary positions, computed on the host in 64 bits and written to
  * `table` (rotary_dim / 2 + 1 doubles): pair i turns by position * f(theta_i),
@@ -548,7 +549,7 @@ int ds3_hip_attention_paged(const ds3_hip_buffer_t *q, ds3_hip_type_t type, uint
  *   the ones of at least min_p times the first's weight (0 or less, NaN: all),
  * always the first one.  Drawn is the first kept token in that order at which the summed
  * weights pass u times all kept ones'.  probs[r] (optional) is its share of them.
- * temperature 0 or less, or a logit of +inf: the first token, share 1.  A row of nothing but
+ * temperature 0 or less or NaN, or a logit of +inf: the first token, share 1.  A row of nothing but
  * -inf and NaN: token -1, share 0.  The settings are one F32 (top_k: int32) a row;
  * NULL: temperature 1, all tokens.
  * Weights are summed in 64 bits, where only sums of many small ones matter each to

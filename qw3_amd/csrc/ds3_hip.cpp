@@ -2878,7 +2878,8 @@ extern "C" int ds3_hip_debug_attention_split(const int32_t *q_offsets, const int
     AttnArgs p{};
     AttnUnits of[2];
     if (!q_offsets || !kv_lens || !split ||
-        !attention_sizes_ok("attention_split", n_tokens, n_seq, n_head, n_head_kv, head_dim, 1, block_size, max_blocks, window, p))
+        !attention_sizes_ok("attention_split", n_tokens, n_seq, n_head, n_head_kv, head_dim, 1, block_size, max_blocks,
+                            window, p))
         return -1;
     p.offsets = q_offsets;
     p.lens = kv_lens;

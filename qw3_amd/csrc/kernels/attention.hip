@@ -78,7 +78,10 @@ __host__ __device__ __forceinline__ int whole_runs(const AttnArgs &p, int M, flo
     return want >= 0x1p30f ? ATT_WHOLE : std::max(((int)want + grain) & -grain, p.least);
 }
 // (span and run up to ATT_WHOLE: their sum passes 2^31)
-__host__ __device__ __forceinline__ int runs_of(int span, int run) { return (int)(((unsigned)span + (unsigned)run - 1) / (unsigned)run); }
+__host__ __device__ __forceinline__ int runs_of(int span, int run)
+{
+    return (int)(((unsigned)span + (unsigned)run - 1) / (unsigned)run);
+}
 __host__ __device__ __forceinline__ int unit_run(const AttnArgs &p, int M, long long work, long long tiles)
 {
     if (tiles >= p.target) return ATT_WHOLE;
@@ -1120,7 +1123,8 @@ bool attention_units(const AttnArgs &p, AttnUnits out[2])
     if (!attention_launch(p, l)) return false;
     for (int k = 0; k < 2; k++) {
         const AttnArgs &a = k == 0 ? l.many : l.few;
-        const int M = k == 0 ? tile_rows(p) : ROWS_M, wgs = k == 0 ? l.many_wgs : l.few_wgs, join = k == 0 ? l.many_join : l.few_join;
+        const int M = k == 0 ? tile_rows(p) : ROWS_M, wgs = k == 0 ? l.many_wgs : l.few_wgs,
+                  join = k == 0 ? l.many_join : l.few_join;
         AttnUnits &o = out[k];
         o = {};
         if (wgs == 0) continue;
@@ -1175,7 +1179,8 @@ static hipError_t attention_dim(const AttnArgs &p, hipStream_t s)
     if (l.many_wgs > 0) attention_tiles<T, DP>(l.many, l.many_wgs, s);
     if (l.few_wgs > 0) attention_few<T, DP>(l.few, l.few_wgs, s);
     if (l.many_join > 0 && l.few_join > 0)
-        hipLaunchKernelGGL((k_attn_join_both<T, DP, M>), dim3(l.many_join + l.few_join), ATT_TPB, 0, s, l.many, l.few, l.many_join);
+        hipLaunchKernelGGL((k_attn_join_both<T, DP, M>), dim3(l.many_join + l.few_join), ATT_TPB, 0, s, l.many, l.few,
+                           l.many_join);
     else if (l.many_join > 0) hipLaunchKernelGGL((k_attn_join<T, DP, M>), dim3(l.many_join), ATT_TPB, 0, s, l.many);
     else if (l.few_join > 0) hipLaunchKernelGGL((k_attn_join<T, DP, ROWS_M>), dim3(l.few_join), ATT_TPB, 0, s, l.few);
     return hipGetLastError();

@@ -110,7 +110,7 @@ __device__ __forceinline__ bool search_unit(const AttnArgs &p, int M, int id, Un
         u.seq = 0;
         u.run = unit_run(p, M, (long long)tiles * span, tiles);
         const int tight = tight_run(p, M, (long long)tiles * span);
-        if (tight < u.run && (long long)tiles * (runs_of(span, tight)) <= p.target) u.run = tight;
+        if (tight < u.run && (long long)tiles * runs_of(span, tight) <= p.target) u.run = tight;
         const int chunks = runs_of(span, u.run);
         if ((long long)id >= (long long)tiles * (TILES ? 1 : chunks)) return false;
         u.tile = TILES ? id : id / chunks;
@@ -125,7 +125,7 @@ __device__ __forceinline__ bool search_unit(const AttnArgs &p, int M, int id, Un
         const long long work = wave_sum((long long)tiles * span);
         u.run = unit_run(p, M, work, wave_sum((long long)tiles));
         const int tight = tight_run(p, M, work);
-        if (tight < u.run && wave_sum((long long)tiles * (runs_of(span, tight))) <= p.target) u.run = tight;
+        if (tight < u.run && wave_sum((long long)tiles * runs_of(span, tight)) <= p.target) u.run = tight;
         const long long units = (long long)tiles * runs_of(span, u.run);
         const long long at = wave_scan(units) - units, first = TILES ? wave_scan((long long)tiles) - tiles : at;
         const uint64_t here = __ballot(id >= first && id < first + (TILES ? tiles : units));
